@@ -1,0 +1,236 @@
+// Shared by the masked attention's forward (attn_masked.hip) and backward
+// (attn_masked_bwd.hip) kernels: rows and their key ranges, the score
+// function, the tiles in LDS.
+//
+//   x_ij = sm_scale q_i.k_j
+//   s_ij = cap tanh(x_ij / cap) - slope_h |p_i - p_j|      (both optional)
+//   o_i  = sum_j softmax_j(s_ij) v_j over the keys that query i sees
+//
+// Rows.  The G = H / Hk query heads of a key head are rows of one problem:
+// row r of problem (b, key head) is token r / G, head r % G of the group, so
+// K and V are read once for the group and a block of rows spans few tokens.
+//
+// Masks are ranges.  A document is a run of queries [q0, q1) and one of keys
+// [k0, k1); query m stands at key coordinate at = m + k1 - q1 (the last query
+// at the last key).  It sees the keys [k0, hi), hi = k1, or under a causal
+// mask min(k1, max(k0 + prefix, at + 1)): ONE range, and the queries that see
+// a key are one range too.  So a tile is outside, inside or on the edge of a
+// block's ranges, and only edge tiles compare indices.
+#pragma once
+
+#include <math.h>
+
+#include "gpa_common.h"
+
+namespace gpa {
+
+constexpr int kMTile = 32;          // keys (forward, dq) or rows (dk, dv) of a tile
+constexpr int kMWaves = 4;
+constexpr int kMThreads = kMWaves * 64;
+constexpr int kMRows = kMWaves * 32;
+constexpr float kMLog2e = 1.4426950408889634f;
+constexpr uint32_t kNoRow = 0x40000000u;   // a DMA offset outside every descriptor: zeros
+
+// Where documents lie, and what limits a query's keys.
+struct MaskArgs {
+  const int32_t* q_off;   // nullable: one document, all queries
+  const int32_t* k_off;   // nullable: one document, all keys
+  const int32_t* lens;    // nullable: key counts of a batch (one document)
+  const int32_t* prefix;  // nullable: prefix_len for every document
+  int64_t qo_sb, ko_sb, prefix_sb;
+  int32_t docs, prefix_len, causal;
+  int32_t M, N;
+};
+
+struct DocSpan { int q0, q1, k0, k1, pre; };
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+// The last of `docs` runs that begins at or before `at` (-1: none), of the
+// run borders off[0 .. docs]; docs where off[docs] lies at or before it.
+__device__ __forceinline__ int find_run(const int32_t* off, int docs, int at) {
+  int lo = 0, hi = docs + 1;        // off[i] <= at holds for i < lo, not for i >= hi
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (off[mid] <= at) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo - 1;
+}
+
+// The document of batch element b's run d, or an empty one.  Whatever the
+// offsets hold, the ranges stay inside the queries and the keys.
+__device__ __forceinline__ DocSpan doc_span(const MaskArgs& a, int64_t b, int d) {
+  DocSpan s{0, 0, 0, 0, 0};
+  if (d < 0 || d >= a.docs) return s;
+  s.q1 = a.M;
+  s.k1 = a.N;
+  if (a.q_off) {
+    const int32_t* q = a.q_off + b * a.qo_sb + d;
+    s.q0 = clampi(q[0], 0, a.M);
+    s.q1 = clampi(q[1], s.q0, a.M);
+  }
+  if (a.k_off) {
+    const int32_t* k = a.k_off + b * a.ko_sb + d;
+    s.k0 = clampi(k[0], 0, a.N);
+    s.k1 = clampi(k[1], s.k0, a.N);
+  }
+  if (a.lens) s.k1 = clampi(a.lens[b], 0, a.N);
+  if (a.causal) s.pre = a.prefix ? clampi(a.prefix[b * a.prefix_sb + d], 0, a.N) : a.prefix_len;
+  return s;
+}
+
+// Keys [lo, hi) that query m of batch element b sees, and its key coordinate.
+struct RowSpan { int lo, hi, at; };
+__device__ __forceinline__ RowSpan row_span(const MaskArgs& a, int64_t b, int m) {
+  const int d = a.q_off ? find_run(a.q_off + b * a.qo_sb, a.docs, m) : 0;
+  const DocSpan s = doc_span(a, b, d);
+  RowSpan r{s.k0, s.k1, m + s.k1 - s.q1};
+  if (a.causal) r.hi = clampi(s.k0 + s.pre > r.at + 1 ? s.k0 + s.pre : r.at + 1, s.k0, s.k1);
+  if (m < s.q0 || m >= s.q1) r.hi = r.lo;
+  return r;
+}
+
+// Queries [lo, hi) that see key j, and what m is added to for its coordinate.
+struct KeySpan { int lo, hi, shift; };
+__device__ __forceinline__ KeySpan key_span(const MaskArgs& a, int64_t b, int j) {
+  const int d = a.k_off ? find_run(a.k_off + b * a.ko_sb, a.docs, j) : 0;
+  const DocSpan s = doc_span(a, b, d);
+  KeySpan k{s.q0, s.q1, s.k1 - s.q1};
+  if (a.causal && j - s.k0 >= s.pre) k.lo = clampi(j - k.shift, s.q0, s.q1);
+  if (j < s.k0 || j >= s.k1) k.hi = k.lo;
+  return k;
+}
+
+// Scores, in log2 units.  `c` is sm_scale log2(e); with a cap c = 2 log2(e)
+// sm_scale / cap (the exponent of e^(2u), u = x / cap) and capl = cap log2(e).
+struct ScoreArgs { float c, capl; };
+
+// tanh(u) = 1 - 2 / (1 + e^(2u)): right at both ends (e^(2u) = 0 or inf), and
+// off by about 2^-23 absolutely, 1e-5 of a score at a cap of 50.
+__device__ __forceinline__ float cap_tanh(float s, float c) {
+  const float e = __builtin_amdgcn_exp2f(s * c);
+  return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+}
+
+// One tile of a tensor in LDS: 32 rows of HD 16-bit values, row-major, their
+// 16-byte chunks XOR-swizzled by row so that both kinds of read are free of
+// bank conflicts: fragments of one chunk of 16 consecutive rows (all 16 slots
+// of 256 bytes are hit once) and ds_read_b64_tr_b16 of 4 chunks of 4 rows.
+template <int HD>
+__device__ __forceinline__ constexpr int tile_swz(int row) {
+  if constexpr (HD == 64) return ((row >> 1 & 1) << 2) | (row >> 2 & 3);   // two rows per 256 bytes
+  else return ((row & 3) << 2) | (row >> 2 & 3);
+}
+// Element offset of a row's 16-byte chunk.
+template <int HD>
+__device__ __forceinline__ constexpr int tile_at(int row, int chunk) {
+  return row * HD + ((chunk ^ tile_swz<HD>(row)) << 3);
+}
+
+// DMA of 4 / 16 bytes per lane into LDS at lds + 4 * lane / lds + 16 * lane.
+__device__ __forceinline__ void m_dma4(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t voff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      r, (__attribute__((address_space(3))) void*)lds, 4, voff, 0, 0, 0);
+}
+__device__ __forceinline__ void m_dma16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t voff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      r, (__attribute__((address_space(3))) void*)lds, 16, voff, 0, 0, 0);
+}
+// Wait until at most N vector-memory instructions of this wave are in flight.
+template <int N>
+__device__ __forceinline__ void m_wait() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// A descriptor over the rows [row, row + 32) of a tensor that ends at `end`
+// (rows; none: nothing is read).  Its base moves in 64 bits, so a tensor may
+// be longer than a 32-bit offset reaches.
+template <int HD>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint16_t* base, int64_t stride,
+                                                            int row, int end) {
+  int n = end - row;
+  n = n > kMTile ? kMTile : n;
+  const uint32_t bytes = n > 0 ? (uint32_t)(n - 1) * (uint32_t)(stride * 2) + HD * 2 : 0u;
+  return make_rsrc(base + (int64_t)row * stride, bytes);
+}
+
+// The A operand of a product over the tile's features: lane (hi, l32) has
+// row l32, features 16 ks + 8 hi .. +7.
+template <int HD>
+__device__ __forceinline__ bf16x8 row_frag(const uint16_t* t, int ks, int l32, int hi) {
+  return *reinterpret_cast<const bf16x8*>(&t[tile_at<HD>(l32, 2 * ks + hi)]);
+}
+
+// The A operand of a product over the tile's rows, transposed: lane (hi, l32)
+// has feature 32 db + l32 of the rows 16 s + 8 e + 4 hi + 0 .. 3 (e = 0, 1), the
+// order in which the score MFMA's result registers hold them, so that its
+// results are the B operand as they stand.
+template <int HD>
+__device__ __forceinline__ bf16x8 tr_frag(const uint16_t* t, int lane, int db, int s) {
+  typedef short i16x4 __attribute__((ext_vector_type(4)));
+  const int hi = lane >> 5, v4 = (lane & 15) >> 2, a = lane & 3, bit4 = (lane >> 4) & 1;
+  const int chunk = 4 * db + 2 * bit4 + (a >> 1);
+  const int row = 16 * s + 4 * hi + v4;
+  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) i16x4*)&t[tile_at<HD>(row, chunk) + (a & 1) * 4]);
+  const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) i16x4*)&t[tile_at<HD>(row + 8, chunk) + (a & 1) * 4]);
+  const bf16x4 l4 = __builtin_bit_cast(bf16x4, lo), u4 = __builtin_bit_cast(bf16x4, up);
+  return bf16x8{l4[0], l4[1], l4[2], l4[3], u4[0], u4[1], u4[2], u4[3]};
+}
+
+// Sixteen fp32 values of a lane as the B operand's two fragments.
+template <bool F16>
+__device__ __forceinline__ void pack_frags(const float (&p)[16], bf16x8 (&out)[2]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const bf16x2 v = pack2<F16>(p[8 * s + e], p[8 * s + e + 1]);
+      out[s][e] = v[0];
+      out[s][e + 1] = v[1];
+    }
+}
+
+// acc += A^T . P over a tile's rows where a row that a lane does not see may
+// hold infinities or NaN: 0 times them is NaN, so such values are taken out of
+// the product and the rows that do see them get them back by their sign: an
+// indicator product over the seen rows tells which (both signs: NaN).
+template <int HD, bool F16>
+__device__ __forceinline__ f32x16 careful_mfma(const uint16_t* t, int lane, int db,
+                                               const bf16x8 (&p)[2], const bf16x8 (&seen)[2],
+                                               f32x16 acc) {
+  const uint16_t expo = F16 ? 0x7c00 : 0x7f80, one = F16 ? 0x3c00 : 0x3f80;
+  f32x16 up{}, down{};
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+    u16x8 x = __builtin_bit_cast(u16x8, tr_frag<HD>(t, lane, db, s)), xp, xn;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint16_t w = x[e];
+      const bool odd = (w & expo) == expo, nan = odd && (w & (0x7fff ^ expo)) != 0;
+      xp[e] = odd && (nan || !(w & 0x8000)) ? one : 0;
+      xn[e] = odd && (nan || (w & 0x8000)) ? one : 0;
+      x[e] = odd ? 0 : w;
+    }
+    acc = mfma32x32x16_t<F16>(__builtin_bit_cast(bf16x8, x), p[s], acc);
+    up = mfma32x32x16_t<F16>(__builtin_bit_cast(bf16x8, xp), seen[s], up);
+    down = mfma32x32x16_t<F16>(__builtin_bit_cast(bf16x8, xn), seen[s], down);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    if (up[r] > 0.f) acc[r] += INFINITY;
+    if (down[r] > 0.f) acc[r] -= INFINITY;
+  }
+  return acc;
+}
+
+// Shared by the entry points: the checks of their arguments (has_o: an output
+// is written to a->o), and the kernels' form of them.
+int masked_check(const char* fn, int dtype, const gpa_attn_masked_args* a, bool has_o);
+void masked_fill(const gpa_attn_masked_args* a, MaskArgs* m, ScoreArgs* s);
+
+}  // namespace gpa

@@ -1,0 +1,680 @@
+// Masked attention, backward (attn_masked.h has the formulas and the masks).
+//
+//   P_ij  = 2^(s_ij log2(e) - lse_i)             (recomputed from q, k and the LSE)
+//   dP_ij = dO_i . V_j,   delta_i = dO_i . O_i - log2(e) dlse_i
+//   dS_ij = P_ij (dP_ij - delta_i) (1 - tanh^2(x_ij / cap))
+//   dV_j  = sum_i P_ij dO_i,   dK_j = sm_scale sum_i dS_ij Q_i,
+//   dQ_i  = sm_scale sum_j dS_ij K_j
+//
+// attn_masked_delta_kernel writes a record of every 32 rows: their LSE, -delta,
+// token and slope.  attn_masked_dkdv_kernel: a wave owns 32 keys (K, V, dK and
+// dV in registers) and walks the rows that see them, all query heads of the
+// key head, so a shared head's gradient is one sum in one order; S = Q . K^T
+// puts a key in each lane, and P and dS are used in place as the B operands of
+// dV^T += dO^T . P and dK^T += Q^T . dS.  attn_masked_dq_kernel mirrors it: a
+// wave owns 32 rows and walks the keys, dQ^T += K^T . dS^T.  No atomics: two
+// kernels compute S and dP twice (7 products instead of 5), and in return
+// the results repeat bit by bit and no fp32 copy of dQ goes through memory.
+//
+// P and dS are rounded to the operand format for the products (the same
+// relative error as the gradients' own rounding); sums are fp32.  In fp16
+// small weights would lose bits below 2^-14, so P is scaled by 2^14 and dS by a
+// power of two that follows its largest value; the sums are scaled back.
+#include "attn_masked.h"
+
+#include <algorithm>
+
+namespace gpa {
+namespace {
+
+constexpr int kRec = 128;                      // floats of a record: lse, -delta, token, slope
+
+struct BwdArgs {
+  const uint16_t *q, *k, *v, *o, *d_o;
+  const float *lse, *d_lse;
+  uint16_t *dq, *dk, *dv;
+  int64_t q_sb, q_sh, q_sm, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, o_sb, o_sh, o_sm;
+  int64_t do_sb, do_sh, do_sm, dq_sb, dq_sh, dq_sm, dk_sb, dk_sh, dk_sn, dv_sb, dv_sh, dv_sn;
+  int64_t lse_sb, lse_sh;
+  const float* slopes;
+  int64_t slopes_sb;
+  float* rec;                                  // [B * Hk][tiles][kRec]
+  int32_t Hk, G, R, tiles;                     // R = M * G rows of a problem
+  float sm_scale;
+  MaskArgs mask;
+  ScoreArgs score;
+};
+
+template <int HD, bool F16>
+__global__ __launch_bounds__(256) void attn_masked_delta_kernel(BwdArgs p) {
+  constexpr int CH = HD / 8;                   // lanes of a row
+  const int tile = blockIdx.x % p.tiles, prob = blockIdx.x / p.tiles;
+  const int b = prob / p.Hk, kvh = prob % p.Hk;
+  float* rec = p.rec + ((int64_t)prob * p.tiles + tile) * kRec;
+  const int ch = threadIdx.x % CH;
+  for (int i = threadIdx.x / CH; i < 32; i += 256 / CH) {
+    const int r = tile * 32 + i;
+    float lse = INFINITY, delta = 0.f, slope = 0.f;   // past the rows: weights of zero
+    int m = 0;
+    if (r < p.R) {
+      m = r / p.G;
+      const int h = kvh * p.G + r % p.G;
+      const bf16x8 x = *reinterpret_cast<const bf16x8*>(p.o + b * p.o_sb + h * p.o_sh + m * p.o_sm + 8 * ch);
+      const bf16x8 y = *reinterpret_cast<const bf16x8*>(p.d_o + b * p.do_sb + h * p.do_sh + m * p.do_sm + 8 * ch);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        delta = __builtin_fmaf(half_to_f32<F16>(x[e]), half_to_f32<F16>(y[e]), delta);
+      lse = p.lse[b * p.lse_sb + h * p.lse_sh + m];
+      if (lse == -INFINITY) lse = INFINITY;    // a row that sees nothing
+      if (p.slopes) slope = p.slopes[b * p.slopes_sb + h] * kMLog2e;
+      if (p.d_lse && ch == 0)
+        delta -= kMLog2e * p.d_lse[((int64_t)b * p.Hk * p.G + h) * p.mask.M + m];
+    }
+#pragma unroll
+    for (int s = 1; s < CH; s <<= 1) delta += __shfl_xor(delta, s);
+    if (ch == 0) {
+      rec[i] = lse;
+      rec[32 + i] = -delta;
+      rec[64 + i] = (float)m;
+      rec[96 + i] = slope;
+    }
+  }
+}
+
+constexpr float kPScale = 16384.0f;            // of P in fp16
+
+// The power of two by which a wave's dS are scaled in fp16: set by the first
+// values, lowered where later ones would pass the format's range.
+struct DsScale {
+  float s = 0.f;
+  // Whether it has to move for these values; `ratio` rescales the sums.
+  __device__ __forceinline__ bool follow(const float (&ds)[16], float& ratio) {
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(ds[i]));
+    if (!__builtin_amdgcn_ballot_w64(mx * s > 32768.0f || (s == 0.f && mx > 0.f))) return false;
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) mx = fmaxf(mx, __shfl_xor(mx, i));
+    // 2^13 at most; a largest value that is not finite leaves the scale alone.
+    const int e = mx < INFINITY ? min(13 - __builtin_amdgcn_frexp_expf(mx), 100) : 0;
+    const float to = mx < INFINITY ? __builtin_amdgcn_ldexpf(1.0f, e) : s == 0.f ? 1.0f : s;
+    ratio = s == 0.f ? 1.0f : to / s;
+    s = to;
+    return true;
+  }
+};
+
+template <int HD>
+struct RowSlot {
+  uint16_t q[kMTile * HD];
+  uint16_t d[kMTile * HD];
+  float st[kRec];
+};
+
+template <int HD, bool F16, bool CAP, bool SLOPE>
+__global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_kernel(BwdArgs p) {
+  constexpr int KS = HD / 16, DB = HD / 32, CH = HD / 8;
+  constexpr int DJ = kMTile * CH / kMThreads;
+  __shared__ __attribute__((aligned(16))) RowSlot<HD> r0, r1, r2, r3;
+  __shared__ __attribute__((aligned(16))) float sink[64];
+  __shared__ int range[2][kMWaves];
+
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int blocks = (p.mask.N + kMRows - 1) / kMRows;
+  const int kb = blockIdx.x % blocks, prob = blockIdx.x / blocks;
+  const int b = prob / p.Hk, kvh = prob % p.Hk;
+  const int j = kb * kMRows + wave * 32 + l32;
+  const bool live = j < p.mask.N;
+  const int jc = live ? j : p.mask.N - 1;
+  const KeySpan ks_ = key_span(p.mask, b, jc);
+  const int lo = ks_.lo * p.G, hi_r = ks_.hi * p.G;   // rows that see this lane's key
+  const float shift = (float)(ks_.shift - jc);
+
+  bf16x8 kf[KS], vf[KS];
+  {
+    const uint16_t* K = p.k + b * p.k_sb + kvh * p.k_sh + jc * p.k_sn;
+    const uint16_t* V = p.v + b * p.v_sb + kvh * p.v_sh + jc * p.v_sn;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kf[ks] = *reinterpret_cast<const bf16x8*>(K + 16 * ks + 8 * hi);
+      vf[ks] = *reinterpret_cast<const bf16x8*>(V + 16 * ks + 8 * hi);
+    }
+  }
+
+  const bool any = live && hi_r > lo;
+  int w_lo = any ? lo : 0x7fffffff, w_hi = any ? hi_r : 0;
+  int a_lo = live ? lo : 0, a_hi = live ? (any ? hi_r : 0) : 0x7fffffff;
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) {
+    w_lo = min(w_lo, __shfl_xor(w_lo, i));
+    w_hi = max(w_hi, __shfl_xor(w_hi, i));
+    a_lo = max(a_lo, __shfl_xor(a_lo, i));
+    a_hi = min(a_hi, __shfl_xor(a_hi, i));
+  }
+  w_lo = __builtin_amdgcn_readfirstlane(w_lo);
+  w_hi = __builtin_amdgcn_readfirstlane(w_hi);
+  a_lo = __builtin_amdgcn_readfirstlane(a_lo);
+  a_hi = __builtin_amdgcn_readfirstlane(a_hi);
+  if (lane == 0) {
+    range[0][wave] = w_lo;
+    range[1][wave] = w_hi;
+  }
+  __syncthreads();
+  int n_lo = range[0][0], n_hi = range[1][0];
+#pragma unroll
+  for (int i = 1; i < kMWaves; ++i) {
+    n_lo = min(n_lo, range[0][i]);
+    n_hi = max(n_hi, range[1][i]);
+  }
+  n_lo = __builtin_amdgcn_readfirstlane(n_lo);
+  n_hi = __builtin_amdgcn_readfirstlane(n_hi);
+  const int t_begin = n_hi > n_lo ? n_lo / 32 : 0, t_end = n_hi > n_lo ? (n_hi + 31) / 32 : 0;
+
+  // Rows of a tile: token and head of row 32 t + i follow from (32 t) / G; where
+  // G divides 32 the offsets inside a tile are the same for all tiles.
+  const uint16_t* Q = p.q + b * p.q_sb + (int64_t)kvh * p.G * p.q_sh;
+  const uint16_t* D = p.d_o + b * p.do_sb + (int64_t)kvh * p.G * p.do_sh;
+  const bool even = 32 % p.G == 0;
+  uint32_t q_voff[DJ], d_voff[DJ];
+  auto offsets = [&](int first) {              // first: (32 t) % G
+#pragma unroll
+    for (int i = 0; i < DJ; ++i) {
+      const int pos = (wave * DJ + i) * 64 + lane, row = pos / CH;
+      const uint32_t ch = (uint32_t)((pos % CH) ^ tile_swz<HD>(row)) * 16u;
+      const uint32_t tok = (uint32_t)(first + row) / (uint32_t)p.G, g = (uint32_t)(first + row) % (uint32_t)p.G;
+      q_voff[i] = tok * (uint32_t)(p.q_sm * 2) + g * (uint32_t)(p.q_sh * 2) + ch;
+      d_voff[i] = tok * (uint32_t)(p.do_sm * 2) + g * (uint32_t)(p.do_sh * 2) + ch;
+    }
+  };
+  offsets(0);
+  const float* rec = p.rec + (int64_t)prob * p.tiles * kRec;
+  auto issue = [&](int t, RowSlot<HD>& T) {
+    const int base = min(t, p.tiles) * 32;     // tiles past the rows: all lanes idle
+    if (!even) offsets(base % p.G);
+    const int64_t tok = base / p.G;
+    const __amdgpu_buffer_rsrc_t qr = make_rsrc(Q + tok * p.q_sm, kNoRow);
+    const __amdgpu_buffer_rsrc_t dr = make_rsrc(D + tok * p.do_sm, kNoRow);
+    const __amdgpu_buffer_rsrc_t rr = make_rsrc(rec + (int64_t)base / 32 * kRec, kRec * 4);
+    const int left = p.R - base;
+#pragma unroll
+    for (int i = 0; i < DJ; ++i) {
+      const bool in = ((wave * DJ + i) * 64 + lane) / CH < left;
+      m_dma16(qr, &T.q[(wave * DJ + i) * 512], in ? q_voff[i] : kNoRow);
+    }
+#pragma unroll
+    for (int i = 0; i < DJ; ++i) {
+      const bool in = ((wave * DJ + i) * 64 + lane) / CH < left;
+      m_dma16(dr, &T.d[(wave * DJ + i) * 512], in ? d_voff[i] : kNoRow);
+    }
+    // Waves 0 and 1 fetch the record; 2 and 3 land zeros beside it, so that
+    // every wave waits for the same number of DMAs.
+    m_dma4(rr, wave < 2 ? &T.st[wave * 64] : &sink[0],
+           wave < 2 && left > 0 ? (uint32_t)(wave * 64 + lane) * 4u : kNoRow);
+  };
+
+  f32x16 dk[DB], dv[DB];
+  DsScale sc;
+  auto restart = [&]() {
+    sc = DsScale{};
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
+  };
+
+  // P and dS of the tile's rows (registers) and this lane's key.
+  auto weights = [&](const RowSlot<HD>& T, int row0, bool edge, float (&w)[16], float (&ds)[16]) {
+    f32x16 s{}, dp;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 nd = *reinterpret_cast<const f32x4*>(&T.st[32 + 8 * g + 4 * hi]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[4 * g + e] = nd[e];
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      s = mfma32x32x16_t<F16>(row_frag<HD>(T.q, ks, l32, hi), kf[ks], s);
+      dp = mfma32x32x16_t<F16>(row_frag<HD>(T.d, ks, l32, hi), vf[ks], dp);
+    }
+    const int from = lo - row0 - 4 * hi, to = hi_r - row0 - 4 * hi;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 ls = *reinterpret_cast<const f32x4*>(&T.st[8 * g + 4 * hi]);
+      f32x4 tok, sl;
+      if constexpr (SLOPE) {
+        tok = *reinterpret_cast<const f32x4*>(&T.st[64 + 8 * g + 4 * hi]);
+        sl = *reinterpret_cast<const f32x4*>(&T.st[96 + 8 * g + 4 * hi]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * g + e;
+        float t = 0.f, x;
+        if constexpr (CAP) {
+          t = cap_tanh(s[i], p.score.c);
+          x = t * p.score.capl;
+        } else {
+          x = s[i] * p.score.c;
+        }
+        if constexpr (SLOPE) x = __builtin_fmaf(-sl[e], fabsf(tok[e] + shift), x);
+        w[i] = __builtin_amdgcn_exp2f(x - ls[e]);
+        ds[i] = w[i] * dp[i];
+        if constexpr (CAP) ds[i] *= __builtin_fmaf(-t, t, 1.0f);
+        if (edge && (mfma_row(i, 0) < from || mfma_row(i, 0) >= to)) w[i] = ds[i] = 0.f;
+      }
+    }
+    if constexpr (F16) {
+      float ratio;
+      if (sc.follow(ds, ratio)) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) dk[db] *= ratio;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        w[i] *= kPScale;
+        ds[i] *= sc.s;
+      }
+    }
+  };
+
+  auto iter = [&](int t, const RowSlot<HD>& cur, RowSlot<HD>& dst) {
+    m_wait<2 * (2 * DJ + 1)>();
+    __syncthreads();
+    issue(t + 3, dst);
+    const int row0 = t * 32;
+    if (row0 >= w_hi || row0 + 32 <= w_lo) return;
+    float w[16], ds[16];
+    weights(cur, row0, row0 < a_lo || row0 + 32 > a_hi, w, ds);
+    bf16x8 wb[2], db_[2];
+    pack_frags<F16>(w, wb);
+    pack_frags<F16>(ds, db_);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        dv[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.d, lane, db, s), wb[s], dv[db]);
+        dk[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.q, lane, db, s), db_[s], dk[db]);
+      }
+  };
+  restart();
+  issue(t_begin, r0);
+  issue(t_begin + 1, r1);
+  issue(t_begin + 2, r2);
+  for (int t = t_begin; t < t_end; t += 4) {
+    iter(t, r0, r3);
+    if (t + 1 >= t_end) break;
+    iter(t + 1, r1, r0);
+    if (t + 2 >= t_end) break;
+    iter(t + 2, r2, r1);
+    if (t + 3 >= t_end) break;
+    iter(t + 3, r3, r2);
+  }
+  m_wait<0>();
+
+  bool odd = false;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      odd |= !(fabsf(dk[db][i]) < INFINITY) || !(fabsf(dv[db][i]) < INFINITY);
+  if (__syncthreads_or(odd && live)) {
+    restart();
+    for (int t = t_begin; t < t_end; ++t) {
+      __syncthreads();
+      issue(t, r0);
+      m_wait<0>();
+      __syncthreads();
+      const int row0 = t * 32, from = lo - row0 - 4 * hi, to = hi_r - row0 - 4 * hi;
+      float w[16], ds[16], sx[16];
+      weights(r0, row0, true, w, ds);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        sx[i] = mfma_row(i, 0) < from || mfma_row(i, 0) >= to ? 0.f : 1.f;
+      bf16x8 wb[2], db_[2], sb[2];
+      pack_frags<F16>(w, wb);
+      pack_frags<F16>(ds, db_);
+      pack_frags<F16>(sx, sb);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        dv[db] = careful_mfma<HD, F16>(r0.d, lane, db, wb, sb, dv[db]);
+        dk[db] = careful_mfma<HD, F16>(r0.q, lane, db, db_, sb, dk[db]);
+      }
+    }
+  }
+  if (!live) return;
+  const float kx = F16 ? (sc.s == 0.f ? 0.f : p.sm_scale / sc.s) : p.sm_scale;
+  const float vx = F16 ? 1.0f / kPScale : 1.0f;
+  uint16_t* DK = p.dk + b * p.dk_sb + kvh * p.dk_sh + j * p.dk_sn;
+  uint16_t* DV = p.dv + b * p.dv_sb + kvh * p.dv_sh + j * p.dv_sn;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int at = db * 32 + 8 * g + 4 * hi;
+      const bf16x2 k0 = pack2<F16>(dk[db][4 * g] * kx, dk[db][4 * g + 1] * kx);
+      const bf16x2 k1 = pack2<F16>(dk[db][4 * g + 2] * kx, dk[db][4 * g + 3] * kx);
+      const bf16x2 v0 = pack2<F16>(dv[db][4 * g] * vx, dv[db][4 * g + 1] * vx);
+      const bf16x2 v1 = pack2<F16>(dv[db][4 * g + 2] * vx, dv[db][4 * g + 3] * vx);
+      *reinterpret_cast<u32x2*>(DK + at) =
+          u32x2{__builtin_bit_cast(uint32_t, k0), __builtin_bit_cast(uint32_t, k1)};
+      *reinterpret_cast<u32x2*>(DV + at) =
+          u32x2{__builtin_bit_cast(uint32_t, v0), __builtin_bit_cast(uint32_t, v1)};
+    }
+}
+
+template <int HD>
+struct KeySlot {
+  uint16_t k[kMTile * HD];
+  uint16_t v[kMTile * HD];
+};
+
+template <int HD, bool F16, bool CAP, bool SLOPE>
+__global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_kernel(BwdArgs p) {
+  constexpr int KS = HD / 16, DB = HD / 32, CH = HD / 8;
+  constexpr int DJ = kMTile * CH / kMThreads;
+  __shared__ __attribute__((aligned(16))) KeySlot<HD> r0, r1, r2, r3;
+  __shared__ int range[2][kMWaves];
+
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int blocks = (p.R + kMRows - 1) / kMRows;
+  const int qb = blockIdx.x % blocks, prob = blockIdx.x / blocks;
+  const int b = prob / p.Hk, kvh = prob % p.Hk;
+  const int r = qb * kMRows + wave * 32 + l32;
+  const bool live = r < p.R;
+  const int rc = live ? r : p.R - 1;
+  const int m_tok = rc / p.G, h = kvh * p.G + rc % p.G;
+  const RowSpan span = row_span(p.mask, b, m_tok);
+  const float* rec = p.rec + ((int64_t)prob * p.tiles + rc / 32) * kRec + rc % 32;
+  const float lse = rec[0], ndelta = rec[32], slope = SLOPE ? rec[96] : 0.f;
+
+  bf16x8 qf[KS], df[KS];
+  {
+    const uint16_t* Q = p.q + b * p.q_sb + h * p.q_sh + m_tok * p.q_sm;
+    const uint16_t* D = p.d_o + b * p.do_sb + h * p.do_sh + m_tok * p.do_sm;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = *reinterpret_cast<const bf16x8*>(Q + 16 * ks + 8 * hi);
+      df[ks] = *reinterpret_cast<const bf16x8*>(D + 16 * ks + 8 * hi);
+    }
+  }
+
+  const bool any = live && span.hi > span.lo;
+  int w_lo = any ? span.lo : 0x7fffffff, w_hi = any ? span.hi : 0;
+  int a_lo = live ? span.lo : 0, a_hi = live ? (any ? span.hi : 0) : 0x7fffffff;
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) {
+    w_lo = min(w_lo, __shfl_xor(w_lo, i));
+    w_hi = max(w_hi, __shfl_xor(w_hi, i));
+    a_lo = max(a_lo, __shfl_xor(a_lo, i));
+    a_hi = min(a_hi, __shfl_xor(a_hi, i));
+  }
+  w_lo = __builtin_amdgcn_readfirstlane(w_lo);
+  w_hi = __builtin_amdgcn_readfirstlane(w_hi);
+  a_lo = __builtin_amdgcn_readfirstlane(a_lo);
+  a_hi = __builtin_amdgcn_readfirstlane(a_hi);
+  if (lane == 0) {
+    range[0][wave] = w_lo;
+    range[1][wave] = w_hi;
+  }
+  __syncthreads();
+  int n_lo = range[0][0], n_hi = range[1][0];
+#pragma unroll
+  for (int i = 1; i < kMWaves; ++i) {
+    n_lo = min(n_lo, range[0][i]);
+    n_hi = max(n_hi, range[1][i]);
+  }
+  n_lo = __builtin_amdgcn_readfirstlane(n_lo);
+  n_hi = __builtin_amdgcn_readfirstlane(n_hi);
+  if (n_hi <= n_lo) n_lo = n_hi = 0;
+  const int t_end = (n_hi - n_lo + kMTile - 1) / kMTile;
+
+  const uint16_t* K = p.k + b * p.k_sb + kvh * p.k_sh;
+  const uint16_t* V = p.v + b * p.v_sb + kvh * p.v_sh;
+  uint32_t k_voff[DJ], v_voff[DJ];
+#pragma unroll
+  for (int i = 0; i < DJ; ++i) {
+    const int pos = (wave * DJ + i) * 64 + lane, key = pos / CH;
+    const uint32_t ch = (uint32_t)((pos % CH) ^ tile_swz<HD>(key)) * 16u;
+    k_voff[i] = key * (uint32_t)(p.k_sn * 2) + ch;
+    v_voff[i] = key * (uint32_t)(p.v_sn * 2) + ch;
+  }
+  auto issue = [&](int t, KeySlot<HD>& T) {
+    const int n0 = n_lo + t * kMTile;
+    const __amdgpu_buffer_rsrc_t kr = tile_rsrc<HD>(K, p.k_sn, n0, n_hi);
+    const __amdgpu_buffer_rsrc_t vr = tile_rsrc<HD>(V, p.v_sn, n0, n_hi);
+#pragma unroll
+    for (int i = 0; i < DJ; ++i) m_dma16(kr, &T.k[(wave * DJ + i) * 512], k_voff[i]);
+#pragma unroll
+    for (int i = 0; i < DJ; ++i) m_dma16(vr, &T.v[(wave * DJ + i) * 512], v_voff[i]);
+  };
+
+  f32x16 dq[DB];
+  DsScale sc;
+  auto restart = [&]() {
+    sc = DsScale{};
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dq[db] = f32x16{};
+  };
+  auto weights = [&](const KeySlot<HD>& T, int n0, bool edge, float (&ds)[16]) {
+    f32x16 s{}, dp;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dp[i] = ndelta;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      s = mfma32x32x16_t<F16>(row_frag<HD>(T.k, ks, l32, hi), qf[ks], s);
+      dp = mfma32x32x16_t<F16>(row_frag<HD>(T.v, ks, l32, hi), df[ks], dp);
+    }
+    const float dist = (float)(span.at - n0 - 4 * hi);
+    const int from = span.lo - n0 - 4 * hi, to = span.hi - n0 - 4 * hi;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float t = 0.f, x;
+      if constexpr (CAP) {
+        t = cap_tanh(s[i], p.score.c);
+        x = t * p.score.capl;
+      } else {
+        x = s[i] * p.score.c;
+      }
+      if constexpr (SLOPE) x = __builtin_fmaf(-slope, fabsf(dist - (float)mfma_row(i, 0)), x);
+      ds[i] = __builtin_amdgcn_exp2f(x - lse) * dp[i];
+      if constexpr (CAP) ds[i] *= __builtin_fmaf(-t, t, 1.0f);
+      if (edge && (mfma_row(i, 0) < from || mfma_row(i, 0) >= to)) ds[i] = 0.f;
+    }
+    if constexpr (F16) {
+      float ratio;
+      if (sc.follow(ds, ratio)) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) dq[db] *= ratio;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[i] *= sc.s;
+    }
+  };
+  auto iter = [&](int t, const KeySlot<HD>& cur, KeySlot<HD>& dst) {
+    m_wait<4 * DJ>();
+    __syncthreads();
+    issue(t + 3, dst);
+    const int n0 = n_lo + t * kMTile;
+    if (n0 >= w_hi || n0 + kMTile <= w_lo) return;
+    float ds[16];
+    weights(cur, n0, n0 < a_lo || n0 + kMTile > a_hi, ds);
+    bf16x8 db_[2];
+    pack_frags<F16>(ds, db_);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        dq[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.k, lane, db, s), db_[s], dq[db]);
+  };
+  restart();
+  issue(0, r0);
+  issue(1, r1);
+  issue(2, r2);
+  for (int t = 0; t < t_end; t += 4) {
+    iter(t, r0, r3);
+    if (t + 1 >= t_end) break;
+    iter(t + 1, r1, r0);
+    if (t + 2 >= t_end) break;
+    iter(t + 2, r2, r1);
+    if (t + 3 >= t_end) break;
+    iter(t + 3, r3, r2);
+  }
+  m_wait<0>();
+
+  bool odd = false;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) odd |= !(fabsf(dq[db][i]) < INFINITY);
+  if (__syncthreads_or(odd && live)) {
+    restart();
+    for (int t = 0; t < t_end; ++t) {
+      __syncthreads();
+      issue(t, r0);
+      m_wait<0>();
+      __syncthreads();
+      const int n0 = n_lo + t * kMTile, from = span.lo - n0 - 4 * hi, to = span.hi - n0 - 4 * hi;
+      float ds[16], sx[16];
+      weights(r0, n0, true, ds);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        sx[i] = mfma_row(i, 0) < from || mfma_row(i, 0) >= to ? 0.f : 1.f;
+      bf16x8 db_[2], sb[2];
+      pack_frags<F16>(ds, db_);
+      pack_frags<F16>(sx, sb);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) dq[db] = careful_mfma<HD, F16>(r0.k, lane, db, db_, sb, dq[db]);
+    }
+  }
+  if (!live) return;
+  const float x = F16 ? (sc.s == 0.f ? 0.f : p.sm_scale / sc.s) : p.sm_scale;
+  uint16_t* DQ = p.dq + b * p.dq_sb + h * p.dq_sh + m_tok * p.dq_sm;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const bf16x2 a = pack2<F16>(dq[db][4 * g] * x, dq[db][4 * g + 1] * x);
+      const bf16x2 c = pack2<F16>(dq[db][4 * g + 2] * x, dq[db][4 * g + 3] * x);
+      *reinterpret_cast<u32x2*>(DQ + db * 32 + 8 * g + 4 * hi) =
+          u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, c)};
+    }
+}
+
+template <int HD, bool F16, bool CAP, bool SLOPE>
+hipError_t launch_one(const BwdArgs& a, int64_t problems, hipStream_t s) {
+  const int64_t kb = (a.mask.N + kMRows - 1) / kMRows, qb = (a.R + kMRows - 1) / kMRows;
+  if (kb > 0)
+    hipLaunchKernelGGL((attn_masked_dkdv_kernel<HD, F16, CAP, SLOPE>), dim3((unsigned)(kb * problems)),
+                       dim3(kMThreads), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((attn_masked_dq_kernel<HD, F16, CAP, SLOPE>), dim3((unsigned)(qb * problems)),
+                     dim3(kMThreads), 0, s, a);
+  return hipGetLastError();
+}
+
+template <int HD, bool F16>
+hipError_t launch(const BwdArgs& a, int64_t problems, bool cap, hipStream_t s) {
+  hipLaunchKernelGGL((attn_masked_delta_kernel<HD, F16>), dim3((unsigned)(problems * a.tiles)),
+                     dim3(256), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (cap) return a.slopes ? launch_one<HD, F16, true, true>(a, problems, s)
+                           : launch_one<HD, F16, true, false>(a, problems, s);
+  return a.slopes ? launch_one<HD, F16, false, true>(a, problems, s)
+                  : launch_one<HD, F16, false, false>(a, problems, s);
+}
+
+}  // namespace
+}  // namespace gpa
+
+using namespace gpa;
+
+extern "C" size_t gpa_attn_masked_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t M) {
+  if (B <= 0 || H <= 0 || Hk <= 0 || M <= 0 || H % Hk) return 0;
+  return (size_t)B * Hk * ((H / Hk * M + 31) / 32) * kRec * sizeof(float);
+}
+
+extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* a,
+                                   const gpa_attn_masked_grads* g, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  const char* fn = "gpa_attn_masked_bwd";
+  gpa_clear_error();
+  const int rc = masked_check(fn, dtype, a, true);
+  if (rc != GPA_OK) return rc;
+  if (!g) {
+    gpa_set_error("%s: null arguments", fn);
+    return GPA_E_INVALID;
+  }
+  if (a->P > 0 || a->lens) {
+    gpa_set_error("%s: no gradients of a shared prefix or of padded batches by lens", fn);
+    return GPA_E_UNSUPPORTED;
+  }
+  if (a->B == 0 || a->H == 0 || a->M == 0) {
+    if (a->B > 0 && a->Hk > 0 && a->N > 0 && a->H > 0 && (g->dk || g->dv)) {
+      gpa_set_error("%s: no query, so dk and dv are zeros that the caller writes", fn);
+      return GPA_E_INVALID;
+    }
+    return GPA_OK;
+  }
+  const bool keys = a->N > 0;
+  if (!a->lse || !g->d_o || !g->dq || (keys && (!g->dk || !g->dv))) {
+    gpa_set_error("%s: null pointer (lse, d_o, dq, dk, dv)", fn);
+    return GPA_E_INVALID;
+  }
+  auto ok = [](const void* p, int64_t s0, int64_t s1, int64_t s2) {
+    return (uintptr_t)p % 16 == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0;
+  };
+  if (!ok(g->d_o, g->do_sb, g->do_sh, g->do_sm) || !ok(g->dq, g->dq_sb, g->dq_sh, g->dq_sm) ||
+      (keys && (!ok(g->dk, g->dk_sb, g->dk_sh, g->dk_sn) || !ok(g->dv, g->dv_sb, g->dv_sh, g->dv_sn)))) {
+    gpa_set_error("%s: rows must be 16-byte aligned", fn);
+    return GPA_E_INVALID;
+  }
+  const int64_t G = a->H / a->Hk, problems = a->B * a->Hk;
+  // A tile's 32 rows (at most 33 tokens, G heads) by 32-bit offsets below kNoRow.
+  for (int i = 0; i < 2; ++i) {
+    const int64_t sm = i ? g->do_sm : a->q_sm, sh = i ? g->do_sh : a->q_sh;
+    if (sm < 0 || sh < 0 || (G - 1) * sh + 33 * sm + a->D >= (int64_t)1 << 29) {
+      gpa_set_error("%s: the query heads of a key head span 2^29 elements or more", fn);
+      return GPA_E_UNSUPPORTED;
+    }
+  }
+  const int64_t tiles = (a->M * G + 31) / 32, kb = (a->N + kMRows - 1) / kMRows;
+  if (problems * std::max(tiles, kb) > 0x7fffffff) {
+    gpa_set_error("%s: too many rows", fn);
+    return GPA_E_UNSUPPORTED;
+  }
+  const size_t need = gpa_attn_masked_bwd_workspace_bytes(a->B, a->H, a->Hk, a->M);
+  if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16) {
+    gpa_set_error("%s: workspace of %zu bytes, 16-byte aligned, needed", fn, need);
+    return GPA_E_WORKSPACE;
+  }
+  BwdArgs f{};
+  f.q = (const uint16_t*)a->q; f.k = (const uint16_t*)a->k; f.v = (const uint16_t*)a->v;
+  f.o = (const uint16_t*)a->o; f.d_o = (const uint16_t*)g->d_o;
+  f.lse = a->lse; f.d_lse = g->d_lse;
+  f.dq = (uint16_t*)g->dq; f.dk = (uint16_t*)g->dk; f.dv = (uint16_t*)g->dv;
+  f.q_sb = a->q_sb; f.q_sh = a->q_sh; f.q_sm = a->q_sm;
+  f.k_sb = a->k_sb; f.k_sh = a->k_sh; f.k_sn = a->k_sn;
+  f.v_sb = a->v_sb; f.v_sh = a->v_sh; f.v_sn = a->v_sn;
+  f.o_sb = a->o_sb; f.o_sh = a->o_sh; f.o_sm = a->o_sm;
+  f.do_sb = g->do_sb; f.do_sh = g->do_sh; f.do_sm = g->do_sm;
+  f.dq_sb = g->dq_sb; f.dq_sh = g->dq_sh; f.dq_sm = g->dq_sm;
+  f.dk_sb = g->dk_sb; f.dk_sh = g->dk_sh; f.dk_sn = g->dk_sn;
+  f.dv_sb = g->dv_sb; f.dv_sh = g->dv_sh; f.dv_sn = g->dv_sn;
+  f.lse_sb = a->lse_sb; f.lse_sh = a->lse_sh;
+  f.slopes = a->slopes; f.slopes_sb = a->slopes_sb;
+  f.rec = (float*)workspace;
+  f.Hk = (int32_t)a->Hk; f.G = (int32_t)G; f.R = (int32_t)(a->M * G); f.tiles = (int32_t)tiles;
+  f.sm_scale = a->sm_scale;
+  masked_fill(a, &f.mask, &f.score);
+  const bool f16 = dtype == GPA_DTYPE_F16, cap = a->cap > 0.f;
+  const hipStream_t s = (hipStream_t)stream;
+  const hipError_t e =
+      a->D == 64 ? (f16 ? launch<64, true>(f, problems, cap, s) : launch<64, false>(f, problems, cap, s))
+                 : (f16 ? launch<128, true>(f, problems, cap, s) : launch<128, false>(f, problems, cap, s));
+  if (e != hipSuccess) {
+    gpa_set_error("%s: launch failed: %s", fn, hipGetErrorString(e));
+    return GPA_E_LAUNCH;
+  }
+  return GPA_OK;
+}

@@ -41,6 +41,18 @@ the custom ops:
     gpa::residual_layernorm(Tensor x, Tensor? y, Tensor? gamma, Tensor? weight,
                             Tensor? bias, float eps, bool want_h)
                             -> (Tensor h, Tensor ln)
+    gpa::attn_masked(Tensor q, Tensor k, Tensor v, float sm_scale, float cap,
+                     Tensor? slopes, bool causal, Tensor? prefix, int prefix_len,
+                     Tensor? q_offsets, Tensor? k_offsets, bool want_lse,
+                     bool lse_grad) -> (Tensor o, Tensor lse)       (differentiable)
+    gpa::attn_masked_bwd(Tensor d_o, Tensor? d_lse, Tensor q, Tensor k, Tensor v,
+                         Tensor o, Tensor lse, float sm_scale, float cap,
+                         Tensor? slopes, bool causal, Tensor? prefix, int prefix_len,
+                         Tensor? q_offsets, Tensor? k_offsets)
+                         -> (Tensor dq, Tensor dk, Tensor dv)
+    gpa::attn_shared_prefix(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor k,
+                            Tensor v, Tensor? lengths, float sm_scale, float cap,
+                            Tensor? slopes, bool want_lse) -> (Tensor o, Tensor lse)
 
 All launch on torch's current stream of the input's device.  There is no
 fallback: a missing library or a non-GPU tensor raises.
@@ -56,7 +68,7 @@ from typing import Optional, Tuple
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libgpa_mi355x.so"
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 GPA_OK = 0
 GPA_E_INVALID = -1
@@ -80,6 +92,26 @@ _DTYPE_CODES = {torch.float32: GPA_DTYPE_F32, torch.bfloat16: GPA_DTYPE_BF16,
                           torch.float16: GPA_DTYPE_F16}
 GPA_MERGE_SUM = 0
 GPA_MERGE_MEAN = 1
+
+
+
+def _struct(name, fields):
+    """A ctypes structure from "kind: names" lines (p pointer, l int64, i int32, f float)."""
+    kinds = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "i": ctypes.c_int32, "f": ctypes.c_float}
+    return type(name, (ctypes.Structure,), {"_fields_": [
+        (n, kinds[kind]) for kind, names in (f.split(":") for f in fields) for n in names.split()]})
+
+
+# gpa_attn_masked_args and gpa_attn_masked_grads, in the header's order.
+_MaskedArgs = _struct("_MaskedArgs", (
+    "p: q k v o lse", "l: B H Hk M N D",
+    "l: q_sb q_sh q_sm k_sb k_sh k_sn v_sb v_sh v_sn o_sb o_sh o_sm lse_sb lse_sh",
+    "p: slopes", "l: slopes_sb", "p: q_offsets k_offsets", "l: qo_sb ko_sb docs",
+    "p: prefix", "l: prefix_sb prefix_len", "p: lens pk pv", "l: P pk_sh pk_sn pv_sh pv_sn",
+    "i: causal", "f: sm_scale cap"))
+_MaskedGrads = _struct("_MaskedGrads", (
+    "p: d_o d_lse dq dk dv",
+    "l: do_sb do_sh do_sm dq_sb dq_sh dq_sm dk_sb dk_sh dk_sn dv_sb dv_sh dv_sn"))
 
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None
@@ -187,6 +219,16 @@ def _bind(lib: ctypes.CDLL) -> None:
     ]
     lib.gpa_residual_layernorm_f16.restype = ctypes.c_int
     lib.gpa_residual_layernorm_f16.argtypes = lib.gpa_residual_layernorm_bf16.argtypes
+    lib.gpa_attn_masked_workspace_bytes.restype = ctypes.c_size_t
+    lib.gpa_attn_masked_workspace_bytes.argtypes = [_i64] * 7
+    lib.gpa_attn_masked.restype = ctypes.c_int
+    lib.gpa_attn_masked.argtypes = [ctypes.c_int, ctypes.POINTER(_MaskedArgs), _vp,
+                                    ctypes.c_size_t, _vp]
+    lib.gpa_attn_masked_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.gpa_attn_masked_bwd_workspace_bytes.argtypes = [_i64] * 4
+    lib.gpa_attn_masked_bwd.restype = ctypes.c_int
+    lib.gpa_attn_masked_bwd.argtypes = [ctypes.c_int, ctypes.POINTER(_MaskedArgs),
+                                        ctypes.POINTER(_MaskedGrads), _vp, ctypes.c_size_t, _vp]
     lib.gpa_merge_order.restype = ctypes.c_int
     lib.gpa_merge_order.argtypes = [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp]
     lib.gpa_merge_plan_workspace_bytes.restype = ctypes.c_size_t
@@ -240,7 +282,9 @@ def exported_symbols() -> Tuple[str, ...]:
             "gpa_attn_keybias_f16", "gpa_residual_layernorm_bf16",
             "gpa_attn_keybias_bf16_noalloc", "gpa_lse_combine_f16", "gpa_qk_norm_rope_f16",
             "gpa_residual_layernorm_f16", "gpa_pool_shared_f16", "gpa_shared_set",
-            "gpa_attn_keybias_join", "gpa_qk_norm_rope_params")
+            "gpa_attn_keybias_join", "gpa_qk_norm_rope_params",
+            "gpa_attn_masked_workspace_bytes", "gpa_attn_masked",
+            "gpa_attn_masked_bwd_workspace_bytes", "gpa_attn_masked_bwd")
 
 
 def _check(rc: int, what: str) -> None:
@@ -301,7 +345,7 @@ def _rows_ok(t: torch.Tensor, align_elems: int) -> bool:
 # --------------------------------------------------------------------------
 #
 # Each op is defined with its schema, its fake implementation and an autograd
-# kernel whose backward raises (the ops are forward-only).  That autograd
+# kernel whose backward raises where the op is forward-only.  That autograd
 # kernel is Python that a call without gradients has no use for: a call whose
 # tensors need none goes to the dispatcher below it.  Everything else
 # (dispatch modes, functorch, tracing) sees the same op as before.  Measured
@@ -316,19 +360,21 @@ _LIB = torch.ops.gpa._library = torch.library.Library("gpa", "FRAGMENT")
 _Below = torch._C._AutoDispatchBelowAutograd
 
 
-def _op(fn):
+def _op(fn, setup_context=None, backward=None):
     """Define gpa::<name of fn> with fn as its implementation on every device
-    (it refuses tensors that are not on a GPU); returns the callable."""
+    (it refuses tensors that are not on a GPU) and, where it has gradients, its
+    backward; returns the callable."""
     name = fn.__name__
     _LIB.define(name + torch.library.infer_schema(fn, mutates_args=()),
                 tags=(torch.Tag.pt2_compliant_tag,))
     _LIB.impl(name, fn, "CompositeExplicitAutograd")
 
-    def backward(ctx, *grads):
+    def forward_only(ctx, *grads):
         raise RuntimeError(f"Trying to backward through gpa.{name}.default but no autograd "
                            "formula was registered: the op is forward-only")
 
-    torch.library.register_autograd(f"gpa::{name}", backward, lib=_LIB)
+    torch.library.register_autograd(f"gpa::{name}", backward or forward_only,
+                                    setup_context=setup_context, lib=_LIB)
     ops = torch.ops.gpa
     getattr(ops, name)                   # so that the namespace holds it
     packets = vars(ops)
@@ -1082,3 +1128,214 @@ def residual_layernorm(x: torch.Tensor, y: Optional[torch.Tensor], gamma: Option
 def _residual_layernorm_fake(x, y, gamma, weight, bias, eps, want_h):
     return (x.new_empty(x.shape if want_h else (0,)),
             x.new_empty(x.shape if weight is not None else (0,)))
+
+
+# --------------------------------------------------------------------------
+# gpa::attn_masked, its gradients, gpa::attn_shared_prefix
+# --------------------------------------------------------------------------
+
+def _like(t):
+    """A new tensor in t's order of dimensions, rows of unit stride."""
+    return torch.empty_like(t) if t.stride(-1) == 1 else t.new_empty(t.shape)
+
+
+def _rows8(t):
+    return t if _rows_ok(t, 8) else t.contiguous()
+
+
+def _masked_shapes(what, q, k, v):
+    """Checks of q [B, H, M, D] and k, v [B, Hk, N, D]."""
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{what} takes bf16 or fp16 q, got {q.dtype}")
+    for name, t in (("k", k), ("v", v)):
+        if t.dtype != q.dtype:
+            raise ValueError(f"{what}: {name} is {t.dtype}, q is {q.dtype}")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] \
+            or k.shape[3] != q.shape[3] or (k.shape[1] == 0) != (q.shape[1] == 0) \
+            or (k.shape[1] and q.shape[1] % k.shape[1]):
+        raise ValueError(f"{what}: q [B,H,M,D], k and v [B,Hk,N,D] with H a multiple of Hk, got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+
+
+def _table(what, name, t, B, width, dtype):
+    """A device table [width] or [B, width]: the tensor with rows of unit stride
+    and its stride between batch elements."""
+    if t.dtype != dtype or t.dim() not in (1, 2) or t.shape[-1] != width \
+            or (t.dim() == 2 and t.shape[0] != B):
+        raise ValueError(f"{what}: {name} must be {dtype} [{width}] or [{B}, {width}], got "
+                         f"{t.dtype} {tuple(t.shape)}")
+    if width > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if t.dim() == 2 and B > 1 else 0
+
+
+def _masked_args(what, q, k, v, o, lse, sm_scale, cap, slopes, causal, prefix=None, prefix_len=0,
+                 q_offsets=None, k_offsets=None, lens=None, pk=None, pv=None):
+    """The filled gpa_attn_masked_args, and the tensors it points into."""
+    B, H, M, D = q.shape
+    Hk, N = k.shape[1], k.shape[2]
+    docs, qo_sb, ko_sb, pre_sb, sl_sb = 1, 0, 0, 0, 0
+    if k_offsets is not None:
+        docs = k_offsets.shape[-1] - 1
+        k_offsets, ko_sb = _table(what, "k_offsets", k_offsets, B, docs + 1, torch.int32)
+    if q_offsets is not None:
+        if k_offsets is None:
+            docs = q_offsets.shape[-1] - 1
+        q_offsets, qo_sb = _table(what, "q_offsets", q_offsets, B, docs + 1, torch.int32)
+    if prefix is not None:
+        prefix, pre_sb = _table(what, "prefix", prefix, B, docs, torch.int32)
+    if slopes is not None:
+        slopes, sl_sb = _table(what, "slopes", slopes, B, H, torch.float32)
+    if lens is not None:
+        lens, _ = _table(what, "lengths", lens, 0, B, torch.int32)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    a = _MaskedArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(o), ptr(lse), B, H, Hk, M, N, D,
+        _st(q, 0), _st(q, 1), _rs(q, 2), _st(k, 0), _st(k, 1), _rs(k, 2),
+        _st(v, 0), _st(v, 1), _rs(v, 2), _st(o, 0), _st(o, 1), _rs(o, 2),
+        0 if lse is None else _st(lse, 0), 0 if lse is None else _st(lse, 1),
+        ptr(slopes), sl_sb, ptr(q_offsets), ptr(k_offsets), qo_sb, ko_sb, docs,
+        ptr(prefix), pre_sb, prefix_len, ptr(lens), ptr(pk), ptr(pv),
+        0 if pk is None else pk.shape[1], *((0, 0, 0, 0) if pk is None else
+                                            (_st(pk, 0), _rs(pk, 1), _st(pv, 0), _rs(pv, 1))),
+        int(causal), sm_scale, cap)
+    return a, (q, k, v, o, lse, slopes, q_offsets, k_offsets, prefix, lens, pk, pv)
+
+
+def _masked_run(what, q, k, v, want_lse, *args, pk=None, pv=None, **kwargs):
+    """Allocate and launch gpa_attn_masked."""
+    dev = q.device
+    o = _like(q)
+    B, H, M, D = q.shape
+    lse = torch.empty((B, H, M) if want_lse else (0,), device=dev, dtype=torch.float32)
+    q, k, v = _rows8(q), _rows8(k), _rows8(v)
+    if pk is not None:
+        pk, pv = _rows8(pk), _rows8(pv)
+    a, held = _masked_args(what, q, k, v, o, lse if want_lse else None, *args, pk=pk, pv=pv, **kwargs)
+    L = lib()
+    P = 0 if pk is None else pk.shape[1]
+    ws_bytes = L.gpa_attn_masked_workspace_bytes(B, H, k.shape[1], M, k.shape[2], P, D)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+    with _on(dev):
+        rc = L.gpa_attn_masked(_DTYPE_CODES[q.dtype], ctypes.byref(a),
+                               None if ws is None else ws.data_ptr(), ws_bytes, _stream(dev))
+    _check(rc, what)
+    return o, lse
+
+
+def _masked_setup(ctx, inputs, output):
+    q, k, v, sm_scale, cap, slopes, causal, prefix, prefix_len, qo, ko, want_lse, lse_grad = inputs
+    o, lse = output
+    if not want_lse:
+        raise RuntimeError("gpa::attn_masked: gradients need the LSE (want_lse)")
+    ctx.set_materialize_grads(False)
+    if not lse_grad:
+        ctx.mark_non_differentiable(lse)
+    ctx.save_for_backward(q, k, v, o, lse, slopes, prefix, qo, ko)
+    ctx.rest = (sm_scale, cap, causal, prefix_len)
+
+
+def _masked_backward(ctx, d_o, d_lse):
+    q, k, v, o, lse, slopes, prefix, qo, ko = ctx.saved_tensors
+    sm_scale, cap, causal, prefix_len = ctx.rest
+    if ctx.needs_input_grad[5]:
+        raise RuntimeError("gpa::attn_masked: the slopes have no gradient")
+    grads = (None, None, None)
+    if d_o is not None or d_lse is not None:
+        grads = attn_masked_bwd(torch.zeros_like(o) if d_o is None else d_o, d_lse, q, k, v, o, lse,
+                                sm_scale, cap, slopes, causal, prefix, prefix_len, qo, ko)
+    return (*grads,) + (None,) * 10
+
+
+def attn_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale: float, cap: float,
+                slopes: Optional[torch.Tensor], causal: bool, prefix: Optional[torch.Tensor],
+                prefix_len: int, q_offsets: Optional[torch.Tensor],
+                k_offsets: Optional[torch.Tensor], want_lse: bool,
+                lse_grad: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """gpa_attn_masked: o like q, and the log2 LSE [B, H, M] fp32 if want_lse
+    (else an empty tensor), which gradients need; lse_grad: the LSE is
+    differentiable too.  cap 0: none."""
+    _require_gpu(*[t for t in (q, k, v, slopes, prefix, q_offsets, k_offsets) if t is not None])
+    _masked_shapes("gpa::attn_masked", q, k, v)
+    return _masked_run("gpa::attn_masked", q, k, v, want_lse, sm_scale, cap, slopes, causal, prefix,
+                       prefix_len, q_offsets, k_offsets)
+
+
+attn_masked = _op(attn_masked, _masked_setup, _masked_backward)
+
+
+@_fake("attn_masked")
+def _attn_masked_fake(q, k, v, sm_scale, cap, slopes, causal, prefix, prefix_len, q_offsets,
+                      k_offsets, want_lse, lse_grad):
+    return _like(q), q.new_empty(q.shape[:3] if want_lse else (0,), dtype=torch.float32)
+
+
+@_op
+def attn_masked_bwd(d_o: torch.Tensor, d_lse: Optional[torch.Tensor], q: torch.Tensor,
+                    k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+                    sm_scale: float, cap: float, slopes: Optional[torch.Tensor], causal: bool,
+                    prefix: Optional[torch.Tensor], prefix_len: int,
+                    q_offsets: Optional[torch.Tensor], k_offsets: Optional[torch.Tensor]
+                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """gpa_attn_masked_bwd: the gradients of q, k and v, in their order of
+    dimensions."""
+    what = "gpa::attn_masked_bwd"
+    dev = _require_gpu(*[t for t in (q, k, v, o, lse, d_o, d_lse, slopes, prefix, q_offsets,
+                                     k_offsets) if t is not None])
+    _masked_shapes(what, q, k, v)
+    if o.shape != q.shape or d_o.shape != q.shape or o.dtype != q.dtype or d_o.dtype != q.dtype \
+            or lse.shape != q.shape[:3] or lse.dtype != torch.float32 \
+            or (d_lse is not None and (d_lse.shape != lse.shape or d_lse.dtype != torch.float32)):
+        raise ValueError(f"{what}: o {o.dtype} {tuple(o.shape)}, d_o {d_o.dtype} {tuple(d_o.shape)}, "
+                         f"lse {lse.dtype} {tuple(lse.shape)} do not match q {tuple(q.shape)}")
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    if q.numel() == 0:
+        return dq, dk.zero_(), dv.zero_()
+    q, k, v, o, d_o = (_rows8(t) for t in (q, k, v, o, d_o))
+    lse = lse if lse.stride(-1) == 1 else lse.contiguous()
+    d_lse = None if d_lse is None else d_lse.contiguous()
+    a, held = _masked_args(what, q, k, v, o, lse, sm_scale, cap, slopes, causal, prefix, prefix_len,
+                           q_offsets, k_offsets)
+    g = _MaskedGrads(d_o.data_ptr(), None if d_lse is None else d_lse.data_ptr(), dq.data_ptr(),
+                     dk.data_ptr(), dv.data_ptr(),
+                     *(s for t in (d_o, dq, dk, dv) for s in (_st(t, 0), _st(t, 1), _rs(t, 2))))
+    L = lib()
+    ws_bytes = L.gpa_attn_masked_bwd_workspace_bytes(q.shape[0], q.shape[1], k.shape[1], q.shape[2])
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    with _on(dev):
+        rc = L.gpa_attn_masked_bwd(_DTYPE_CODES[q.dtype], ctypes.byref(a), ctypes.byref(g),
+                                   ws.data_ptr(), ws_bytes, _stream(dev))
+    _check(rc, what)
+    return dq, dk, dv
+
+
+@_fake("attn_masked_bwd")
+def _attn_masked_bwd_fake(d_o, d_lse, q, k, v, o, lse, sm_scale, cap, slopes, causal, prefix,
+                          prefix_len, q_offsets, k_offsets):
+    return _like(q), _like(k), _like(v)
+
+
+@_op
+def attn_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
+                       k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor],
+                       sm_scale: float, cap: float, slopes: Optional[torch.Tensor],
+                       want_lse: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """gpa_attn_masked with a shared prefix [Hk, P, D] before each batch
+    element's own keys [B, Hk, N, D] (lengths int32 [B] of them; None: all), the
+    queries being the last M own tokens."""
+    what = "gpa::attn_shared_prefix"
+    _require_gpu(*[t for t in (q, prefix_k, prefix_v, k, v, lengths, slopes) if t is not None])
+    _masked_shapes(what, q, k, v)
+    if prefix_k.dtype != q.dtype or prefix_v.dtype != q.dtype or prefix_k.dim() != 3 \
+            or prefix_k.shape != prefix_v.shape or prefix_k.shape[0] != k.shape[1] \
+            or prefix_k.shape[2] != q.shape[3]:
+        raise ValueError(f"{what}: the prefix must be {q.dtype} [{k.shape[1]}, P, {q.shape[3]}], got "
+                         f"{prefix_k.dtype} {tuple(prefix_k.shape)} and {prefix_v.dtype} "
+                         f"{tuple(prefix_v.shape)}")
+    return _masked_run(what, q, k, v, want_lse, sm_scale, cap, slopes, True, lens=lengths,
+                       pk=prefix_k, pv=prefix_v)
+
+
+@_fake("attn_shared_prefix")
+def _attn_shared_prefix_fake(q, prefix_k, prefix_v, k, v, lengths, sm_scale, cap, slopes, want_lse):
+    return _like(q), q.new_empty(q.shape[:3] if want_lse else (0,), dtype=torch.float32)

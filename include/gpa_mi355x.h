@@ -36,6 +36,10 @@
  *   gpa_residual_layernorm_bf16 (and _f16) — residual + LayerScale + LayerNorm of the
  *                           caller's blocks (replaces vggt/layers/block.py:84-96
  *                           torch ops).
+ *   gpa_attn_masked (and _bwd) — attention of packed documents, causal and
+ *                           prefix masks, capped and distance-biased scores,
+ *                           shared key heads; a prefix that a batch shares;
+ *                           and its gradients.
  *
  * Conventions shared by every entry point:
  *   - All tensor pointers are device pointers owned by the caller.  The
@@ -65,7 +69,7 @@
 extern "C" {
 #endif
 
-#define GPA_ABI_VERSION 18
+#define GPA_ABI_VERSION 19
 
 enum {
   GPA_OK = 0,
@@ -491,6 +495,77 @@ int gpa_residual_layernorm_f16(const void* x, const void* y, const void* gamma,
                                int64_t rows, int64_t C, int64_t x_sn, int64_t y_sn,
                                void* h_out, int64_t h_sn, void* ln_out, int64_t ln_sn,
                                void* stream);
+
+/*
+ * Masked attention (no counterpart in the reference).  q and o [B, H, M, D],
+ * k and v [B, Hk, N, D], all bf16 or all fp16; D = 64 or 128; query head h
+ * reads key head h / (H / Hk).
+ *   x = sm_scale q.k;  s = cap > 0 ? cap tanh(x / cap) : x;
+ *   s -= slopes[h] |at - j|                       (slopes != NULL)
+ *   o = sum_j softmax(s)_j v_j over the keys that the query sees;
+ *   lse[b*lse_sb + h*lse_sh + m] = log2 sum_j e^s  (lse != NULL)
+ * A query that sees no key gets zeros and -inf.
+ * Documents: run d of batch element b holds the queries q_offsets[b*qo_sb + d]
+ * .. q_offsets[b*qo_sb + d + 1] - 1 and the keys of k_offsets likewise (docs + 1
+ * values each, not decreasing; NULL, for docs = 1 only: all of them).  Query
+ * m of a document stands at key at = m + k1 - q1 (its last query at its last
+ * key) and sees the document's keys, under `causal` those j <= at and the
+ * first prefix[b*prefix_sb + d] (NULL: prefix_len) ones.  Tokens of no document
+ * see nothing.  Offsets, lens and prefixes are read on the device; what lies
+ * outside the tensors is cut to them.
+ * Shared prefix (P > 0): keys pk and pv [Hk, P, D] come before those of every
+ * batch element and are seen by all queries; lens (int32 [B], NULL: all N)
+ * says how many of the N own keys each element has.  Both go with docs = 1 and
+ * no offsets; lens alone is a padded batch.
+ * workspace: gpa_attn_masked_workspace_bytes(...) bytes, 16-byte aligned,
+ * overwritten (0: none).  Key rows (k_sn, v_sn, pk_sn, pv_sn) are less than
+ * 2^23 elements apart; a head's keys may span any distance.
+ */
+typedef struct gpa_attn_masked_args {
+  const void *q, *k, *v;
+  void* o;
+  float* lse;
+  int64_t B, H, Hk, M, N, D;
+  int64_t q_sb, q_sh, q_sm, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, o_sb, o_sh, o_sm, lse_sb, lse_sh;
+  const float* slopes;            /* [H] or NULL; slopes_sb between batch elements (0: shared) */
+  int64_t slopes_sb;
+  const int32_t *q_offsets, *k_offsets;
+  int64_t qo_sb, ko_sb, docs;
+  const int32_t* prefix;
+  int64_t prefix_sb, prefix_len;
+  const int32_t* lens;
+  const void *pk, *pv;
+  int64_t P, pk_sh, pk_sn, pv_sh, pv_sn;
+  int32_t causal;
+  float sm_scale, cap;
+} gpa_attn_masked_args;
+
+size_t gpa_attn_masked_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t M, int64_t N,
+                                       int64_t P, int64_t D);
+int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/*
+ * Its gradients, from the forward's output o and log2 LSE (args->o and
+ * args->lse, both required) and the output's gradient d_o, with d_lse the LSE's
+ * (NULL: none; contiguous [B, H, M]): dq, dk and dv in the operands' format,
+ * those of a shared key head summed over its query heads.  No shared prefix
+ * (P = 0, lens = NULL).  Sums run in a fixed order: two calls give the same
+ * bits.  A batch element's query heads of one key head, and 32 tokens, span
+ * less than 2^29 elements of q and of d_o.  workspace:
+ * gpa_attn_masked_bwd_workspace_bytes(...), 16-byte aligned.
+ */
+typedef struct gpa_attn_masked_grads {
+  const void* d_o;
+  const float* d_lse;
+  void *dq, *dk, *dv;
+  int64_t do_sb, do_sh, do_sm, dq_sb, dq_sh, dq_sm, dk_sb, dk_sh, dk_sn, dv_sb, dv_sh, dv_sn;
+} gpa_attn_masked_grads;
+
+size_t gpa_attn_masked_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t M);
+int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* args,
+                        const gpa_attn_masked_grads* grads, void* workspace,
+                        size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
