@@ -53,6 +53,15 @@ the custom ops:
     gpa::attn_shared_prefix(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor k,
                             Tensor v, Tensor? lengths, float sm_scale, float cap,
                             Tensor? slopes, bool want_lse) -> (Tensor o, Tensor lse)
+    gpa::norm_gate(Tensor x, Tensor y, Tensor? post_w, Tensor? post_b, Tensor? gate,
+                   Tensor pre_w, Tensor? pre_b, float scale, bool layer, float eps,
+                   bool want_stats) -> (Tensor h, Tensor out, Tensor stats)
+                                                                   (differentiable)
+    gpa::norm_gate_bwd(Tensor? dh, Tensor? dout, Tensor x, Tensor y, Tensor? post_w,
+                       Tensor? post_b, Tensor? gate, Tensor pre_w, Tensor? pre_b,
+                       Tensor stats, float scale, bool layer)
+                       -> (Tensor dx, Tensor dy, Tensor dpost_w, Tensor dpost_b,
+                           Tensor dgate, Tensor dpre_w, Tensor dpre_b)
 
 All launch on torch's current stream of the input's device.  There is no
 fallback: a missing library or a non-GPU tensor raises.
@@ -112,6 +121,12 @@ _MaskedArgs = _struct("_MaskedArgs", (
 _MaskedGrads = _struct("_MaskedGrads", (
     "p: d_o d_lse dq dk dv",
     "l: do_sb do_sh do_sm dq_sb dq_sh dq_sm dk_sb dk_sh dk_sn dv_sb dv_sh dv_sn"))
+
+# gpa_norm_gate_args and gpa_norm_gate_grads.
+_NormArgs = _struct("_NormArgs", ("p: x y gate w1 b1 w2 b2 stats", "l: rows C groups x_sn y_sn",
+                                  "i: layer", "f: scale eps"))
+_NormGrads = _struct("_NormGrads", ("p: dh dout dx dy dgate dw1 db1 dw2 db2",
+                                    "l: dh_sn dout_sn dx_sn dy_sn"))
 
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None
@@ -229,6 +244,14 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.gpa_attn_masked_bwd.restype = ctypes.c_int
     lib.gpa_attn_masked_bwd.argtypes = [ctypes.c_int, ctypes.POINTER(_MaskedArgs),
                                         ctypes.POINTER(_MaskedGrads), _vp, ctypes.c_size_t, _vp]
+    lib.gpa_norm_gate.restype = ctypes.c_int
+    lib.gpa_norm_gate.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.POINTER(_NormArgs), _vp, _i64,
+                                  _vp, _i64, _vp]
+    lib.gpa_norm_gate_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.gpa_norm_gate_bwd_workspace_bytes.argtypes = [_i64] * 3
+    lib.gpa_norm_gate_bwd.restype = ctypes.c_int
+    lib.gpa_norm_gate_bwd.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.POINTER(_NormArgs),
+                                      ctypes.POINTER(_NormGrads), _vp, ctypes.c_size_t, _vp]
     lib.gpa_merge_order.restype = ctypes.c_int
     lib.gpa_merge_order.argtypes = [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp]
     lib.gpa_merge_plan_workspace_bytes.restype = ctypes.c_size_t
@@ -284,7 +307,8 @@ def exported_symbols() -> Tuple[str, ...]:
             "gpa_residual_layernorm_f16", "gpa_pool_shared_f16", "gpa_shared_set",
             "gpa_attn_keybias_join", "gpa_qk_norm_rope_params",
             "gpa_attn_masked_workspace_bytes", "gpa_attn_masked",
-            "gpa_attn_masked_bwd_workspace_bytes", "gpa_attn_masked_bwd")
+            "gpa_attn_masked_bwd_workspace_bytes", "gpa_attn_masked_bwd", "gpa_norm_gate",
+            "gpa_norm_gate_bwd_workspace_bytes", "gpa_norm_gate_bwd")
 
 
 def _check(rc: int, what: str) -> None:
@@ -1339,3 +1363,148 @@ def attn_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
 @_fake("attn_shared_prefix")
 def _attn_shared_prefix_fake(q, prefix_k, prefix_v, k, v, lengths, sm_scale, cap, slopes, want_lse):
     return _like(q), q.new_empty(q.shape[:3] if want_lse else (0,), dtype=torch.float32)
+
+
+# --------------------------------------------------------------------------
+# gpa::norm_gate and its gradients
+# --------------------------------------------------------------------------
+
+def _norm_check(what, x, y, w1, b1, gate, w2, b2):
+    """Checks, and (rows, C, the gate's groups)."""
+    params = [t for t in (w1, b1, gate, w2, b2) if t is not None]
+    C = x.shape[-1] if x.dim() else 0
+    if x.dtype not in _DTYPE_CODES:
+        raise ValueError(f"{what}: dtype {x.dtype} is not fp32, bf16 or fp16")
+    if x.dim() < 1 or y.shape != x.shape or y.dtype != x.dtype:
+        raise ValueError(f"{what}: x {x.dtype} {tuple(x.shape)} and y {y.dtype} {tuple(y.shape)} differ")
+    if any(t.dtype != w2.dtype for t in params) or w2.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{what}: parameters are all of the rows' type {x.dtype}, or all fp32, got "
+                         f"{[t.dtype for t in params]}")
+    for name, t in (("post_weight", w1), ("post_bias", b1), ("pre_weight", w2), ("pre_bias", b2)):
+        if t is not None and t.shape != (C,):
+            raise ValueError(f"{what}: {name} must be [{C}], got {tuple(t.shape)}")
+    if b1 is not None and w1 is None:
+        raise ValueError(f"{what}: post_bias without post_weight")
+    rows = x.numel() // C if C else 0
+    groups = 1
+    if gate is not None:
+        groups = gate.shape[0]
+        if gate.dim() != 2 or gate.shape[1] != C or (rows % groups if groups else rows):
+            raise ValueError(f"{what}: gate [groups, {C}] over {rows} rows, got {tuple(gate.shape)}")
+        groups = max(groups, 1)
+    return rows, C, groups
+
+
+def _norm_rows(t, C):
+    """t as rows of C features with one stride (copied where it has none)."""
+    t = t.reshape(-1, C)
+    return t if t.stride(1) == 1 or C == 1 else t.contiguous()
+
+
+def _norm_setup(ctx, inputs, output):
+    x, y, w1, b1, gate, w2, b2, scale, layer, eps, want_stats = inputs
+    if not want_stats:
+        raise RuntimeError("gpa::norm_gate: gradients need the statistics (want_stats)")
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[2])
+    ctx.save_for_backward(x, y, w1, b1, gate, w2, b2, output[2])
+    ctx.rest = (scale, layer)
+
+
+def _norm_backward(ctx, dh, dout, _):
+    x, y, w1, b1, gate, w2, b2, stats = ctx.saved_tensors
+    if dh is None and dout is None:
+        return (None,) * 11
+    got = norm_gate_bwd(dh, dout, x, y, w1, b1, gate, w2, b2, stats, *ctx.rest)
+    dx, dy, dw1, db1, dgate, dw2, db2 = got
+    none = lambda g, t: None if t is None else g  # noqa: E731
+    return (dx, dy, none(dw1, w1), none(db1, b1), none(dgate, gate), dw2, none(db2, b2),
+            None, None, None, None)
+
+
+def norm_gate(x: torch.Tensor, y: torch.Tensor, post_w: Optional[torch.Tensor],
+              post_b: Optional[torch.Tensor], gate: Optional[torch.Tensor], pre_w: torch.Tensor,
+              pre_b: Optional[torch.Tensor], scale: float, layer: bool, eps: float,
+              want_stats: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """gpa_norm_gate over the last dim of x and y: h and out in their type and
+    shape, and the row statistics [rows, 4] fp32 if want_stats (else an empty
+    tensor), which gradients need.  gate [groups, C]: each row of it serves
+    rows / groups consecutive rows."""
+    what = "gpa::norm_gate"
+    dev = _require_gpu(*[t for t in (x, y, post_w, post_b, gate, pre_w, pre_b) if t is not None])
+    rows, C, groups = _norm_check(what, x, y, post_w, post_b, gate, pre_w, pre_b)
+    h = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    out = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    stats = torch.empty((rows, 4) if want_stats else (0,), device=dev, dtype=torch.float32)
+    if rows == 0:
+        return h, out, stats
+    xr, yr = _norm_rows(x, C), _norm_rows(y, C)
+    par = [None if t is None else t.contiguous() for t in (gate, post_w, post_b, pre_w, pre_b)]
+    a = _NormArgs(xr.data_ptr(), yr.data_ptr(), *(None if t is None else t.data_ptr() for t in par),
+                  stats.data_ptr() if want_stats else None, rows, C, groups, _rs(xr, 0), _rs(yr, 0),
+                  int(layer), scale, eps)
+    with _on(dev):
+        rc = lib().gpa_norm_gate(_DTYPE_CODES[x.dtype], _DTYPE_CODES[pre_w.dtype], ctypes.byref(a),
+                                 h.data_ptr(), C, out.data_ptr(), C, _stream(dev))
+    _check(rc, what)
+    return h, out, stats
+
+
+norm_gate = _op(norm_gate, _norm_setup, _norm_backward)
+
+
+@_fake("norm_gate")
+def _norm_gate_fake(x, y, post_w, post_b, gate, pre_w, pre_b, scale, layer, eps, want_stats):
+    C = x.shape[-1]
+    return (x.new_empty(x.shape), x.new_empty(x.shape),
+            x.new_empty((x.numel() // C, 4) if want_stats else (0,), dtype=torch.float32))
+
+
+@_op
+def norm_gate_bwd(dh: Optional[torch.Tensor], dout: Optional[torch.Tensor], x: torch.Tensor,
+                  y: torch.Tensor, post_w: Optional[torch.Tensor], post_b: Optional[torch.Tensor],
+                  gate: Optional[torch.Tensor], pre_w: torch.Tensor, pre_b: Optional[torch.Tensor],
+                  stats: torch.Tensor, scale: float, layer: bool
+                  ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                             torch.Tensor, torch.Tensor]:
+    """gpa_norm_gate_bwd: the gradients of x, y, post_w, post_b, gate, pre_w and
+    pre_b (empty tensors for absent ones) from those of h and out (None:
+    zeros)."""
+    what = "gpa::norm_gate_bwd"
+    dev = _require_gpu(*[t for t in (x, y, dh, dout, stats, post_w, post_b, gate, pre_w, pre_b)
+                         if t is not None])
+    rows, C, groups = _norm_check(what, x, y, post_w, post_b, gate, pre_w, pre_b)
+    for name, t in (("dh", dh), ("dout", dout)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"{what}: {name} {t.dtype} {tuple(t.shape)} does not match x")
+    if stats.dtype != torch.float32 or stats.shape != (rows, 4) or not stats.is_contiguous():
+        raise ValueError(f"{what}: stats must be contiguous fp32 [{rows}, 4], got {stats.dtype} "
+                         f"{tuple(stats.shape)}")
+    dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    dy = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    grads = [pre_w.new_empty(0 if t is None else t.shape) for t in (post_w, post_b, gate, pre_w, pre_b)]
+    if rows == 0:
+        return (dx, dy, *(g.zero_() for g in grads))
+    xr, yr = _norm_rows(x, C), _norm_rows(y, C)
+    dhr, dor = (None if t is None else _norm_rows(t, C) for t in (dh, dout))
+    par = [None if t is None else t.contiguous() for t in (gate, post_w, post_b, pre_w, pre_b)]
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    a = _NormArgs(xr.data_ptr(), yr.data_ptr(), *map(ptr, par), stats.data_ptr(), rows, C, groups,
+                  _rs(xr, 0), _rs(yr, 0), int(layer), scale, 0.0)
+    dw1, db1, dg, dw2, db2 = (g.data_ptr() if g.numel() else None for g in grads)
+    g = _NormGrads(ptr(dhr), ptr(dor), dx.data_ptr(), dy.data_ptr(), dg, dw1, db1, dw2, db2,
+                   0 if dhr is None else _rs(dhr, 0), 0 if dor is None else _rs(dor, 0), C, C)
+    L = lib()
+    ws_bytes = L.gpa_norm_gate_bwd_workspace_bytes(rows, C, groups)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    with _on(dev):
+        rc = L.gpa_norm_gate_bwd(_DTYPE_CODES[x.dtype], _DTYPE_CODES[pre_w.dtype], ctypes.byref(a),
+                                 ctypes.byref(g), ws.data_ptr(), ws_bytes, _stream(dev))
+    _check(rc, what)
+    return (dx, dy, *grads)
+
+
+@_fake("norm_gate_bwd")
+def _norm_gate_bwd_fake(dh, dout, x, y, post_w, post_b, gate, pre_w, pre_b, stats, scale, layer):
+    return (x.new_empty(x.shape), x.new_empty(x.shape),
+            *(pre_w.new_empty((0,) if t is None else t.shape) for t in (post_w, post_b, gate, pre_w, pre_b)))

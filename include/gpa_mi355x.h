@@ -40,6 +40,8 @@
  *                           prefix masks, capped and distance-biased scores,
  *                           shared key heads; a prefix that a batch shares;
  *                           and its gradients.
+ *   gpa_norm_gate (and _bwd) — the norms after and before a block with its
+ *                           gate and residual scale, and their gradients.
  *
  * Conventions shared by every entry point:
  *   - All tensor pointers are device pointers owned by the caller.  The
@@ -566,6 +568,43 @@ size_t gpa_attn_masked_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int
 int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* args,
                         const gpa_attn_masked_grads* grads, void* workspace,
                         size_t workspace_bytes, void* stream);
+
+/*
+ * The norms around a block with its gate and residual (no counterpart in the
+ * reference), over rows of C features (1 to 8192):
+ *   u = w1 ? N(y) w1 + b1 : y;  h = x + scale gate u;  out = N(h) w2 + b2
+ * N: (t - mean) / sqrt(var + eps) (layer != 0, biased variance) or
+ * t / sqrt(mean t^2 + eps).  gate [groups, C] (NULL: 1): row r takes gate row
+ * r / (rows / groups); w1, b1, b2 may be NULL.  Rows are of `dtype` (any
+ * GPA_DTYPE), parameters all of `param_dtype` (the rows' or fp32); fp32 inside, h
+ * and out rounded once.  stats (NULL: not kept): fp32 [rows][4], 16-byte
+ * aligned, for the backward.
+ */
+typedef struct gpa_norm_gate_args {
+  const void *x, *y, *gate, *w1, *b1, *w2, *b2;
+  float* stats;
+  int64_t rows, C, groups, x_sn, y_sn;
+  int32_t layer;
+  float scale, eps;
+} gpa_norm_gate_args;
+
+int gpa_norm_gate(int dtype, int param_dtype, const gpa_norm_gate_args* args, void* h, int64_t h_sn,
+                  void* out, int64_t out_sn, void* stream);
+
+/* Its gradients, from those of h and out (either NULL: zeros) and the
+ * forward's stats: dx and dy in the rows' type, the parameters' (NULL: not wanted)
+ * contiguous in theirs.  Sums run in a fixed order.  workspace:
+ * gpa_norm_gate_bwd_workspace_bytes(...), 16-byte aligned. */
+typedef struct gpa_norm_gate_grads {
+  const void *dh, *dout;
+  void *dx, *dy, *dgate, *dw1, *db1, *dw2, *db2;
+  int64_t dh_sn, dout_sn, dx_sn, dy_sn;
+} gpa_norm_gate_grads;
+
+size_t gpa_norm_gate_bwd_workspace_bytes(int64_t rows, int64_t C, int64_t groups);
+int gpa_norm_gate_bwd(int dtype, int param_dtype, const gpa_norm_gate_args* args,
+                      const gpa_norm_gate_grads* grads, void* workspace, size_t workspace_bytes,
+                      void* stream);
 
 #ifdef __cplusplus
 }
