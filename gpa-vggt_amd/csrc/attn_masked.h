@@ -228,9 +228,19 @@ __device__ __forceinline__ f32x16 careful_mfma(const uint16_t* t, int lane, int 
   return acc;
 }
 
+// Whether the rows of a [n0, n1, n2, D] tensor of 16-bit values are 16-byte aligned;
+// a dimension of one has any stride.
+inline bool rows_aligned(const void* p, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2,
+                         int64_t s2) {
+  return (uintptr_t)p % 16 == 0 && (n0 < 2 || s0 % 8 == 0) && (n1 < 2 || s1 % 8 == 0) &&
+         (n2 < 2 || s2 % 8 == 0);
+}
+
 // Shared by the entry points: the checks of their arguments (has_o: an output
 // is written to a->o), and the kernels' form of them.
 int masked_check(const char* fn, int dtype, const gpa_attn_masked_args* a, bool has_o);
+// The arguments with a plain stride for every dimension of one.
+gpa_attn_masked_args masked_plain(const gpa_attn_masked_args* a);
 void masked_fill(const gpa_attn_masked_args* a, MaskArgs* m, ScoreArgs* s);
 
 }  // namespace gpa

@@ -456,23 +456,37 @@ int gpa::masked_check(const char* fn, int dtype, const gpa_attn_masked_args* a, 
     gpa_set_error("%s: null pointer", fn);
     return GPA_E_INVALID;
   }
-  auto ok = [](const void* p, int64_t s0, int64_t s1, int64_t s2) {
-    return (uintptr_t)p % 16 == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0;
-  };
-  if (!ok(a->q, a->q_sb, a->q_sh, a->q_sm) || (has_o && !ok(a->o, a->o_sb, a->o_sh, a->o_sm)) ||
-      (keys && (!ok(a->k, a->k_sb, a->k_sh, a->k_sn) || !ok(a->v, a->v_sb, a->v_sh, a->v_sn))) ||
-      (pre && (!ok(a->pk, 0, a->pk_sh, a->pk_sn) || !ok(a->pv, 0, a->pv_sh, a->pv_sn)))) {
+  const int64_t B = a->B, H = a->H, Hk = a->Hk;
+  if (!rows_aligned(a->q, B, a->q_sb, H, a->q_sh, a->M, a->q_sm) ||
+      (has_o && !rows_aligned(a->o, B, a->o_sb, H, a->o_sh, a->M, a->o_sm)) ||
+      (keys && (!rows_aligned(a->k, B, a->k_sb, Hk, a->k_sh, a->N, a->k_sn) ||
+                !rows_aligned(a->v, B, a->v_sb, Hk, a->v_sh, a->N, a->v_sn))) ||
+      (pre && (!rows_aligned(a->pk, 1, 0, Hk, a->pk_sh, a->P, a->pk_sn) ||
+               !rows_aligned(a->pv, 1, 0, Hk, a->pv_sh, a->P, a->pv_sn)))) {
     gpa_set_error("%s: rows must be 16-byte aligned", fn);
     return GPA_E_INVALID;
   }
   // A tile's 32 rows are addressed by 32-bit offsets from its first one.
   const int64_t row_lim = (int64_t)1 << 23;
-  for (const int64_t s : {keys ? a->k_sn : 0, keys ? a->v_sn : 0, pre ? a->pk_sn : 0, pre ? a->pv_sn : 0})
+  const bool many = a->N > 1, pre_many = a->P > 1;
+  for (const int64_t s : {many ? a->k_sn : 0, many ? a->v_sn : 0, pre_many ? a->pk_sn : 0,
+                          pre_many ? a->pv_sn : 0})
     if (s < 0 || s >= row_lim) {
       gpa_set_error("%s: key row stride %lld unsupported (0 to 2^23)", fn, (long long)s);
       return GPA_E_UNSUPPORTED;
     }
   return GPA_OK;
+}
+
+gpa_attn_masked_args gpa::masked_plain(const gpa_attn_masked_args* a) {
+  gpa_attn_masked_args x = *a;
+  if (a->B < 2) x.q_sb = x.k_sb = x.v_sb = x.o_sb = x.lse_sb = x.slopes_sb = x.qo_sb = x.ko_sb = x.prefix_sb = 0;
+  if (a->H < 2) x.q_sh = x.o_sh = x.lse_sh = 0;
+  if (a->Hk < 2) x.k_sh = x.v_sh = x.pk_sh = x.pv_sh = 0;
+  if (a->M < 2) x.q_sm = x.o_sm = a->D;
+  if (a->N < 2) x.k_sn = x.v_sn = a->D;
+  if (a->P < 2) x.pk_sn = x.pv_sn = a->D;
+  return x;
 }
 
 void gpa::masked_fill(const gpa_attn_masked_args* a, MaskArgs* m, ScoreArgs* s) {
@@ -498,12 +512,13 @@ extern "C" size_t gpa_attn_masked_workspace_bytes(int64_t B, int64_t H, int64_t 
   return z > 1 ? (size_t)z * B * H * M * (D + 2) * sizeof(float) : 0;
 }
 
-extern "C" int gpa_attn_masked(int dtype, const gpa_attn_masked_args* a, void* workspace,
+extern "C" int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void* workspace,
                                size_t workspace_bytes, void* stream) {
   const char* fn = "gpa_attn_masked";
   gpa_clear_error();
-  const int rc = masked_check(fn, dtype, a, true);
+  const int rc = masked_check(fn, dtype, args, true);
   if (rc != GPA_OK) return rc;
+  const gpa_attn_masked_args plain_args = masked_plain(args), *a = &plain_args;
   if (a->B == 0 || a->H == 0 || a->M == 0) return GPA_OK;
   const int64_t G = a->H / a->Hk;
   const Plan x = plan(a->B, a->Hk, G, a->M, a->N, a->P);

@@ -594,13 +594,14 @@ extern "C" size_t gpa_attn_masked_bwd_workspace_bytes(int64_t B, int64_t H, int6
   return (size_t)B * Hk * ((H / Hk * M + 31) / 32) * kRec * sizeof(float);
 }
 
-extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* a,
+extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* args,
                                    const gpa_attn_masked_grads* g, void* workspace,
                                    size_t workspace_bytes, void* stream) {
   const char* fn = "gpa_attn_masked_bwd";
   gpa_clear_error();
-  const int rc = masked_check(fn, dtype, a, true);
+  const int rc = masked_check(fn, dtype, args, true);
   if (rc != GPA_OK) return rc;
+  const gpa_attn_masked_args plain_args = masked_plain(args), *a = &plain_args;
   if (!g) {
     gpa_set_error("%s: null arguments", fn);
     return GPA_E_INVALID;
@@ -621,18 +622,17 @@ extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* a,
     gpa_set_error("%s: null pointer (lse, d_o, dq, dk, dv)", fn);
     return GPA_E_INVALID;
   }
-  auto ok = [](const void* p, int64_t s0, int64_t s1, int64_t s2) {
-    return (uintptr_t)p % 16 == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0;
-  };
-  if (!ok(g->d_o, g->do_sb, g->do_sh, g->do_sm) || !ok(g->dq, g->dq_sb, g->dq_sh, g->dq_sm) ||
-      (keys && (!ok(g->dk, g->dk_sb, g->dk_sh, g->dk_sn) || !ok(g->dv, g->dv_sb, g->dv_sh, g->dv_sn)))) {
+  if (!rows_aligned(g->d_o, a->B, g->do_sb, a->H, g->do_sh, a->M, g->do_sm) ||
+      !rows_aligned(g->dq, a->B, g->dq_sb, a->H, g->dq_sh, a->M, g->dq_sm) ||
+      (keys && (!rows_aligned(g->dk, a->B, g->dk_sb, a->Hk, g->dk_sh, a->N, g->dk_sn) ||
+                !rows_aligned(g->dv, a->B, g->dv_sb, a->Hk, g->dv_sh, a->N, g->dv_sn)))) {
     gpa_set_error("%s: rows must be 16-byte aligned", fn);
     return GPA_E_INVALID;
   }
   const int64_t G = a->H / a->Hk, problems = a->B * a->Hk;
   // A tile's 32 rows (at most 33 tokens, G heads) by 32-bit offsets below kNoRow.
   for (int i = 0; i < 2; ++i) {
-    const int64_t sm = i ? g->do_sm : a->q_sm, sh = i ? g->do_sh : a->q_sh;
+    const int64_t sm = a->M < 2 ? a->D : i ? g->do_sm : a->q_sm, sh = G < 2 ? 0 : i ? g->do_sh : a->q_sh;
     if (sm < 0 || sh < 0 || (G - 1) * sh + 33 * sm + a->D >= (int64_t)1 << 29) {
       gpa_set_error("%s: the query heads of a key head span 2^29 elements or more", fn);
       return GPA_E_UNSUPPORTED;
@@ -657,7 +657,7 @@ extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* a,
   f.k_sb = a->k_sb; f.k_sh = a->k_sh; f.k_sn = a->k_sn;
   f.v_sb = a->v_sb; f.v_sh = a->v_sh; f.v_sn = a->v_sn;
   f.o_sb = a->o_sb; f.o_sh = a->o_sh; f.o_sm = a->o_sm;
-  f.do_sb = g->do_sb; f.do_sh = g->do_sh; f.do_sm = g->do_sm;
+  f.do_sb = a->B < 2 ? 0 : g->do_sb; f.do_sh = a->H < 2 ? 0 : g->do_sh; f.do_sm = a->M < 2 ? a->D : g->do_sm;
   f.dq_sb = g->dq_sb; f.dq_sh = g->dq_sh; f.dq_sm = g->dq_sm;
   f.dk_sb = g->dk_sb; f.dk_sh = g->dk_sh; f.dk_sn = g->dk_sn;
   f.dv_sb = g->dv_sb; f.dv_sh = g->dv_sh; f.dv_sn = g->dv_sn;
