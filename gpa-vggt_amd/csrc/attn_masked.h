@@ -102,15 +102,29 @@ __device__ __forceinline__ KeySpan key_span(const MaskArgs& a, int64_t b, int j)
   return k;
 }
 
-// Scores, in log2 units.  `c` is sm_scale log2(e); with a cap c = 2 log2(e)
-// sm_scale / cap (the exponent of e^(2u), u = x / cap) and capl = cap log2(e).
-struct ScoreArgs { float c, capl; };
+// Scores, in log2 units.  c1 = sm_scale log2(e).  With a cap: ce = 2 log2(e)
+// sm_scale / cap (the exponent of e^(2u), u = x / cap), capl = cap log2(e), and for
+// |u| <= kPolyMax, a product |q.k| <= lim, the coefficients of an odd polynomial.
+struct ScoreArgs { float c1, ce, capl, lim, poly[4]; };
 
 // tanh(u) = 1 - 2 / (1 + e^(2u)): right at both ends (e^(2u) = 0 or inf), and
 // off by about 2^-23 absolutely, 1e-5 of a score at a cap of 50.
-__device__ __forceinline__ float cap_tanh(float s, float c) {
-  const float e = __builtin_amdgcn_exp2f(s * c);
+__device__ __forceinline__ float cap_tanh(float s, float ce) {
+  const float e = __builtin_amdgcn_exp2f(s * ce);
   return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+}
+
+// tanh(u) / u as a polynomial in u^2, for |u| <= 0.5 off by less than 1.3e-7 of
+// tanh (weighted least squares towards the smallest largest error).  Four FMA-rate
+// instructions and the one that subtracts the offset, where the exponential and
+// the reciprocal above (half rate each) take the time of eight: scores seldom
+// come nearer to their cap, and a tile in which one does takes the other form.
+constexpr float kPolyMax = 0.5f;
+constexpr double kPoly[4] = {0.999997676, -0.333206552, 0.131451453, -0.043372476};
+// The score of a product s over s, in log2 units, by the polynomial.
+__device__ __forceinline__ float cap_poly(float s, const ScoreArgs& a) {
+  const float z = s * s;
+  return __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(a.poly[3], z, a.poly[2]), z, a.poly[1]), z, a.poly[0]);
 }
 
 // One tile of a tensor in LDS: 32 rows of HD 16-bit values, row-major, their
@@ -126,6 +140,21 @@ __device__ __forceinline__ constexpr int tile_swz(int row) {
 template <int HD>
 __device__ __forceinline__ constexpr int tile_at(int row, int chunk) {
   return row * HD + ((chunk ^ tile_swz<HD>(row)) << 3);
+}
+
+// Item L of blocks x problems: heavy blocks first (the last rows of a causal
+// document see the most keys, so a launch's tail is short), and the blocks of one
+// problem on one XCD (workgroups go round the eight of them), whose L2 then holds
+// the problem's tiles.
+__device__ __forceinline__ void item_of(int L, int blocks, int problems, int& block, int& prob) {
+  const int per = problems / 8;
+  if (problems % 8 == 0) {
+    prob = L % 8 + 8 * (L / 8 % per);
+    block = L / 8 / per;
+  } else {
+    prob = L % problems;
+    block = L / problems;
+  }
 }
 
 // DMA of 4 / 16 bytes per lane into LDS at lds + 4 * lane / lds + 16 * lane.
@@ -204,6 +233,7 @@ __device__ __forceinline__ f32x16 careful_mfma(const uint16_t* t, int lane, int 
                                                f32x16 acc) {
   const uint16_t expo = F16 ? 0x7c00 : 0x7f80, one = F16 ? 0x3c00 : 0x3f80;
   f32x16 up{}, down{};
+  __builtin_amdgcn_sched_barrier(0);           // one feature block at a time: registers, not speed
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));

@@ -3,17 +3,26 @@
 // keys that a whole batch shares (attn_masked.h has the formulas and the
 // ranges that the masks are).
 //
-// attn_masked_kernel.  A workgroup has 128 rows (32 a wave) of one problem
-// and walks the keys that any of them sees, 32 a tile, through a four-slot
-// LDS ring filled by DMA three tiles ahead.  Scores are computed transposed,
-// S^T = K . Q^T on v_mfma_f32_32x32x16, so that a lane owns one row and the
-// softmax needs no exchange but one between lane halves; P^T is used in place
-// as the B operand of O^T += V^T . P^T.  The softmax offset starts at the first
-// tile's row max and moves only where a later one exceeds it by more than
-// the format of P allows (64 for bf16, 15 for fp16, in log2 units).  Sums are
-// fp32; P is rounded to the operand format for the product with V, as the
-// framework's other attention does (its relative error, 2^-9 or 2^-12, is
-// that of the output's own rounding).
+// Scores are computed transposed, S^T = K . Q^T on v_mfma_f32_32x32x16, so that a
+// lane owns one row and the softmax needs no exchange but one between lane
+// halves; P^T is used in place as the B operand of O^T += V^T . P^T.  The softmax
+// offset starts at the first tile's row max and moves only where a later one
+// exceeds it by more than the format of P allows (64 for bf16, 15 for fp16, in log2
+// units): the largest |q.k| of a tile bounds its scores (caps and slopes only
+// lower them), so a tile's exact maximum is formed only where the bound passes
+// that.  Sums are fp32; P is rounded to the operand format for the product with V,
+// as the framework's other attention does (its relative error, 2^-9 or 2^-12,
+// is that of the output's own rounding).
+//
+// attn_masked_kernel, many rows: a workgroup has 128 rows (32 a wave) of one
+// problem and walks the keys that any of them sees, 32 a tile, through a
+// four-slot LDS ring filled by DMA; S of the next tile is computed beside the
+// softmax of this one.
+//
+// attn_masked_few_kernel, up to 32 rows (new tokens): all four waves have the same
+// rows, and each walks every fourth tile through buffers of its own, K's free again
+// after the scores and V's after the product, with no barrier in the loop; their
+// results are added up in LDS.
 //
 // Few rows and many keys leave most of the chip without work: the key range
 // of a block is then split over workgroups, whose unnormalised outputs, offsets
@@ -22,8 +31,9 @@
 // the same way.
 //
 // A masked key's value does not reach a row: its weight is zero, and where
-// zero times it is not (an infinity or NaN), the workgroup finds a non-finite
-// output at its end and walks its keys again, with such values taken out.
+// zero times it is not (an infinity or NaN), the workgroup (the wave, where it
+// walks alone) finds a non-finite output at its end and walks its keys again,
+// with such values taken out.
 #include "attn_masked.h"
 
 #include <algorithm>
@@ -60,6 +70,200 @@ struct FwdArgs {
   FwdSet set[2];          // the own keys; the shared prefix (no blocks: none)
 };
 
+// A lane's row of a set's problem, and the ranges of a wave's 32 rows.
+struct Row {
+  bool live;
+  int b, h, kvh, tok;
+  int lo, hi, at;         // keys [lo, hi) are seen; the row's key coordinate
+  int w_lo, w_hi;         // keys that some row of the wave sees
+  int a_lo, a_hi;         // keys that every row sees
+};
+
+__device__ __forceinline__ Row locate(const FwdArgs& p, const FwdSet& S, int prob, int r) {
+  Row x;
+  x.live = r < S.R;
+  const int rc = x.live ? r : S.R - 1;
+  const int per = p.mask.M * p.G;
+  x.kvh = S.folded ? prob : prob % p.Hk;
+  x.b = S.folded ? rc / per : prob / p.Hk;
+  const int rr = S.folded ? rc % per : rc;
+  x.tok = rr / p.G;
+  x.h = x.kvh * p.G + rr % p.G;
+  const RowSpan s = row_span(p.mask, x.b, x.tok);
+  x.lo = S.folded ? 0 : s.lo;
+  x.hi = S.folded ? S.N : s.hi;
+  x.at = S.folded ? s.at + S.N : s.at;
+  const bool any = x.live && x.hi > x.lo;
+  x.w_lo = any ? x.lo : 0x7fffffff;
+  x.w_hi = any ? x.hi : 0;
+  x.a_lo = x.live ? x.lo : 0;
+  x.a_hi = !x.live ? 0x7fffffff : any ? x.hi : 0;
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) {
+    x.w_lo = min(x.w_lo, __shfl_xor(x.w_lo, i));
+    x.w_hi = max(x.w_hi, __shfl_xor(x.w_hi, i));
+    x.a_lo = max(x.a_lo, __shfl_xor(x.a_lo, i));
+    x.a_hi = min(x.a_hi, __shfl_xor(x.a_hi, i));
+  }
+  x.w_lo = __builtin_amdgcn_readfirstlane(x.w_lo);
+  x.w_hi = __builtin_amdgcn_readfirstlane(x.w_hi);
+  x.a_lo = __builtin_amdgcn_readfirstlane(x.a_lo);
+  x.a_hi = __builtin_amdgcn_readfirstlane(x.a_hi);
+  return x;
+}
+
+// A wave's 32 rows: their queries, softmax state and outputs.
+template <int HD, bool F16, bool CAP, bool SLOPE>
+struct Rows {
+  static constexpr int KS = HD / 16, DB = HD / 32;
+  const ScoreArgs& sc;
+  const int lane, hi, l32;
+  int lo, end, at;
+  float slope;
+  bf16x8 qf[KS];
+  f32x16 o[DB];
+  float m, l;
+
+  __device__ __forceinline__ Rows(const FwdArgs& p, const Row& x, int lane_)
+      : sc(p.score), lane(lane_), hi(lane_ >> 5), l32(lane_ & 31), lo(x.lo), end(x.hi), at(x.at), slope(0.f) {
+    if constexpr (SLOPE) slope = p.slopes[x.b * p.slopes_sb + x.h] * kMLog2e;
+    const uint16_t* Q = p.q + x.b * p.q_sb + x.h * p.q_sh + x.tok * p.q_sm;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(Q + 16 * ks + 8 * hi);
+  }
+  __device__ __forceinline__ void restart() {
+    m = -1.0e30f;                              // finite: -inf - m is -inf
+    l = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[db] = f32x16{};
+  }
+  // The products of a tile's 32 keys (registers) and this lane's query.
+  __device__ __forceinline__ f32x16 products(const uint16_t* k) const {
+    f32x16 s{};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = mfma32x32x16_t<F16>(row_frag<HD>(k, ks, l32, hi), qf[ks], s);
+    return s;
+  }
+  __device__ __forceinline__ void masked(float (&x)[16], int n0) const {
+    const int from = lo - n0 - 4 * hi, to = end - n0 - 4 * hi;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (mfma_row(i, 0) < from || mfma_row(i, 0) >= to) x[i] = -INFINITY;
+  }
+  __device__ __forceinline__ void sloped(float (&x)[16], int n0) const {
+    if constexpr (SLOPE) {
+      const float dist = (float)(at - n0 - 4 * hi);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(-slope, fabsf(dist - (float)mfma_row(i, 0)), x[i]);
+    }
+  }
+  // Scores in log2 units, -inf where the row does not see the key, less `off`.
+  __device__ __forceinline__ void scores(const f32x16& s, int n0, bool edge, bool poly, float off, float (&x)[16]) const {
+    if (!CAP) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(s[i], sc.c1, -off);
+    } else if (poly) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(s[i], cap_poly(s[i], sc), -off);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(cap_tanh(s[i], sc.ce), sc.capl, -off);
+    }
+    sloped(x, n0);
+    if (edge) masked(x, n0);
+  }
+  // Products to weights.  Where a tile's largest |product| does not tell that all
+  // scores lie below the offset's reach, the offset follows the row's maximum, and
+  // the sum and the output with it.
+  __device__ __forceinline__ void weigh(const f32x16& s, int n0, bool edge, float (&x)[16]) {
+    float a = fmaxf(fabsf(s[0]), fabsf(s[1]));
+#pragma unroll
+    for (int i = 2; i < 16; i += 2) a = fmaxf(fmaxf(a, fabsf(s[i])), fabsf(s[i + 1]));
+    const bool poly = CAP && __builtin_amdgcn_ballot_w64(!(a <= sc.lim)) == 0;
+    if (__builtin_amdgcn_ballot_w64(!(a * sc.c1 <= m + kUp<F16>))) {
+      scores(s, n0, edge, poly, 0.f, x);
+      float mx = x[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+      mx = max_halves(mx);
+      const float m_new = mx > m + kUp<F16> ? mx : m;
+      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] *= alpha;
+    }
+    scores(s, n0, edge, poly, m, x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] = __builtin_amdgcn_exp2f(x[i]);
+      l += x[i];
+    }
+  }
+  __device__ __forceinline__ void add(const uint16_t* v, const float (&x)[16]) {
+    bf16x8 pb[2];
+    pack_frags<F16>(x, pb);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) o[db] = mfma32x32x16_t<F16>(tr_frag<HD>(v, lane, db, s), pb[s], o[db]);
+  }
+  // A tile whose values may hold infinities or NaN that a row does not see.
+  __device__ __forceinline__ void careful(const uint16_t* k, const uint16_t* v, int n0) {
+    float x[16], seen[16];
+    weigh(products(k), n0, true, x);
+    const int from = lo - n0 - 4 * hi, to = end - n0 - 4 * hi;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) seen[i] = mfma_row(i, 0) < from || mfma_row(i, 0) >= to ? 0.f : 1.f;
+    bf16x8 pb[2], sb[2];
+    pack_frags<F16>(x, pb);
+    pack_frags<F16>(seen, sb);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[db] = careful_mfma<HD, F16>(v, lane, db, pb, sb, o[db]);
+  }
+  __device__ __forceinline__ bool odd() const {
+    bool x = false;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x |= !(fabsf(o[db][i]) < INFINITY);
+    return x;
+  }
+  // The rows' outputs, or their part of them; `total` is the sum over both halves.
+  __device__ __forceinline__ void finish(const FwdArgs& p, const FwdSet& S, const Row& x, int z, float total) {
+    if (!x.live) return;
+    if (p.part) {
+      const int64_t row = (((int64_t)x.b * p.Hk + x.kvh) * p.mask.M + x.tok) * p.G + (x.h - x.kvh * p.G);
+      const int64_t to = (int64_t)(S.z0 + z) * p.rows + row;
+      float* O = p.part + to * HD;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(O + db * 32 + 8 * g + 4 * hi) =
+              f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+      if (hi == 0) {
+        p.stat[2 * to] = m;
+        p.stat[2 * to + 1] = total;
+      }
+      return;
+    }
+    const float inv = total == 0.f ? 0.f : 1.0f / total;   // no key seen: zeros
+    uint16_t* O = p.o + x.b * p.o_sb + x.h * p.o_sh + x.tok * p.o_sm;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const bf16x2 a = pack2<F16>(o[db][4 * g + 0] * inv, o[db][4 * g + 1] * inv);
+        const bf16x2 b = pack2<F16>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv);
+        *reinterpret_cast<u32x2*>(O + db * 32 + 8 * g + 4 * hi) =
+            u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+      }
+    if (p.lse && hi == 0)
+      p.lse[x.b * p.lse_sb + x.h * p.lse_sh + x.tok] = total == 0.f ? -INFINITY : m + __log2f(total);
+  }
+};
+
 template <int HD>
 struct Slot {
   uint16_t k[kMTile * HD];
@@ -67,62 +271,25 @@ struct Slot {
 };
 
 template <int HD, bool F16, bool CAP, bool SLOPE>
-__global__ __launch_bounds__(kMThreads, 2) void attn_masked_kernel(FwdArgs p) {
-  constexpr int KS = HD / 16, DB = HD / 32, CH = HD / 8;
+__global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_kernel(FwdArgs p, int which) {
+  constexpr int CH = HD / 8;
   constexpr int DJ = kMTile * CH / kMThreads;  // 16-byte DMAs per wave, tile and tensor
   __shared__ __attribute__((aligned(16))) Slot<HD> r0, r1, r2, r3;
   __shared__ int range[2][kMWaves];
 
-  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, l32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int item = blockIdx.x;
-  const int own_items = p.set[0].blocks * p.set[0].problems * p.set[0].splits;
-  const bool second = item >= own_items;
-  const FwdSet& S = p.set[second ? 1 : 0];
-  if (second) item -= own_items;
-  const int qb = item % S.blocks, prob = item / S.blocks % S.problems,
-            z = item / S.blocks / S.problems;
+  const FwdSet& S = p.set[which];
+  const int z = blockIdx.x / (S.blocks * S.problems);
+  int qb, prob;
+  item_of(blockIdx.x % (S.blocks * S.problems), S.blocks, S.problems, qb, prob);
+  qb = S.blocks - 1 - qb;
+  const Row row = locate(p, S, prob, qb * kMRows + wave * 32 + (lane & 31));
+  Rows<HD, F16, CAP, SLOPE> R(p, row, lane);
 
-  // This lane's row.
-  const int r = qb * kMRows + wave * 32 + l32;
-  const bool live = r < S.R;
-  const int rc = live ? r : S.R - 1;
-  const int per = p.mask.M * p.G;
-  const int kvh = S.folded ? prob : prob % p.Hk;
-  const int b = S.folded ? rc / per : prob / p.Hk;
-  const int rr = S.folded ? rc % per : rc;
-  const int m_tok = rr / p.G, h = kvh * p.G + rr % p.G;
-  RowSpan span = row_span(p.mask, b, m_tok);
-  if (S.folded) span = RowSpan{0, S.N, span.at + S.N};
-  float slope = 0.f;
-  if constexpr (SLOPE) slope = p.slopes[b * p.slopes_sb + h] * kMLog2e;
-
-  bf16x8 qf[KS];
-  {
-    const uint16_t* Q = p.q + b * p.q_sb + h * p.q_sh + m_tok * p.q_sm;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(Q + 16 * ks + 8 * hi);
-  }
-
-  // The keys that this wave's rows see, and that the workgroup's do.
-  const bool any = live && span.hi > span.lo;
-  int w_lo = any ? span.lo : 0x7fffffff, w_hi = any ? span.hi : 0;   // some row's
-  int a_lo = live ? span.lo : 0, a_hi = live ? span.hi : 0x7fffffff;  // every row's
-  if (live && !any) a_hi = 0;
-#pragma unroll
-  for (int i = 1; i < 32; i <<= 1) {
-    w_lo = min(w_lo, __shfl_xor(w_lo, i));
-    w_hi = max(w_hi, __shfl_xor(w_hi, i));
-    a_lo = max(a_lo, __shfl_xor(a_lo, i));
-    a_hi = min(a_hi, __shfl_xor(a_hi, i));
-  }
-  w_lo = __builtin_amdgcn_readfirstlane(w_lo);
-  w_hi = __builtin_amdgcn_readfirstlane(w_hi);
-  a_lo = __builtin_amdgcn_readfirstlane(a_lo);
-  a_hi = __builtin_amdgcn_readfirstlane(a_hi);
   if (lane == 0) {
-    range[0][wave] = w_lo;
-    range[1][wave] = w_hi;
+    range[0][wave] = row.w_lo;
+    range[1][wave] = row.w_hi;
   }
   __syncthreads();
   int n_lo = range[0][0], n_hi = range[1][0];
@@ -134,13 +301,13 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_kernel(FwdArgs p) {
   n_lo = __builtin_amdgcn_readfirstlane(n_lo);
   n_hi = __builtin_amdgcn_readfirstlane(n_hi);
   if (n_hi <= n_lo) n_lo = n_hi = 0;           // nothing seen: no tile, empty DMAs
-  const int all_tiles = n_hi > n_lo ? (n_hi - n_lo + kMTile - 1) / kMTile : 0;
+  const int all_tiles = (n_hi - n_lo + kMTile - 1) / kMTile;
   const int t_begin = (int)((int64_t)all_tiles * z / S.splits);
   const int t_end = (int)((int64_t)all_tiles * (z + 1) / S.splits);
 
   const int64_t kb = S.folded ? 0 : prob / p.Hk;
-  const uint16_t* K = S.k + kb * S.k_sb + kvh * S.k_sh;
-  const uint16_t* V = S.v + kb * S.v_sb + kvh * S.v_sh;
+  const uint16_t* K = S.k + kb * S.k_sb + row.kvh * S.k_sh;
+  const uint16_t* V = S.v + kb * S.v_sb + row.kvh * S.v_sh;
   uint32_t k_voff[DJ], v_voff[DJ];
 #pragma unroll
   for (int j = 0; j < DJ; ++j) {
@@ -160,219 +327,272 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_kernel(FwdArgs p) {
 #pragma unroll
     for (int j = 0; j < DJ; ++j) m_dma16(vr, &T.v[(wave * DJ + j) * 512], v_voff[j]);
   };
+  auto sees = [&](int n0) { return n0 < row.w_hi && n0 + kMTile > row.w_lo; };
 
-  f32x16 o_acc[DB];
-  float m, l;
-
-  // Tile t's scores, in log2 units, -inf where the row does not see the key.
-  auto scores = [&](const Slot<HD>& T, int n0, bool edge, float (&x)[16]) {
-    f32x16 sv{};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      sv = mfma32x32x16_t<F16>(row_frag<HD>(T.k, ks, l32, hi), qf[ks], sv);
-    const float dist = (float)(span.at - n0 - 4 * hi);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float y = CAP ? cap_tanh(sv[i], p.score.c) * p.score.capl : sv[i] * p.score.c;
-      if constexpr (SLOPE) y = __builtin_fmaf(-slope, fabsf(dist - (float)mfma_row(i, 0)), y);
-      x[i] = y;
-    }
-    if (edge) {
-      const int from = span.lo - n0 - 4 * hi, to = span.hi - n0 - 4 * hi;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (mfma_row(i, 0) < from || mfma_row(i, 0) >= to) x[i] = -INFINITY;
-    }
-  };
-  auto weigh = [&](float (&x)[16]) {           // x to weights; m, l and O move
-    float mx = x[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
-    mx = max_halves(mx);
-    const bool move = mx > m + kUp<F16>;
-    if (__builtin_amdgcn_ballot_w64(move)) {
-      const float m_new = move ? mx : m;
-      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-      m = m_new;
-      l *= alpha;
-#pragma unroll
-      for (int db = 0; db < DB; ++db) o_acc[db] *= alpha;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[i] = __builtin_amdgcn_exp2f(x[i] - m);
-      l += x[i];
-    }
-  };
-  auto restart = [&]() {
-    m = -1.0e30f;                              // finite: -inf - m is -inf
-    l = 0.f;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) o_acc[db] = f32x16{};
-  };
-
-  auto iter = [&](int t, const Slot<HD>& cur, Slot<HD>& dst) {
-    m_wait<4 * DJ>();                          // tile t landed (two more in flight)
-    __syncthreads();                           // ... for every wave; `dst` is free
+  // Iteration t: tile t in `cur`, its products in s; tile t + 1 in `nxt`; tile t + 3
+  // issued into `dst`, the slot of tile t - 1, free once every wave passed the barrier.
+  f32x16 s;
+  auto iter = [&](int t, const Slot<HD>& cur, const Slot<HD>& nxt, Slot<HD>& dst) {
+    m_wait<2 * DJ>();                          // tile t + 1 landed (tile t + 2 in flight)
+    __syncthreads();                           // ... for every wave
     issue(t + 3, dst);
     const int n0 = n_lo + t * kMTile;
-    if (n0 >= w_hi || n0 + kMTile <= w_lo) return;
-    float x[16];
-    scores(cur, n0, n0 < a_lo || n0 + kMTile > a_hi, x);
-    weigh(x);
-    bf16x8 pb[2];
-    pack_frags<F16>(x, pb);
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        o_acc[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.v, lane, db, s), pb[s], o_acc[db]);
+    const f32x16 next = R.products(nxt.k);
+    if (sees(n0)) {
+      float x[16];
+      R.weigh(s, n0, n0 < row.a_lo || n0 + kMTile > row.a_hi, x);
+      R.add(cur.v, x);
+    }
+    s = next;
   };
-  restart();
+  R.restart();
   issue(t_begin, r0);
   issue(t_begin + 1, r1);
   issue(t_begin + 2, r2);
+  m_wait<4 * DJ>();
+  __syncthreads();
+  s = R.products(r0.k);
   for (int t = t_begin; t < t_end; t += 4) {
-    iter(t, r0, r3);
+    iter(t, r0, r1, r3);
     if (t + 1 >= t_end) break;
-    iter(t + 1, r1, r0);
+    iter(t + 1, r1, r2, r0);
     if (t + 2 >= t_end) break;
-    iter(t + 2, r2, r1);
+    iter(t + 2, r2, r3, r1);
     if (t + 3 >= t_end) break;
-    iter(t + 3, r3, r2);
+    iter(t + 3, r3, r0, r2);
   }
   m_wait<0>();                                 // no DMA may land after the workgroup ends
 
-  float total = sum_halves(l);
-  bool odd = false;
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) odd |= !(fabsf(o_acc[db][i]) < INFINITY);
-  if (__syncthreads_or(odd && live)) {
-    // Again, one tile at a time, without the values that a row does not see.
-    restart();
+  if (__syncthreads_or(R.odd() && row.live)) {
+    R.restart();
     for (int t = t_begin; t < t_end; ++t) {
       __syncthreads();
       issue(t, r0);
       m_wait<0>();
       __syncthreads();
-      const int n0 = n_lo + t * kMTile;
-      float x[16], sx[16];
-      scores(r0, n0, true, x);
-      const int from = span.lo - n0 - 4 * hi, to = span.hi - n0 - 4 * hi;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        sx[i] = mfma_row(i, 0) < from || mfma_row(i, 0) >= to ? 0.f : 1.f;
-      weigh(x);
-      bf16x8 pb[2], sb[2];
-      pack_frags<F16>(x, pb);
-      pack_frags<F16>(sx, sb);
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-        o_acc[db] = careful_mfma<HD, F16>(r0.v, lane, db, pb, sb, o_acc[db]);
+      R.careful(r0.k, r0.v, n_lo + t * kMTile);
     }
-    total = sum_halves(l);
   }
-  if (!live) return;
+  R.finish(p, S, row, z, sum_halves(R.l));
+}
 
-  if (p.part) {
-    const int64_t row = (((int64_t)b * p.Hk + kvh) * p.mask.M + m_tok) * p.G + (h - kvh * p.G);
-    const int64_t at = (int64_t)(S.z0 + z) * p.rows + row;
-    float* O = p.part + at * HD;
+template <int HD, bool F16, bool CAP, bool SLOPE>
+__global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_few_kernel(FwdArgs p, int which) {
+  constexpr int CH = HD / 8, DB = HD / 32;
+  constexpr int DJ = kMTile * CH / 64;         // 16-byte DMAs per tile and tensor: one wave's
+  constexpr int ROW = 64 / CH;                 // rows of a DMA
+  __shared__ __attribute__((aligned(16))) uint16_t kt[kMWaves][kMTile * HD];
+  __shared__ __attribute__((aligned(16))) uint16_t vt[kMWaves][kMTile * HD];
+  __shared__ float stat[kMWaves][2][32];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const FwdSet& S = p.set[which];
+  const int prob = blockIdx.x % S.problems, z = blockIdx.x / S.problems;
+  const Row row = locate(p, S, prob, lane & 31);
+  Rows<HD, F16, CAP, SLOPE> R(p, row, lane);
+  const int n_lo = row.w_hi > row.w_lo ? row.w_lo : 0, n_hi = row.w_hi > row.w_lo ? row.w_hi : 0;
+  const int all_tiles = (n_hi - n_lo + kMTile - 1) / kMTile;
+  const int t_begin = (int)((int64_t)all_tiles * z / S.splits) + wave;
+  const int t_end = (int)((int64_t)all_tiles * (z + 1) / S.splits);
+
+  const int64_t kb = S.folded ? 0 : prob / p.Hk;
+  const uint16_t* K = S.k + kb * S.k_sb + row.kvh * S.k_sh;
+  const uint16_t* V = S.v + kb * S.v_sb + row.kvh * S.v_sh;
+  uint16_t *kw = kt[wave], *vw = vt[wave];
+  // Tiles past the wave's last one are issued too, empty: the waits count them.
+  auto issue = [&](const uint16_t* base, int64_t stride, int t, uint16_t* T) {
+    const __amdgpu_buffer_rsrc_t r = tile_rsrc<HD>(base, stride, n_lo + t * kMTile, t < t_end ? n_hi : 0);
+#pragma unroll
+    for (int j = 0; j < DJ; ++j) {
+      const int key = j * ROW + lane / CH;
+      m_dma16(r, T + j * 512, key * (uint32_t)(stride * 2) + (uint32_t)((lane % CH) ^ tile_swz<HD>(key)) * 16u);
+    }
+  };
+  R.restart();
+  issue(K, S.k_sn, t_begin, kw);
+  issue(V, S.v_sn, t_begin, vw);
+  for (int t = t_begin; t < t_end; t += kMWaves) {
+    const int n0 = n_lo + t * kMTile;
+    m_wait<DJ>();                              // K landed, V in flight
+    const f32x16 s = R.products(kw);
+    __builtin_amdgcn_s_waitcnt(0xc07f);        // lgkmcnt(0): K is read, its buffer free
+    issue(K, S.k_sn, t + kMWaves, kw);
+    const bool edge = n0 < row.a_lo || n0 + kMTile > row.a_hi;
+    float x[16];
+    R.weigh(s, n0, edge, x);
+    m_wait<DJ>();                              // V landed, the next K in flight
+    R.add(vw, x);
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    issue(V, S.v_sn, t + kMWaves, vw);
+  }
+  m_wait<0>();
+  if (__builtin_amdgcn_ballot_w64(R.odd() && row.live)) {
+    R.restart();
+    for (int t = t_begin; t < t_end; t += kMWaves) {
+      issue(K, S.k_sn, t, kw);
+      issue(V, S.v_sn, t, vw);
+      m_wait<0>();
+      R.careful(kw, vw, n_lo + t * kMTile);
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+    }
+  }
+
+  // The four waves' results in wave 0, by way of K's buffers, all at one offset.
+  float total = sum_halves(R.l);
+  if (lane < 32) {
+    stat[wave][0][lane] = R.m;
+    stat[wave][1][lane] = total;
+  }
+  __syncthreads();
+  float m = stat[0][0][lane & 31];
+#pragma unroll
+  for (int i = 1; i < kMWaves; ++i) m = fmaxf(m, stat[i][0][lane & 31]);
+  total = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMWaves; ++i)
+    total = __builtin_fmaf(__builtin_amdgcn_exp2f(stat[i][0][lane & 31] - m), stat[i][1][lane & 31], total);
+  const float alpha = __builtin_amdgcn_exp2f(R.m - m);
+#pragma unroll
+  for (int db = 0; db < DB; ++db) R.o[db] *= alpha;
+  R.m = m;
+  f32x4* ex = reinterpret_cast<f32x4*>(&kt[0][0]) + lane;   // [2][DB * 4][64]
+  auto give = [&](int at) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(O + db * 32 + 8 * g + 4 * hi) =
-            f32x4{o_acc[db][4 * g], o_acc[db][4 * g + 1], o_acc[db][4 * g + 2], o_acc[db][4 * g + 3]};
-    if (hi == 0) {
-      p.stat[2 * at] = m;
-      p.stat[2 * at + 1] = total;
-    }
-    return;
-  }
-  const float inv = total == 0.f ? 0.f : 1.0f / total;   // no key seen: zeros
-  uint16_t* O = p.o + b * p.o_sb + h * p.o_sh + m_tok * p.o_sm;
+        ex[(at * DB * 4 + db * 4 + g) * 64] = f32x4{R.o[db][4 * g], R.o[db][4 * g + 1], R.o[db][4 * g + 2],
+                                                   R.o[db][4 * g + 3]};
+  };
+  auto take = [&](int at) {
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const bf16x2 lo = pack2<F16>(o_acc[db][4 * g + 0] * inv, o_acc[db][4 * g + 1] * inv);
-      const bf16x2 up = pack2<F16>(o_acc[db][4 * g + 2] * inv, o_acc[db][4 * g + 3] * inv);
-      *reinterpret_cast<u32x2*>(O + db * 32 + 8 * g + 4 * hi) =
-          u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, up)};
-    }
-  if (p.lse && hi == 0)
-    p.lse[b * p.lse_sb + h * p.lse_sh + m_tok] = total == 0.f ? -INFINITY : m + __log2f(total);
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = ex[(at * DB * 4 + db * 4 + g) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) R.o[db][4 * g + e] += v[e];
+      }
+  };
+  if (wave >= 2) give(wave - 2);
+  __syncthreads();
+  if (wave < 2) take(wave);
+  __syncthreads();
+  if (wave == 1) give(0);
+  __syncthreads();
+  if (wave > 0) return;
+  take(0);
+  R.finish(p, S, row, z, total);
 }
 
-// One wave a row: the partial outputs of its splits put together.
-template <int HD, bool F16>
+// The partial outputs of a row's splits put together, by WAVES waves.
+constexpr int kMaxSplits = 512;
+template <int HD, bool F16, int WAVES>
 __global__ __launch_bounds__(256) void attn_masked_join_kernel(FwdArgs p) {
-  constexpr int E = HD / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= p.rows) return;
-  const int g = (int)(row % p.G);
-  const int64_t t = row / p.G;
-  const int m_tok = (int)(t % p.mask.M);
-  const int64_t bh = t / p.mask.M, b = bh / p.Hk;
-  const int h = (int)(bh % p.Hk) * p.G + g;
-
-  // The splits' offsets and sums, one lane a split (64 at a time).
-  float top = -INFINITY;
-  for (int z = lane; z < p.splits; z += 64) top = fmaxf(top, p.stat[2 * (z * p.rows + row)]);
+  constexpr int ROWS = 4 / WAVES, T = WAVES * 64, L = HD / 4, GR = T / L;   // L lanes have the row once
+  constexpr int MAXZ = WAVES == 1 ? 16 : kMaxSplits;
+  __shared__ float weight[ROWS][MAXZ];
+  __shared__ float red[4];
+  __shared__ f32x4 acc[4][L];
+  const int slot = threadIdx.x / T, tid = threadIdx.x % T, lane = tid & 63, wave = threadIdx.x >> 6;
+  const int64_t row = std::min((int64_t)blockIdx.x * ROWS + slot, p.rows - 1);
+  auto over = [&](float v, auto op) {          // over the row's lanes
 #pragma unroll
-  for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
-  float total = 0.f, o[E] = {};
-  for (int z0 = 0; z0 < p.splits; z0 += 64) {
-    const int z = z0 + lane;
-    float w = 0.f;
+    for (int i = 1; i < 64; i <<= 1) v = op(v, __shfl_xor(v, i));
+    if constexpr (WAVES > 1) {
+      __syncthreads();
+      if (lane == 0) red[wave] = v;
+      __syncthreads();
+      v = op(op(red[0], red[1]), op(red[2], red[3]));
+    }
+    return v;
+  };
+  constexpr int PER = (MAXZ + T - 1) / T;
+  float m[PER], l[PER], top = -INFINITY, total = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int z = tid + i * T;
+    m[i] = -INFINITY;
+    l[i] = 0.f;
     if (z < p.splits) {
-      const int64_t at = z * p.rows + row;
-      w = __builtin_amdgcn_exp2f(p.stat[2 * at] - top);
-      const float sum = p.stat[2 * at + 1];
-      total = __builtin_fmaf(w, sum, total);
-      if (sum == 0.f) w = 0.f;
+      const float2 s = reinterpret_cast<const float2*>(p.stat)[z * p.rows + row];
+      m[i] = s.x;
+      l[i] = s.y;
     }
-    const int n = min(64, p.splits - z0);
-    for (int i = 0; i < n; ++i) {
-      const float wi = __shfl(w, i);
-      const float* O = p.part + ((int64_t)(z0 + i) * p.rows + row) * HD;
+    top = fmaxf(top, m[i]);
+  }
+  top = over(top, [](float a, float b) { return fmaxf(a, b); });
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(wi, O[lane * E + e], o[e]);
-    }
+  for (int i = 0; i < PER; ++i) {
+    const int z = tid + i * T;
+    const float w = l[i] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m[i] - top);
+    total = __builtin_fmaf(w, l[i], total);
+    if (z < p.splits) weight[slot][z] = w;
+  }
+  total = over(total, [](float a, float b) { return a + b; });
+  __syncthreads();
+  const int at = tid % L, group = tid / L;
+  f32x4 o{};
+  const f32x4* P = reinterpret_cast<const f32x4*>(p.part) + row * L + at;
+#pragma unroll 4
+  for (int z = group; z < p.splits; z += GR) {
+    const f32x4 v = P[(int64_t)z * p.rows * L];
+    const float w = weight[slot][z];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, v[e], o[e]);
   }
 #pragma unroll
-  for (int i = 1; i < 64; i <<= 1) total += __shfl_xor(total, i);
+  for (int i = L; i < 64; i <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], i);
+  if constexpr (WAVES > 1) {
+    if (lane < L) acc[wave][at] = o;
+    __syncthreads();
+    o = acc[0][at];
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += acc[i][at][e];
+  }
+  if (tid >= L || (int64_t)blockIdx.x * ROWS + slot >= p.rows) return;
+  const int g = (int)(row % p.G);
+  const int64_t t = row / p.G, tok = t % p.mask.M, b = t / p.mask.M / p.Hk;
+  const int64_t h = t / p.mask.M % p.Hk * p.G + g;
   const float inv = total == 0.f ? 0.f : 1.0f / total;
-  uint16_t* O = p.o + b * p.o_sb + h * p.o_sh + m_tok * p.o_sm;
-  if constexpr (E == 2) {
-    const bf16x2 v = pack2<F16>(o[0] * inv, o[1] * inv);
-    *reinterpret_cast<uint32_t*>(O + 2 * lane) = __builtin_bit_cast(uint32_t, v);
-  } else {
-    O[lane] = __builtin_bit_cast(uint16_t, f32_to_half<F16>(o[0] * inv));
+  const bf16x2 lo = pack2<F16>(o[0] * inv, o[1] * inv), hi = pack2<F16>(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<u32x2*>(p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sm + 4 * at) =
+      u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+  if (p.lse && at == 0)
+    p.lse[b * p.lse_sb + h * p.lse_sh + tok] = total == 0.f ? -INFINITY : top + __log2f(total);
+}
+
+template <int HD, bool F16, bool CAP, bool SLOPE>
+hipError_t launch_sets(const FwdArgs& a, hipStream_t s) {
+  for (int i = 1; i >= 0; --i) {               // the prefix, then the own keys
+    const FwdSet& t = a.set[i];
+    const unsigned items = (unsigned)t.blocks * t.problems * t.splits;
+    if (items == 0) continue;
+    if (t.R <= 32)
+      hipLaunchKernelGGL((attn_masked_few_kernel<HD, F16, CAP, SLOPE>), dim3(items), dim3(kMThreads), 0, s, a, i);
+    else
+      hipLaunchKernelGGL((attn_masked_kernel<HD, F16, CAP, SLOPE>), dim3(items), dim3(kMThreads), 0, s, a, i);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
-  if (p.lse && lane == 0)
-    p.lse[b * p.lse_sb + h * p.lse_sh + m_tok] = total == 0.f ? -INFINITY : top + __log2f(total);
+  return hipSuccess;
 }
 
 template <int HD, bool F16>
 hipError_t launch(const FwdArgs& a, bool cap, hipStream_t s) {
-  int64_t items = 0;
-  for (const FwdSet& t : a.set) items += (int64_t)t.blocks * t.problems * t.splits;
-  const dim3 grid((unsigned)items), block(kMThreads);
-  if (cap && a.slopes) hipLaunchKernelGGL((attn_masked_kernel<HD, F16, true, true>), grid, block, 0, s, a);
-  else if (cap) hipLaunchKernelGGL((attn_masked_kernel<HD, F16, true, false>), grid, block, 0, s, a);
-  else if (a.slopes) hipLaunchKernelGGL((attn_masked_kernel<HD, F16, false, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((attn_masked_kernel<HD, F16, false, false>), grid, block, 0, s, a);
-  if (a.part) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attn_masked_join_kernel<HD, F16>), dim3((unsigned)((a.rows + 3) / 4)),
-                       dim3(256), 0, s, a);
-  }
+  const hipError_t e = cap ? (a.slopes ? launch_sets<HD, F16, true, true>(a, s) : launch_sets<HD, F16, true, false>(a, s))
+                           : (a.slopes ? launch_sets<HD, F16, false, true>(a, s) : launch_sets<HD, F16, false, false>(a, s));
+  if (e != hipSuccess || !a.part) return e;
+  // A wave a row reads a few splits, four waves many.
+  if (a.splits <= 16)
+    hipLaunchKernelGGL((attn_masked_join_kernel<HD, F16, 1>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((attn_masked_join_kernel<HD, F16, 4>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
@@ -383,8 +603,7 @@ hipError_t launch(const FwdArgs& a, bool cap, hipStream_t s) {
 constexpr int64_t kWant = 512, kLeast = 8;
 int splits_of(int64_t items, int64_t keys) {
   const int64_t tiles = (keys + kMTile - 1) / kMTile;
-  int64_t z = items > 0 ? kWant / items : 1;
-  z = std::min(z, tiles / kLeast);
+  const int64_t z = std::min({items > 0 ? kWant / items : 1, tiles / kLeast, (int64_t)kMaxSplits / 2});
   return (int)std::max<int64_t>(z, 1);
 }
 
@@ -500,8 +719,15 @@ void gpa::masked_fill(const gpa_attn_masked_args* a, MaskArgs* m, ScoreArgs* s) 
   m->causal = a->causal != 0;
   m->M = (int32_t)a->M;
   m->N = (int32_t)a->N;
-  s->c = a->cap > 0.f ? 2.0f * kMLog2e * a->sm_scale / a->cap : a->sm_scale * kMLog2e;
-  s->capl = a->cap * kMLog2e;
+  s->c1 = a->sm_scale * kMLog2e;
+  if (a->cap > 0.f) {
+    const double g = (double)a->sm_scale / a->cap, l2e = 1.4426950408889634;
+    s->ce = (float)(2.0 * l2e * g);
+    s->capl = a->cap * kMLog2e;
+    s->lim = (float)std::min(kPolyMax / g, 1e18);   // s^2 stays finite
+    double scale = a->sm_scale * l2e;
+    for (int i = 0; i < 4; ++i, scale *= g * g) s->poly[i] = (float)(kPoly[i] * scale);
+  }
 }
 
 extern "C" size_t gpa_attn_masked_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t M,

@@ -122,7 +122,8 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int blocks = (p.mask.N + kMRows - 1) / kMRows;
-  const int kb = blockIdx.x % blocks, prob = blockIdx.x / blocks;
+  int kb, prob;
+  item_of(blockIdx.x, blocks, gridDim.x / blocks, kb, prob);
   const int b = prob / p.Hk, kvh = prob % p.Hk;
   const int j = kb * kMRows + wave * 32 + l32;
   const bool live = j < p.mask.N;
@@ -249,10 +250,10 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
         const int i = 4 * g + e;
         float t = 0.f, x;
         if constexpr (CAP) {
-          t = cap_tanh(s[i], p.score.c);
+          t = cap_tanh(s[i], p.score.ce);
           x = t * p.score.capl;
         } else {
-          x = s[i] * p.score.c;
+          x = s[i] * p.score.c1;
         }
         if constexpr (SLOPE) x = __builtin_fmaf(-sl[e], fabsf(tok[e] + shift), x);
         w[i] = __builtin_amdgcn_exp2f(x - ls[e]);
@@ -376,7 +377,9 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_ke
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int blocks = (p.R + kMRows - 1) / kMRows;
-  const int qb = blockIdx.x % blocks, prob = blockIdx.x / blocks;
+  int qb, prob;
+  item_of(blockIdx.x, blocks, gridDim.x / blocks, qb, prob);
+  qb = blocks - 1 - qb;
   const int b = prob / p.Hk, kvh = prob % p.Hk;
   const int r = qb * kMRows + wave * 32 + l32;
   const bool live = r < p.R;
@@ -469,10 +472,10 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_ke
     for (int i = 0; i < 16; ++i) {
       float t = 0.f, x;
       if constexpr (CAP) {
-        t = cap_tanh(s[i], p.score.c);
+        t = cap_tanh(s[i], p.score.ce);
         x = t * p.score.capl;
       } else {
-        x = s[i] * p.score.c;
+        x = s[i] * p.score.c1;
       }
       if constexpr (SLOPE) x = __builtin_fmaf(-slope, fabsf(dist - (float)mfma_row(i, 0)), x);
       ds[i] = __builtin_amdgcn_exp2f(x - lse) * dp[i];
