@@ -6,15 +6,25 @@
 //   dV_j  = sum_i P_ij dO_i,   dK_j = sm_scale sum_i dS_ij Q_i,
 //   dQ_i  = sm_scale sum_j dS_ij K_j
 //
-// attn_masked_delta_kernel writes a record of every 32 rows: their LSE, -delta,
-// token and slope.  attn_masked_dkdv_kernel: a wave owns 32 keys (K, V, dK and
-// dV in registers) and walks the rows that see them, all query heads of the
-// key head, so a shared head's gradient is one sum in one order; S = Q . K^T
-// puts a key in each lane, and P and dS are used in place as the B operands of
-// dV^T += dO^T . P and dK^T += Q^T . dS.  attn_masked_dq_kernel mirrors it: a
-// wave owns 32 rows and walks the keys, dQ^T += K^T . dS^T.  No atomics: two
-// kernels compute S and dP twice (7 products instead of 5), and in return
-// the results repeat bit by bit and no fp32 copy of dQ goes through memory.
+// attn_masked_delta_kernel writes a record of every 64 rows: their LSE, -delta,
+// token and slope.
+//
+// attn_masked_dkdv_kernel: a workgroup has 64 keys and walks the rows that see
+// them, all query heads of the key head, so a shared head's gradient is one sum
+// in one order.  A wave owns 32 of the keys (K, V, dK and dV in registers) and
+// one half of each 64-row tile; the two halves are added at the end.  (With 128
+// keys to a workgroup, one row tile for all four waves, a launch of 4,096 keys
+// and 8 heads had 256 workgroups of very different lengths.)  S = Q . K^T puts a
+// key in each lane, and P and dS are used in place as the B operands of dV^T +=
+// dO^T . P and dK^T += Q^T . dS.
+//
+// attn_masked_dq_kernel mirrors it: a wave owns 32 rows and walks the keys, dQ^T +=
+// K^T . dS^T.  In both the next tile's S and dP are computed beside this one's
+// weights.  No atomics: two kernels compute S and dP twice (7 products instead of
+// 5), and in return the results repeat bit by bit and no fp32 copy of dQ goes
+// through memory.
+//
+// With a cap, r = 1 / (1 + e^(2u)) gives both: tanh = 1 - 2r, 1 - tanh^2 = 4 (r - r^2).
 //
 // P and dS are rounded to the operand format for the products (the same
 // relative error as the gradients' own rounding); sums are fp32.  In fp16
@@ -27,7 +37,9 @@
 namespace gpa {
 namespace {
 
-constexpr int kRec = 128;                      // floats of a record: lse, -delta, token, slope
+constexpr int kRowTile = 64;                   // rows of a record, and of a dk, dv tile
+constexpr int kRec = 4 * kRowTile;             // lse (less cap log2(e)), -delta, token, slope
+constexpr int kKeys = 64;                      // keys of a dk, dv workgroup
 
 struct BwdArgs {
   const uint16_t *q, *k, *v, *o, *d_o;
@@ -52,8 +64,8 @@ __global__ __launch_bounds__(256) void attn_masked_delta_kernel(BwdArgs p) {
   const int b = prob / p.Hk, kvh = prob % p.Hk;
   float* rec = p.rec + ((int64_t)prob * p.tiles + tile) * kRec;
   const int ch = threadIdx.x % CH;
-  for (int i = threadIdx.x / CH; i < 32; i += 256 / CH) {
-    const int r = tile * 32 + i;
+  for (int i = threadIdx.x / CH; i < kRowTile; i += 256 / CH) {
+    const int r = tile * kRowTile + i;
     float lse = INFINITY, delta = 0.f, slope = 0.f;   // past the rows: weights of zero
     int m = 0;
     if (r < p.R) {
@@ -73,10 +85,10 @@ __global__ __launch_bounds__(256) void attn_masked_delta_kernel(BwdArgs p) {
 #pragma unroll
     for (int s = 1; s < CH; s <<= 1) delta += __shfl_xor(delta, s);
     if (ch == 0) {
-      rec[i] = lse;
-      rec[32 + i] = -delta;
-      rec[64 + i] = (float)m;
-      rec[96 + i] = slope;
+      rec[i] = lse - p.score.capl;             // capl: 0 without a cap
+      rec[kRowTile + i] = -delta;
+      rec[2 * kRowTile + i] = (float)m;
+      rec[3 * kRowTile + i] = slope;
     }
   }
 }
@@ -104,28 +116,41 @@ struct DsScale {
   }
 };
 
+// P and dS of one product s and dP - delta; `lse` is a record's.
+template <bool CAP>
+struct Pair { float x, der; };
+template <bool CAP>
+__device__ __forceinline__ Pair<CAP> log_weight(float s, float lse, const ScoreArgs& a) {
+  if constexpr (CAP) {
+    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * a.ce));
+    return {__builtin_fmaf(r, -2.0f * a.capl, -lse), __builtin_fmaf(-r, r, r)};   // der: a quarter of it
+  } else {
+    return {__builtin_fmaf(s, a.c1, -lse), 1.0f};
+  }
+}
+
 template <int HD>
 struct RowSlot {
-  uint16_t q[kMTile * HD];
-  uint16_t d[kMTile * HD];
+  uint16_t q[kRowTile * HD];
+  uint16_t d[kRowTile * HD];
   float st[kRec];
 };
 
 template <int HD, bool F16, bool CAP, bool SLOPE>
 __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_kernel(BwdArgs p) {
   constexpr int KS = HD / 16, DB = HD / 32, CH = HD / 8;
-  constexpr int DJ = kMTile * CH / kMThreads;
+  constexpr int DJ = kRowTile * CH / kMThreads;
   __shared__ __attribute__((aligned(16))) RowSlot<HD> r0, r1, r2, r3;
-  __shared__ __attribute__((aligned(16))) float sink[64];
   __shared__ int range[2][kMWaves];
 
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int blocks = (p.mask.N + kMRows - 1) / kMRows;
+  const int half = wave >> 1;                  // of a row tile
+  const int blocks = (p.mask.N + kKeys - 1) / kKeys;
   int kb, prob;
   item_of(blockIdx.x, blocks, gridDim.x / blocks, kb, prob);
   const int b = prob / p.Hk, kvh = prob % p.Hk;
-  const int j = kb * kMRows + wave * 32 + l32;
+  const int j = kb * kKeys + (wave & 1) * 32 + l32;
   const bool live = j < p.mask.N;
   const int jc = live ? j : p.mask.N - 1;
   const KeySpan ks_ = key_span(p.mask, b, jc);
@@ -170,15 +195,16 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   }
   n_lo = __builtin_amdgcn_readfirstlane(n_lo);
   n_hi = __builtin_amdgcn_readfirstlane(n_hi);
-  const int t_begin = n_hi > n_lo ? n_lo / 32 : 0, t_end = n_hi > n_lo ? (n_hi + 31) / 32 : 0;
+  const int t_begin = n_hi > n_lo ? n_lo / kRowTile : 0;
+  const int t_end = n_hi > n_lo ? (n_hi + kRowTile - 1) / kRowTile : 0;
 
-  // Rows of a tile: token and head of row 32 t + i follow from (32 t) / G; where
-  // G divides 32 the offsets inside a tile are the same for all tiles.
+  // Rows of a tile: token and head of row 64 t + i follow from (64 t) / G; where
+  // G divides 64 the offsets inside a tile are the same for all tiles.
   const uint16_t* Q = p.q + b * p.q_sb + (int64_t)kvh * p.G * p.q_sh;
   const uint16_t* D = p.d_o + b * p.do_sb + (int64_t)kvh * p.G * p.do_sh;
-  const bool even = 32 % p.G == 0;
+  const bool even = kRowTile % p.G == 0;
   uint32_t q_voff[DJ], d_voff[DJ];
-  auto offsets = [&](int first) {              // first: (32 t) % G
+  auto offsets = [&](int first) {              // first: (64 t) % G
 #pragma unroll
     for (int i = 0; i < DJ; ++i) {
       const int pos = (wave * DJ + i) * 64 + lane, row = pos / CH;
@@ -191,13 +217,13 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   offsets(0);
   const float* rec = p.rec + (int64_t)prob * p.tiles * kRec;
   auto issue = [&](int t, RowSlot<HD>& T) {
-    const int base = min(t, p.tiles) * 32;     // tiles past the rows: all lanes idle
+    const int base = min(t, p.tiles) * kRowTile;   // tiles past the rows: all lanes idle
     if (!even) offsets(base % p.G);
     const int64_t tok = base / p.G;
     const __amdgpu_buffer_rsrc_t qr = make_rsrc(Q + tok * p.q_sm, kNoRow);
     const __amdgpu_buffer_rsrc_t dr = make_rsrc(D + tok * p.do_sm, kNoRow);
-    const __amdgpu_buffer_rsrc_t rr = make_rsrc(rec + (int64_t)base / 32 * kRec, kRec * 4);
     const int left = p.R - base;
+    const __amdgpu_buffer_rsrc_t rr = make_rsrc(rec + (int64_t)base / kRowTile * kRec, left > 0 ? kRec * 4 : 0);
 #pragma unroll
     for (int i = 0; i < DJ; ++i) {
       const bool in = ((wave * DJ + i) * 64 + lane) / CH < left;
@@ -208,10 +234,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
       const bool in = ((wave * DJ + i) * 64 + lane) / CH < left;
       m_dma16(dr, &T.d[(wave * DJ + i) * 512], in ? d_voff[i] : kNoRow);
     }
-    // Waves 0 and 1 fetch the record; 2 and 3 land zeros beside it, so that
-    // every wave waits for the same number of DMAs.
-    m_dma4(rr, wave < 2 ? &T.st[wave * 64] : &sink[0],
-           wave < 2 && left > 0 ? (uint32_t)(wave * 64 + lane) * 4u : kNoRow);
+    m_dma4(rr, &T.st[wave * 64], (uint32_t)(wave * 64 + lane) * 4u);
   };
 
   f32x16 dk[DB], dv[DB];
@@ -221,46 +244,49 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
 #pragma unroll
     for (int db = 0; db < DB; ++db) dk[db] = dv[db] = f32x16{};
   };
-
-  // P and dS of the tile's rows (registers) and this lane's key.
-  auto weights = [&](const RowSlot<HD>& T, int row0, bool edge, float (&w)[16], float (&ds)[16]) {
-    f32x16 s{}, dp;
+  // S and dP - delta of the rows of this wave's half (registers) and this lane's key.
+  auto products = [&](const RowSlot<HD>& T, f32x16& s, f32x16& dp) {
+    s = f32x16{};
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const f32x4 nd = *reinterpret_cast<const f32x4*>(&T.st[32 + 8 * g + 4 * hi]);
+      const f32x4 nd = *reinterpret_cast<const f32x4*>(&T.st[kRowTile + half * 32 + 8 * g + 4 * hi]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * g + e] = nd[e];
     }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      s = mfma32x32x16_t<F16>(row_frag<HD>(T.q, ks, l32, hi), kf[ks], s);
-      dp = mfma32x32x16_t<F16>(row_frag<HD>(T.d, ks, l32, hi), vf[ks], dp);
+      s = mfma32x32x16_t<F16>(row_frag<HD>(T.q + half * 32 * HD, ks, l32, hi), kf[ks], s);
+      dp = mfma32x32x16_t<F16>(row_frag<HD>(T.d + half * 32 * HD, ks, l32, hi), vf[ks], dp);
     }
-    const int from = lo - row0 - 4 * hi, to = hi_r - row0 - 4 * hi;
+  };
+  // P and dS.
+  auto weights = [&](const RowSlot<HD>& T, const f32x16& s, const f32x16& dp, int row0, bool edge,
+                     float (&w)[16], float (&ds)[16]) {
+    const float* st = &T.st[half * 32 + 4 * hi];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const f32x4 ls = *reinterpret_cast<const f32x4*>(&T.st[8 * g + 4 * hi]);
+      const f32x4 ls = *reinterpret_cast<const f32x4*>(&st[8 * g]);
       f32x4 tok, sl;
       if constexpr (SLOPE) {
-        tok = *reinterpret_cast<const f32x4*>(&T.st[64 + 8 * g + 4 * hi]);
-        sl = *reinterpret_cast<const f32x4*>(&T.st[96 + 8 * g + 4 * hi]);
+        tok = *reinterpret_cast<const f32x4*>(&st[2 * kRowTile + 8 * g]);
+        sl = *reinterpret_cast<const f32x4*>(&st[3 * kRowTile + 8 * g]);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * g + e;
-        float t = 0.f, x;
-        if constexpr (CAP) {
-          t = cap_tanh(s[i], p.score.ce);
-          x = t * p.score.capl;
-        } else {
-          x = s[i] * p.score.c1;
-        }
+        const Pair<CAP> y = log_weight<CAP>(s[i], ls[e], p.score);
+        float x = y.x;
         if constexpr (SLOPE) x = __builtin_fmaf(-sl[e], fabsf(tok[e] + shift), x);
-        w[i] = __builtin_amdgcn_exp2f(x - ls[e]);
+        w[i] = __builtin_amdgcn_exp2f(x);
         ds[i] = w[i] * dp[i];
-        if constexpr (CAP) ds[i] *= __builtin_fmaf(-t, t, 1.0f);
-        if (edge && (mfma_row(i, 0) < from || mfma_row(i, 0) >= to)) w[i] = ds[i] = 0.f;
+        if constexpr (CAP) ds[i] *= y.der;
       }
+    }
+    if (edge) {
+      const int from = lo - row0 - 4 * hi, to = hi_r - row0 - 4 * hi;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (mfma_row(i, 0) < from || mfma_row(i, 0) >= to) w[i] = ds[i] = 0.f;
     }
     if constexpr (F16) {
       float ratio;
@@ -276,37 +302,46 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
     }
   };
 
-  auto iter = [&](int t, const RowSlot<HD>& cur, RowSlot<HD>& dst) {
-    m_wait<2 * (2 * DJ + 1)>();
-    __syncthreads();
+  f32x16 s, dp;
+  auto iter = [&](int t, const RowSlot<HD>& cur, const RowSlot<HD>& nxt, RowSlot<HD>& dst) {
+    m_wait<2 * DJ + 1>();                      // tile t + 1 landed (tile t + 2 in flight)
+    __syncthreads();                           // ... for every wave; `dst` is free
     issue(t + 3, dst);
-    const int row0 = t * 32;
-    if (row0 >= w_hi || row0 + 32 <= w_lo) return;
-    float w[16], ds[16];
-    weights(cur, row0, row0 < a_lo || row0 + 32 > a_hi, w, ds);
-    bf16x8 wb[2], db_[2];
-    pack_frags<F16>(w, wb);
-    pack_frags<F16>(ds, db_);
+    f32x16 s_next, dp_next;
+    products(nxt, s_next, dp_next);
+    const int row0 = t * kRowTile + half * 32;
+    if (row0 < w_hi && row0 + 32 > w_lo) {
+      float w[16], ds[16];
+      weights(cur, s, dp, row0, row0 < a_lo || row0 + 32 > a_hi, w, ds);
+      bf16x8 wb[2], db_[2];
+      pack_frags<F16>(w, wb);
+      pack_frags<F16>(ds, db_);
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        dv[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.d, lane, db, s), wb[s], dv[db]);
-        dk[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.q, lane, db, s), db_[s], dk[db]);
-      }
+        for (int i = 0; i < 2; ++i) {
+          dv[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.d + half * 32 * HD, lane, db, i), wb[i], dv[db]);
+          dk[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.q + half * 32 * HD, lane, db, i), db_[i], dk[db]);
+        }
+    }
+    s = s_next;
+    dp = dp_next;
   };
   restart();
   issue(t_begin, r0);
   issue(t_begin + 1, r1);
   issue(t_begin + 2, r2);
+  m_wait<2 * (2 * DJ + 1)>();
+  __syncthreads();
+  products(r0, s, dp);
   for (int t = t_begin; t < t_end; t += 4) {
-    iter(t, r0, r3);
+    iter(t, r0, r1, r3);
     if (t + 1 >= t_end) break;
-    iter(t + 1, r1, r0);
+    iter(t + 1, r1, r2, r0);
     if (t + 2 >= t_end) break;
-    iter(t + 2, r2, r1);
+    iter(t + 2, r2, r3, r1);
     if (t + 3 >= t_end) break;
-    iter(t + 3, r3, r2);
+    iter(t + 3, r3, r0, r2);
   }
   m_wait<0>();
 
@@ -323,9 +358,10 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
       issue(t, r0);
       m_wait<0>();
       __syncthreads();
-      const int row0 = t * 32, from = lo - row0 - 4 * hi, to = hi_r - row0 - 4 * hi;
+      const int row0 = t * kRowTile + half * 32, from = lo - row0 - 4 * hi, to = hi_r - row0 - 4 * hi;
       float w[16], ds[16], sx[16];
-      weights(r0, row0, true, w, ds);
+      products(r0, s, dp);
+      weights(r0, s, dp, row0, true, w, ds);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         sx[i] = mfma_row(i, 0) < from || mfma_row(i, 0) >= to ? 0.f : 1.f;
@@ -335,14 +371,49 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
       pack_frags<F16>(sx, sb);
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        dv[db] = careful_mfma<HD, F16>(r0.d, lane, db, wb, sb, dv[db]);
-        dk[db] = careful_mfma<HD, F16>(r0.q, lane, db, db_, sb, dk[db]);
+        dv[db] = careful_mfma<HD, F16>(r0.d + half * 32 * HD, lane, db, wb, sb, dv[db]);
+        dk[db] = careful_mfma<HD, F16>(r0.q + half * 32 * HD, lane, db, db_, sb, dk[db]);
       }
     }
+    __syncthreads();
   }
-  if (!live) return;
-  const float kx = F16 ? (sc.s == 0.f ? 0.f : p.sm_scale / sc.s) : p.sm_scale;
+
+  // The second half's sums by way of the ring, slots of 16 bytes a lane.
+  const float kx = (CAP ? 4.0f : 1.0f) * p.sm_scale * (F16 ? (sc.s == 0.f ? 0.f : 1.0f / sc.s) : 1.0f);
   const float vx = F16 ? 1.0f / kPScale : 1.0f;
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    dk[db] *= kx;
+    dv[db] *= vx;
+  }
+  static_assert(sizeof(RowSlot<HD>) >= 2 * DB * 4 * 64 * 16, "two waves' sums of one tensor in a slot");
+  auto give = [&](uint16_t* to, const f32x16 (&v)[DB]) {
+    f32x4* at = reinterpret_cast<f32x4*>(to) + (wave & 1) * DB * 4 * 64 + lane;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        at[(db * 4 + g) * 64] = f32x4{v[db][4 * g], v[db][4 * g + 1], v[db][4 * g + 2], v[db][4 * g + 3]};
+  };
+  auto take = [&](const uint16_t* from, f32x16 (&v)[DB]) {
+    const f32x4* at = reinterpret_cast<const f32x4*>(from) + (wave & 1) * DB * 4 * 64 + lane;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = at[(db * 4 + g) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[db][4 * g + e] += x[e];
+      }
+  };
+  if (half == 1) {
+    give(r0.q, dk);
+    give(r1.q, dv);
+  }
+  __syncthreads();
+  if (half == 1 || !live) return;
+  take(r0.q, dk);
+  take(r1.q, dv);
   uint16_t* DK = p.dk + b * p.dk_sb + kvh * p.dk_sh + j * p.dk_sn;
   uint16_t* DV = p.dv + b * p.dv_sb + kvh * p.dv_sh + j * p.dv_sn;
 #pragma unroll
@@ -350,10 +421,10 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int at = db * 32 + 8 * g + 4 * hi;
-      const bf16x2 k0 = pack2<F16>(dk[db][4 * g] * kx, dk[db][4 * g + 1] * kx);
-      const bf16x2 k1 = pack2<F16>(dk[db][4 * g + 2] * kx, dk[db][4 * g + 3] * kx);
-      const bf16x2 v0 = pack2<F16>(dv[db][4 * g] * vx, dv[db][4 * g + 1] * vx);
-      const bf16x2 v1 = pack2<F16>(dv[db][4 * g + 2] * vx, dv[db][4 * g + 3] * vx);
+      const bf16x2 k0 = pack2<F16>(dk[db][4 * g], dk[db][4 * g + 1]);
+      const bf16x2 k1 = pack2<F16>(dk[db][4 * g + 2], dk[db][4 * g + 3]);
+      const bf16x2 v0 = pack2<F16>(dv[db][4 * g], dv[db][4 * g + 1]);
+      const bf16x2 v1 = pack2<F16>(dv[db][4 * g + 2], dv[db][4 * g + 3]);
       *reinterpret_cast<u32x2*>(DK + at) =
           u32x2{__builtin_bit_cast(uint32_t, k0), __builtin_bit_cast(uint32_t, k1)};
       *reinterpret_cast<u32x2*>(DV + at) =
@@ -368,7 +439,7 @@ struct KeySlot {
 };
 
 template <int HD, bool F16, bool CAP, bool SLOPE>
-__global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_kernel(BwdArgs p) {
+__global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p) {
   constexpr int KS = HD / 16, DB = HD / 32, CH = HD / 8;
   constexpr int DJ = kMTile * CH / kMThreads;
   __shared__ __attribute__((aligned(16))) KeySlot<HD> r0, r1, r2, r3;
@@ -386,8 +457,8 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_ke
   const int rc = live ? r : p.R - 1;
   const int m_tok = rc / p.G, h = kvh * p.G + rc % p.G;
   const RowSpan span = row_span(p.mask, b, m_tok);
-  const float* rec = p.rec + ((int64_t)prob * p.tiles + rc / 32) * kRec + rc % 32;
-  const float lse = rec[0], ndelta = rec[32], slope = SLOPE ? rec[96] : 0.f;
+  const float* rec = p.rec + ((int64_t)prob * p.tiles + rc / kRowTile) * kRec + rc % kRowTile;
+  const float lse = rec[0], ndelta = rec[kRowTile], slope = SLOPE ? rec[3 * kRowTile] : 0.f;
 
   bf16x8 qf[KS], df[KS];
   {
@@ -457,8 +528,8 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_ke
 #pragma unroll
     for (int db = 0; db < DB; ++db) dq[db] = f32x16{};
   };
-  auto weights = [&](const KeySlot<HD>& T, int n0, bool edge, float (&ds)[16]) {
-    f32x16 s{}, dp;
+  auto products = [&](const KeySlot<HD>& T, f32x16& s, f32x16& dp) {
+    s = f32x16{};
 #pragma unroll
     for (int i = 0; i < 16; ++i) dp[i] = ndelta;
 #pragma unroll
@@ -466,21 +537,22 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_ke
       s = mfma32x32x16_t<F16>(row_frag<HD>(T.k, ks, l32, hi), qf[ks], s);
       dp = mfma32x32x16_t<F16>(row_frag<HD>(T.v, ks, l32, hi), df[ks], dp);
     }
+  };
+  auto weights = [&](const f32x16& s, const f32x16& dp, int n0, bool edge, float (&ds)[16]) {
     const float dist = (float)(span.at - n0 - 4 * hi);
-    const int from = span.lo - n0 - 4 * hi, to = span.hi - n0 - 4 * hi;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float t = 0.f, x;
-      if constexpr (CAP) {
-        t = cap_tanh(s[i], p.score.ce);
-        x = t * p.score.capl;
-      } else {
-        x = s[i] * p.score.c1;
-      }
+      const Pair<CAP> y = log_weight<CAP>(s[i], lse, p.score);
+      float x = y.x;
       if constexpr (SLOPE) x = __builtin_fmaf(-slope, fabsf(dist - (float)mfma_row(i, 0)), x);
-      ds[i] = __builtin_amdgcn_exp2f(x - lse) * dp[i];
-      if constexpr (CAP) ds[i] *= __builtin_fmaf(-t, t, 1.0f);
-      if (edge && (mfma_row(i, 0) < from || mfma_row(i, 0) >= to)) ds[i] = 0.f;
+      ds[i] = __builtin_amdgcn_exp2f(x) * dp[i];
+      if constexpr (CAP) ds[i] *= y.der;
+    }
+    if (edge) {
+      const int from = span.lo - n0 - 4 * hi, to = span.hi - n0 - 4 * hi;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (mfma_row(i, 0) < from || mfma_row(i, 0) >= to) ds[i] = 0.f;
     }
     if constexpr (F16) {
       float ratio;
@@ -492,34 +564,43 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_ke
       for (int i = 0; i < 16; ++i) ds[i] *= sc.s;
     }
   };
-  auto iter = [&](int t, const KeySlot<HD>& cur, KeySlot<HD>& dst) {
-    m_wait<4 * DJ>();
+  f32x16 s, dp;
+  auto iter = [&](int t, const KeySlot<HD>& cur, const KeySlot<HD>& nxt, KeySlot<HD>& dst) {
+    m_wait<2 * DJ>();                          // tile t + 1 landed (tile t + 2 in flight)
     __syncthreads();
     issue(t + 3, dst);
+    f32x16 s_next, dp_next;
+    products(nxt, s_next, dp_next);
     const int n0 = n_lo + t * kMTile;
-    if (n0 >= w_hi || n0 + kMTile <= w_lo) return;
-    float ds[16];
-    weights(cur, n0, n0 < a_lo || n0 + kMTile > a_hi, ds);
-    bf16x8 db_[2];
-    pack_frags<F16>(ds, db_);
+    if (n0 < w_hi && n0 + kMTile > w_lo) {
+      float ds[16];
+      weights(s, dp, n0, n0 < a_lo || n0 + kMTile > a_hi, ds);
+      bf16x8 db_[2];
+      pack_frags<F16>(ds, db_);
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        dq[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.k, lane, db, s), db_[s], dq[db]);
+        for (int i = 0; i < 2; ++i)
+          dq[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.k, lane, db, i), db_[i], dq[db]);
+    }
+    s = s_next;
+    dp = dp_next;
   };
   restart();
   issue(0, r0);
   issue(1, r1);
   issue(2, r2);
+  m_wait<4 * DJ>();
+  __syncthreads();
+  products(r0, s, dp);
   for (int t = 0; t < t_end; t += 4) {
-    iter(t, r0, r3);
+    iter(t, r0, r1, r3);
     if (t + 1 >= t_end) break;
-    iter(t + 1, r1, r0);
+    iter(t + 1, r1, r2, r0);
     if (t + 2 >= t_end) break;
-    iter(t + 2, r2, r1);
+    iter(t + 2, r2, r3, r1);
     if (t + 3 >= t_end) break;
-    iter(t + 3, r3, r2);
+    iter(t + 3, r3, r0, r2);
   }
   m_wait<0>();
 
@@ -537,7 +618,8 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_ke
       __syncthreads();
       const int n0 = n_lo + t * kMTile, from = span.lo - n0 - 4 * hi, to = span.hi - n0 - 4 * hi;
       float ds[16], sx[16];
-      weights(r0, n0, true, ds);
+      products(r0, s, dp);
+      weights(s, dp, n0, true, ds);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         sx[i] = mfma_row(i, 0) < from || mfma_row(i, 0) >= to ? 0.f : 1.f;
@@ -549,7 +631,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_ke
     }
   }
   if (!live) return;
-  const float x = F16 ? (sc.s == 0.f ? 0.f : p.sm_scale / sc.s) : p.sm_scale;
+  const float x = (CAP ? 4.0f : 1.0f) * p.sm_scale * (F16 ? (sc.s == 0.f ? 0.f : 1.0f / sc.s) : 1.0f);
   uint16_t* DQ = p.dq + b * p.dq_sb + h * p.dq_sh + m_tok * p.dq_sm;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -564,7 +646,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dq_ke
 
 template <int HD, bool F16, bool CAP, bool SLOPE>
 hipError_t launch_one(const BwdArgs& a, int64_t problems, hipStream_t s) {
-  const int64_t kb = (a.mask.N + kMRows - 1) / kMRows, qb = (a.R + kMRows - 1) / kMRows;
+  const int64_t kb = (a.mask.N + kKeys - 1) / kKeys, qb = (a.R + kMRows - 1) / kMRows;
   if (kb > 0)
     hipLaunchKernelGGL((attn_masked_dkdv_kernel<HD, F16, CAP, SLOPE>), dim3((unsigned)(kb * problems)),
                        dim3(kMThreads), 0, s, a);
@@ -594,7 +676,7 @@ using namespace gpa;
 
 extern "C" size_t gpa_attn_masked_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t M) {
   if (B <= 0 || H <= 0 || Hk <= 0 || M <= 0 || H % Hk) return 0;
-  return (size_t)B * Hk * ((H / Hk * M + 31) / 32) * kRec * sizeof(float);
+  return (size_t)B * Hk * ((H / Hk * M + kRowTile - 1) / kRowTile) * kRec * sizeof(float);
 }
 
 extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* args,
@@ -633,16 +715,16 @@ extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* args,
     return GPA_E_INVALID;
   }
   const int64_t G = a->H / a->Hk, problems = a->B * a->Hk;
-  // A tile's 32 rows (at most 33 tokens, G heads) by 32-bit offsets below kNoRow.
+  // A tile's 64 rows (at most 65 tokens, G heads) by 32-bit offsets below kNoRow.
   for (int i = 0; i < 2; ++i) {
     const int64_t sm = a->M < 2 ? a->D : i ? g->do_sm : a->q_sm, sh = G < 2 ? 0 : i ? g->do_sh : a->q_sh;
-    if (sm < 0 || sh < 0 || (G - 1) * sh + 33 * sm + a->D >= (int64_t)1 << 29) {
+    if (sm < 0 || sh < 0 || (G - 1) * sh + (kRowTile + 1) * sm + a->D >= (int64_t)1 << 29) {
       gpa_set_error("%s: the query heads of a key head span 2^29 elements or more", fn);
       return GPA_E_UNSUPPORTED;
     }
   }
-  const int64_t tiles = (a->M * G + 31) / 32, kb = (a->N + kMRows - 1) / kMRows;
-  if (problems * std::max(tiles, kb) > 0x7fffffff) {
+  const int64_t tiles = (a->M * G + kRowTile - 1) / kRowTile, kb = (a->N + kKeys - 1) / kKeys;
+  if (problems * std::max({tiles, kb, (a->M * G + kMRows - 1) / kMRows}) > 0x7fffffff) {
     gpa_set_error("%s: too many rows", fn);
     return GPA_E_UNSUPPORTED;
   }

@@ -553,7 +553,7 @@ int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void* workspace
  * (NULL: none; contiguous [B, H, M]): dq, dk and dv in the operands' format,
  * those of a shared key head summed over its query heads.  No shared prefix
  * (P = 0, lens = NULL).  Sums run in a fixed order: two calls give the same
- * bits.  A batch element's query heads of one key head, and 32 tokens, span
+ * bits.  A batch element's query heads of one key head, and 65 tokens, span
  * less than 2^29 elements of q and of d_o.  workspace:
  * gpa_attn_masked_bwd_workspace_bytes(...), 16-byte aligned.
  */

@@ -60,7 +60,7 @@ def test_null_arguments_and_workspace_alignment():
     assert need > 0 and _forward(N=100_000, ws=FAKE + 4, ws_bytes=need) == WSP
     assert _forward(N=100_000, ws=FAKE, ws_bytes=need - 1) == WSP
     assert L.gpa_attn_masked_workspace_bytes(2, 4, 2, 10, 10, 0, 64) == 0
-    assert L.gpa_attn_masked_bwd_workspace_bytes(2, 4, 2, 10) == 2 * 2 * 1 * 128 * 4
+    assert L.gpa_attn_masked_bwd_workspace_bytes(2, 4, 2, 10) == 2 * 2 * 1 * 256 * 4
 
 
 def test_nothing_to_do_is_ok():
