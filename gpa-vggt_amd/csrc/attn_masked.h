@@ -185,30 +185,49 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint16_t* base
   return make_rsrc(base + (int64_t)row * stride, bytes);
 }
 
-// The A operand of a product over the tile's features: lane (hi, l32) has
-// row l32, features 16 ks + 8 hi .. +7.
+// Reads of a tile's operands.  A lane's offsets inside a tile are kept, and the
+// tile's own place goes into the instructions' offset fields: `fresh`, once a
+// tile, keeps the compiler from holding the sums of both in registers (a set of
+// them for each of the ring's slots).
 template <int HD>
-__device__ __forceinline__ bf16x8 row_frag(const uint16_t* t, int ks, int l32, int hi) {
-  return *reinterpret_cast<const bf16x8*>(&t[tile_at<HD>(l32, 2 * ks + hi)]);
-}
-
-// The A operand of a product over the tile's rows, transposed: lane (hi, l32)
-// has feature 32 db + l32 of the rows 16 s + 8 e + 4 hi + 0 .. 3 (e = 0, 1), the
-// order in which the score MFMA's result registers hold them, so that its
-// results are the B operand as they stand.
-template <int HD>
-__device__ __forceinline__ bf16x8 tr_frag(const uint16_t* t, int lane, int db, int s) {
-  typedef short i16x4 __attribute__((ext_vector_type(4)));
-  const int hi = lane >> 5, v4 = (lane & 15) >> 2, a = lane & 3, bit4 = (lane >> 4) & 1;
-  const int chunk = 4 * db + 2 * bit4 + (a >> 1);
-  const int row = 16 * s + 4 * hi + v4;
-  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (__attribute__((address_space(3))) i16x4*)&t[tile_at<HD>(row, chunk) + (a & 1) * 4]);
-  const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (__attribute__((address_space(3))) i16x4*)&t[tile_at<HD>(row + 8, chunk) + (a & 1) * 4]);
-  const bf16x4 l4 = __builtin_bit_cast(bf16x4, lo), u4 = __builtin_bit_cast(bf16x4, up);
-  return bf16x8{l4[0], l4[1], l4[2], l4[3], u4[0], u4[1], u4[2], u4[3]};
-}
+struct TileReader {
+  uint32_t row[HD / 16], tr[HD / 32][2];       // bytes
+  __device__ __forceinline__ explicit TileReader(int lane) {
+    const int hi = lane >> 5, l32 = lane & 31, v4 = (lane & 15) >> 2, a = lane & 3, bit4 = (lane >> 4) & 1;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) row[ks] = 2 * tile_at<HD>(l32, 2 * ks + hi);
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        tr[db][e] = 2 * (tile_at<HD>(8 * e + 4 * hi + v4, 4 * db + 2 * bit4 + (a >> 1)) + (a & 1) * 4);
+  }
+  __device__ __forceinline__ void fresh() {
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) asm volatile("" : "+v"(row[ks]));
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db) asm volatile("" : "+v"(tr[db][0]), "+v"(tr[db][1]));
+  }
+  typedef __attribute__((address_space(3))) const char* lds_ptr;
+  static __device__ __forceinline__ lds_ptr lds(const uint16_t* t) { return (lds_ptr)t; }
+  // The A operand of a product over the tile's features: lane (hi, l32) has row
+  // l32, features 16 ks + 8 hi .. +7.
+  __device__ __forceinline__ bf16x8 rows(const uint16_t* t, int ks) const {
+    return *reinterpret_cast<__attribute__((address_space(3))) const bf16x8*>(lds(t) + row[ks]);
+  }
+  // The A operand of a product over the tile's rows, transposed: lane (hi, l32)
+  // has feature 32 db + l32 of the rows 16 s + 8 e + 4 hi + 0 .. 3 (e = 0, 1), the
+  // order in which the score MFMA's result registers hold them, so that its
+  // results are the B operand as they stand.
+  __device__ __forceinline__ bf16x8 turned(const uint16_t* t, int db, int s) const {
+    typedef short i16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) i16x4* tr_ptr;
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(lds(t) + tr[db][0] + 32 * s * HD));
+    const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(lds(t) + tr[db][1] + 32 * s * HD));
+    const bf16x4 l4 = __builtin_bit_cast(bf16x4, lo), u4 = __builtin_bit_cast(bf16x4, up);
+    return bf16x8{l4[0], l4[1], l4[2], l4[3], u4[0], u4[1], u4[2], u4[3]};
+  }
+};
 
 // Sixteen fp32 values of a lane as the B operand's two fragments.
 template <bool F16>
@@ -228,7 +247,7 @@ __device__ __forceinline__ void pack_frags(const float (&p)[16], bf16x8 (&out)[2
 // the product and the rows that do see them get them back by their sign: an
 // indicator product over the seen rows tells which (both signs: NaN).
 template <int HD, bool F16>
-__device__ __forceinline__ f32x16 careful_mfma(const uint16_t* t, int lane, int db,
+__device__ __forceinline__ f32x16 careful_mfma(const TileReader<HD>& rd, const uint16_t* t, int db,
                                                const bf16x8 (&p)[2], const bf16x8 (&seen)[2],
                                                f32x16 acc) {
   const uint16_t expo = F16 ? 0x7c00 : 0x7f80, one = F16 ? 0x3c00 : 0x3f80;
@@ -237,7 +256,7 @@ __device__ __forceinline__ f32x16 careful_mfma(const uint16_t* t, int lane, int 
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-    u16x8 x = __builtin_bit_cast(u16x8, tr_frag<HD>(t, lane, db, s)), xp, xn;
+    u16x8 x = __builtin_bit_cast(u16x8, rd.turned(t, db, s)), xp, xn;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint16_t w = x[e];

@@ -117,15 +117,16 @@ template <int HD, bool F16, bool CAP, bool SLOPE>
 struct Rows {
   static constexpr int KS = HD / 16, DB = HD / 32;
   const ScoreArgs& sc;
-  const int lane, hi, l32;
+  TileReader<HD> rd;
+  const int hi;
   int lo, end, at;
   float slope;
   bf16x8 qf[KS];
   f32x16 o[DB];
   float m, l;
 
-  __device__ __forceinline__ Rows(const FwdArgs& p, const Row& x, int lane_)
-      : sc(p.score), lane(lane_), hi(lane_ >> 5), l32(lane_ & 31), lo(x.lo), end(x.hi), at(x.at), slope(0.f) {
+  __device__ __forceinline__ Rows(const FwdArgs& p, const Row& x, int lane)
+      : sc(p.score), rd(lane), hi(lane >> 5), lo(x.lo), end(x.hi), at(x.at), slope(0.f) {
     if constexpr (SLOPE) slope = p.slopes[x.b * p.slopes_sb + x.h] * kMLog2e;
     const uint16_t* Q = p.q + x.b * p.q_sb + x.h * p.q_sh + x.tok * p.q_sm;
 #pragma unroll
@@ -141,24 +142,13 @@ struct Rows {
   __device__ __forceinline__ f32x16 products(const uint16_t* k) const {
     f32x16 s{};
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = mfma32x32x16_t<F16>(row_frag<HD>(k, ks, l32, hi), qf[ks], s);
+    for (int ks = 0; ks < KS; ++ks) s = mfma32x32x16_t<F16>(rd.rows(k, ks), qf[ks], s);
     return s;
   }
-  __device__ __forceinline__ void masked(float (&x)[16], int n0) const {
-    const int from = lo - n0 - 4 * hi, to = end - n0 - 4 * hi;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (mfma_row(i, 0) < from || mfma_row(i, 0) >= to) x[i] = -INFINITY;
-  }
-  __device__ __forceinline__ void sloped(float (&x)[16], int n0) const {
-    if constexpr (SLOPE) {
-      const float dist = (float)(at - n0 - 4 * hi);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(-slope, fabsf(dist - (float)mfma_row(i, 0)), x[i]);
-    }
-  }
-  // Scores in log2 units, -inf where the row does not see the key, less `off`.
-  __device__ __forceinline__ void scores(const f32x16& s, int n0, bool edge, bool poly, float off, float (&x)[16]) const {
+  // Scores in log2 units, less `off`.  (AHEAD: the distances are formed anew, so that
+  // the two uses in a tile share no values, which would live across a branch.)
+  template <bool AHEAD>
+  __device__ __forceinline__ void scores(const f32x16& s, int n0, bool poly, float off, float (&x)[16]) const {
     if (!CAP) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(s[i], sc.c1, -off);
@@ -169,36 +159,58 @@ struct Rows {
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(cap_tanh(s[i], sc.ce), sc.capl, -off);
     }
-    sloped(x, n0);
-    if (edge) masked(x, n0);
+    if constexpr (SLOPE) {
+      int own = at;
+      if constexpr (AHEAD) asm volatile("" : "+v"(own));
+      const float dist = (float)(own - n0 - 4 * hi);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(-slope, fabsf(dist - (float)mfma_row(i, 0)), x[i]);
+    }
   }
-  // Products to weights.  Where a tile's largest |product| does not tell that all
+  // `none` where the row does not see the key.
+  __device__ __forceinline__ void masked(float (&x)[16], int n0, float none) const {
+    const int from = lo - n0 - 4 * hi, to = end - n0 - 4 * hi;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (mfma_row(i, 0) < from || mfma_row(i, 0) >= to) x[i] = none;
+  }
+  // Before a tile's weights: where its largest |product| does not tell that all
   // scores lie below the offset's reach, the offset follows the row's maximum, and
-  // the sum and the output with it.
-  __device__ __forceinline__ void weigh(const f32x16& s, int n0, bool edge, float (&x)[16]) {
+  // the sum and the output with it (two branches, the second with nothing but the
+  // scaling: as one, the outputs had other registers after it, and every tile that
+  // took the other way copied them, 32 moves).  Whether the polynomial serves all
+  // products.
+  __device__ __forceinline__ bool settle(const f32x16& s, int n0, bool edge) {
     float a = fmaxf(fabsf(s[0]), fabsf(s[1]));
 #pragma unroll
     for (int i = 2; i < 16; i += 2) a = fmaxf(fmaxf(a, fabsf(s[i])), fabsf(s[i + 1]));
     const bool poly = CAP && __builtin_amdgcn_ballot_w64(!(a <= sc.lim)) == 0;
+    float m_new = m;
     if (__builtin_amdgcn_ballot_w64(!(a * sc.c1 <= m + kUp<F16>))) {
-      scores(s, n0, edge, poly, 0.f, x);
+      float x[16];
+      scores<true>(s, n0, poly, 0.f, x);
+      if (edge) masked(x, n0, -INFINITY);
       float mx = x[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
       mx = max_halves(mx);
-      const float m_new = mx > m + kUp<F16> ? mx : m;
+      if (mx > m + kUp<F16>) m_new = mx;
+    }
+    if (__builtin_amdgcn_ballot_w64(m_new != m)) {
       const float alpha = __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
       l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
     }
-    scores(s, n0, edge, poly, m, x);
+    return poly;
+  }
+  __device__ __forceinline__ void weigh(int n0, bool edge, float (&x)[16]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[i] = __builtin_amdgcn_exp2f(x[i]);
-      l += x[i];
-    }
+    for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(x[i]);
+    if (edge) masked(x, n0, 0.f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) l += x[i];
   }
   __device__ __forceinline__ void add(const uint16_t* v, const float (&x)[16]) {
     bf16x8 pb[2];
@@ -206,12 +218,15 @@ struct Rows {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) o[db] = mfma32x32x16_t<F16>(tr_frag<HD>(v, lane, db, s), pb[s], o[db]);
+      for (int s = 0; s < 2; ++s) o[db] = mfma32x32x16_t<F16>(rd.turned(v, db, s), pb[s], o[db]);
   }
   // A tile whose values may hold infinities or NaN that a row does not see.
   __device__ __forceinline__ void careful(const uint16_t* k, const uint16_t* v, int n0) {
     float x[16], seen[16];
-    weigh(products(k), n0, true, x);
+    const f32x16 s = products(k);
+    const bool poly = settle(s, n0, true);
+    scores<false>(s, n0, poly, m, x);
+    weigh(n0, true, x);
     const int from = lo - n0 - 4 * hi, to = end - n0 - 4 * hi;
 #pragma unroll
     for (int i = 0; i < 16; ++i) seen[i] = mfma_row(i, 0) < from || mfma_row(i, 0) >= to ? 0.f : 1.f;
@@ -219,7 +234,7 @@ struct Rows {
     pack_frags<F16>(x, pb);
     pack_frags<F16>(seen, sb);
 #pragma unroll
-    for (int db = 0; db < DB; ++db) o[db] = careful_mfma<HD, F16>(v, lane, db, pb, sb, o[db]);
+    for (int db = 0; db < DB; ++db) o[db] = careful_mfma<HD, F16>(rd, v, db, pb, sb, o[db]);
   }
   __device__ __forceinline__ bool odd() const {
     bool x = false;
@@ -327,7 +342,6 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_kerne
 #pragma unroll
     for (int j = 0; j < DJ; ++j) m_dma16(vr, &T.v[(wave * DJ + j) * 512], v_voff[j]);
   };
-  auto sees = [&](int n0) { return n0 < row.w_hi && n0 + kMTile > row.w_lo; };
 
   // Iteration t: tile t in `cur`, its products in s; tile t + 1 in `nxt`; tile t + 3
   // issued into `dst`, the slot of tile t - 1, free once every wave passed the barrier.
@@ -336,14 +350,20 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_kerne
     m_wait<2 * DJ>();                          // tile t + 1 landed (tile t + 2 in flight)
     __syncthreads();                           // ... for every wave
     issue(t + 3, dst);
+    R.rd.fresh();
     const int n0 = n_lo + t * kMTile;
-    const f32x16 next = R.products(nxt.k);
-    if (sees(n0)) {
+    const bool edge = n0 < row.a_lo || n0 + kMTile > row.a_hi;
+    if (n0 < row.w_hi && n0 + kMTile > row.w_lo) {
+      const bool poly = R.settle(s, n0, edge);
       float x[16];
-      R.weigh(s, n0, n0 < row.a_lo || n0 + kMTile > row.a_hi, x);
+      R.template scores<false>(s, n0, poly, R.m, x);
+      const f32x16 next = R.products(nxt.k);   // beside the exponentials
+      R.weigh(n0, edge, x);
       R.add(cur.v, x);
+      s = next;
+    } else {
+      s = R.products(nxt.k);
     }
-    s = next;
   };
   R.restart();
   issue(t_begin, r0);
@@ -420,7 +440,9 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_few_k
     issue(K, S.k_sn, t + kMWaves, kw);
     const bool edge = n0 < row.a_lo || n0 + kMTile > row.a_hi;
     float x[16];
-    R.weigh(s, n0, edge, x);
+    const bool poly = R.settle(s, n0, edge);
+    R.template scores<false>(s, n0, poly, R.m, x);
+    R.weigh(n0, edge, x);
     m_wait<DJ>();                              // V landed, the next K in flight
     R.add(vw, x);
     __builtin_amdgcn_s_waitcnt(0xc07f);

@@ -237,6 +237,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
     m_dma4(rr, &T.st[wave * 64], (uint32_t)(wave * 64 + lane) * 4u);
   };
 
+  TileReader<HD> rd(lane);
   f32x16 dk[DB], dv[DB];
   DsScale sc;
   auto restart = [&]() {
@@ -255,8 +256,8 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
     }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      s = mfma32x32x16_t<F16>(row_frag<HD>(T.q + half * 32 * HD, ks, l32, hi), kf[ks], s);
-      dp = mfma32x32x16_t<F16>(row_frag<HD>(T.d + half * 32 * HD, ks, l32, hi), vf[ks], dp);
+      s = mfma32x32x16_t<F16>(rd.rows(T.q + half * 32 * HD, ks), kf[ks], s);
+      dp = mfma32x32x16_t<F16>(rd.rows(T.d + half * 32 * HD, ks), vf[ks], dp);
     }
   };
   // P and dS.
@@ -307,10 +308,11 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
     m_wait<2 * DJ + 1>();                      // tile t + 1 landed (tile t + 2 in flight)
     __syncthreads();                           // ... for every wave; `dst` is free
     issue(t + 3, dst);
-    f32x16 s_next, dp_next;
-    products(nxt, s_next, dp_next);
+    rd.fresh();
     const int row0 = t * kRowTile + half * 32;
     if (row0 < w_hi && row0 + 32 > w_lo) {
+      f32x16 s_next, dp_next;
+      products(nxt, s_next, dp_next);
       float w[16], ds[16];
       weights(cur, s, dp, row0, row0 < a_lo || row0 + 32 > a_hi, w, ds);
       bf16x8 wb[2], db_[2];
@@ -320,12 +322,14 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          dv[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.d + half * 32 * HD, lane, db, i), wb[i], dv[db]);
-          dk[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.q + half * 32 * HD, lane, db, i), db_[i], dk[db]);
+          dv[db] = mfma32x32x16_t<F16>(rd.turned(cur.d + half * 32 * HD, db, i), wb[i], dv[db]);
+          dk[db] = mfma32x32x16_t<F16>(rd.turned(cur.q + half * 32 * HD, db, i), db_[i], dk[db]);
         }
+      s = s_next;
+      dp = dp_next;
+    } else {
+      products(nxt, s, dp);
     }
-    s = s_next;
-    dp = dp_next;
   };
   restart();
   issue(t_begin, r0);
@@ -371,8 +375,8 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
       pack_frags<F16>(sx, sb);
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        dv[db] = careful_mfma<HD, F16>(r0.d + half * 32 * HD, lane, db, wb, sb, dv[db]);
-        dk[db] = careful_mfma<HD, F16>(r0.q + half * 32 * HD, lane, db, db_, sb, dk[db]);
+        dv[db] = careful_mfma<HD, F16>(rd, r0.d + half * 32 * HD, db, wb, sb, dv[db]);
+        dk[db] = careful_mfma<HD, F16>(rd, r0.q + half * 32 * HD, db, db_, sb, dk[db]);
       }
     }
     __syncthreads();
@@ -521,6 +525,7 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
     for (int i = 0; i < DJ; ++i) m_dma16(vr, &T.v[(wave * DJ + i) * 512], v_voff[i]);
   };
 
+  TileReader<HD> rd(lane);
   f32x16 dq[DB];
   DsScale sc;
   auto restart = [&]() {
@@ -534,8 +539,8 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
     for (int i = 0; i < 16; ++i) dp[i] = ndelta;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      s = mfma32x32x16_t<F16>(row_frag<HD>(T.k, ks, l32, hi), qf[ks], s);
-      dp = mfma32x32x16_t<F16>(row_frag<HD>(T.v, ks, l32, hi), df[ks], dp);
+      s = mfma32x32x16_t<F16>(rd.rows(T.k, ks), qf[ks], s);
+      dp = mfma32x32x16_t<F16>(rd.rows(T.v, ks), df[ks], dp);
     }
   };
   auto weights = [&](const f32x16& s, const f32x16& dp, int n0, bool edge, float (&ds)[16]) {
@@ -569,10 +574,11 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
     m_wait<2 * DJ>();                          // tile t + 1 landed (tile t + 2 in flight)
     __syncthreads();
     issue(t + 3, dst);
-    f32x16 s_next, dp_next;
-    products(nxt, s_next, dp_next);
+    rd.fresh();
     const int n0 = n_lo + t * kMTile;
     if (n0 < w_hi && n0 + kMTile > w_lo) {
+      f32x16 s_next, dp_next;
+      products(nxt, s_next, dp_next);
       float ds[16];
       weights(s, dp, n0, n0 < a_lo || n0 + kMTile > a_hi, ds);
       bf16x8 db_[2];
@@ -581,10 +587,12 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          dq[db] = mfma32x32x16_t<F16>(tr_frag<HD>(cur.k, lane, db, i), db_[i], dq[db]);
+          dq[db] = mfma32x32x16_t<F16>(rd.turned(cur.k, db, i), db_[i], dq[db]);
+      s = s_next;
+      dp = dp_next;
+    } else {
+      products(nxt, s, dp);
     }
-    s = s_next;
-    dp = dp_next;
   };
   restart();
   issue(0, r0);
@@ -627,7 +635,7 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
       pack_frags<F16>(ds, db_);
       pack_frags<F16>(sx, sb);
 #pragma unroll
-      for (int db = 0; db < DB; ++db) dq[db] = careful_mfma<HD, F16>(r0.k, lane, db, db_, sb, dq[db]);
+      for (int db = 0; db < DB; ++db) dq[db] = careful_mfma<HD, F16>(rd, r0.k, db, db_, sb, dq[db]);
     }
   }
   if (!live) return;
