@@ -173,6 +173,13 @@ __device__ __forceinline__ void m_wait() {
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
 }
 
+// The same, then the workgroup's barrier.  (__syncthreads is a fence as well: the
+// compiler waits for every DMA in flight before it, and the ring hides nothing.)
+template <int N>
+__device__ __forceinline__ void m_wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
 // A descriptor over the rows [row, row + 32) of a tensor that ends at `end`
 // (rows; none: nothing is read).  Its base moves in 64 bits, so a tensor may
 // be longer than a 32-bit offset reaches.

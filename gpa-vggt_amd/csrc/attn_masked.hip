@@ -347,8 +347,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_kerne
   // issued into `dst`, the slot of tile t - 1, free once every wave passed the barrier.
   f32x16 s;
   auto iter = [&](int t, const Slot<HD>& cur, const Slot<HD>& nxt, Slot<HD>& dst) {
-    m_wait<2 * DJ>();                          // tile t + 1 landed (tile t + 2 in flight)
-    __syncthreads();                           // ... for every wave
+    m_wait_barrier<2 * DJ>();                  // tile t + 1 landed (t + 2 in flight) for every wave
     issue(t + 3, dst);
     R.rd.fresh();
     const int n0 = n_lo + t * kMTile;
@@ -369,8 +368,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_kerne
   issue(t_begin, r0);
   issue(t_begin + 1, r1);
   issue(t_begin + 2, r2);
-  m_wait<4 * DJ>();
-  __syncthreads();
+  m_wait_barrier<4 * DJ>();
   s = R.products(r0.k);
   for (int t = t_begin; t < t_end; t += 4) {
     iter(t, r0, r1, r3);

@@ -305,8 +305,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
 
   f32x16 s, dp;
   auto iter = [&](int t, const RowSlot<HD>& cur, const RowSlot<HD>& nxt, RowSlot<HD>& dst) {
-    m_wait<2 * DJ + 1>();                      // tile t + 1 landed (tile t + 2 in flight)
-    __syncthreads();                           // ... for every wave; `dst` is free
+    m_wait_barrier<2 * DJ + 1>();              // tile t + 1 landed (t + 2 in flight) for every wave
     issue(t + 3, dst);
     rd.fresh();
     const int row0 = t * kRowTile + half * 32;
@@ -335,8 +334,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   issue(t_begin, r0);
   issue(t_begin + 1, r1);
   issue(t_begin + 2, r2);
-  m_wait<2 * (2 * DJ + 1)>();
-  __syncthreads();
+  m_wait_barrier<2 * (2 * DJ + 1)>();
   products(r0, s, dp);
   for (int t = t_begin; t < t_end; t += 4) {
     iter(t, r0, r1, r3);
@@ -571,8 +569,7 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
   };
   f32x16 s, dp;
   auto iter = [&](int t, const KeySlot<HD>& cur, const KeySlot<HD>& nxt, KeySlot<HD>& dst) {
-    m_wait<2 * DJ>();                          // tile t + 1 landed (tile t + 2 in flight)
-    __syncthreads();
+    m_wait_barrier<2 * DJ>();                  // tile t + 1 landed (t + 2 in flight) for every wave
     issue(t + 3, dst);
     rd.fresh();
     const int n0 = n_lo + t * kMTile;
@@ -598,8 +595,7 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
   issue(0, r0);
   issue(1, r1);
   issue(2, r2);
-  m_wait<4 * DJ>();
-  __syncthreads();
+  m_wait_barrier<4 * DJ>();
   products(r0, s, dp);
   for (int t = 0; t < t_end; t += 4) {
     iter(t, r0, r1, r3);
