@@ -30,6 +30,11 @@
 // is one more set of rows, those of all sequences, over its own keys, joined
 // the same way.
 //
+// Many rows under a mask: blocks see between none and all of the keys, and a launch
+// lasts as long as the longest ones and what starts last.  Two small kernels count
+// each block's tiles, cut the longest and list the pieces by length, and
+// attn_masked_piece_kernel takes them in that order (`deal`).
+//
 // A masked key's value does not reach a row: its weight is zero, and where
 // zero times it is not (an infinity or NaN), the workgroup (the wave, where it
 // walks alone) finds a non-finite output at its end and walks its keys again,
@@ -54,6 +59,20 @@ struct FwdSet {
   int32_t folded;         // the rows of all sequences over one sequence of keys, all seen
 };
 
+// Workgroups of a kernel to a CU, and of a launch that is resident at once.
+template <int HD> constexpr int kPerCu = HD == 64 ? 3 : 2;
+constexpr int kCus = 256;
+constexpr int kDealItems = 2048;               // (sequence, block) pairs that are dealt out at most
+constexpr int64_t kLeast = 8;                  // tiles of a share of a block at least
+
+// The pieces of a problem's blocks, the same for every key head of a sequence.
+struct Deal {
+  int32_t pieces, cuts, pad[2];
+  int4 piece[kDealItems + kCus * 3];           // sequence and block, number, of how many, first part (-1: whole)
+  int4 cut[kCus * 3];                          // sequence and block, pieces, first part
+  int32_t count[kDealItems];                   // tiles of a sequence's block
+};
+
 struct FwdArgs {
   const uint16_t* q;
   uint16_t* o;
@@ -63,6 +82,7 @@ struct FwdArgs {
   int64_t slopes_sb;
   float* part;            // partial outputs [splits][rows][HD]; null: none
   float* stat;            // their (offset, sum) [splits][rows][2]
+  Deal* deal;             // null: splits.  Otherwise parts are [part][key head][128 rows]
   int64_t rows;           // B * Hk * M * G
   int32_t B, Hk, G, splits;
   MaskArgs mask;
@@ -110,6 +130,23 @@ __device__ __forceinline__ Row locate(const FwdArgs& p, const FwdSet& S, int pro
   x.a_lo = __builtin_amdgcn_readfirstlane(x.a_lo);
   x.a_hi = __builtin_amdgcn_readfirstlane(x.a_hi);
   return x;
+}
+
+// Where a row's unnormalised outputs, offset and sum go (null: to no partial).
+struct Part {
+  float* o;
+  float2* stat;
+};
+template <int HD>
+__device__ __forceinline__ Part part_at(const FwdArgs& p, int64_t i) {
+  return {p.part + i * HD, reinterpret_cast<float2*>(p.stat) + i};
+}
+// Split z of a set, in which a row's number is that of (sequence, key head, token, head).
+template <int HD>
+__device__ __forceinline__ Part split_part(const FwdArgs& p, const FwdSet& S, const Row& x, int z) {
+  if (!p.part) return {};
+  const int64_t row = (((int64_t)x.b * p.Hk + x.kvh) * p.mask.M + x.tok) * p.G + (x.h - x.kvh * p.G);
+  return part_at<HD>(p, (int64_t)(S.z0 + z) * p.rows + row);
 }
 
 // A wave's 32 rows: their queries, softmax state and outputs.
@@ -244,23 +281,18 @@ struct Rows {
       for (int i = 0; i < 16; ++i) x |= !(fabsf(o[db][i]) < INFINITY);
     return x;
   }
-  // The rows' outputs, or their part of them; `total` is the sum over both halves.
-  __device__ __forceinline__ void finish(const FwdArgs& p, const FwdSet& S, const Row& x, int z, float total) {
+  // The rows' outputs, or with `to` this lane's part of them; `total` is the sum over
+  // both halves.
+  __device__ __forceinline__ void finish(const FwdArgs& p, const Row& x, Part to, float total) {
     if (!x.live) return;
-    if (p.part) {
-      const int64_t row = (((int64_t)x.b * p.Hk + x.kvh) * p.mask.M + x.tok) * p.G + (x.h - x.kvh * p.G);
-      const int64_t to = (int64_t)(S.z0 + z) * p.rows + row;
-      float* O = p.part + to * HD;
+    if (to.o) {
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(O + db * 32 + 8 * g + 4 * hi) =
+          *reinterpret_cast<f32x4*>(to.o + db * 32 + 8 * g + 4 * hi) =
               f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-      if (hi == 0) {
-        p.stat[2 * to] = m;
-        p.stat[2 * to + 1] = total;
-      }
+      if (hi == 0) *to.stat = float2{m, total};
       return;
     }
     const float inv = total == 0.f ? 0.f : 1.0f / total;   // no key seen: zeros
@@ -285,8 +317,10 @@ struct Slot {
   uint16_t v[kMTile * HD];
 };
 
-template <int HD, bool F16, bool CAP, bool SLOPE>
-__global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_kernel(FwdArgs p, int which) {
+// Block qb of a problem: `share(tiles)` says which of its tiles are this workgroup's
+// (x, y), `part(row)` where a row's part of the outputs goes.
+template <int HD, bool F16, bool CAP, bool SLOPE, class Share, class ToPart>
+__device__ __forceinline__ void walk(const FwdArgs& p, const FwdSet& S, int prob, int qb, Share share, ToPart part) {
   constexpr int CH = HD / 8;
   constexpr int DJ = kMTile * CH / kMThreads;  // 16-byte DMAs per wave, tile and tensor
   __shared__ __attribute__((aligned(16))) Slot<HD> r0, r1, r2, r3;
@@ -294,11 +328,6 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_kerne
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const FwdSet& S = p.set[which];
-  const int z = blockIdx.x / (S.blocks * S.problems);
-  int qb, prob;
-  item_of(blockIdx.x % (S.blocks * S.problems), S.blocks, S.problems, qb, prob);
-  qb = S.blocks - 1 - qb;
   const Row row = locate(p, S, prob, qb * kMRows + wave * 32 + (lane & 31));
   Rows<HD, F16, CAP, SLOPE> R(p, row, lane);
 
@@ -317,8 +346,8 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_kerne
   n_hi = __builtin_amdgcn_readfirstlane(n_hi);
   if (n_hi <= n_lo) n_lo = n_hi = 0;           // nothing seen: no tile, empty DMAs
   const int all_tiles = (n_hi - n_lo + kMTile - 1) / kMTile;
-  const int t_begin = (int)((int64_t)all_tiles * z / S.splits);
-  const int t_end = (int)((int64_t)all_tiles * (z + 1) / S.splits);
+  const int2 mine = share(all_tiles);
+  const int t_begin = mine.x, t_end = mine.y;
 
   const int64_t kb = S.folded ? 0 : prob / p.Hk;
   const uint16_t* K = S.k + kb * S.k_sb + row.kvh * S.k_sh;
@@ -391,7 +420,175 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_kerne
       R.careful(r0.k, r0.v, n_lo + t * kMTile);
     }
   }
-  R.finish(p, S, row, z, sum_halves(R.l));
+  R.finish(p, row, part(row), sum_halves(R.l));
+}
+
+// A block, or split z of it.
+template <int HD, bool F16, bool CAP, bool SLOPE>
+__global__ __launch_bounds__(kMThreads, kPerCu<HD>) void attn_masked_kernel(FwdArgs p, int which) {
+  const FwdSet& S = p.set[which];
+  const int z = blockIdx.x / (S.blocks * S.problems);
+  int qb, prob;
+  item_of(blockIdx.x % (S.blocks * S.problems), S.blocks, S.problems, qb, prob);
+  walk<HD, F16, CAP, SLOPE>(
+      p, S, prob, S.blocks - 1 - qb,
+      [&](int tiles) { return int2{(int)((int64_t)tiles * z / S.splits), (int)((int64_t)tiles * (z + 1) / S.splits)}; },
+      [&](const Row& x) { return split_part<HD>(p, S, x, z); });
+}
+
+// ---- blocks of unequal length.
+
+// The tiles of the row blocks of a sequence (blockIdx.x: sequence, block), at least one.
+__global__ __launch_bounds__(kMRows) void attn_masked_count_kernel(FwdArgs p) {
+  __shared__ int range[2][kMRows / 64];
+  const FwdSet& S = p.set[0];
+  const int b = blockIdx.x / S.blocks, r = blockIdx.x % S.blocks * kMRows + threadIdx.x;
+  RowSpan s{0x7fffffff, 0, 0};
+  if (r < S.R) s = row_span(p.mask, b, r / p.G);
+  int lo = s.hi > s.lo ? s.lo : 0x7fffffff, hi = s.hi > s.lo ? s.hi : 0;
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) {
+    lo = min(lo, __shfl_xor(lo, i));
+    hi = max(hi, __shfl_xor(hi, i));
+  }
+  if (threadIdx.x % 64 == 0) {
+    range[0][threadIdx.x / 64] = lo;
+    range[1][threadIdx.x / 64] = hi;
+  }
+  __syncthreads();
+  if (threadIdx.x > 0) return;
+  lo = min(range[0][0], range[0][1]);
+  hi = max(range[1][0], range[1][1]);
+  p.deal->count[blockIdx.x] = hi > lo ? (hi - lo + kMTile - 1) / kMTile : 1;
+}
+
+// The blocks' pieces, long ones first.  With T tiles in all for `spans` workgroups
+// that are resident at once, a block of more than C = T / spans is cut into equal
+// pieces of C at most, so no piece outlasts the rest.  With one causal document,
+// whose lengths go from the shortest to the longest evenly, C is half as much
+// again: fewer parts, 7 to 14 % less time on 128 to 512 blocks; where a block lies
+// astride two documents and walks both, that C costs 15 % (16 heads, 10,992 tokens).
+// The atomics order pieces of about one length among themselves, which changes no result.
+__global__ __launch_bounds__(1024) void attn_masked_deal_kernel(FwdArgs p, int spans) {
+  constexpr int EACH = kDealItems / 1024, KEYS = 256;
+  __shared__ int part[16];
+  __shared__ int at[KEYS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = p.B * p.set[0].blocks;
+  // The sum of the threads before this one, and the total.
+  auto scan = [&](int v, int& total) {
+    auto upto = [&](int x, int width) {
+#pragma unroll
+      for (int i = 1; i < width; i <<= 1) {
+        const int y = __shfl_up(x, i);
+        x += lane >= i ? y : 0;
+      }
+      return x;
+    };
+    const int x = upto(v, 64);
+    __syncthreads();
+    if (lane == 63) part[wave] = x;
+    __syncthreads();
+    const int s = upto(part[lane & 15], 16);
+    total = __shfl(s, 15);
+    const int before = __shfl(s, (wave - 1) & 15);
+    return x - v + (wave > 0 ? before : 0);
+  };
+  int c[EACH], tiles = 0, all;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    c[i] = tid * EACH + i < n ? p.deal->count[tid * EACH + i] : 0;
+    tiles += c[i];
+  }
+  if (tid < KEYS) at[tid] = 0;
+  scan(tiles, all);
+  const int64_t line = (int64_t)all * p.Hk * (p.mask.q_off || p.mask.k_off || p.mask.lens ? 2 : 3) / 2;
+  const int most = (int)std::max<int64_t>((line + spans - 1) / spans, kLeast);
+  int pieces[EACH], key[EACH], cut = 0, total;   // cut blocks, and 2^12 for each of their pieces
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    pieces[i] = (c[i] + most - 1) / most;
+    const int len = pieces[i] > 1 ? (c[i] + pieces[i] - 1) / pieces[i] : c[i];
+    key[i] = KEYS - 1 - (int)((int64_t)std::max(len - 1, 0) * KEYS / most);
+    if (pieces[i] > 1) cut += (pieces[i] << 12) + 1;
+    if (pieces[i] > 0) atomicAdd(&at[key[i]], pieces[i]);
+  }
+  cut = scan(cut, total);
+  const int num = tid < KEYS ? at[tid] : 0;
+  int listed;
+  const int first = scan(num, listed);
+  if (tid < KEYS) at[tid] = first;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int e = tid * EACH + i;
+    const bool whole = pieces[i] < 2;
+    if (pieces[i] == 0) continue;
+    const int to = atomicAdd(&at[key[i]], pieces[i]), slot = cut >> 12;
+    for (int k = 0; k < pieces[i]; ++k) p.deal->piece[to + k] = int4{e, k, pieces[i], whole ? -1 : slot + k};
+    if (whole) continue;
+    p.deal->cut[cut & 4095] = int4{e, pieces[i], slot, 0};
+    cut += (pieces[i] << 12) + 1;
+  }
+  if (tid == 0) {
+    p.deal->pieces = listed;
+    p.deal->cuts = total & 4095;
+  }
+}
+
+// A piece of a block.  The heads of a sequence take the same piece together, each on
+// an XCD of its own where they are a multiple of the eight.
+template <int HD, bool F16, bool CAP, bool SLOPE>
+__global__ __launch_bounds__(kMThreads, kPerCu<HD>) void attn_masked_piece_kernel(FwdArgs p) {
+  const FwdSet& S = p.set[0];
+  const int kvh = blockIdx.x % p.Hk, at = blockIdx.x / p.Hk;
+  if (at >= p.deal->pieces) return;
+  const int4 x = p.deal->piece[at];
+  walk<HD, F16, CAP, SLOPE>(
+      p, S, x.x / S.blocks * p.Hk + kvh, x.x % S.blocks,
+      [&](int tiles) { return int2{(int)((int64_t)tiles * x.y / x.z), (int)((int64_t)tiles * (x.y + 1) / x.z)}; },
+      [&](const Row&) {
+        if (x.w < 0) return Part{};
+        return part_at<HD>(p, ((int64_t)x.w * p.Hk + kvh) * kMRows + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31));
+      });
+}
+
+// Four values of a row's outputs.
+template <bool F16>
+__device__ __forceinline__ void emit(const FwdArgs& p, int64_t b, int64_t h, int64_t tok, int at, f32x4 o, float total) {
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  const bf16x2 lo = pack2<F16>(o[0] * inv, o[1] * inv), hi = pack2<F16>(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<u32x2*>(p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sm + 4 * at) =
+      u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+
+// The pieces of a block that was cut, put together, HD / 4 lanes a row.
+template <int HD, bool F16>
+__global__ __launch_bounds__(256) void attn_masked_piece_join_kernel(FwdArgs p) {
+  constexpr int L = HD / 4;
+  const int kvh = blockIdx.x % p.Hk, c = blockIdx.x / p.Hk, nb = p.set[0].blocks;
+  if (c >= p.deal->cuts) return;
+  const int4 s = p.deal->cut[c];
+  const int local = blockIdx.y * (256 / L) + threadIdx.x / L, at = threadIdx.x % L;
+  const int r = s.x % nb * kMRows + local;
+  if (r >= p.set[0].R) return;
+  auto slot = [&](int i) { return ((int64_t)(s.z + i) * p.Hk + kvh) * kMRows + local; };
+  const float2* stat = reinterpret_cast<const float2*>(p.stat);
+  float top = -INFINITY, total = 0.f;
+  for (int i = 0; i < s.y; ++i) top = fmaxf(top, stat[slot(i)].x);
+  f32x4 o{};
+#pragma unroll 4
+  for (int i = 0; i < s.y; ++i) {
+    const float2 t = stat[slot(i)];
+    const f32x4 v = reinterpret_cast<const f32x4*>(p.part)[slot(i) * L + at];
+    const float a = t.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(t.x - top);
+    total = __builtin_fmaf(a, t.y, total);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(a, v[e], o[e]);
+  }
+  const int64_t b = s.x / nb, h = (int64_t)kvh * p.G + r % p.G, tok = r / p.G;
+  emit<F16>(p, b, h, tok, at, o, total);
+  if (p.lse && at == 0)
+    p.lse[b * p.lse_sb + h * p.lse_sh + tok] = total == 0.f ? -INFINITY : top + __log2f(total);
 }
 
 template <int HD, bool F16, bool CAP, bool SLOPE>
@@ -503,7 +700,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_few_k
   __syncthreads();
   if (wave > 0) return;
   take(0);
-  R.finish(p, S, row, z, total);
+  R.finish(p, row, split_part<HD>(p, S, row, z), total);
 }
 
 // The partial outputs of a row's splits put together, by WAVES waves.
@@ -579,16 +776,29 @@ __global__ __launch_bounds__(256) void attn_masked_join_kernel(FwdArgs p) {
   const int g = (int)(row % p.G);
   const int64_t t = row / p.G, tok = t % p.mask.M, b = t / p.mask.M / p.Hk;
   const int64_t h = t / p.mask.M % p.Hk * p.G + g;
-  const float inv = total == 0.f ? 0.f : 1.0f / total;
-  const bf16x2 lo = pack2<F16>(o[0] * inv, o[1] * inv), hi = pack2<F16>(o[2] * inv, o[3] * inv);
-  *reinterpret_cast<u32x2*>(p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sm + 4 * at) =
-      u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+  emit<F16>(p, b, h, tok, at, o, total);
   if (p.lse && at == 0)
     p.lse[b * p.lse_sb + h * p.lse_sh + tok] = total == 0.f ? -INFINITY : top + __log2f(total);
 }
 
 template <int HD, bool F16, bool CAP, bool SLOPE>
 hipError_t launch_sets(const FwdArgs& a, hipStream_t s) {
+  if (a.deal) {
+    hipLaunchKernelGGL(attn_masked_count_kernel, dim3((unsigned)(a.B * a.set[0].blocks)), dim3(kMRows), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int spans = kCus * kPerCu<HD>, Hk = a.Hk;
+    hipLaunchKernelGGL(attn_masked_deal_kernel, dim3(1), dim3(1024), 0, s, a, spans);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    // A head has fewer cut blocks than spans / Hk, and at most that many pieces more than blocks.
+    const unsigned most = (unsigned)(a.B * a.set[0].blocks + spans / Hk) * Hk, cuts = (unsigned)(spans / Hk) * Hk;
+    hipLaunchKernelGGL((attn_masked_piece_kernel<HD, F16, CAP, SLOPE>), dim3(most), dim3(kMThreads), 0, s, a);
+    e = hipGetLastError();
+    if (e != hipSuccess || cuts == 0) return e;
+    hipLaunchKernelGGL((attn_masked_piece_join_kernel<HD, F16>), dim3(cuts, kMRows * HD / 4 / 256), dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
   for (int i = 1; i >= 0; --i) {               // the prefix, then the own keys
     const FwdSet& t = a.set[i];
     const unsigned items = (unsigned)t.blocks * t.problems * t.splits;
@@ -607,7 +817,7 @@ template <int HD, bool F16>
 hipError_t launch(const FwdArgs& a, bool cap, hipStream_t s) {
   const hipError_t e = cap ? (a.slopes ? launch_sets<HD, F16, true, true>(a, s) : launch_sets<HD, F16, true, false>(a, s))
                            : (a.slopes ? launch_sets<HD, F16, false, true>(a, s) : launch_sets<HD, F16, false, false>(a, s));
-  if (e != hipSuccess || !a.part) return e;
+  if (e != hipSuccess || a.deal || !a.part) return e;
   // A wave a row reads a few splits, four waves many.
   if (a.splits <= 16)
     hipLaunchKernelGGL((attn_masked_join_kernel<HD, F16, 1>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0, s, a);
@@ -620,15 +830,43 @@ hipError_t launch(const FwdArgs& a, bool cap, hipStream_t s) {
 // blocks over many keys are bound by one workgroup's walk; kWant workgroups
 // (two a CU) fill the chip.  A split has at least kLeast tiles: below that
 // the join costs what the shorter walk saves.
-constexpr int64_t kWant = 512, kLeast = 8;
+constexpr int64_t kWant = 512;
 int splits_of(int64_t items, int64_t keys) {
   const int64_t tiles = (keys + kMTile - 1) / kMTile;
   const int64_t z = std::min({items > 0 ? kWant / items : 1, tiles / kLeast, (int64_t)kMaxSplits / 2});
   return (int)std::max<int64_t>(z, 1);
 }
 
-struct Plan { int blocks, problems, splits, p_blocks, p_problems, p_splits; };
-Plan plan(int64_t B, int64_t Hk, int64_t G, int64_t M, int64_t N, int64_t P) {
+// What makes row blocks see key ranges of unequal length.
+enum class Unequal { no, causal, documents };
+Unequal unequal_of(const gpa_attn_masked_args& a) {
+  return a.q_offsets || a.k_offsets || a.lens ? Unequal::documents : a.causal ? Unequal::causal : Unequal::no;
+}
+
+// Whether a launch's blocks are counted, cut and sorted first.  That takes two small
+// kernels and a join, 9 us, and pays where the mask makes blocks unequal and their
+// number is between what the splits above fill the chip with and what evens
+// itself out.  Measured (us, without and with; bf16):
+//   one causal document, 8 heads of 64, 4,096 tokens (256 blocks)     71    52
+//   16 of 64, 4,096 tokens (512)                                      78    71
+//   2 x 16 of 64, 4,096 tokens (1,024)                               100   111
+//   8 of 128, 4,096 tokens (256)                                      85    66
+//   16 of 128, 4,096 tokens (512)                                    102   106
+//   four documents, 16 of 64, 10,992 tokens (1,376)                  417   330
+//   three documents, 4 x 16 of 64, 4,096 tokens (2,048)              129   130
+bool deal(Unequal u, int64_t P, int64_t rows, int64_t items, int64_t entries, int64_t N, int64_t spans) {
+  const int64_t tiles = (N + kMTile - 1) / kMTile;
+  if (u == Unequal::no || P > 0 || rows <= 32 || items < 128 || tiles < 64) return false;
+  if (entries > kDealItems || N >= (int64_t)1 << 24) return false;   // the list's length; 32-bit sums
+  return u == Unequal::documents ? items <= 2 * spans : 2 * items <= spans || (items < spans && tiles >= 128);
+}
+
+struct Plan {
+  int blocks, problems, splits, p_blocks, p_problems, p_splits;
+  bool deal;
+  size_t parts, bytes;    // parts of a row of outputs, workspace
+};
+Plan plan(int64_t B, int64_t Hk, int64_t G, int64_t M, int64_t N, int64_t P, int64_t D, Unequal unequal) {
   Plan x{};
   x.blocks = (int)((M * G + kMRows - 1) / kMRows);
   x.problems = (int)(B * Hk);
@@ -638,6 +876,12 @@ Plan plan(int64_t B, int64_t Hk, int64_t G, int64_t M, int64_t N, int64_t P) {
     x.p_splits = splits_of((int64_t)x.p_blocks * Hk, P);
   }
   x.splits = splits_of((int64_t)x.blocks * x.problems, N);
+  const int64_t items = (int64_t)x.blocks * x.problems, spans = kCus * (D == 64 ? kPerCu<64> : kPerCu<128>);
+  x.deal = deal(unequal, P, M * G, items, B * x.blocks, N, spans);
+  if (x.deal) x.splits = 1;
+  const int z = x.splits + x.p_splits;
+  x.parts = x.deal ? (size_t)(2 * spans * kMRows) : z > 1 ? (size_t)z * B * Hk * G * M : 0;
+  x.bytes = x.parts * (D + 2) * sizeof(float) + (x.deal ? sizeof(Deal) : 0);
   return x;
 }
 
@@ -753,9 +997,10 @@ void gpa::masked_fill(const gpa_attn_masked_args* a, MaskArgs* m, ScoreArgs* s) 
 extern "C" size_t gpa_attn_masked_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t M,
                                                   int64_t N, int64_t P, int64_t D) {
   if (B <= 0 || H <= 0 || Hk <= 0 || M <= 0 || N < 0 || P < 0 || H % Hk) return 0;
-  const Plan x = plan(B, Hk, H / Hk, M, N, P);
-  const int z = x.splits + x.p_splits;
-  return z > 1 ? (size_t)z * B * H * M * (D + 2) * sizeof(float) : 0;
+  size_t most = 0;                             // whatever the mask
+  for (const Unequal u : {Unequal::no, Unequal::causal, Unequal::documents})
+    most = std::max(most, plan(B, Hk, H / Hk, M, N, P, D, u).bytes);
+  return most;
 }
 
 extern "C" int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void* workspace,
@@ -767,10 +1012,10 @@ extern "C" int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void
   const gpa_attn_masked_args plain_args = masked_plain(args), *a = &plain_args;
   if (a->B == 0 || a->H == 0 || a->M == 0) return GPA_OK;
   const int64_t G = a->H / a->Hk;
-  const Plan x = plan(a->B, a->Hk, G, a->M, a->N, a->P);
+  const Plan x = plan(a->B, a->Hk, G, a->M, a->N, a->P, a->D, unequal_of(*a));
   const int64_t items = (int64_t)x.blocks * x.problems * x.splits +
                         (int64_t)x.p_blocks * x.p_problems * x.p_splits;
-  const size_t need = gpa_attn_masked_workspace_bytes(a->B, a->H, a->Hk, a->M, a->N, a->P, a->D);
+  const size_t need = x.bytes;
   if (items > 0x7fffffff || a->B * a->H * a->M >= (int64_t)1 << 31) {
     gpa_set_error("%s: too many rows", fn);
     return GPA_E_UNSUPPORTED;
@@ -794,7 +1039,8 @@ extern "C" int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void
   masked_fill(a, &f.mask, &f.score);
   if (need > 0) {
     f.part = (float*)workspace;
-    f.stat = f.part + (int64_t)f.splits * f.rows * a->D;
+    f.stat = f.part + x.parts * a->D;
+    if (x.deal) f.deal = (Deal*)(f.stat + x.parts * 2);
   }
   FwdSet& own = f.set[0];
   own.k = (const uint16_t*)a->k; own.v = (const uint16_t*)a->v;

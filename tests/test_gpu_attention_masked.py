@@ -134,6 +134,34 @@ def test_long_and_wide(dev):
     _check(dev, 1, 1, 1, 2, 40_000, 64, BF, seed=3, back=False, causal=True, slopes=torch.tensor([0.01]))
 
 
+def test_blocks_of_unequal_length(dev):
+    """Many row blocks under a mask: cut and taken in order of their lengths."""
+    _check(dev, 1, 8, 8, 2100, 2100, 64, BF, seed=21, back=False, causal=True, slopes=torch.rand(8))
+    _check(dev, 1, 8, 8, 2100, 2100, 128, HF, seed=22, back=False, causal=True, prefix=900, cap=20.0)
+    off = [40, 41, 600, 600, 1990, 2060]
+    _check(dev, 1, 12, 4, 2100, 2100, 128, BF, seed=23, back=False, offsets=off)
+    _check(dev, 1, 15, 5, 2100, 2100, 64, HF, seed=24, back=False, offsets=off, causal=True, prefix=[1, 0, 5, 3000, 2])
+    lens = [[0, n] for n in (2100, 0, 1, 2099, 64, 1025)]
+    _check(dev, 6, 22, 11, 70, 2100, 64, BF, seed=25, back=False, causal=True, k_offsets=lens, cap=30.0)
+    _check(dev, 6, 22, 11, 70, 2100, 128, BF, seed=26, back=False, k_offsets=lens)
+
+
+def test_more_heads_than_workgroups_at_once(dev):
+    _check(dev, 1, 800, 800, 33, 2020, 64, BF, seed=27, back=False, causal=True, offsets=[0, 3, 33],
+           k_offsets=[0, 1000, 2020])
+
+
+def test_masked_values_of_blocks_in_pieces(dev):
+    """Infinities and NaN in keys of no document change no bit."""
+    q, k, v, _, _ = (t.to(dev) for t in _inputs(1, 8, 8, 2200, 2200, 64, BF, 28))
+    off = torch.tensor([0, 50, 2150], dtype=torch.int32, device=dev)
+    want = attention_masked(q, k, v, 0.125, offsets=off, return_lse=True)
+    k[:, :, 2150:], v[:, :, 2150:] = math.nan, math.inf
+    v[:, :, 2160:] = math.nan
+    got = attention_masked(q, k, v, 0.125, offsets=off, return_lse=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_no_tokens(dev):
     for B, M, N in ((0, 4, 4), (2, 0, 5), (2, 5, 0)):
         q = torch.randn(B, 4, M, 64, device=dev, dtype=BF, requires_grad=True)
