@@ -142,6 +142,12 @@ __device__ __forceinline__ constexpr int tile_at(int row, int chunk) {
   return row * HD + ((chunk ^ tile_swz<HD>(row)) << 3);
 }
 
+// Where part k of n equal parts of `tiles` begins: the same for all lanes, which the
+// compiler does not see through a division.
+__device__ __forceinline__ int share_of(int tiles, int k, int n) {
+  return __builtin_amdgcn_readfirstlane((int)((int64_t)tiles * k / n));
+}
+
 // Item L of blocks x problems: heavy blocks first (the last rows of a causal
 // document see the most keys, so a launch's tail is short), and the blocks of one
 // problem on one XCD (workgroups go round the eight of them), whose L2 then holds

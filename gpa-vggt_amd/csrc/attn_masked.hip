@@ -33,13 +33,13 @@
 // Many rows under a mask: blocks see between none and all of the keys, and a launch
 // lasts as long as the longest ones and what starts last.  Two small kernels count
 // each block's tiles, cut the longest and list the pieces by length, and
-// attn_masked_piece_kernel takes them in that order (`deal`).
+// attn_masked_piece_kernel takes them in that order (`deals`).
 //
 // A masked key's value does not reach a row: its weight is zero, and where
 // zero times it is not (an infinity or NaN), the workgroup (the wave, where it
 // walks alone) finds a non-finite output at its end and walks its keys again,
 // with such values taken out.
-#include "attn_masked.h"
+#include "attn_masked_deal.h"
 
 #include <algorithm>
 
@@ -59,19 +59,7 @@ struct FwdSet {
   int32_t folded;         // the rows of all sequences over one sequence of keys, all seen
 };
 
-// Workgroups of a kernel to a CU, and of a launch that is resident at once.
-template <int HD> constexpr int kPerCu = HD == 64 ? 3 : 2;
-constexpr int kCus = 256;
-constexpr int kDealItems = 2048;               // (sequence, block) pairs that are dealt out at most
-constexpr int64_t kLeast = 8;                  // tiles of a share of a block at least
-
-// The pieces of a problem's blocks, the same for every key head of a sequence.
-struct Deal {
-  int32_t pieces, cuts, pad[2];
-  int4 piece[kDealItems + kCus * 3];           // sequence and block, number, of how many, first part (-1: whole)
-  int4 cut[kCus * 3];                          // sequence and block, pieces, first part
-  int32_t count[kDealItems];                   // tiles of a sequence's block
-};
+template <int HD> constexpr int kPerCu = HD == 64 ? 3 : 2;   // workgroups to a CU
 
 struct FwdArgs {
   const uint16_t* q;
@@ -432,107 +420,8 @@ __global__ __launch_bounds__(kMThreads, kPerCu<HD>) void attn_masked_kernel(FwdA
   item_of(blockIdx.x % (S.blocks * S.problems), S.blocks, S.problems, qb, prob);
   walk<HD, F16, CAP, SLOPE>(
       p, S, prob, S.blocks - 1 - qb,
-      [&](int tiles) { return int2{(int)((int64_t)tiles * z / S.splits), (int)((int64_t)tiles * (z + 1) / S.splits)}; },
+      [&](int tiles) { return int2{share_of(tiles, z, S.splits), share_of(tiles, z + 1, S.splits)}; },
       [&](const Row& x) { return split_part<HD>(p, S, x, z); });
-}
-
-// ---- blocks of unequal length.
-
-// The tiles of the row blocks of a sequence (blockIdx.x: sequence, block), at least one.
-__global__ __launch_bounds__(kMRows) void attn_masked_count_kernel(FwdArgs p) {
-  __shared__ int range[2][kMRows / 64];
-  const FwdSet& S = p.set[0];
-  const int b = blockIdx.x / S.blocks, r = blockIdx.x % S.blocks * kMRows + threadIdx.x;
-  RowSpan s{0x7fffffff, 0, 0};
-  if (r < S.R) s = row_span(p.mask, b, r / p.G);
-  int lo = s.hi > s.lo ? s.lo : 0x7fffffff, hi = s.hi > s.lo ? s.hi : 0;
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) {
-    lo = min(lo, __shfl_xor(lo, i));
-    hi = max(hi, __shfl_xor(hi, i));
-  }
-  if (threadIdx.x % 64 == 0) {
-    range[0][threadIdx.x / 64] = lo;
-    range[1][threadIdx.x / 64] = hi;
-  }
-  __syncthreads();
-  if (threadIdx.x > 0) return;
-  lo = min(range[0][0], range[0][1]);
-  hi = max(range[1][0], range[1][1]);
-  p.deal->count[blockIdx.x] = hi > lo ? (hi - lo + kMTile - 1) / kMTile : 1;
-}
-
-// The blocks' pieces, long ones first.  With T tiles in all for `spans` workgroups
-// that are resident at once, a block of more than C = T / spans is cut into equal
-// pieces of C at most, so no piece outlasts the rest.  With one causal document,
-// whose lengths go from the shortest to the longest evenly, C is half as much
-// again: fewer parts, 7 to 14 % less time on 128 to 512 blocks; where a block lies
-// astride two documents and walks both, that C costs 15 % (16 heads, 10,992 tokens).
-// The atomics order pieces of about one length among themselves, which changes no result.
-__global__ __launch_bounds__(1024) void attn_masked_deal_kernel(FwdArgs p, int spans) {
-  constexpr int EACH = kDealItems / 1024, KEYS = 256;
-  __shared__ int part[16];
-  __shared__ int at[KEYS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = p.B * p.set[0].blocks;
-  // The sum of the threads before this one, and the total.
-  auto scan = [&](int v, int& total) {
-    auto upto = [&](int x, int width) {
-#pragma unroll
-      for (int i = 1; i < width; i <<= 1) {
-        const int y = __shfl_up(x, i);
-        x += lane >= i ? y : 0;
-      }
-      return x;
-    };
-    const int x = upto(v, 64);
-    __syncthreads();
-    if (lane == 63) part[wave] = x;
-    __syncthreads();
-    const int s = upto(part[lane & 15], 16);
-    total = __shfl(s, 15);
-    const int before = __shfl(s, (wave - 1) & 15);
-    return x - v + (wave > 0 ? before : 0);
-  };
-  int c[EACH], tiles = 0, all;
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    c[i] = tid * EACH + i < n ? p.deal->count[tid * EACH + i] : 0;
-    tiles += c[i];
-  }
-  if (tid < KEYS) at[tid] = 0;
-  scan(tiles, all);
-  const int64_t line = (int64_t)all * p.Hk * (p.mask.q_off || p.mask.k_off || p.mask.lens ? 2 : 3) / 2;
-  const int most = (int)std::max<int64_t>((line + spans - 1) / spans, kLeast);
-  int pieces[EACH], key[EACH], cut = 0, total;   // cut blocks, and 2^12 for each of their pieces
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    pieces[i] = (c[i] + most - 1) / most;
-    const int len = pieces[i] > 1 ? (c[i] + pieces[i] - 1) / pieces[i] : c[i];
-    key[i] = KEYS - 1 - (int)((int64_t)std::max(len - 1, 0) * KEYS / most);
-    if (pieces[i] > 1) cut += (pieces[i] << 12) + 1;
-    if (pieces[i] > 0) atomicAdd(&at[key[i]], pieces[i]);
-  }
-  cut = scan(cut, total);
-  const int num = tid < KEYS ? at[tid] : 0;
-  int listed;
-  const int first = scan(num, listed);
-  if (tid < KEYS) at[tid] = first;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const int e = tid * EACH + i;
-    const bool whole = pieces[i] < 2;
-    if (pieces[i] == 0) continue;
-    const int to = atomicAdd(&at[key[i]], pieces[i]), slot = cut >> 12;
-    for (int k = 0; k < pieces[i]; ++k) p.deal->piece[to + k] = int4{e, k, pieces[i], whole ? -1 : slot + k};
-    if (whole) continue;
-    p.deal->cut[cut & 4095] = int4{e, pieces[i], slot, 0};
-    cut += (pieces[i] << 12) + 1;
-  }
-  if (tid == 0) {
-    p.deal->pieces = listed;
-    p.deal->cuts = total & 4095;
-  }
 }
 
 // A piece of a block.  The heads of a sequence take the same piece together, each on
@@ -542,10 +431,10 @@ __global__ __launch_bounds__(kMThreads, kPerCu<HD>) void attn_masked_piece_kerne
   const FwdSet& S = p.set[0];
   const int kvh = blockIdx.x % p.Hk, at = blockIdx.x / p.Hk;
   if (at >= p.deal->pieces) return;
-  const int4 x = p.deal->piece[at];
+  const int4 x = same(p.deal->piece[at]);
   walk<HD, F16, CAP, SLOPE>(
       p, S, x.x / S.blocks * p.Hk + kvh, x.x % S.blocks,
-      [&](int tiles) { return int2{(int)((int64_t)tiles * x.y / x.z), (int)((int64_t)tiles * (x.y + 1) / x.z)}; },
+      [&](int tiles) { return int2{share_of(tiles, x.y, x.z), share_of(tiles, x.y + 1, x.z)}; },
       [&](const Row&) {
         if (x.w < 0) return Part{};
         return part_at<HD>(p, ((int64_t)x.w * p.Hk + kvh) * kMRows + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31));
@@ -608,8 +497,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_few_k
   Rows<HD, F16, CAP, SLOPE> R(p, row, lane);
   const int n_lo = row.w_hi > row.w_lo ? row.w_lo : 0, n_hi = row.w_hi > row.w_lo ? row.w_hi : 0;
   const int all_tiles = (n_hi - n_lo + kMTile - 1) / kMTile;
-  const int t_begin = (int)((int64_t)all_tiles * z / S.splits) + wave;
-  const int t_end = (int)((int64_t)all_tiles * (z + 1) / S.splits);
+  const int t_begin = share_of(all_tiles, z, S.splits) + wave, t_end = share_of(all_tiles, z + 1, S.splits);
 
   const int64_t kb = S.folded ? 0 : prob / p.Hk;
   const uint16_t* K = S.k + kb * S.k_sb + row.kvh * S.k_sh;
@@ -784,12 +672,8 @@ __global__ __launch_bounds__(256) void attn_masked_join_kernel(FwdArgs p) {
 template <int HD, bool F16, bool CAP, bool SLOPE>
 hipError_t launch_sets(const FwdArgs& a, hipStream_t s) {
   if (a.deal) {
-    hipLaunchKernelGGL(attn_masked_count_kernel, dim3((unsigned)(a.B * a.set[0].blocks)), dim3(kMRows), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
     const int spans = kCus * kPerCu<HD>, Hk = a.Hk;
-    hipLaunchKernelGGL(attn_masked_deal_kernel, dim3(1), dim3(1024), 0, s, a, spans);
-    e = hipGetLastError();
+    hipError_t e = deal_out(a.mask, a.B, Hk, a.G, {a.deal, a.set[0].blocks, spans}, {}, s);
     if (e != hipSuccess) return e;
     // A head has fewer cut blocks than spans / Hk, and at most that many pieces more than blocks.
     const unsigned most = (unsigned)(a.B * a.set[0].blocks + spans / Hk) * Hk, cuts = (unsigned)(spans / Hk) * Hk;
@@ -837,12 +721,6 @@ int splits_of(int64_t items, int64_t keys) {
   return (int)std::max<int64_t>(z, 1);
 }
 
-// What makes row blocks see key ranges of unequal length.
-enum class Unequal { no, causal, documents };
-Unequal unequal_of(const gpa_attn_masked_args& a) {
-  return a.q_offsets || a.k_offsets || a.lens ? Unequal::documents : a.causal ? Unequal::causal : Unequal::no;
-}
-
 // Whether a launch's blocks are counted, cut and sorted first.  That takes two small
 // kernels and a join, 9 us, and pays where the mask makes blocks unequal and their
 // number is between what the splits above fill the chip with and what evens
@@ -854,7 +732,7 @@ Unequal unequal_of(const gpa_attn_masked_args& a) {
 //   16 of 128, 4,096 tokens (512)                                    102   106
 //   four documents, 16 of 64, 10,992 tokens (1,376)                  417   330
 //   three documents, 4 x 16 of 64, 4,096 tokens (2,048)              129   130
-bool deal(Unequal u, int64_t P, int64_t rows, int64_t items, int64_t entries, int64_t N, int64_t spans) {
+bool deals(Unequal u, int64_t P, int64_t rows, int64_t items, int64_t entries, int64_t N, int64_t spans) {
   const int64_t tiles = (N + kMTile - 1) / kMTile;
   if (u == Unequal::no || P > 0 || rows <= 32 || items < 128 || tiles < 64) return false;
   if (entries > kDealItems || N >= (int64_t)1 << 24) return false;   // the list's length; 32-bit sums
@@ -877,7 +755,7 @@ Plan plan(int64_t B, int64_t Hk, int64_t G, int64_t M, int64_t N, int64_t P, int
   }
   x.splits = splits_of((int64_t)x.blocks * x.problems, N);
   const int64_t items = (int64_t)x.blocks * x.problems, spans = kCus * (D == 64 ? kPerCu<64> : kPerCu<128>);
-  x.deal = deal(unequal, P, M * G, items, B * x.blocks, N, spans);
+  x.deal = deals(unequal, P, M * G, items, B * x.blocks, N, spans);
   if (x.deal) x.splits = 1;
   const int z = x.splits + x.p_splits;
   x.parts = x.deal ? (size_t)(2 * spans * kMRows) : z > 1 ? (size_t)z * B * Hk * G * M : 0;

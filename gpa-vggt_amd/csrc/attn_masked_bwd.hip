@@ -24,13 +24,16 @@
 // 5), and in return the results repeat bit by bit and no fp32 copy of dQ goes
 // through memory.
 //
+// Where few key blocks decide how long a launch lasts, blocks are cut and taken by
+// length as in the forward pass; attn_masked_grad_join_kernel adds up the parts.
+//
 // With a cap, r = 1 / (1 + e^(2u)) gives both: tanh = 1 - 2r, 1 - tanh^2 = 4 (r - r^2).
 //
 // P and dS are rounded to the operand format for the products (the same
 // relative error as the gradients' own rounding); sums are fp32.  In fp16
 // small weights would lose bits below 2^-14, so P is scaled by 2^14 and dS by a
 // power of two that follows its largest value; the sums are scaled back.
-#include "attn_masked.h"
+#include "attn_masked_deal.h"
 
 #include <algorithm>
 
@@ -53,9 +56,26 @@ struct BwdArgs {
   float* rec;                                  // [B * Hk][tiles][kRec]
   int32_t Hk, G, R, tiles;                     // R = M * G rows of a problem
   float sm_scale;
+  const Deal *keys, *rows;                     // null: every block whole, heavy ones first
+  float *kpart, *qpart;                        // [part][key head][dk, dv of 64 keys; dq of 128 rows][HD]
   MaskArgs mask;
   ScoreArgs score;
 };
+
+// Workgroup L's piece of a block (k of n), and where its part goes (-1: it is whole).
+struct Piece { int block, prob, k, n, part; };
+__device__ __forceinline__ Piece piece_of(const Deal* d, int L, int blocks, int problems, int Hk) {
+  Piece x{0, 0, 0, 1, -1};
+  if (!d) {
+    item_of(L, blocks, problems, x.block, x.prob);
+    return x;
+  }
+  x.n = 0;
+  if (L / Hk >= d->pieces) return x;
+  const int4 y = same(d->piece[L / Hk]);
+  const int b = y.x / blocks, kvh = L % Hk;
+  return {y.x - b * blocks, b * Hk + kvh, y.y, y.z, y.w < 0 ? -1 : y.w * Hk + kvh};
+}
 
 template <int HD, bool F16>
 __global__ __launch_bounds__(256) void attn_masked_delta_kernel(BwdArgs p) {
@@ -147,9 +167,10 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = wave >> 1;                  // of a row tile
   const int blocks = (p.mask.N + kKeys - 1) / kKeys;
-  int kb, prob;
-  item_of(blockIdx.x, blocks, gridDim.x / blocks, kb, prob);
-  const int b = prob / p.Hk, kvh = prob % p.Hk;
+  const Piece piece = piece_of(p.keys, blockIdx.x, blocks, gridDim.x / blocks, p.Hk);
+  if (piece.n == 0) return;
+  const int kb = piece.block, prob = __builtin_amdgcn_readfirstlane(piece.prob);
+  const int b = __builtin_amdgcn_readfirstlane(prob / p.Hk), kvh = __builtin_amdgcn_readfirstlane(prob % p.Hk);
   const int j = kb * kKeys + (wave & 1) * 32 + l32;
   const bool live = j < p.mask.N;
   const int jc = live ? j : p.mask.N - 1;
@@ -195,8 +216,10 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   }
   n_lo = __builtin_amdgcn_readfirstlane(n_lo);
   n_hi = __builtin_amdgcn_readfirstlane(n_hi);
-  const int t_begin = n_hi > n_lo ? n_lo / kRowTile : 0;
-  const int t_end = n_hi > n_lo ? (n_hi + kRowTile - 1) / kRowTile : 0;
+  const int t_lo = n_hi > n_lo ? n_lo / kRowTile : 0;
+  const int all_tiles = n_hi > n_lo ? (n_hi + kRowTile - 1) / kRowTile - t_lo : 0;
+  const int t_begin = t_lo + share_of(all_tiles, piece.k, piece.n);
+  const int t_end = t_lo + share_of(all_tiles, piece.k + 1, piece.n);
 
   // Rows of a tile: token and head of row 64 t + i follow from (64 t) / G; where
   // G divides 64 the offsets inside a tile are the same for all tiles.
@@ -416,6 +439,19 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   if (half == 1 || !live) return;
   take(r0.q, dk);
   take(r1.q, dv);
+  if (piece.part >= 0) {
+    float* P = p.kpart + ((int64_t)piece.part * 2 * kKeys + (wave & 1) * 32 + l32) * HD;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = db * 32 + 8 * g + 4 * hi;
+        *reinterpret_cast<f32x4*>(P + at) = f32x4{dk[db][4 * g], dk[db][4 * g + 1], dk[db][4 * g + 2], dk[db][4 * g + 3]};
+        *reinterpret_cast<f32x4*>(P + kKeys * HD + at) =
+            f32x4{dv[db][4 * g], dv[db][4 * g + 1], dv[db][4 * g + 2], dv[db][4 * g + 3]};
+      }
+    return;
+  }
   uint16_t* DK = p.dk + b * p.dk_sb + kvh * p.dk_sh + j * p.dk_sn;
   uint16_t* DV = p.dv + b * p.dv_sb + kvh * p.dv_sh + j * p.dv_sn;
 #pragma unroll
@@ -450,10 +486,11 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int blocks = (p.R + kMRows - 1) / kMRows;
-  int qb, prob;
-  item_of(blockIdx.x, blocks, gridDim.x / blocks, qb, prob);
-  qb = blocks - 1 - qb;
-  const int b = prob / p.Hk, kvh = prob % p.Hk;
+  const Piece piece = piece_of(p.rows, blockIdx.x, blocks, gridDim.x / blocks, p.Hk);
+  if (piece.n == 0) return;
+  const int qb = p.rows ? piece.block : blocks - 1 - piece.block;
+  const int prob = __builtin_amdgcn_readfirstlane(piece.prob);
+  const int b = __builtin_amdgcn_readfirstlane(prob / p.Hk), kvh = __builtin_amdgcn_readfirstlane(prob % p.Hk);
   const int r = qb * kMRows + wave * 32 + l32;
   const bool live = r < p.R;
   const int rc = live ? r : p.R - 1;
@@ -501,7 +538,8 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
   n_lo = __builtin_amdgcn_readfirstlane(n_lo);
   n_hi = __builtin_amdgcn_readfirstlane(n_hi);
   if (n_hi <= n_lo) n_lo = n_hi = 0;
-  const int t_end = (n_hi - n_lo + kMTile - 1) / kMTile;
+  const int all_tiles = (n_hi - n_lo + kMTile - 1) / kMTile;
+  const int t_begin = share_of(all_tiles, piece.k, piece.n), t_end = share_of(all_tiles, piece.k + 1, piece.n);
 
   const uint16_t* K = p.k + b * p.k_sb + kvh * p.k_sh;
   const uint16_t* V = p.v + b * p.v_sb + kvh * p.v_sh;
@@ -592,12 +630,12 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
     }
   };
   restart();
-  issue(0, r0);
-  issue(1, r1);
-  issue(2, r2);
+  issue(t_begin, r0);
+  issue(t_begin + 1, r1);
+  issue(t_begin + 2, r2);
   m_wait_barrier<4 * DJ>();
   products(r0, s, dp);
-  for (int t = 0; t < t_end; t += 4) {
+  for (int t = t_begin; t < t_end; t += 4) {
     iter(t, r0, r1, r3);
     if (t + 1 >= t_end) break;
     iter(t + 1, r1, r2, r0);
@@ -615,7 +653,7 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
     for (int i = 0; i < 16; ++i) odd |= !(fabsf(dq[db][i]) < INFINITY);
   if (__syncthreads_or(odd && live)) {
     restart();
-    for (int t = 0; t < t_end; ++t) {
+    for (int t = t_begin; t < t_end; ++t) {
       __syncthreads();
       issue(t, r0);
       m_wait<0>();
@@ -636,6 +674,16 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
   }
   if (!live) return;
   const float x = (CAP ? 4.0f : 1.0f) * p.sm_scale * (F16 ? (sc.s == 0.f ? 0.f : 1.0f / sc.s) : 1.0f);
+  if (piece.part >= 0) {
+    float* P = p.qpart + ((int64_t)piece.part * kMRows + wave * 32 + l32) * HD;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(P + db * 32 + 8 * g + 4 * hi) =
+            f32x4{dq[db][4 * g] * x, dq[db][4 * g + 1] * x, dq[db][4 * g + 2] * x, dq[db][4 * g + 3] * x};
+    return;
+  }
   uint16_t* DQ = p.dq + b * p.dq_sb + h * p.dq_sh + m_tok * p.dq_sm;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -648,16 +696,64 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
     }
 }
 
+// The parts of blocks that were cut, added up: of dk and dv in the first `key_cuts`
+// workgroups, then of dq; HD / 4 lanes a row.
+template <int HD, bool F16>
+__global__ __launch_bounds__(256) void attn_masked_grad_join_kernel(BwdArgs p, int key_cuts) {
+  constexpr int L = HD / 4;
+  const bool of_keys = (int)blockIdx.x < key_cuts;
+  const int i = blockIdx.x - (of_keys ? 0 : key_cuts), kvh = i % p.Hk;
+  const Deal* d = of_keys ? p.keys : p.rows;
+  if (i / p.Hk >= d->cuts) return;
+  const int4 c = d->cut[i / p.Hk];
+  const int row = blockIdx.y * (256 / L) + threadIdx.x / L, at = threadIdx.x % L;
+  const f32x4* P = reinterpret_cast<const f32x4*>(of_keys ? p.kpart : p.qpart) +
+                   (((int64_t)c.z * p.Hk + kvh) * kMRows + row) * L + at;
+  f32x4 x = P[0];
+#pragma unroll 4
+  for (int k = 1; k < c.y; ++k) x += P[(int64_t)k * p.Hk * kMRows * L];
+  uint16_t* to;
+  if (of_keys) {
+    const int blocks = (p.mask.N + kKeys - 1) / kKeys, b = c.x / blocks;
+    const int64_t j = c.x % blocks * kKeys + row % kKeys;
+    if (j >= p.mask.N) return;
+    to = row < kKeys ? p.dk + b * p.dk_sb + kvh * p.dk_sh + j * p.dk_sn
+                     : p.dv + b * p.dv_sb + kvh * p.dv_sh + j * p.dv_sn;
+  } else {
+    const int blocks = (p.R + kMRows - 1) / kMRows, b = c.x / blocks, r = c.x % blocks * kMRows + row;
+    if (r >= p.R) return;
+    to = p.dq + b * p.dq_sb + ((int64_t)kvh * p.G + r % p.G) * p.dq_sh + (int64_t)(r / p.G) * p.dq_sm;
+  }
+  const bf16x2 lo = pack2<F16>(x[0], x[1]), hi = pack2<F16>(x[2], x[3]);
+  *reinterpret_cast<u32x2*>(to + 4 * at) = u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+
+// Workgroups that are resident at once.
+template <int HD> constexpr int kKeySpans = kCus * (HD == 64 ? 2 : 1);
+constexpr int kRowSpans = kCus * 2;
+
 template <int HD, bool F16, bool CAP, bool SLOPE>
 hipError_t launch_one(const BwdArgs& a, int64_t problems, hipStream_t s) {
-  const int64_t kb = (a.mask.N + kKeys - 1) / kKeys, qb = (a.R + kMRows - 1) / kMRows;
+  const int64_t kb = (a.mask.N + kKeys - 1) / kKeys, qb = (a.R + kMRows - 1) / kMRows, B = problems / a.Hk;
+  // As in the forward: a head's pieces are fewer than its blocks and spans / Hk.
+  const int64_t k_cuts = kKeySpans<HD> / a.Hk * a.Hk, q_cuts = kRowSpans / a.Hk * a.Hk;
+  hipError_t e;
+  if (a.rows) {
+    e = deal_out(a.mask, (int)B, a.Hk, a.G, {const_cast<Deal*>(a.rows), (int)qb, kRowSpans},
+                 {const_cast<Deal*>(a.keys), (int)kb, kKeySpans<HD>}, s);
+    if (e != hipSuccess) return e;
+  }
   if (kb > 0)
-    hipLaunchKernelGGL((attn_masked_dkdv_kernel<HD, F16, CAP, SLOPE>), dim3((unsigned)(kb * problems)),
-                       dim3(kMThreads), 0, s, a);
-  const hipError_t e = hipGetLastError();
+    hipLaunchKernelGGL((attn_masked_dkdv_kernel<HD, F16, CAP, SLOPE>),
+                       dim3((unsigned)(kb * problems + (a.keys ? k_cuts : 0))), dim3(kMThreads), 0, s, a);
+  e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((attn_masked_dq_kernel<HD, F16, CAP, SLOPE>), dim3((unsigned)(qb * problems)),
-                     dim3(kMThreads), 0, s, a);
+  hipLaunchKernelGGL((attn_masked_dq_kernel<HD, F16, CAP, SLOPE>),
+                     dim3((unsigned)(qb * problems + (a.rows ? q_cuts : 0))), dim3(kMThreads), 0, s, a);
+  e = hipGetLastError();
+  if (e != hipSuccess || !a.rows || k_cuts + q_cuts == 0) return e;
+  hipLaunchKernelGGL((attn_masked_grad_join_kernel<HD, F16>), dim3((unsigned)(k_cuts + q_cuts), kMRows * HD / 4 / 256),
+                     dim3(256), 0, s, a, (int)k_cuts);
   return hipGetLastError();
 }
 
@@ -673,6 +769,30 @@ hipError_t launch(const BwdArgs& a, int64_t problems, bool cap, hipStream_t s) {
                   : launch_one<HD, F16, false, false>(a, problems, s);
 }
 
+// Whether the blocks are counted, cut and sorted first, as far as the rows decide it,
+// and then.  It costs 17 us in all, and pays where the key blocks are few enough for
+// the longest to decide (shared key heads above all).  Measured (us of all kernels,
+// without and with; bf16, causal):
+//   2 x 16 heads of 64 on 2 x 4, 2,048 tokens (256 key blocks)       157   115
+//   8 of 64, 4,096 tokens (512)                                      143   122
+//   16 of 64, 4,096 tokens (1,024)                                   177   184
+//   8 of 64, 8,192 tokens (1,024)                                    315   305
+//   4 x 16 of 64, 2,048 tokens, four documents (2,048)               131   152
+//   8 of 128, 4,096 tokens (512)                                     247   214
+//   2 x 16 of 128 on 2 x 4, 2,048 tokens, four documents (256)       229   185
+bool may_deal(int64_t problems, int64_t B, int64_t R) {
+  const int64_t qb = (R + kMRows - 1) / kMRows;
+  return qb * problems >= 128 && R >= 2048 && R < (int64_t)1 << 24 && qb * B <= kDealItems;
+}
+bool deals(Unequal u, int64_t problems, int64_t B, int64_t R, int64_t N) {
+  const int64_t kb = (N + kKeys - 1) / kKeys;
+  return u != Unequal::no && may_deal(problems, B, R) && N >= 2048 && kb * problems < 4 * kCus && kb * B <= kDealItems;
+}
+size_t record_floats(int64_t problems, int64_t R) { return (size_t)problems * ((R + kRowTile - 1) / kRowTile) * kRec; }
+// Parts of the lists at most: two for each resident workgroup.
+template <int HD> constexpr size_t kKeyPart = (size_t)2 * kKeySpans<HD> * 2 * kKeys * HD;
+template <int HD> constexpr size_t kRowPart = (size_t)2 * kRowSpans * kMRows * HD;
+
 }  // namespace
 }  // namespace gpa
 
@@ -680,7 +800,9 @@ using namespace gpa;
 
 extern "C" size_t gpa_attn_masked_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t M) {
   if (B <= 0 || H <= 0 || Hk <= 0 || M <= 0 || H % Hk) return 0;
-  return (size_t)B * Hk * ((H / Hk * M + kRowTile - 1) / kRowTile) * kRec * sizeof(float);
+  const int64_t R = H / Hk * M;
+  const size_t rec = record_floats(B * Hk, R) * sizeof(float);
+  return may_deal(B * Hk, B, R) ? rec + 2 * sizeof(Deal) + (kKeyPart<128> + kRowPart<128>) * sizeof(float) : rec;
 }
 
 extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* args,
@@ -753,6 +875,13 @@ extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* args,
   f.lse_sb = a->lse_sb; f.lse_sh = a->lse_sh;
   f.slopes = a->slopes; f.slopes_sb = a->slopes_sb;
   f.rec = (float*)workspace;
+  if (deals(unequal_of(*a), problems, a->B, a->M * G, a->N)) {
+    Deal* d = (Deal*)(f.rec + record_floats(problems, a->M * G));
+    f.rows = d;
+    f.keys = d + 1;
+    f.kpart = (float*)(d + 2);
+    f.qpart = f.kpart + (a->D == 64 ? kKeyPart<64> : kKeyPart<128>);
+  }
   f.Hk = (int32_t)a->Hk; f.G = (int32_t)G; f.R = (int32_t)(a->M * G); f.tiles = (int32_t)tiles;
   f.sm_scale = a->sm_scale;
   masked_fill(a, &f.mask, &f.score);

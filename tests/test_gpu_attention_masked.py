@@ -146,6 +146,18 @@ def test_blocks_of_unequal_length(dev):
     _check(dev, 6, 22, 11, 70, 2100, 128, BF, seed=26, back=False, k_offsets=lens)
 
 
+def test_gradients_of_blocks_of_unequal_length(dev):
+    _check(dev, 1, 8, 8, 2100, 2100, 64, BF, seed=31, causal=True, slopes=torch.rand(8))
+    _check(dev, 1, 8, 8, 2100, 2100, 128, HF, seed=32, causal=True, prefix=900, cap=20.0)
+    off = [40, 41, 600, 600, 1990, 2060]
+    _check(dev, 1, 12, 4, 2100, 2100, 128, BF, seed=33, offsets=off, with_lse_grad=True)
+    _check(dev, 1, 15, 5, 2100, 2100, 64, HF, seed=34, offsets=off, causal=True, prefix=[1, 0, 5, 3000, 2])
+    lens = [[0, n] for n in (2100, 0, 1, 2099, 64, 1025)]
+    _check(dev, 6, 33, 3, 190, 2100, 64, BF, seed=35, causal=True, k_offsets=lens, cap=30.0)
+    _check(dev, 1, 520, 520, 40, 2050, 128, BF, seed=36, causal=True)      # rows too few to be dealt out
+    _check(dev, 1, 2048, 1, 10, 2050, 64, BF, seed=37, causal=True)        # one head: every part its own
+
+
 def test_more_heads_than_workgroups_at_once(dev):
     _check(dev, 1, 800, 800, 33, 2020, 64, BF, seed=27, back=False, causal=True, offsets=[0, 3, 33],
            k_offsets=[0, 1000, 2020])
