@@ -255,6 +255,23 @@ __device__ __forceinline__ void pack_frags(const float (&p)[16], bf16x8 (&out)[2
     }
 }
 
+// sum + the sum of a fragment's values, as the matrix instructions take them.
+template <bool F16>
+__device__ __forceinline__ float sum_frag(const bf16x8& x, float sum) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+  const u32x4 y = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = y[i];                   // a bit_cast of the element itself reads another one
+    if constexpr (F16)
+      sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), f16x2{1, 1}, sum, false);
+    else
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b16x2, w), b16x2{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
+  }
+  return sum;
+}
+
 // acc += A^T . P over a tile's rows where a row that a lane does not see may
 // hold infinities or NaN: 0 times them is NaN, so such values are taken out of
 // the product and the rows that do see them get them back by their sign: an

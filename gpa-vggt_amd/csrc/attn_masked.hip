@@ -64,6 +64,7 @@ template <int HD> constexpr int kPerCu = HD == 64 ? 3 : 2;   // workgroups to a 
 struct FwdArgs {
   const uint16_t* q;
   uint16_t* o;
+  uint16_t* rest;         // what rounding took from o (nullable), laid out as it
   float* lse;             // nullable
   int64_t q_sb, q_sh, q_sm, o_sb, o_sh, o_sm, lse_sb, lse_sh;
   const float* slopes;
@@ -120,6 +121,18 @@ __device__ __forceinline__ Row locate(const FwdArgs& p, const FwdSet& S, int pro
   return x;
 }
 
+// What rounding took from four values, rounded itself; none of a value that is not finite.
+template <bool F16>
+__device__ __forceinline__ u32x2 rest_of(f32x4 x, bf16x2 lo, bf16x2 hi) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[e] -= half_to_f32<F16>(e < 2 ? lo[e] : hi[e - 2]);
+    x[e] = fabsf(x[e]) < INFINITY ? x[e] : 0.f;
+  }
+  const bf16x2 a = pack2<F16>(x[0], x[1]), b = pack2<F16>(x[2], x[3]);
+  return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+}
+
 // Where a row's unnormalised outputs, offset and sum go (null: to no partial).
 struct Part {
   float* o;
@@ -148,7 +161,7 @@ struct Rows {
   float slope;
   bf16x8 qf[KS];
   f32x16 o[DB];
-  float m, l;
+  float m, l, n;           // offset; sums of the weights, and of the rounded ones
 
   __device__ __forceinline__ Rows(const FwdArgs& p, const Row& x, int lane)
       : sc(p.score), rd(lane), hi(lane >> 5), lo(x.lo), end(x.hi), at(x.at), slope(0.f) {
@@ -159,7 +172,7 @@ struct Rows {
   }
   __device__ __forceinline__ void restart() {
     m = -1.0e30f;                              // finite: -inf - m is -inf
-    l = 0.f;
+    l = n = 0.f;
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = f32x16{};
   }
@@ -225,6 +238,7 @@ struct Rows {
       const float alpha = __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
       l *= alpha;
+      n *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] *= alpha;
     }
@@ -240,6 +254,8 @@ struct Rows {
   __device__ __forceinline__ void add(const uint16_t* v, const float (&x)[16]) {
     bf16x8 pb[2];
     pack_frags<F16>(x, pb);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) n = sum_frag<F16>(pb[s], n);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -259,6 +275,8 @@ struct Rows {
     pack_frags<F16>(x, pb);
     pack_frags<F16>(seen, sb);
 #pragma unroll
+    for (int s = 0; s < 2; ++s) n = sum_frag<F16>(pb[s], n);
+#pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = careful_mfma<HD, F16>(rd, v, db, pb, sb, o[db]);
   }
   __device__ __forceinline__ bool odd() const {
@@ -269,11 +287,17 @@ struct Rows {
       for (int i = 0; i < 16; ++i) x |= !(fabsf(o[db][i]) < INFINITY);
     return x;
   }
-  // The rows' outputs, or with `to` this lane's part of them; `total` is the sum over
-  // both halves.
-  __device__ __forceinline__ void finish(const FwdArgs& p, const Row& x, Part to, float total) {
+  // The rows' outputs, or with `to` this lane's part of them; `total` and `norm` are l
+  // and n over both halves.  Outputs are divided by the sum of the weights as they
+  // were rounded, so a weight that stands alone loses nothing: 0.6 to 1.0 instead of
+  // 1.7 thousandths of the output's norm in bf16.  The LSE has the exact weights;
+  // parts are scaled to go with their sum.
+  __device__ __forceinline__ void finish(const FwdArgs& p, const Row& x, Part to, float total, float norm) {
     if (!x.live) return;
     if (to.o) {
+      const float a = norm == 0.f ? 0.f : total / norm;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] *= a;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -283,7 +307,7 @@ struct Rows {
       if (hi == 0) *to.stat = float2{m, total};
       return;
     }
-    const float inv = total == 0.f ? 0.f : 1.0f / total;   // no key seen: zeros
+    const float inv = norm == 0.f ? 0.f : 1.0f / norm;   // no key seen: zeros
     uint16_t* O = p.o + x.b * p.o_sb + x.h * p.o_sh + x.tok * p.o_sm;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -293,6 +317,9 @@ struct Rows {
         const bf16x2 b = pack2<F16>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv);
         *reinterpret_cast<u32x2*>(O + db * 32 + 8 * g + 4 * hi) =
             u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+        if (p.rest)
+          *reinterpret_cast<u32x2*>(p.rest + (O - p.o) + db * 32 + 8 * g + 4 * hi) =
+              rest_of<F16>(f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]} * inv, a, b);
       }
     if (p.lse && hi == 0)
       p.lse[x.b * p.lse_sb + x.h * p.lse_sh + x.tok] = total == 0.f ? -INFINITY : m + __log2f(total);
@@ -408,7 +435,7 @@ __device__ __forceinline__ void walk(const FwdArgs& p, const FwdSet& S, int prob
       R.careful(r0.k, r0.v, n_lo + t * kMTile);
     }
   }
-  R.finish(p, row, part(row), sum_halves(R.l));
+  R.finish(p, row, part(row), sum_halves(R.l), sum_halves(R.n));
 }
 
 // A block, or split z of it.
@@ -446,8 +473,9 @@ template <bool F16>
 __device__ __forceinline__ void emit(const FwdArgs& p, int64_t b, int64_t h, int64_t tok, int at, f32x4 o, float total) {
   const float inv = total == 0.f ? 0.f : 1.0f / total;
   const bf16x2 lo = pack2<F16>(o[0] * inv, o[1] * inv), hi = pack2<F16>(o[2] * inv, o[3] * inv);
-  *reinterpret_cast<u32x2*>(p.o + b * p.o_sb + h * p.o_sh + tok * p.o_sm + 4 * at) =
-      u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+  const int64_t to = b * p.o_sb + h * p.o_sh + tok * p.o_sm + 4 * at;
+  *reinterpret_cast<u32x2*>(p.o + to) = u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+  if (p.rest) *reinterpret_cast<u32x2*>(p.rest + to) = rest_of<F16>(o * inv, lo, hi);
 }
 
 // The pieces of a block that was cut, put together, HD / 4 lanes a row.
@@ -545,6 +573,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_few_k
 
   // The four waves' results in wave 0, by way of K's buffers, all at one offset.
   float total = sum_halves(R.l);
+  const float norm = sum_halves(R.n), even = norm == 0.f ? 0.f : total / norm;
   if (lane < 32) {
     stat[wave][0][lane] = R.m;
     stat[wave][1][lane] = total;
@@ -557,7 +586,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_few_k
 #pragma unroll
   for (int i = 0; i < kMWaves; ++i)
     total = __builtin_fmaf(__builtin_amdgcn_exp2f(stat[i][0][lane & 31] - m), stat[i][1][lane & 31], total);
-  const float alpha = __builtin_amdgcn_exp2f(R.m - m);
+  const float alpha = __builtin_amdgcn_exp2f(R.m - m) * even;
 #pragma unroll
   for (int db = 0; db < DB; ++db) R.o[db] *= alpha;
   R.m = m;
@@ -588,7 +617,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_few_k
   __syncthreads();
   if (wave > 0) return;
   take(0);
-  R.finish(p, row, split_part<HD>(p, S, row, z), total);
+  R.finish(p, row, split_part<HD>(p, S, row, z), total, total);
 }
 
 // The partial outputs of a row's splits put together, by WAVES waves.
@@ -819,7 +848,7 @@ int gpa::masked_check(const char* fn, int dtype, const gpa_attn_masked_args* a, 
   }
   const int64_t B = a->B, H = a->H, Hk = a->Hk;
   if (!rows_aligned(a->q, B, a->q_sb, H, a->q_sh, a->M, a->q_sm) ||
-      (has_o && !rows_aligned(a->o, B, a->o_sb, H, a->o_sh, a->M, a->o_sm)) ||
+      (has_o && (!rows_aligned(a->o, B, a->o_sb, H, a->o_sh, a->M, a->o_sm) || (uintptr_t)a->o_rest % 16)) ||
       (keys && (!rows_aligned(a->k, B, a->k_sb, Hk, a->k_sh, a->N, a->k_sn) ||
                 !rows_aligned(a->v, B, a->v_sb, Hk, a->v_sh, a->N, a->v_sn))) ||
       (pre && (!rows_aligned(a->pk, 1, 0, Hk, a->pk_sh, a->P, a->pk_sn) ||
@@ -905,6 +934,7 @@ extern "C" int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void
   FwdArgs f{};
   f.q = (const uint16_t*)a->q;
   f.o = (uint16_t*)a->o;
+  f.rest = (uint16_t*)a->o_rest;
   f.lse = a->lse;
   f.q_sb = a->q_sb; f.q_sh = a->q_sh; f.q_sm = a->q_sm;
   f.o_sb = a->o_sb; f.o_sh = a->o_sh; f.o_sm = a->o_sm;

@@ -7,7 +7,10 @@
 //   dQ_i  = sm_scale sum_j dS_ij K_j
 //
 // attn_masked_delta_kernel writes a record of every 64 rows: their LSE, -delta,
-// token and slope.
+// token and slope.  delta comes from O and what rounding took from it: where a
+// row's weights are sharp, dP - delta is small beside both, and delta from the
+// rounded O alone put dq and dk 1.9 to 2.5 roundings off (1.4 with the rest; that
+// of dS is left).
 //
 // attn_masked_dkdv_kernel: a workgroup has 64 keys and walks the rows that see
 // them, all query heads of the key head, so a shared head's gradient is one sum
@@ -45,7 +48,7 @@ constexpr int kRec = 4 * kRowTile;             // lse (less cap log2(e)), -delta
 constexpr int kKeys = 64;                      // keys of a dk, dv workgroup
 
 struct BwdArgs {
-  const uint16_t *q, *k, *v, *o, *d_o;
+  const uint16_t *q, *k, *v, *o, *rest, *d_o;
   const float *lse, *d_lse;
   uint16_t *dq, *dk, *dv;
   int64_t q_sb, q_sh, q_sm, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, o_sb, o_sh, o_sm;
@@ -91,11 +94,18 @@ __global__ __launch_bounds__(256) void attn_masked_delta_kernel(BwdArgs p) {
     if (r < p.R) {
       m = r / p.G;
       const int h = kvh * p.G + r % p.G;
-      const bf16x8 x = *reinterpret_cast<const bf16x8*>(p.o + b * p.o_sb + h * p.o_sh + m * p.o_sm + 8 * ch);
+      const int64_t at = b * p.o_sb + h * p.o_sh + m * p.o_sm + 8 * ch;
+      const bf16x8 x = *reinterpret_cast<const bf16x8*>(p.o + at);
       const bf16x8 y = *reinterpret_cast<const bf16x8*>(p.d_o + b * p.do_sb + h * p.do_sh + m * p.do_sm + 8 * ch);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         delta = __builtin_fmaf(half_to_f32<F16>(x[e]), half_to_f32<F16>(y[e]), delta);
+      if (p.rest) {
+        const bf16x8 z = *reinterpret_cast<const bf16x8*>(p.rest + at);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          delta = __builtin_fmaf(half_to_f32<F16>(z[e]), half_to_f32<F16>(y[e]), delta);
+      }
       lse = p.lse[b * p.lse_sb + h * p.lse_sh + m];
       if (lse == -INFINITY) lse = INFINITY;    // a row that sees nothing
       if (p.slopes) slope = p.slopes[b * p.slopes_sb + h] * kMLog2e;
@@ -861,7 +871,7 @@ extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* args,
   }
   BwdArgs f{};
   f.q = (const uint16_t*)a->q; f.k = (const uint16_t*)a->k; f.v = (const uint16_t*)a->v;
-  f.o = (const uint16_t*)a->o; f.d_o = (const uint16_t*)g->d_o;
+  f.o = (const uint16_t*)a->o; f.rest = (const uint16_t*)a->o_rest; f.d_o = (const uint16_t*)g->d_o;
   f.lse = a->lse; f.d_lse = g->d_lse;
   f.dq = (uint16_t*)g->dq; f.dk = (uint16_t*)g->dk; f.dv = (uint16_t*)g->dv;
   f.q_sb = a->q_sb; f.q_sh = a->q_sh; f.q_sm = a->q_sm;

@@ -44,9 +44,10 @@ the custom ops:
     gpa::attn_masked(Tensor q, Tensor k, Tensor v, float sm_scale, float cap,
                      Tensor? slopes, bool causal, Tensor? prefix, int prefix_len,
                      Tensor? q_offsets, Tensor? k_offsets, bool want_lse,
-                     bool lse_grad) -> (Tensor o, Tensor lse)       (differentiable)
+                     bool lse_grad, bool want_rest)
+                     -> (Tensor o, Tensor lse, Tensor rest)         (differentiable)
     gpa::attn_masked_bwd(Tensor d_o, Tensor? d_lse, Tensor q, Tensor k, Tensor v,
-                         Tensor o, Tensor lse, float sm_scale, float cap,
+                         Tensor o, Tensor? rest, Tensor lse, float sm_scale, float cap,
                          Tensor? slopes, bool causal, Tensor? prefix, int prefix_len,
                          Tensor? q_offsets, Tensor? k_offsets)
                          -> (Tensor dq, Tensor dk, Tensor dv)
@@ -124,7 +125,7 @@ _MaskedArgs = _struct("_MaskedArgs", (
     "l: q_sb q_sh q_sm k_sb k_sh k_sn v_sb v_sh v_sn o_sb o_sh o_sm lse_sb lse_sh",
     "p: slopes", "l: slopes_sb", "p: q_offsets k_offsets", "l: qo_sb ko_sb docs",
     "p: prefix", "l: prefix_sb prefix_len", "p: lens pk pv", "l: P pk_sh pk_sn pv_sh pv_sn",
-    "i: causal", "f: sm_scale cap"))
+    "i: causal", "f: sm_scale cap", "p: o_rest"))
 _MaskedGrads = _struct("_MaskedGrads", (
     "p: d_o d_lse dq dk dv",
     "l: do_sb do_sh do_sm dq_sb dq_sh dq_sm dk_sb dk_sh dk_sn dv_sb dv_sh dv_sn"))
@@ -1229,7 +1230,7 @@ def _table(what, name, t, B, width, dtype):
 
 
 def _masked_args(what, q, k, v, o, lse, sm_scale, cap, slopes, causal, prefix=None, prefix_len=0,
-                 q_offsets=None, k_offsets=None, lens=None, pk=None, pv=None):
+                 q_offsets=None, k_offsets=None, lens=None, pk=None, pv=None, rest=None):
     """The filled gpa_attn_masked_args, and the tensors it points into."""
     B, H, M, D = q.shape
     Hk, N = k.shape[1], k.shape[2]
@@ -1255,20 +1256,22 @@ def _masked_args(what, q, k, v, o, lse, sm_scale, cap, slopes, causal, prefix=No
         ptr(slopes), sl_sb, ptr(q_offsets), ptr(k_offsets), qo_sb, ko_sb, docs,
         ptr(prefix), pre_sb, prefix_len, ptr(lens), ptr(pk), ptr(pv),
         *((0, 0, 0, 0, 0) if pk is None else (pk.shape[1], *pk.stride()[:2], *pv.stride()[:2])),
-        int(causal), sm_scale, cap)
-    return a, (q, k, v, o, lse, slopes, q_offsets, k_offsets, prefix, lens, pk, pv)
+        int(causal), sm_scale, cap, ptr(rest))
+    return a, (q, k, v, o, lse, slopes, q_offsets, k_offsets, prefix, lens, pk, pv, rest)
 
 
-def _masked_run(what, q, k, v, want_lse, *args, pk=None, pv=None, **kwargs):
-    """Allocate and launch gpa_attn_masked."""
+def _masked_run(what, q, k, v, want_lse, *args, want_rest=False, pk=None, pv=None, **kwargs):
+    """Allocate and launch gpa_attn_masked: (o, lse, rest)."""
     dev = q.device
     o = _like(q)
+    rest = _like(q) if want_rest else q.new_empty(0)
     B, H, M, D = q.shape
     lse = torch.empty((B, H, M) if want_lse else (0,), device=dev, dtype=torch.float32)
     q, k, v = _rows8(q), _rows8(k), _rows8(v)
     if pk is not None:
         pk, pv = _rows8(pk), _rows8(pv)
-    a, held = _masked_args(what, q, k, v, o, lse if want_lse else None, *args, pk=pk, pv=pv, **kwargs)
+    a, held = _masked_args(what, q, k, v, o, lse if want_lse else None, *args, pk=pk, pv=pv,
+                           rest=rest if want_rest else None, **kwargs)
     L = lib()
     P = 0 if pk is None else pk.shape[1]
     ws_bytes = L.gpa_attn_masked_workspace_bytes(B, H, k.shape[1], M, k.shape[2], P, D)
@@ -1276,45 +1279,44 @@ def _masked_run(what, q, k, v, want_lse, *args, pk=None, pv=None, **kwargs):
     with _on(dev):
         rc = L.gpa_attn_masked(_DTYPE_CODES[q.dtype], a, None if ws is None else ws.data_ptr(), ws_bytes, _stream(dev))
     _check(rc, what)
-    return o, lse
+    return o, lse, rest
 
 
 def _masked_setup(ctx, inputs, output):
-    q, k, v, sm_scale, cap, slopes, causal, prefix, prefix_len, qo, ko, want_lse, lse_grad = inputs
-    o, lse = output
-    if not want_lse:
-        raise RuntimeError("gpa::attn_masked: gradients need the LSE (want_lse)")
+    q, k, v, sm_scale, cap, slopes, causal, prefix, prefix_len, qo, ko, want_lse, lse_grad, want_rest = inputs
+    o, lse, rest = output
+    if not (want_lse and want_rest):
+        raise RuntimeError("gpa::attn_masked: gradients need the LSE and the rest (want_lse, want_rest)")
     ctx.set_materialize_grads(False)
-    if not lse_grad:
-        ctx.mark_non_differentiable(lse)
-    ctx.save_for_backward(q, k, v, o, lse, slopes, prefix, qo, ko)
+    ctx.mark_non_differentiable(*((rest,) if lse_grad else (lse, rest)))
+    ctx.save_for_backward(q, k, v, o, rest, lse, slopes, prefix, qo, ko)
     ctx.rest = (sm_scale, cap, causal, prefix_len)
 
 
-def _masked_backward(ctx, d_o, d_lse):
-    q, k, v, o, lse, slopes, prefix, qo, ko = ctx.saved_tensors
+def _masked_backward(ctx, d_o, d_lse, _d_rest):
+    q, k, v, o, rest, lse, slopes, prefix, qo, ko = ctx.saved_tensors
     sm_scale, cap, causal, prefix_len = ctx.rest
     if ctx.needs_input_grad[5]:
         raise RuntimeError("gpa::attn_masked: the slopes have no gradient")
     grads = (None, None, None)
     if d_o is not None or d_lse is not None:
-        grads = attn_masked_bwd(torch.zeros_like(o) if d_o is None else d_o, d_lse, q, k, v, o, lse,
+        grads = attn_masked_bwd(torch.zeros_like(o) if d_o is None else d_o, d_lse, q, k, v, o, rest, lse,
                                 sm_scale, cap, slopes, causal, prefix, prefix_len, qo, ko)
-    return (*grads,) + (None,) * 10
+    return (*grads,) + (None,) * 11
 
 
 def attn_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale: float, cap: float,
                 slopes: Optional[torch.Tensor], causal: bool, prefix: Optional[torch.Tensor],
                 prefix_len: int, q_offsets: Optional[torch.Tensor],
                 k_offsets: Optional[torch.Tensor], want_lse: bool,
-                lse_grad: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """gpa_attn_masked: o like q, and the log2 LSE [B, H, M] fp32 if want_lse
-    (else an empty tensor), which gradients need; lse_grad: the LSE is
-    differentiable too.  cap 0: none."""
+                lse_grad: bool, want_rest: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """gpa_attn_masked: o like q, the log2 LSE [B, H, M] fp32 if want_lse and
+    what rounding took from o if want_rest (else empty tensors); gradients need
+    both.  lse_grad: the LSE is differentiable too.  cap 0: none."""
     _require_gpu(*[t for t in (q, k, v, slopes, prefix, q_offsets, k_offsets) if t is not None])
     _masked_shapes("gpa::attn_masked", q, k, v)
     return _masked_run("gpa::attn_masked", q, k, v, want_lse, sm_scale, cap, slopes, causal, prefix,
-                       prefix_len, q_offsets, k_offsets)
+                       prefix_len, q_offsets, k_offsets, want_rest=want_rest)
 
 
 attn_masked = _op(attn_masked, _masked_setup, _masked_backward)
@@ -1322,24 +1324,26 @@ attn_masked = _op(attn_masked, _masked_setup, _masked_backward)
 
 @_fake("attn_masked")
 def _attn_masked_fake(q, k, v, sm_scale, cap, slopes, causal, prefix, prefix_len, q_offsets,
-                      k_offsets, want_lse, lse_grad):
-    return _like(q), q.new_empty(q.shape[:3] if want_lse else (0,), dtype=torch.float32)
+                      k_offsets, want_lse, lse_grad, want_rest):
+    return (_like(q), q.new_empty(q.shape[:3] if want_lse else (0,), dtype=torch.float32),
+            _like(q) if want_rest else q.new_empty(0))
 
 
 @_op
 def attn_masked_bwd(d_o: torch.Tensor, d_lse: Optional[torch.Tensor], q: torch.Tensor,
-                    k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
-                    sm_scale: float, cap: float, slopes: Optional[torch.Tensor], causal: bool,
+                    k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
+                    rest: Optional[torch.Tensor], lse: torch.Tensor, sm_scale: float, cap: float, slopes: Optional[torch.Tensor], causal: bool,
                     prefix: Optional[torch.Tensor], prefix_len: int,
                     q_offsets: Optional[torch.Tensor], k_offsets: Optional[torch.Tensor]
                     ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """gpa_attn_masked_bwd: the gradients of q, k and v, in their order of
-    dimensions."""
+    dimensions.  rest: what rounding took from o (None: not known)."""
     what = "gpa::attn_masked_bwd"
-    dev = _require_gpu(*[t for t in (q, k, v, o, lse, d_o, d_lse, slopes, prefix, q_offsets,
+    dev = _require_gpu(*[t for t in (q, k, v, o, rest, lse, d_o, d_lse, slopes, prefix, q_offsets,
                                      k_offsets) if t is not None])
     _masked_shapes(what, q, k, v)
     if o.shape != q.shape or d_o.shape != q.shape or o.dtype != q.dtype or d_o.dtype != q.dtype \
+            or (rest is not None and (rest.shape != q.shape or rest.dtype != q.dtype)) \
             or lse.shape != q.shape[:3] or lse.dtype != torch.float32 \
             or (d_lse is not None and (d_lse.shape != lse.shape or d_lse.dtype != torch.float32)):
         raise ValueError(f"{what}: o {o.dtype} {tuple(o.shape)}, d_o {d_o.dtype} {tuple(d_o.shape)}, "
@@ -1348,10 +1352,12 @@ def attn_masked_bwd(d_o: torch.Tensor, d_lse: Optional[torch.Tensor], q: torch.T
     if q.numel() == 0:
         return dq, dk.zero_(), dv.zero_()
     q, k, v, o, d_o = (_rows8(t) for t in (q, k, v, o, d_o))
+    if rest is not None and (rest.stride() != o.stride() or rest.data_ptr() & 15):
+        rest = torch.empty_strided(o.shape, o.stride(), dtype=o.dtype, device=dev).copy_(rest)
     lse = lse if lse.stride(-1) == 1 else lse.contiguous()
     d_lse = None if d_lse is None else d_lse.contiguous()
     a, held = _masked_args(what, q, k, v, o, lse, sm_scale, cap, slopes, causal, prefix, prefix_len,
-                           q_offsets, k_offsets)
+                           q_offsets, k_offsets, rest=rest)
     g = _MaskedGrads.packed(d_o.data_ptr(), 0 if d_lse is None else d_lse.data_ptr(), dq.data_ptr(),
                             dk.data_ptr(), dv.data_ptr(), *d_o.stride()[:3], *dq.stride()[:3],
                             *dk.stride()[:3], *dv.stride()[:3])
@@ -1365,7 +1371,7 @@ def attn_masked_bwd(d_o: torch.Tensor, d_lse: Optional[torch.Tensor], q: torch.T
 
 
 @_fake("attn_masked_bwd")
-def _attn_masked_bwd_fake(d_o, d_lse, q, k, v, o, lse, sm_scale, cap, slopes, causal, prefix,
+def _attn_masked_bwd_fake(d_o, d_lse, q, k, v, o, rest, lse, sm_scale, cap, slopes, causal, prefix,
                           prefix_len, q_offsets, k_offsets):
     return _like(q), _like(k), _like(v)
 
@@ -1388,7 +1394,7 @@ def attn_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.
                          f"{prefix_k.dtype} {tuple(prefix_k.shape)} and {prefix_v.dtype} "
                          f"{tuple(prefix_v.shape)}")
     return _masked_run(what, q, k, v, want_lse, sm_scale, cap, slopes, True, lens=lengths,
-                       pk=prefix_k, pv=prefix_v)
+                       pk=prefix_k, pv=prefix_v)[:2]
 
 
 @_fake("attn_shared_prefix")

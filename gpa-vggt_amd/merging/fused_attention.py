@@ -174,8 +174,8 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale
             if prefix_len < 0:
                 raise ValueError(f"{what}: prefix {prefix_len} is negative")
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-    o, lse = _native.attn_masked(q, k, v, sm_scale, cap, slopes, bool(causal), prefix, prefix_len,
-                                 offsets, k_offsets, bool(return_lse) or grad, bool(return_lse))
+    o, lse, _ = _native.attn_masked(q, k, v, sm_scale, cap, slopes, bool(causal), prefix, prefix_len,
+                                 offsets, k_offsets, bool(return_lse) or grad, bool(return_lse), grad)
     return (o, lse) if return_lse else o
 
 

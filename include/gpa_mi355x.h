@@ -519,6 +519,8 @@ int gpa_residual_layernorm_f16(const void* x, const void* y, const void* gamma,
  * batch element and are seen by all queries; lens (int32 [B], NULL: all N)
  * says how many of the N own keys each element has.  Both go with docs = 1 and
  * no offsets; lens alone is a padded batch.
+ * o_rest (NULL: not wanted; laid out as o): what rounding took from o, in o's
+ * format.  The gradients take delta = dO . (o + o_rest) from it.
  * workspace: gpa_attn_masked_workspace_bytes(...) bytes, 16-byte aligned,
  * overwritten (0: none).  Key rows (k_sn, v_sn, pk_sn, pv_sn) are less than
  * 2^23 elements apart; a head's keys may span any distance.
@@ -540,6 +542,7 @@ typedef struct gpa_attn_masked_args {
   int64_t P, pk_sh, pk_sn, pv_sh, pv_sn;
   int32_t causal;
   float sm_scale, cap;
+  void* o_rest;
 } gpa_attn_masked_args;
 
 size_t gpa_attn_masked_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t M, int64_t N,
@@ -549,7 +552,8 @@ int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void* workspace
 
 /*
  * Its gradients, from the forward's output o and log2 LSE (args->o and
- * args->lse, both required) and the output's gradient d_o, with d_lse the LSE's
+ * args->lse, both required), args->o_rest (NULL: taken as zero, which costs
+ * where weights are sharp: dq and dk are then off by twice their rounding) and the output's gradient d_o, with d_lse the LSE's
  * (NULL: none; contiguous [B, H, M]): dq, dk and dv in the operands' format,
  * those of a shared key head summed over its query heads.  No shared prefix
  * (P = 0, lens = NULL).  Sums run in a fixed order: two calls give the same

@@ -291,6 +291,38 @@ def test_fp16_gradients_keep_their_bits(dev, size):
         assert rel <= 2 * 2.0 ** -11 + (2.0 ** -25 * math.sqrt(want.numel()) / want.norm().item()), (name, rel)
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("M", [1, 40])
+def test_many_small_weights(dev, M, dt):
+    """20,000 keys at 2^-15 to 2^-17 of the first one's weight, subnormal in fp16, together
+    outweigh a third of it."""
+    q, k, v, _, _ = _inputs(1, 1, 1, M, 20_000, 64, dt, 42, std=0.0)
+    q[..., 0], k[..., 0] = 8.0, -torch.rand(20_000, dtype=torch.float64).to(dt) * 1.4 - 10.4
+    k[:, :, 0, 0] = 0.0
+    ref = masked_attention(q, k, v, 0.125, u=torch.finfo(dt).eps / 2)
+    o, lse = attention_masked(q.to(dev), k.to(dev), v.to(dev), 0.125, return_lse=True)
+    _near("o", o, ref.o, ref.o_bound, dt)
+    assert ((lse.cpu().double() - ref.lse).abs() <= ref.lse_bound).all()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradients_of_sharp_weights(dev, D, dt):
+    """Scores with a spread of 6: dP - delta cancels, so delta has to come from more than
+    the rounded output.  dS and the result are rounded once each, by 0.425 u of a
+    norm (values spread evenly over a binade's logarithm): 0.60 u together, where
+    delta from the rounded output adds 0.8 u."""
+    u = torch.finfo(dt).eps / 2
+    q, k, v, d_o, _ = _inputs(1, 2, 2, 600, 600, D, dt, 41, std=math.sqrt(6.0))
+    x = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    for kw in (dict(), dict(slopes=torch.tensor([0.5, 0.1]))):
+        ref = masked_attention(q, k, v, D ** -0.5, causal=True, d_o=d_o, u=u, **kw)
+        o = attention_masked(*x, D ** -0.5, causal=True, **{n: t.to(dev) for n, t in kw.items()})
+        for name, g, want in zip("qk", torch.autograd.grad(o, x, d_o.to(dev)), ref[2:4]):
+            rel = ((g.cpu().double() - want).norm() / want.norm()).item()
+            assert rel <= 0.75 * u, (name, rel / u)
+
+
 def test_other_stream_and_graph(dev):
     """Captured forward and backward, replayed on new inputs between eager calls."""
     off = torch.tensor([0, 100, 260], dtype=torch.int32, device=dev)
@@ -347,9 +379,10 @@ def test_op_checks(dev):
     q = torch.randn(1, 4, 50, 64, device=dev, dtype=BF, requires_grad=True)
     k = torch.randn(1, 50, 2, 64, device=dev, dtype=BF).transpose(1, 2).requires_grad_()
     torch.library.opcheck(torch.ops.gpa.attn_masked.default,
-                          (q, k, k, 0.125, 20.0, None, True, None, 3, off, off, True, True))
+                          (q, k, k, 0.125, 20.0, None, True, None, 3, off, off, True, True, True))
     from merging import _native
     d = q.detach()
-    o, lse = _native.attn_masked(d, k.detach(), k.detach(), 0.125, 0.0, None, False, None, 0, None, None, True, False)
+    o, lse, rest = _native.attn_masked(d, k.detach(), k.detach(), 0.125, 0.0, None, False, None, 0, None, None, True,
+                                       False, True)
     torch.library.opcheck(torch.ops.gpa.attn_masked_bwd.default,
-                          (d, None, d, k.detach(), k.detach(), o, lse, 0.125, 0.0, None, False, None, 0, None, None))
+                          (d, None, d, k.detach(), k.detach(), o, rest, lse, 0.125, 0.0, None, False, None, 0, None, None))
