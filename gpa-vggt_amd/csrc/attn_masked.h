@@ -255,6 +255,19 @@ __device__ __forceinline__ void pack_frags(const float (&p)[16], bf16x8 (&out)[2
     }
 }
 
+// What rounding took from the first fragment's values, as one more.
+template <bool F16>
+__device__ __forceinline__ bf16x8 rest_frag(const float (&p)[16], const bf16x8& x) {
+  bf16x8 out;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const bf16x2 v = pack2<F16>(p[e] - half_to_f32<F16>(x[e]), p[e + 1] - half_to_f32<F16>(x[e + 1]));
+    out[e] = v[0];
+    out[e + 1] = v[1];
+  }
+  return out;
+}
+
 // sum + the sum of a fragment's values, as the matrix instructions take them.
 template <bool F16>
 __device__ __forceinline__ float sum_frag(const bf16x8& x, float sum) {

@@ -9,8 +9,7 @@
 // attn_masked_delta_kernel writes a record of every 64 rows: their LSE, -delta,
 // token and slope.  delta comes from O and what rounding took from it: where a
 // row's weights are sharp, dP - delta is small beside both, and delta from the
-// rounded O alone put dq and dk 1.9 to 2.5 roundings off (1.4 with the rest; that
-// of dS is left).
+// rounded O alone put dq and dk 1.9 to 2.5 roundings off (1.55 with the rest).
 //
 // attn_masked_dkdv_kernel: a workgroup has 64 keys and walks the rows that see
 // them, all query heads of the key head, so a shared head's gradient is one sum
@@ -33,13 +32,21 @@
 // With a cap, r = 1 / (1 + e^(2u)) gives both: tanh = 1 - 2r, 1 - tanh^2 = 4 (r - r^2).
 //
 // P and dS are rounded to the operand format for the products (the same
-// relative error as the gradients' own rounding); sums are fp32.  Together dq and
-// dk are off by 1.5 times what their own rounding does.  A second product with what
-// rounding took from dS made that 1.1 and the two passes 9 (head dim 128) to
-// 15 % (64) slower: 532 instead of 487 us, 582 instead of 509 (2 x 16 heads on 2 x 4,
-// 4,096 tokens; 8 heads, 8,191 tokens).  In fp16
-// small weights would lose bits below 2^-14, so P is scaled by 2^14 and dS by a
-// power of two that follows its largest value; the sums are scaled back.
+// relative error as the gradients' own rounding); sums are fp32.  Of the two
+// fragments that dS of a tile makes, one goes into a second product with what
+// rounding took from it.  dq and dk are then off by 1.4 times what their own
+// rounding does, against 1.55 without and 1.15 with both fragments; the two passes
+// take 505 us against 487 and 532 (2 x 16 heads of 128 on 2 x 4, 4,096 tokens), and
+// 545 against 500 and 582 (8 heads of 64, 8,191 tokens).  In fp16 small weights
+// would lose bits below 2^-14, so P is scaled by 2^14 and dS by a power of two that
+// follows its largest value; the sums are scaled back.
+//
+// Measured (us): dk, dv 265 and dq 127 at 2 x 16 heads of 128 on 2 x 4, four causal
+// documents of 4,096 tokens in all (375 and 590 TFLOP/s, four and three products);
+// 225 and 203 at 8 of 64, 8,191 tokens, causal with a prefix and slopes (630 and
+// 520).  At head dim 128 dk and dv are bound by LDS reads, 1 KB a matrix
+// instruction, with one wave a SIMD (dK, dV, K and V fill 512 registers); at 64 by
+// vector issue.  delta reads 100 MB in 17.
 #include "attn_masked_deal.h"
 
 #include <algorithm>
@@ -354,12 +361,15 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
       bf16x8 wb[2], db_[2];
       pack_frags<F16>(w, wb);
       pack_frags<F16>(ds, db_);
+      const bf16x8 dr = rest_frag<F16>(ds, db_[0]);
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          const bf16x8 qt = rd.turned(cur.q + half * 32 * HD, db, i);
+          if (i == 0) dk[db] = mfma32x32x16_t<F16>(qt, dr, dk[db]);
           dv[db] = mfma32x32x16_t<F16>(rd.turned(cur.d + half * 32 * HD, db, i), wb[i], dv[db]);
-          dk[db] = mfma32x32x16_t<F16>(rd.turned(cur.q + half * 32 * HD, db, i), db_[i], dk[db]);
+          dk[db] = mfma32x32x16_t<F16>(qt, db_[i], dk[db]);
         }
       s = s_next;
       dp = dp_next;
@@ -632,11 +642,15 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
       weights(s, dp, n0, n0 < a_lo || n0 + kMTile > a_hi, ds);
       bf16x8 db_[2];
       pack_frags<F16>(ds, db_);
+      const bf16x8 dr = rest_frag<F16>(ds, db_[0]);
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          dq[db] = mfma32x32x16_t<F16>(rd.turned(cur.k, db, i), db_[i], dq[db]);
+        for (int i = 0; i < 2; ++i) {
+          const bf16x8 kt = rd.turned(cur.k, db, i);
+          if (i == 0) dq[db] = mfma32x32x16_t<F16>(kt, dr, dq[db]);
+          dq[db] = mfma32x32x16_t<F16>(kt, db_[i], dq[db]);
+        }
       s = s_next;
       dp = dp_next;
     } else {
