@@ -747,13 +747,15 @@ hipError_t launch(const FwdArgs& a, bool cap, hipStream_t s) {
 }
 
 // Splits of a set's key range.  A workgroup walks its keys alone, so few row
-// blocks over many keys are bound by one workgroup's walk; kWant workgroups
-// (two a CU) fill the chip.  A split has at least kLeast tiles: below that
-// the join costs what the shorter walk saves.
-constexpr int64_t kWant = 512;
-int splits_of(int64_t items, int64_t keys) {
+// blocks over many keys are bound by one workgroup's walk; two workgroups a CU fill
+// the chip, and three of 128 rows at head dim 64 (16 heads over 32,771 shared keys:
+// 46 us on 512 workgroups, 38 on 768; the few-row kernel, whose waves walk alone,
+// gains nothing from them).  A split has at least kLeast tiles: below that the join
+// costs what the shorter walk saves.
+int splits_of(int64_t items, int64_t rows, int64_t keys, int64_t D) {
   const int64_t tiles = (keys + kMTile - 1) / kMTile;
-  const int64_t z = std::min({items > 0 ? kWant / items : 1, tiles / kLeast, (int64_t)kMaxSplits / 2});
+  const int64_t want = kCus * (rows > 32 && D == 64 ? kPerCu<64> : 2);
+  const int64_t z = std::min({items > 0 ? want / items : 1, tiles / kLeast, (int64_t)kMaxSplits / 2});
   return (int)std::max<int64_t>(z, 1);
 }
 
@@ -787,9 +789,9 @@ Plan plan(int64_t B, int64_t Hk, int64_t G, int64_t M, int64_t N, int64_t P, int
   if (P > 0) {
     x.p_blocks = (int)((B * M * G + kMRows - 1) / kMRows);
     x.p_problems = (int)Hk;
-    x.p_splits = splits_of((int64_t)x.p_blocks * Hk, P);
+    x.p_splits = splits_of((int64_t)x.p_blocks * Hk, B * M * G, P, D);
   }
-  x.splits = splits_of((int64_t)x.blocks * x.problems, N);
+  x.splits = splits_of((int64_t)x.blocks * x.problems, M * G, N, D);
   const int64_t items = (int64_t)x.blocks * x.problems, spans = kCus * (D == 64 ? kPerCu<64> : kPerCu<128>);
   x.deal = deals(unequal, P, M * G, items, B * x.blocks, N, spans);
   if (x.deal) x.splits = 1;

@@ -57,6 +57,7 @@ namespace {
 constexpr int kRowTile = 64;                   // rows of a record, and of a dk, dv tile
 constexpr int kRec = 4 * kRowTile;             // lse (less cap log2(e)), -delta, token, slope
 constexpr int kKeys = 64;                      // keys of a dk, dv workgroup
+static_assert(kRowTile == 64 && kKeys == 64, "attn_masked_count_kernel counts these");
 
 struct BwdArgs {
   const uint16_t *q, *k, *v, *o, *rest, *d_o;

@@ -63,6 +63,28 @@ def test_null_arguments_and_workspace_alignment():
     assert L.gpa_attn_masked_bwd_workspace_bytes(2, 4, 2, 10) == 2 * 2 * 1 * 256 * 4
 
 
+def test_rest_of_the_output_is_aligned():
+    assert _forward(o_rest=FAKE + 8) == INV
+    assert _native.lib().gpa_last_error()
+
+
+def test_workspaces_of_blocks_in_pieces():
+    """Sized for any mask of the sizes; a call asks for what its own mask needs."""
+    L = _native.lib()
+    big = dict(B=1, H=8, Hk=8, M=4096, N=4096, q_sb=0, k_sb=0, v_sb=0, o_sb=0, q_sh=4096 * 64, k_sh=4096 * 64,
+               v_sh=4096 * 64, o_sh=4096 * 64, q_sm=64, k_sn=64, v_sn=64, o_sm=64)
+    need = L.gpa_attn_masked_workspace_bytes(1, 8, 8, 4096, 4096, 0, 64)
+    assert need > 0
+    assert _forward(ws=FAKE, ws_bytes=need - 1, causal=1, **big) == WSP
+    assert _forward(ws=FAKE, ws_bytes=0, causal=1, **big) == WSP
+    rec = 8 * (4096 // 64) * 256 * 4
+    need = L.gpa_attn_masked_bwd_workspace_bytes(1, 8, 8, 4096)
+    assert need > rec
+    shape = dict(do_sb=0, do_sh=4096 * 64, do_sm=64, dq_sb=0, dq_sh=4096 * 64, dq_sm=64, dk_sb=0, dk_sh=4096 * 64,
+                 dk_sn=64, dv_sb=0, dv_sh=4096 * 64, dv_sn=64)
+    assert _backward(ws_bytes=need - 1, g=shape, lse=FAKE, causal=1, **big) == WSP
+
+
 def test_nothing_to_do_is_ok():
     assert _forward(B=0) == 0 and _forward(M=0) == 0
 

@@ -374,6 +374,14 @@ def test_gradients_by_differences(dev):
             assert abs((up - down) / (2 * eps) - want.reshape(-1)[at]) < 1e-7
 
 
+def test_gradients_need_what_the_forward_kept(dev):
+    from merging import _native
+    q = torch.randn(1, 2, 9, 64, device=dev, dtype=BF, requires_grad=True)
+    for kept in ((False, False), (True, False), (False, True)):
+        with pytest.raises(RuntimeError, match="gradients need"):
+            _native.attn_masked(q, q, q, 0.125, 0.0, None, False, None, 0, None, None, kept[0], False, kept[1])
+
+
 def test_op_checks(dev):
     off = torch.tensor([0, 20, 50], dtype=torch.int32, device=dev)
     q = torch.randn(1, 4, 50, 64, device=dev, dtype=BF, requires_grad=True)
