@@ -7,6 +7,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from merging.fused_attention import attention_masked, attention_shared_prefix
 from merging.fused_norms import norm_gate_residual
@@ -184,3 +185,30 @@ def test_training_on_two_streams(dev):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for runs, w in zip(got, want) for run in runs for a, b in zip(run, w))
     assert not math.isnan(float(want[0][0].float().sum()))
+
+
+def test_compiled_and_checkpointed_blocks(dev):
+    """A block traced as one graph, and one whose forward runs again in the backward
+    pass, give the eager call's bits; a second derivative is refused."""
+    g = torch.Generator(device=dev).manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=g, device=dev).to(BF).requires_grad_()  # noqa: E731
+    x, q, k, v = r(2, 130, 256), r(2, 4, 130, 64), r(2, 2, 130, 64), r(2, 2, 130, 64)
+    w = torch.ones(256, device=dev, dtype=BF, requires_grad=True)
+    off = torch.tensor([0, 40, 130], dtype=torch.int32, device=dev)
+
+    def block(x, q, k, v, w):
+        o = attention_masked(q, k, v, 0.125, causal=True, cap=20.0, offsets=off)
+        return norm_gate_residual(x, o.transpose(1, 2).reshape(2, 130, 256), w, post_weight=w)
+    leaves = [x, q, k, v, w]
+    d = [torch.randn(2, 130, 256, generator=g, device=dev).to(BF) for _ in range(2)]
+
+    def run(fn):
+        out = fn(*leaves)
+        return [*out, *torch.autograd.grad(out, leaves, d)]
+    want = run(block)
+    for fn in (torch.compile(block, backend="aot_eager", fullgraph=True),
+               lambda *a: torch.utils.checkpoint.checkpoint(block, *a, use_reentrant=False)):
+        assert all(torch.equal(a, b) for a, b in zip(run(fn), want))
+    first = torch.autograd.grad(attention_masked(q, k, v, 0.125).float().square().sum(), q, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.float().sum(), q)
