@@ -760,7 +760,7 @@ int splits_of(int64_t items, int64_t rows, int64_t keys, int64_t D) {
 }
 
 // Whether a launch's blocks are counted, cut and sorted first.  That takes two small
-// kernels and a join, 9 us, and pays where the mask makes blocks unequal and their
+// kernels and a join, 10 to 15 us, and pays where the mask makes blocks unequal and their
 // number is between what the splits above fill the chip with and what evens
 // itself out.  Measured (us, without and with; bf16):
 //   one causal document, 8 heads of 64, 4,096 tokens (256 blocks)     71    52
