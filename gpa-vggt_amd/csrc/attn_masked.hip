@@ -8,9 +8,10 @@
 // halves; P^T is used in place as the B operand of O^T += V^T . P^T.  The softmax
 // offset starts at the first tile's row max and moves only where a later one
 // exceeds it by more than the format of P allows (64 for bf16, 15 for fp16, in log2
-// units): the largest |q.k| of a tile bounds its scores (caps and slopes only
-// lower them), so a tile's exact maximum is formed only where the bound passes
-// that.  Sums are fp32; P is rounded to the operand format for the product with V,
+// units): the largest |q.k| of a tile, and what a slope below zero adds to it at the
+// tile's largest distance, bound its scores (caps and slopes above zero only lower
+// them), so a tile's exact maximum is formed only where the bound passes that.
+// Sums are fp32; P is rounded to the operand format for the product with V,
 // as the framework's other attention does (its relative error, 2^-9 or 2^-12,
 // is that of the output's own rounding).
 //
@@ -165,14 +166,17 @@ struct Rows {
   TileReader<HD> rd;
   const int hi;
   int lo, end, at;
-  float slope;
+  float slope, lift;       // lift: what a key of distance 1 gains, 0 but for slopes below zero
   bf16x8 qf[KS];
   f32x16 o[DB];
   float m, l, n;           // offset; sums of the weights, and of the rounded ones
 
   __device__ __forceinline__ Rows(const FwdArgs& p, const Row& x, int lane)
-      : sc(p.score), rd(lane), hi(lane >> 5), lo(x.lo), end(x.hi), at(x.at), slope(0.f) {
-    if constexpr (SLOPE) slope = p.slopes[x.b * p.slopes_sb + x.h] * kMLog2e;
+      : sc(p.score), rd(lane), hi(lane >> 5), lo(x.lo), end(x.hi), at(x.at), slope(0.f), lift(0.f) {
+    if constexpr (SLOPE) {
+      slope = p.slopes[x.b * p.slopes_sb + x.h] * kMLog2e;
+      lift = fmaxf(-slope, 0.f);
+    }
     const uint16_t* Q = p.q + x.b * p.q_sb + x.h * p.q_sh + x.tok * p.q_sm;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(Q + 16 * ks + 8 * hi);
@@ -219,8 +223,8 @@ struct Rows {
     for (int i = 0; i < 16; ++i)
       if (mfma_row(i, 0) < from || mfma_row(i, 0) >= to) x[i] = none;
   }
-  // Before a tile's weights: where its largest |product| does not tell that all
-  // scores lie below the offset's reach, the offset follows the row's maximum, and
+  // Before a tile's weights: where its largest |product| (and distance) does not tell that
+  // all scores lie below the offset's reach, the offset follows the row's maximum, and
   // the sum and the output with it (two branches, the second with nothing but the
   // scaling: as one, the outputs had other registers after it, and every tile that
   // took the other way copied them, 32 moves).  Whether the polynomial serves all
@@ -230,8 +234,12 @@ struct Rows {
 #pragma unroll
     for (int i = 2; i < 16; i += 2) a = fmaxf(fmaxf(a, fabsf(s[i])), fabsf(s[i + 1]));
     const bool poly = CAP && __builtin_amdgcn_ballot_w64(!(a <= sc.lim)) == 0;
-    float m_new = m;
-    if (__builtin_amdgcn_ballot_w64(!(a * sc.c1 <= m + kUp<F16>))) {
+    float m_new = m, bound = a * sc.c1;
+    if constexpr (SLOPE) {
+      const float dist = (float)(at - n0);     // of the tile's first key; its last: 31 less
+      bound = __builtin_fmaf(lift, fmaxf(fabsf(dist), fabsf(dist - (kMTile - 1))), bound);
+    }
+    if (__builtin_amdgcn_ballot_w64(!(bound <= m + kUp<F16>))) {
       float x[16];
       scores<true>(s, n0, poly, 0.f, x);
       if (edge) masked(x, n0, -INFINITY);

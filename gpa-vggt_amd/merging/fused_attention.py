@@ -133,7 +133,7 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale
     key head h // (H // Hk).
 
     x = sm_scale q.k;  s = cap tanh(x / cap) (cap None: x), less
-    slopes[h] * |p_q - p_k| (slopes fp32 [H] or [B, H], constants).
+    slopes[h] * |p_q - p_k| (slopes fp32 [H] or [B, H], of either sign, constants).
 
     Documents: run d holds the queries offsets[d] .. offsets[d + 1] - 1 and the
     keys of k_offsets likewise (int32 [docs + 1], or [B, docs + 1] where they

@@ -75,7 +75,7 @@ def masked_attention(q, k, v, sm_scale, *, cap=None, slopes=None, causal=False, 
                 if slopes is not None:
                     sl = float(slopes[b][h] if slopes.dim() == 2 else slopes[h])
                     s = s - sl * (at - j).abs()
-                    err += 4 * f * sl * max(n, m)
+                    err += 4 * f * abs(sl) * max(n, m)
                 s = s.masked_fill(~seen, -math.inf)
                 ls = torch.logsumexp(s, -1)
                 p = torch.exp(s - ls.clamp_min(-1e300)[:, None])
