@@ -46,7 +46,9 @@
 // A masked key's value does not reach a row: its weight is zero, and where
 // zero times it is not (an infinity or NaN), the workgroup (the wave, where it
 // walks alone) finds a non-finite output at its end and walks its keys again,
-// with such values taken out.
+// with such values taken out.  Weights of up to 2^64 can also take finite bf16
+// values out of fp32's range: an output that is still not below kBig is formed
+// once more, with weights that no sum of finite values passes it with.
 #include "attn_masked_deal.h"
 
 #include <algorithm>
@@ -55,6 +57,9 @@ namespace gpa {
 namespace {
 
 template <bool F16> constexpr float kUp = F16 ? 15.0f : 64.0f;
+// Outputs up to here, in 2^9 parts at once, add up to a finite sum.  Weights of 2^-30
+// keep those of 2^30 keys finite whatever the values are.
+constexpr float kBig = 0x1p100f, kDown = -30.0f;
 
 // One set of rows over one set of keys.
 struct FwdSet {
@@ -229,7 +234,8 @@ struct Rows {
   // scaling: as one, the outputs had other registers after it, and every tile that
   // took the other way copied them, 32 moves).  Whether the polynomial serves all
   // products.
-  __device__ __forceinline__ bool settle(const f32x16& s, int n0, bool edge) {
+  // `up`: how far scores may lie above the offset (below zero: have to lie below it).
+  __device__ __forceinline__ bool settle(const f32x16& s, int n0, bool edge, float up = kUp<F16>) {
     float a = fmaxf(fabsf(s[0]), fabsf(s[1]));
 #pragma unroll
     for (int i = 2; i < 16; i += 2) a = fmaxf(fmaxf(a, fabsf(s[i])), fabsf(s[i + 1]));
@@ -239,7 +245,7 @@ struct Rows {
       const float dist = (float)(at - n0);     // of the tile's first key; its last: 31 less
       bound = __builtin_fmaf(lift, fmaxf(fabsf(dist), fabsf(dist - (kMTile - 1))), bound);
     }
-    if (__builtin_amdgcn_ballot_w64(!(bound <= m + kUp<F16>))) {
+    if (__builtin_amdgcn_ballot_w64(!(bound <= m + up))) {
       float x[16];
       scores<true>(s, n0, poly, 0.f, x);
       if (edge) masked(x, n0, -INFINITY);
@@ -247,7 +253,7 @@ struct Rows {
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
       mx = max_halves(mx);
-      if (mx > m + kUp<F16>) m_new = mx;
+      if (mx > m + up) m_new = mx - fminf(up, 0.f);
     }
     if (__builtin_amdgcn_ballot_w64(m_new != m)) {
       const float alpha = __builtin_amdgcn_exp2f(m - m_new);
@@ -277,10 +283,10 @@ struct Rows {
       for (int s = 0; s < 2; ++s) o[db] = mfma32x32x16_t<F16>(rd.turned(v, db, s), pb[s], o[db]);
   }
   // A tile whose values may hold infinities or NaN that a row does not see.
-  __device__ __forceinline__ void careful(const uint16_t* k, const uint16_t* v, int n0) {
+  __device__ __forceinline__ void careful(const uint16_t* k, const uint16_t* v, int n0, float up) {
     float x[16], seen[16];
     const f32x16 s = products(k);
-    const bool poly = settle(s, n0, true);
+    const bool poly = settle(s, n0, true, up);
     scores<false>(s, n0, poly, m, x);
     weigh(n0, true, x);
     const int from = lo - n0 - 4 * hi, to = end - n0 - 4 * hi;
@@ -299,7 +305,7 @@ struct Rows {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x |= !(fabsf(o[db][i]) < INFINITY);
+      for (int i = 0; i < 16; ++i) x |= !(fabsf(o[db][i]) < kBig);
     return x;
   }
   // The rows' outputs, or with `to` this lane's part of them; `total` and `norm` are l
@@ -440,15 +446,16 @@ __device__ __forceinline__ void walk(const FwdArgs& p, const FwdSet& S, int prob
   }
   m_wait<0>();                                 // no DMA may land after the workgroup ends
 
-  if (__syncthreads_or(R.odd() && row.live)) {
+  for (float up = kUp<F16>; __syncthreads_or(R.odd() && row.live); up = kDown) {
     R.restart();
     for (int t = t_begin; t < t_end; ++t) {
       __syncthreads();
       issue(t, r0);
       m_wait<0>();
       __syncthreads();
-      R.careful(r0.k, r0.v, n_lo + t * kMTile);
+      R.careful(r0.k, r0.v, n_lo + t * kMTile, up);
     }
+    if (F16 || up < 0.f) break;                // fp16's values times its weights are finite
   }
   R.finish(p, row, part(row), sum_halves(R.l), sum_halves(R.n));
 }
@@ -575,15 +582,16 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_masked_few_k
     issue(V, S.v_sn, t + kMWaves, vw);
   }
   m_wait<0>();
-  if (__builtin_amdgcn_ballot_w64(R.odd() && row.live)) {
+  for (float up = kUp<F16>; __builtin_amdgcn_ballot_w64(R.odd() && row.live); up = kDown) {
     R.restart();
     for (int t = t_begin; t < t_end; t += kMWaves) {
       issue(K, S.k_sn, t, kw);
       issue(V, S.v_sn, t, vw);
       m_wait<0>();
-      R.careful(kw, vw, n_lo + t * kMTile);
+      R.careful(kw, vw, n_lo + t * kMTile, up);
       __builtin_amdgcn_s_waitcnt(0xc07f);
     }
+    if (F16 || up < 0.f) break;
   }
 
   // The four waves' results in wave 0, by way of K's buffers, all at one offset.

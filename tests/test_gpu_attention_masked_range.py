@@ -43,3 +43,28 @@ def test_slopes_below_zero_in_cut_blocks(dev, D, dt):
 def test_slopes_below_zero_over_a_shared_prefix(dev, D, dt):
     _check_prefix(dev, 3, 4, 2, 2, 3000, 70, D, dt, [70, 2, 33], slopes=DOWN)
     _check_prefix(dev, 2, 4, 2, 40, 700, 200, D, dt, [200, 41], slopes=DOWN)
+
+
+# --- values near the end of bf16's range ----------------------------------------
+
+@pytest.mark.parametrize("M,N", [(1, 500), (40, 500), (2, 20_000), (200, 3000)])
+def test_large_values(dev, M, N):
+    """Weights grow by 2^60 over a row's tiles, which an offset that stays where the first
+    tile put it allows; times values of 1e25 that passes fp32."""
+    q, k, v, _, _ = _inputs(1, 2, 1, M, N, 64, BF, 61, std=0.0)
+    q[..., 0], k[:, :, 128:, 0] = 8.0, 42.0
+    k[:, :, :128, 0] = torch.rand(128, generator=torch.Generator().manual_seed(1)).to(BF)
+    for big in (v * 1e25, torch.full_like(v, 3e38)):
+        ref = masked_attention(q, k, big, 0.125)
+        o, lse = attention_masked(q.to(dev), k.to(dev), big.to(dev), 0.125, return_lse=True)
+        _near("o", o, ref.o, ref.o_bound, BF)
+        assert ((lse.cpu().double() - ref.lse).abs() <= ref.lse_bound).all()
+
+
+def test_large_values_in_cut_blocks(dev):
+    q, k, v, _, _ = _inputs(1, 8, 8, 2100, 2100, 64, BF, 62, std=0.0)
+    q[..., 0], k[:, :, 128:, 0] = 8.0, 42.0
+    v = v * 1e25
+    ref = masked_attention(q, k, v, 0.125, causal=True)
+    o = attention_masked(q.to(dev), k.to(dev), v.to(dev), 0.125, causal=True)
+    _near("o", o, ref.o, ref.o_bound, BF)
