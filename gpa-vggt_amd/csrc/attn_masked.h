@@ -104,8 +104,9 @@ __device__ __forceinline__ KeySpan key_span(const MaskArgs& a, int64_t b, int j)
 
 // Scores, in log2 units.  c1 = sm_scale log2(e).  With a cap: ce = 2 log2(e)
 // sm_scale / cap (the exponent of e^(2u), u = x / cap), capl = cap log2(e), and for
-// |u| <= kPolyMax, a product |q.k| <= lim, the coefficients of an odd polynomial.
-struct ScoreArgs { float c1, ce, capl, lim, poly[4]; };
+// |u| <= kPolyMax, a product |q.k| <= lim, the coefficients of an odd polynomial;
+// half = 1 / (2 capl).
+struct ScoreArgs { float c1, ce, capl, lim, half, poly[4]; };
 
 // tanh(u) = 1 - 2 / (1 + e^(2u)): right at both ends (e^(2u) = 0 or inf), and
 // off by about 2^-23 absolutely, 1e-5 of a score at a cap of 50.

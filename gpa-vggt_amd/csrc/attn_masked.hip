@@ -921,6 +921,7 @@ void gpa::masked_fill(const gpa_attn_masked_args* a, MaskArgs* m, ScoreArgs* s) 
     s->ce = (float)(2.0 * l2e * g);
     s->capl = a->cap * kMLog2e;
     s->lim = (float)std::min(kPolyMax / g, 1e18);   // s^2 stays finite
+    s->half = (float)(0.5 / (l2e * a->cap));
     double scale = a->sm_scale * l2e;
     for (int i = 0; i < 4; ++i, scale *= g * g) s->poly[i] = (float)(kPoly[i] * scale);
   }

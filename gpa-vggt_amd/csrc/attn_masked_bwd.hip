@@ -30,6 +30,8 @@
 // length as in the forward pass; attn_masked_grad_join_kernel adds up the parts.
 //
 // With a cap, r = 1 / (1 + e^(2u)) gives both: tanh = 1 - 2r, 1 - tanh^2 = 4 (r - r^2).
+// Scores that are small beside the cap lose what r rounds away, so with caps above kNarrow
+// they come from the forward's polynomial.
 //
 // P and dS are rounded to the operand format for the products (the same
 // relative error as the gradients' own rounding); sums are fp32.  Of the two
@@ -55,7 +57,7 @@ namespace gpa {
 namespace {
 
 constexpr int kRowTile = 64;                   // rows of a record, and of a dk, dv tile
-constexpr int kRec = 4 * kRowTile;             // lse (less cap log2(e)), -delta, token, slope
+constexpr int kRec = 4 * kRowTile;             // lse (kNarrowCap: less cap log2(e)), -delta, token, slope
 constexpr int kKeys = 64;                      // keys of a dk, dv workgroup
 static_assert(kRowTile == 64 && kKeys == 64, "attn_masked_count_kernel counts these");
 
@@ -70,7 +72,7 @@ struct BwdArgs {
   int64_t slopes_sb;
   float* rec;                                  // [B * Hk][tiles][kRec]
   int32_t Hk, G, R, tiles;                     // R = M * G rows of a problem
-  float sm_scale;
+  float sm_scale, lse_off;
   const Deal *keys, *rows;                     // null: every block whole, heavy ones first
   float *kpart, *qpart;                        // [part][key head][dk, dv of 64 keys; dq of 128 rows][HD]
   MaskArgs mask;
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(256) void attn_masked_delta_kernel(BwdArgs p) {
 #pragma unroll
     for (int s = 1; s < CH; s <<= 1) delta += __shfl_xor(delta, s);
     if (ch == 0) {
-      rec[i] = lse - p.score.capl;             // capl: 0 without a cap
+      rec[i] = lse - p.lse_off;
       rec[kRowTile + i] = -delta;
       rec[2 * kRowTile + i] = (float)m;
       rec[3 * kRowTile + i] = slope;
@@ -158,17 +160,25 @@ struct DsScale {
   }
 };
 
-// P and dS of one product s and dP - delta; `lse` is a record's.
-template <bool CAP>
+// How scores are capped.  From r alone they are off by about 5 2^-24 cap (log2 units): for
+// caps up to kNarrow P by less than a seventeenth of what rounding takes from it.  Above,
+// products within `lim` go through the polynomial, selected one by one.  Measured (us,
+// forward and backward, cap 100 and 200 with kNarrow between): 1,005 and 1,122 at
+// 2 x 16 heads of 128 on 2 x 4, 4,096 tokens, causal; 592 and 762 at 8 of 64, 8,191 tokens.
+template <bool F16> constexpr float kNarrow = F16 ? 128.0f : 1024.0f;
+enum Cap { kNoCap, kNarrowCap, kWideCap };
+
+// log2 of P, and 1 - tanh^2 (of which a quarter with a cap), of one product s; `lse` is a record's.
 struct Pair { float x, der; };
-template <bool CAP>
-__device__ __forceinline__ Pair<CAP> log_weight(float s, float lse, const ScoreArgs& a) {
-  if constexpr (CAP) {
-    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * a.ce));
-    return {__builtin_fmaf(r, -2.0f * a.capl, -lse), __builtin_fmaf(-r, r, r)};   // der: a quarter of it
-  } else {
-    return {__builtin_fmaf(s, a.c1, -lse), 1.0f};
-  }
+template <Cap CAP>
+__device__ __forceinline__ Pair log_weight(float s, float lse, const ScoreArgs& a) {
+  if constexpr (CAP == kNoCap) return {__builtin_fmaf(s, a.c1, -lse), 1.0f};
+  const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * a.ce));
+  if constexpr (CAP == kNarrowCap) return {__builtin_fmaf(r, -2.0f * a.capl, -lse), __builtin_fmaf(-r, r, r)};
+  const float near = s * cap_poly(s, a), t = near * a.half;
+  const bool in = fabsf(s) <= a.lim;
+  return {(in ? near : __builtin_fmaf(r, -2.0f * a.capl, a.capl)) - lse,
+          in ? __builtin_fmaf(-t, t, 0.25f) : __builtin_fmaf(-r, r, r)};
 }
 
 template <int HD>
@@ -178,7 +188,7 @@ struct RowSlot {
   float st[kRec];
 };
 
-template <int HD, bool F16, bool CAP, bool SLOPE>
+template <int HD, bool F16, Cap CAP, bool SLOPE>
 __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_kernel(BwdArgs p) {
   constexpr int KS = HD / 16, DB = HD / 32, CH = HD / 8;
   constexpr int DJ = kRowTile * CH / kMThreads;
@@ -320,12 +330,12 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * g + e;
-        const Pair<CAP> y = log_weight<CAP>(s[i], ls[e], p.score);
+        const Pair y = log_weight<CAP>(s[i], ls[e], p.score);
         float x = y.x;
         if constexpr (SLOPE) x = __builtin_fmaf(-sl[e], fabsf(tok[e] + shift), x);
         w[i] = __builtin_amdgcn_exp2f(x);
         ds[i] = w[i] * dp[i];
-        if constexpr (CAP) ds[i] *= y.der;
+        if constexpr (CAP != kNoCap) ds[i] *= y.der;
       }
     }
     if (edge) {
@@ -429,7 +439,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   }
 
   // The second half's sums by way of the ring, slots of 16 bytes a lane.
-  const float kx = (CAP ? 4.0f : 1.0f) * p.sm_scale * (F16 ? (sc.s == 0.f ? 0.f : 1.0f / sc.s) : 1.0f);
+  const float kx = (CAP != kNoCap ? 4.0f : 1.0f) * p.sm_scale * (F16 ? (sc.s == 0.f ? 0.f : 1.0f / sc.s) : 1.0f);
   const float vx = F16 ? 1.0f / kPScale : 1.0f;
 #pragma unroll
   for (int db = 0; db < DB; ++db) {
@@ -501,7 +511,7 @@ struct KeySlot {
   uint16_t v[kMTile * HD];
 };
 
-template <int HD, bool F16, bool CAP, bool SLOPE>
+template <int HD, bool F16, Cap CAP, bool SLOPE>
 __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p) {
   constexpr int KS = HD / 16, DB = HD / 32, CH = HD / 8;
   constexpr int DJ = kMTile * CH / kMThreads;
@@ -608,11 +618,11 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
     const float dist = (float)(span.at - n0 - 4 * hi);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const Pair<CAP> y = log_weight<CAP>(s[i], lse, p.score);
+      const Pair y = log_weight<CAP>(s[i], lse, p.score);
       float x = y.x;
       if constexpr (SLOPE) x = __builtin_fmaf(-slope, fabsf(dist - (float)mfma_row(i, 0)), x);
       ds[i] = __builtin_amdgcn_exp2f(x) * dp[i];
-      if constexpr (CAP) ds[i] *= y.der;
+      if constexpr (CAP != kNoCap) ds[i] *= y.der;
     }
     if (edge) {
       const int from = span.lo - n0 - 4 * hi, to = span.hi - n0 - 4 * hi;
@@ -702,7 +712,7 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
     }
   }
   if (!live) return;
-  const float x = (CAP ? 4.0f : 1.0f) * p.sm_scale * (F16 ? (sc.s == 0.f ? 0.f : 1.0f / sc.s) : 1.0f);
+  const float x = (CAP != kNoCap ? 4.0f : 1.0f) * p.sm_scale * (F16 ? (sc.s == 0.f ? 0.f : 1.0f / sc.s) : 1.0f);
   if (piece.part >= 0) {
     float* P = p.qpart + ((int64_t)piece.part * kMRows + wave * 32 + l32) * HD;
 #pragma unroll
@@ -761,7 +771,7 @@ __global__ __launch_bounds__(256) void attn_masked_grad_join_kernel(BwdArgs p, i
 template <int HD> constexpr int kKeySpans = kCus * (HD == 64 ? 2 : 1);
 constexpr int kRowSpans = kCus * 2;
 
-template <int HD, bool F16, bool CAP, bool SLOPE>
+template <int HD, bool F16, Cap CAP, bool SLOPE>
 hipError_t launch_one(const BwdArgs& a, int64_t problems, hipStream_t s) {
   const int64_t kb = (a.mask.N + kKeys - 1) / kKeys, qb = (a.R + kMRows - 1) / kMRows, B = problems / a.Hk;
   // As in the forward: a head's pieces are fewer than its blocks and spans / Hk.
@@ -787,15 +797,17 @@ hipError_t launch_one(const BwdArgs& a, int64_t problems, hipStream_t s) {
 }
 
 template <int HD, bool F16>
-hipError_t launch(const BwdArgs& a, int64_t problems, bool cap, hipStream_t s) {
+hipError_t launch(const BwdArgs& a, int64_t problems, Cap cap, hipStream_t s) {
   hipLaunchKernelGGL((attn_masked_delta_kernel<HD, F16>), dim3((unsigned)(problems * a.tiles)),
                      dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if (cap) return a.slopes ? launch_one<HD, F16, true, true>(a, problems, s)
-                           : launch_one<HD, F16, true, false>(a, problems, s);
-  return a.slopes ? launch_one<HD, F16, false, true>(a, problems, s)
-                  : launch_one<HD, F16, false, false>(a, problems, s);
+  if (cap == kWideCap) return a.slopes ? launch_one<HD, F16, kWideCap, true>(a, problems, s)
+                                       : launch_one<HD, F16, kWideCap, false>(a, problems, s);
+  if (cap == kNarrowCap) return a.slopes ? launch_one<HD, F16, kNarrowCap, true>(a, problems, s)
+                                         : launch_one<HD, F16, kNarrowCap, false>(a, problems, s);
+  return a.slopes ? launch_one<HD, F16, kNoCap, true>(a, problems, s)
+                  : launch_one<HD, F16, kNoCap, false>(a, problems, s);
 }
 
 // Whether the blocks are counted, cut and sorted first, as far as the rows decide it,
@@ -914,7 +926,9 @@ extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* args,
   f.Hk = (int32_t)a->Hk; f.G = (int32_t)G; f.R = (int32_t)(a->M * G); f.tiles = (int32_t)tiles;
   f.sm_scale = a->sm_scale;
   masked_fill(a, &f.mask, &f.score);
-  const bool f16 = dtype == GPA_DTYPE_F16, cap = a->cap > 0.f;
+  const bool f16 = dtype == GPA_DTYPE_F16;
+  const Cap cap = a->cap > (f16 ? kNarrow<true> : kNarrow<false>) ? kWideCap : a->cap > 0.f ? kNarrowCap : kNoCap;
+  if (cap == kNarrowCap) f.lse_off = f.score.capl;
   const hipStream_t s = (hipStream_t)stream;
   const hipError_t e =
       a->D == 64 ? (f16 ? launch<64, true>(f, problems, cap, s) : launch<64, false>(f, problems, cap, s))

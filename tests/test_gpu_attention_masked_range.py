@@ -68,3 +68,39 @@ def test_large_values_in_cut_blocks(dev):
     ref = masked_attention(q, k, v, 0.125, causal=True)
     o = attention_masked(q.to(dev), k.to(dev), v.to(dev), 0.125, causal=True)
     _near("o", o, ref.o, ref.o_bound, BF)
+
+
+# --- caps far above and below the scores -------------------------------------------
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [1e4, 1e6, 1e12])
+def test_caps_far_above_the_scores(dev, cap, D, dt):
+    """Bounds from the uncapped scores, so that they do not grow with the cap.  The
+    capped score's polynomial is off by 2.2 f of it and rounded six times, beside the
+    product's D + 8 >= 72 f of no less: an eighth more."""
+    q, k, v, d_o, d_lse = _inputs(2, 4, 2, 150, 150, D, dt, 71)
+    kw = dict(causal=True, slopes=torch.tensor([0.5, 0.0, 0.03, 2.0]), d_o=d_o, d_lse=d_lse, u=torch.finfo(dt).eps / 2)
+    ref, free = (masked_attention(q, k, v, D ** -0.5, cap=c, **kw) for c in (cap, None))
+    x = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    o, lse = attention_masked(*x, D ** -0.5, cap=cap, causal=True, slopes=kw["slopes"].to(dev), return_lse=True)
+    assert ((lse.detach().cpu().double() - ref.lse).abs() <= 1.125 * free.lse_bound).all()
+    got = [o, *torch.autograd.grad([o, lse], x, [d_o.to(dev), d_lse.to(dev)])]
+    for name in ("o", "dq", "dk", "dv"):
+        want, loose, bound = (getattr(r, n) for r, n in ((ref, name), (free, name), (free, name + "_bound")))
+        _near(name, got[("o", "dq", "dk", "dv").index(name)], want, 1.125 * bound + (want - loose).abs(), dt)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [100.0, 200.0, 2000.0])
+def test_caps_that_scores_reach(dev, cap, D, dt):
+    """Rows of scores from far below to far above the cap, beside each other."""
+    q, k, v, d_o, _ = _inputs(1, 4, 2, 150, 150, D, dt, 73)
+    q = (q.float() * torch.logspace(-2, 2, 150)[:, None]).to(dt)
+    ref = masked_attention(q, k, v, D ** -0.5, cap=cap, d_o=d_o, u=torch.finfo(dt).eps / 2)
+    x = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    o = attention_masked(*x, D ** -0.5, cap=cap)
+    got = [o, *torch.autograd.grad(o, x, d_o.to(dev))]
+    for name, t in zip(("o", "dq", "dk", "dv"), got):
+        _near(name, t, getattr(ref, name), getattr(ref, name + "_bound"), dt)
