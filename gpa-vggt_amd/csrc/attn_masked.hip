@@ -918,12 +918,13 @@ void gpa::masked_fill(const gpa_attn_masked_args* a, MaskArgs* m, ScoreArgs* s) 
   s->c1 = a->sm_scale * kMLog2e;
   if (a->cap > 0.f) {
     const double g = (double)a->sm_scale / a->cap, l2e = 1.4426950408889634;
-    s->ce = (float)(2.0 * l2e * g);
+    s->ce = (float)std::min(2.0 * l2e * g, 1e38);   // times a product of 0: 0
     s->capl = a->cap * kMLog2e;
     s->lim = (float)std::min(kPolyMax / g, 1e18);   // s^2 stays finite
     s->half = (float)(0.5 / (l2e * a->cap));
     double scale = a->sm_scale * l2e;
     for (int i = 0; i < 4; ++i, scale *= g * g) s->poly[i] = (float)(kPoly[i] * scale);
+    if (!isfinite(s->poly[3])) s->lim = -1.f;   // a cap so small that no product but 0 would take them
   }
 }
 

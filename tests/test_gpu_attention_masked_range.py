@@ -104,3 +104,17 @@ def test_caps_that_scores_reach(dev, cap, D, dt):
     got = [o, *torch.autograd.grad(o, x, d_o.to(dev))]
     for name, t in zip(("o", "dq", "dk", "dv"), got):
         _near(name, t, getattr(ref, name), getattr(ref, name + "_bound"), dt)
+
+
+@pytest.mark.parametrize("M", [5, 150])
+@pytest.mark.parametrize("cap", [1e-4, 1e-8, 1e-30])
+def test_caps_far_below_the_scores(dev, cap, M):
+    """Scores of plus or minus the cap, and of zero where a query or key is zero."""
+    q, k, v, d_o, _ = _inputs(1, 2, 1, M, 150, 64, BF, 72)
+    q[:, :, ::3], k[:, :, :40] = 0, 0
+    ref = masked_attention(q, k, v, 0.125, cap=cap, d_o=d_o)
+    x = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    o = attention_masked(*x, 0.125, cap=cap)
+    got = [o, *torch.autograd.grad(o, x, d_o.to(dev))]
+    for name, t in zip(("o", "dq", "dk", "dv"), got):
+        _near(name, t, getattr(ref, name), getattr(ref, name + "_bound"), BF)
