@@ -20,7 +20,6 @@ gradients, and a prefix that a whole batch shares (`csrc/attn_masked.hip`).
 """
 from __future__ import annotations
 
-import math
 from typing import Optional, Union
 
 import torch
@@ -31,6 +30,7 @@ __all__ = ["attention_keybias", "attention_join", "attention_masked", "attention
            "attention_shared_prefix", "combine_by_lse", "LOG2E"]
 
 LOG2E = 1.4426950408889634
+_F32_MIN, _F32_MAX = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 def _autocast_dtype() -> torch.dtype:
@@ -104,10 +104,10 @@ def combine_by_lse(out_a: torch.Tensor, lse_a: torch.Tensor, out_b: torch.Tensor
 
 def _score_args(what, sm_scale, cap, slopes):
     sm_scale = float(sm_scale)
-    if not (sm_scale > 0 and math.isfinite(sm_scale)):
-        raise ValueError(f"{what}: sm_scale must be finite and positive, got {sm_scale}")
-    if cap is not None and not (cap > 0 and math.isfinite(cap)):
-        raise ValueError(f"{what}: cap must be finite and positive, or None, got {cap}")
+    if not _F32_MIN <= sm_scale <= _F32_MAX:
+        raise ValueError(f"{what}: sm_scale must be finite and positive in fp32, got {sm_scale}")
+    if cap is not None and not _F32_MIN <= cap <= _F32_MAX:
+        raise ValueError(f"{what}: cap must be finite and positive in fp32, or None, got {cap}")
     if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: the slopes are constants (they have no gradient)")
     return sm_scale, 0.0 if cap is None else float(cap)

@@ -9,7 +9,6 @@ has RMS norms too, and is differentiable (`csrc/norm_gate.hip`).
 """
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -17,6 +16,8 @@ import torch
 from . import _native
 
 __all__ = ["norm_gate_residual"]
+
+_F32_MAX = torch.finfo(torch.float32).max
 
 
 def _gate_rows(x: torch.Tensor, gate: torch.Tensor) -> torch.Tensor:
@@ -52,8 +53,8 @@ def norm_gate_residual(x: torch.Tensor, y: torch.Tensor, pre_weight: torch.Tenso
     what = "norm_gate_residual"
     if kind not in ("rms", "layer"):
         raise ValueError(f"{what}: kind {kind!r} is not 'rms' or 'layer'")
-    if not (eps >= 0 and math.isfinite(eps) and math.isfinite(scale)):
-        raise ValueError(f"{what}: eps must be finite and >= 0, scale finite, got {eps} and {scale}")
+    if not (0 <= eps <= _F32_MAX and abs(scale) <= _F32_MAX):
+        raise ValueError(f"{what}: eps must be finite and >= 0, scale finite, in fp32, got {eps} and {scale}")
     if not 1 <= x.dim() or x.shape != y.shape:
         raise ValueError(f"{what}: x {tuple(x.shape)} and y {tuple(y.shape)} differ")
     if x.shape[-1] > 8192 or x.shape[-1] < 1:
