@@ -7,7 +7,7 @@
 //   dQ_i  = sm_scale sum_j dS_ij K_j
 //
 // attn_masked_delta_kernel writes a record of every 64 rows: their LSE, -delta,
-// token and slope.  delta comes from O and what rounding took from it: where a
+// token (counted from the first row's, so that it is exact in fp32) and slope.  delta comes from O and what rounding took from it: where a
 // row's weights are sharp, dP - delta is small beside both, and delta from the
 // rounded O alone put dq and dk 1.9 to 2.5 roundings off (1.55 with the rest).
 //
@@ -104,9 +104,10 @@ __global__ __launch_bounds__(256) void attn_masked_delta_kernel(BwdArgs p) {
   for (int i = threadIdx.x / CH; i < kRowTile; i += 256 / CH) {
     const int r = tile * kRowTile + i;
     float lse = INFINITY, delta = 0.f, slope = 0.f;   // past the rows: weights of zero
-    int m = 0;
+    float tok = 0.f;
     if (r < p.R) {
-      m = r / p.G;
+      const int m = r / p.G;
+      tok = (float)(m - tile * kRowTile / p.G);
       const int h = kvh * p.G + r % p.G;
       const int64_t at = b * p.o_sb + h * p.o_sh + m * p.o_sm + 8 * ch;
       const bf16x8 x = *reinterpret_cast<const bf16x8*>(p.o + at);
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(256) void attn_masked_delta_kernel(BwdArgs p) {
     if (ch == 0) {
       rec[i] = lse - p.lse_off;
       rec[kRowTile + i] = -delta;
-      rec[2 * kRowTile + i] = (float)m;
+      rec[2 * kRowTile + i] = tok;
       rec[3 * kRowTile + i] = slope;
     }
   }
@@ -208,7 +209,8 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   const int jc = live ? j : p.mask.N - 1;
   const KeySpan ks_ = key_span(p.mask, b, jc);
   const int lo = ks_.lo * p.G, hi_r = ks_.hi * p.G;   // rows that see this lane's key
-  const float shift = (float)(ks_.shift - jc);
+  // A tile's first token, as a distance from this lane's key.
+  auto place_of = [&](int t) { return t * kRowTile / p.G + ks_.shift - jc; };
 
   bf16x8 kf[KS], vf[KS];
   {
@@ -317,7 +319,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   };
   // P and dS.
   auto weights = [&](const RowSlot<HD>& T, const f32x16& s, const f32x16& dp, int row0, bool edge,
-                     float (&w)[16], float (&ds)[16]) {
+                     float first_at, float (&w)[16], float (&ds)[16]) {
     const float* st = &T.st[half * 32 + 4 * hi];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -332,7 +334,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
         const int i = 4 * g + e;
         const Pair y = log_weight<CAP>(s[i], ls[e], p.score);
         float x = y.x;
-        if constexpr (SLOPE) x = __builtin_fmaf(-sl[e], fabsf(tok[e] + shift), x);
+        if constexpr (SLOPE) x = __builtin_fmaf(-sl[e], fabsf(tok[e] + first_at), x);
         w[i] = __builtin_amdgcn_exp2f(x);
         ds[i] = w[i] * dp[i];
         if constexpr (CAP != kNoCap) ds[i] *= y.der;
@@ -359,16 +361,20 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   };
 
   f32x16 s, dp;
+  int place = SLOPE ? place_of(t_begin) : 0;
+  const int step = kRowTile / p.G;             // from tile to tile, where G divides one
   auto iter = [&](int t, const RowSlot<HD>& cur, const RowSlot<HD>& nxt, RowSlot<HD>& dst) {
     m_wait_barrier<2 * DJ + 1>();              // tile t + 1 landed (t + 2 in flight) for every wave
     issue(t + 3, dst);
     rd.fresh();
+    const float first_at = (float)place;
+    if constexpr (SLOPE) place = even ? place + step : place_of(t + 1);
     const int row0 = t * kRowTile + half * 32;
     if (row0 < w_hi && row0 + 32 > w_lo) {
       f32x16 s_next, dp_next;
       products(nxt, s_next, dp_next);
       float w[16], ds[16];
-      weights(cur, s, dp, row0, row0 < a_lo || row0 + 32 > a_hi, w, ds);
+      weights(cur, s, dp, row0, row0 < a_lo || row0 + 32 > a_hi, first_at, w, ds);
       bf16x8 wb[2], db_[2];
       pack_frags<F16>(w, wb);
       pack_frags<F16>(ds, db_);
@@ -421,7 +427,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
       const int row0 = t * kRowTile + half * 32, from = lo - row0 - 4 * hi, to = hi_r - row0 - 4 * hi;
       float w[16], ds[16], sx[16];
       products(r0, s, dp);
-      weights(r0, s, dp, row0, true, w, ds);
+      weights(r0, s, dp, row0, true, SLOPE ? (float)place_of(t) : 0.f, w, ds);
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         sx[i] = mfma_row(i, 0) < from || mfma_row(i, 0) >= to ? 0.f : 1.f;

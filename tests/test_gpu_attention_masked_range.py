@@ -118,3 +118,36 @@ def test_caps_far_below_the_scores(dev, cap, M):
     got = [o, *torch.autograd.grad(o, x, d_o.to(dev))]
     for name, t in zip(("o", "dq", "dk", "dv"), got):
         _near(name, t, getattr(ref, name), getattr(ref, name + "_bound"), BF)
+
+
+# --- positions above 2^24 -----------------------------------------------------------
+
+def test_documents_behind_2_24_tokens(dev):
+    """A document behind 2^24 tokens of none: distances are its own, so results and
+    gradients are those of the document alone, bit by bit."""
+    far, D = 2 ** 24, 64
+    g = torch.Generator(device=dev).manual_seed(81)
+    short = [torch.randn(1, h, 320, D, generator=g, device=dev).to(BF) for h in (2, 1, 1, 2)]
+    slopes = torch.tensor([0.5, 0.03], device=dev)
+
+    def step(q, k, v, d_o, at):
+        x = [t.requires_grad_() for t in (q, k, v)]
+        off = torch.tensor([at, at + 3, at + 320], dtype=torch.int32, device=dev)
+        o = attention_masked(*x, 0.125, causal=True, slopes=slopes, offsets=off)
+        return [o.detach(), *torch.autograd.grad(o, x, d_o)]
+
+    def behind(t):
+        out = torch.zeros(1, far + 320, t.shape[1], D, dtype=BF, device=dev).transpose(1, 2)
+        out[:, :, far:] = t
+        return out
+    want = step(*(t.clone() for t in short), 0)
+    for name, got, ref in zip(("o", "dq", "dk", "dv"), step(*(behind(t) for t in short), far), want):
+        assert torch.equal(got[:, :, far:], ref), name
+        assert not got[:, :, :far].any(), name
+
+
+@pytest.mark.parametrize("dt,D", [(BF, 64), (HF, 128)])
+@pytest.mark.parametrize("H,Hk", [(6, 2), (5, 1), (40, 1), (64, 1), (100, 1)])
+def test_slopes_of_head_groups_astride_row_tiles(dev, H, Hk, D, dt):
+    slopes = torch.rand(H, generator=torch.Generator().manual_seed(H)) * 0.3
+    _check(dev, 1, H, Hk, 77, 130, D, dt, seed=H, slopes=slopes, offsets=[0, 20, 77], k_offsets=[3, 60, 130])
