@@ -253,8 +253,6 @@ __global__ __launch_bounds__(kBwdThreads<LANES>, WHOLE ? 2 : 4) void norm_gate_b
   const int lane = threadIdx.x % LANES, wave = lane / 64;
   const int i = lane * 8;                      // this lane's features
   const float inv_c = 1.0f / a.C;
-  // Factors instead of branches in the loop: no mean (RMS), no norm after the block.
-  const float layer = a.layer ? inv_c : 0.f, post = a.w1 ? inv_c : 0.f, post0 = a.w1 ? layer : 0.f;
 
   // A sum over the workgroup's rows in hand, in slot 0's registers.
   auto join = [&](float (&v)[8]) {
@@ -295,7 +293,7 @@ __global__ __launch_bounds__(kBwdThreads<LANES>, WHOLE ? 2 : 4) void norm_gate_b
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         gw[e] = a.scale * gt[e] * w1[e];
-        gb[e] = a.scale * gt[e] * b1[e];
+        gb[e] = a.b1 ? a.scale * gt[e] * b1[e] : 0.f;
       }
     }
     const int64_t end = (g + 1) * a.per, first = g * a.per + skip;
@@ -310,26 +308,32 @@ __global__ __launch_bounds__(kBwdThreads<LANES>, WHOLE ? 2 : 4) void norm_gate_b
       load8<T, VEC>(row_rsrc<T>(a.x, row * a.x_sn, n), i, h);
       load8<T, VEC>(row_rsrc<T>(a.dout, row * a.dout_sn, n), i, o);
       load8<T, VEC>(row_rsrc<T>(a.dh, row * a.dh_sn, n), i, d);
-      // Features past C: o, d, gate and weights are zeros there (a weight or gate that
-      // is absent is 1), so no sum of the row has them.
-      float s1 = 0.f, s0 = 0.f;
+      // A norm that is absent, or whose output has no gradient, is left out, and a mean that
+      // RMS does not take is not multiplied by 0: where a value or a sum is not finite, 0
+      // times it is NaN for the whole row.  Features past C: o, gate and weights are zeros
+      // there (a weight or gate that is absent is 1), so no sum of the row has them.
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        u[e] = (u[e] - st[0]) * st[1];
-        h[e] = (h[e] + __builtin_fmaf(gw[e], u[e], gb[e]) - st[2]) * st[3];
-        dw2[e] = __builtin_fmaf(o[e], h[e], dw2[e]);
-        db2[e] += o[e];
-        o[e] *= w2[e];
-        s1 = __builtin_fmaf(o[e], h[e], s1);
-        s0 += o[e];
+      for (int e = 0; e < 8; ++e) u[e] = (u[e] - st[0]) * st[1];
+      if (a.dout) {
+        float s1 = 0.f, s0 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          h[e] = (h[e] + __builtin_fmaf(gw[e], u[e], gb[e]) - st[2]) * st[3];
+          dw2[e] = __builtin_fmaf(o[e], h[e], dw2[e]);
+          db2[e] += o[e];
+          o[e] *= w2[e];
+          s1 = __builtin_fmaf(o[e], h[e], s1);
+          s0 += o[e];
+        }
+        red.sum2(s1, s0, slot, wave);
+        s1 *= inv_c;
+        s0 = a.layer ? s0 * inv_c : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] += st[3] * (o[e] - s0 - h[e] * s1);
       }
-      red.sum2(s1, s0, slot, wave);
-      s1 *= inv_c;
-      s0 *= layer;
       float t1 = 0.f, t0 = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        d[e] += st[3] * (o[e] - s0 - h[e] * s1);
         A[e] = __builtin_fmaf(d[e], u[e], A[e]);
         D[e] += d[e];
         o[e] = gw[e] * d[e];
@@ -337,11 +341,13 @@ __global__ __launch_bounds__(kBwdThreads<LANES>, WHOLE ? 2 : 4) void norm_gate_b
         t0 += o[e];
       }
       store8<T, VEC>(row_rsrc<T>(a.dx, row * a.dx_sn, n), i, d);
-      red.sum2(t1, t0, slot, wave);
-      t1 *= post;
-      t0 *= post0;
+      if (a.w1) {
+        red.sum2(t1, t0, slot, wave);
+        t1 *= inv_c;
+        t0 = a.layer ? t0 * inv_c : 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = st[1] * (o[e] - t0 - u[e] * t1);
+        for (int e = 0; e < 8; ++e) o[e] = st[1] * (o[e] - t0 - u[e] * t1);
+      }
       store8<T, VEC>(row_rsrc<T>(a.dy, row * a.dy_sn, n), i, o);
     }
     float w1[8], b1[8], gt[8];
@@ -352,7 +358,7 @@ __global__ __launch_bounds__(kBwdThreads<LANES>, WHOLE ? 2 : 4) void norm_gate_b
     for (int e = 0; e < 8; ++e) {
       dw1[e] = __builtin_fmaf(a.scale * gt[e], A[e], dw1[e]);
       db1[e] = __builtin_fmaf(a.scale * gt[e], D[e], db1[e]);
-      A[e] = a.scale * __builtin_fmaf(w1[e], A[e], b1[e] * D[e]);      // dgate
+      A[e] = a.scale * (a.b1 ? __builtin_fmaf(w1[e], A[e], b1[e] * D[e]) : w1[e] * A[e]);   // dgate
       D[e] = 0.f;
     }
     if constexpr (WHOLE) {
