@@ -1,8 +1,12 @@
 """Arguments of the language-model operators at the ends of their ranges; none of this
 needs a GPU."""
+import math
+import random
+
 import pytest
 import torch
 
+from merging import _native
 from merging.fused_attention import attention_masked, attention_shared_prefix
 from merging.fused_norms import norm_gate_residual
 
@@ -30,3 +34,22 @@ def test_numbers_outside_fp32_are_refused(value):
     else:
         with pytest.raises(ValueError, match="GPU"):         # 0 in fp32, as eps and scale may be
             norm_gate_residual(x, x, x[0], eps=value, scale=value)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_workspaces_stay_below_their_stated_sizes(seed):
+    """8 (D + 2) bytes for each of 98,304 (head dim 64) or 65,536 (128) rows and a list of
+    66,000; over a shared prefix for each query and head, where they are more.  The
+    backward: 101 MB, and 16 bytes for each query and head of whole 64-row tiles."""
+    rng = random.Random(seed)
+    L = _native.lib()
+    D, hk, G = rng.choice([64, 128]), rng.choice([1, 2, 5, 8, 64]), rng.choice([1, 3, 4, 32])
+    size = lambda top: int(math.exp(rng.uniform(0, math.log(top))))  # noqa: E731
+    B, M, N, P = size(300), size(20_000), size(300_000), size(300_000)
+    least = {64: 98_304, 128: 65_536}[D]
+    each = 8 * (D + 2)
+    assert L.gpa_attn_masked_workspace_bytes(B, hk * G, hk, M, N, 0, D) <= each * least + 66_000
+    got = L.gpa_attn_masked_workspace_bytes(B, hk * G, hk, M, N, P, D)
+    assert each * B * hk * G * M <= got <= each * max(least, B * hk * G * M) + 66_000
+    tiles = B * hk * (-(-G * M // 64))
+    assert L.gpa_attn_masked_bwd_workspace_bytes(B, hk * G, hk, M) <= 101_000_000 + 16 * 64 * tiles
