@@ -1191,8 +1191,13 @@ def _residual_layernorm_fake(x, y, gamma, weight, bias, eps, want_h):
 # --------------------------------------------------------------------------
 
 def _like(t):
-    """A new tensor in t's order of dimensions, rows of unit stride."""
-    return torch.empty_like(t) if t.stride(-1) == 1 else t.new_empty(t.shape)
+    """A new tensor in t's order of dimensions, rows of unit stride (where t's rows
+    overlap, its order may not have them innermost)."""
+    if t.stride(-1) == 1:
+        new = torch.empty_like(t)
+        if new.stride(-1) == 1:
+            return new
+    return t.new_empty(t.shape)
 
 
 def _rows8(t):

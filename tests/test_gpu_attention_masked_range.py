@@ -151,3 +151,19 @@ def test_documents_behind_2_24_tokens(dev):
 def test_slopes_of_head_groups_astride_row_tiles(dev, H, Hk, D, dt):
     slopes = torch.rand(H, generator=torch.Generator().manual_seed(H)) * 0.3
     _check(dev, 1, H, Hk, 77, 130, D, dt, seed=H, slopes=slopes, offsets=[0, 20, 77], k_offsets=[3, 60, 130])
+
+
+# --- rows that overlap ----------------------------------------------------------------
+
+def test_windows_that_slide_over_a_sequence(dev):
+    """Queries, keys and values whose rows overlap, fewer of them than features."""
+    g = torch.Generator(device=dev).manual_seed(91)
+    t = torch.randn(3, 200, generator=g, device=dev).to(BF)
+    q, k, v = (x.unfold(0, 64, 1)[:40].expand(1, 2, 40, 64).requires_grad_() for x in t)
+    d_o = torch.randn(1, 2, 40, 64, generator=g, device=dev).to(BF)
+
+    def step(*x):
+        o = attention_masked(*x, 0.125, causal=True)
+        return [o.detach(), *torch.autograd.grad(o, x, d_o)]
+    plain = [x.detach().contiguous().requires_grad_() for x in (q, k, v)]
+    assert all(torch.equal(a, b) for a, b in zip(step(q, k, v), step(*plain)))

@@ -53,3 +53,11 @@ def test_workspaces_stay_below_their_stated_sizes(seed):
     assert each * B * hk * G * M <= got <= each * max(least, B * hk * G * M) + 66_000
     tiles = B * hk * (-(-G * M // 64))
     assert L.gpa_attn_masked_bwd_workspace_bytes(B, hk * G, hk, M) <= 101_000_000 + 16 * 64 * tiles
+
+
+@pytest.mark.parametrize("rows,step", [(40, 1), (100, 1), (40, 8), (1, 1)])
+def test_results_of_overlapping_rows_have_rows(rows, step):
+    """Windows that slide over a sequence: rows that overlap, in an order of their own."""
+    t = torch.arange(4000.0).unfold(0, 64, step)[:rows].expand(2, 3, rows, 64)
+    new = _native._like(t)
+    assert new.shape == t.shape and new.stride(-1) == 1 and _native._rows_ok(new, 8)
