@@ -1252,7 +1252,9 @@ def _masked_args(what, q, k, v, o, lse, sm_scale, cap, slopes, causal, prefix=No
     if slopes is not None:
         slopes, sl_sb = _table(what, "slopes", slopes, B, H, torch.float32)
     if lens is not None:
-        lens, _ = _table(what, "lengths", lens, 0, B, torch.int32)
+        if lens.dtype != torch.int32 or lens.shape != (B,):
+            raise ValueError(f"{what}: lengths must be torch.int32 [{B}], got {lens.dtype} {tuple(lens.shape)}")
+        lens = lens.contiguous()
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     a = _MaskedArgs.packed(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ptr(lse), B, H, Hk, M, N, D,

@@ -61,3 +61,11 @@ def test_results_of_overlapping_rows_have_rows(rows, step):
     t = torch.arange(4000.0).unfold(0, 64, step)[:rows].expand(2, 3, rows, 64)
     new = _native._like(t)
     assert new.shape == t.shape and new.stride(-1) == 1 and _native._rows_ok(new, 8)
+
+
+@pytest.mark.parametrize("lens", [torch.zeros(0, 2, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32),
+                                  torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int64)])
+def test_lengths_are_one_row(lens):
+    q = torch.zeros(2, 2, 3, 64, dtype=BF)
+    with pytest.raises(ValueError, match=r"lengths must be torch.int32 \[2\]"):
+        _native._masked_args("x", q, q, q, q, None, 0.125, 0.0, None, True, lens=lens)
