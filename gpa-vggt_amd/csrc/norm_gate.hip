@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256) void norm_gate_kernel(NormArgs a) {
   Sum red{buf};
   const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x / LANES);
   const int lane = threadIdx.x % LANES, wave = lane / 64;
-  const int64_t row = (int64_t)blockIdx.x * ROWS + slot;
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * ROWS + slot;
   const bool live = row < a.rows;
   const int n = live ? a.C : 0;
   const float inv_c = 1.0f / a.C;
@@ -437,8 +437,10 @@ Split split_rows(int64_t rows, int64_t per) {
 
 template <typename T, int LANES, int NV, bool VEC>
 void forward(const NormArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((norm_gate_kernel<T, LANES, NV, VEC>), dim3((unsigned)((a.rows * LANES + 255) / 256)),
-                     dim3(256), 0, s, a);
+  // A dimension of a grid has less than 2^32 threads; workgroups past the rows do nothing.
+  const int64_t wgs = (a.rows * LANES + 255) / 256, most = (int64_t)1 << 23;
+  hipLaunchKernelGGL((norm_gate_kernel<T, LANES, NV, VEC>),
+                     dim3((unsigned)std::min(wgs, most), (unsigned)((wgs + most - 1) / most)), dim3(256), 0, s, a);
 }
 template <typename T>
 void launch_forward(const NormArgs& a, bool vec, hipStream_t s) {
