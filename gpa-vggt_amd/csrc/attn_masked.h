@@ -28,6 +28,7 @@ constexpr int kMTile = 32;          // keys (forward, dq) or rows (dk, dv) of a 
 constexpr int kMWaves = 4;
 constexpr int kMThreads = kMWaves * 64;
 constexpr int kMRows = kMWaves * 32;
+constexpr int64_t kMostWgs = 0xffffffff / kMThreads;
 constexpr float kMLog2e = 1.4426950408889634f;
 constexpr uint32_t kNoRow = 0x40000000u;   // a DMA offset outside every descriptor: zeros
 

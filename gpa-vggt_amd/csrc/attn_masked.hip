@@ -950,7 +950,9 @@ extern "C" int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void
   const int64_t items = (int64_t)x.blocks * x.problems * x.splits +
                         (int64_t)x.p_blocks * x.p_problems * x.p_splits;
   const size_t need = x.bytes;
-  if (items > 0x7fffffff || a->B * a->H * a->M >= (int64_t)1 << 31) {
+  // A launch has less than 2^32 threads; the join has a wave a row.
+  const int64_t rows = a->B * a->H * a->M;
+  if (items > kMostWgs || rows >= (int64_t)1 << 31 || (need > 0 && !x.deal && rows > kMostWgs * 4)) {
     gpa_set_error("%s: too many rows", fn);
     return GPA_E_UNSUPPORTED;
   }
@@ -968,7 +970,7 @@ extern "C" int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void
   f.lse_sb = a->lse_sb; f.lse_sh = a->lse_sh;
   f.slopes = a->slopes;
   f.slopes_sb = a->slopes_sb;
-  f.rows = a->B * a->H * a->M;
+  f.rows = rows;
   f.B = (int32_t)a->B; f.Hk = (int32_t)a->Hk; f.G = (int32_t)G;
   f.splits = x.splits + x.p_splits;
   masked_fill(a, &f.mask, &f.score);

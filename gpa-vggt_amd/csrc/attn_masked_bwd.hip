@@ -897,7 +897,7 @@ extern "C" int gpa_attn_masked_bwd(int dtype, const gpa_attn_masked_args* args,
     }
   }
   const int64_t tiles = (a->M * G + kRowTile - 1) / kRowTile, kb = (a->N + kKeys - 1) / kKeys;
-  if (problems * std::max({tiles, kb, (a->M * G + kMRows - 1) / kMRows}) > 0x7fffffff) {
+  if (problems * std::max({tiles, kb, (a->M * G + kMRows - 1) / kMRows}) > kMostWgs) {
     gpa_set_error("%s: too many rows", fn);
     return GPA_E_UNSUPPORTED;
   }

@@ -9,6 +9,7 @@ import torch
 from merging import _native
 from merging.fused_attention import attention_masked, attention_shared_prefix
 from merging.fused_norms import norm_gate_residual
+from test_attention_masked_host import FAKE, _backward, _forward
 
 BF = torch.bfloat16
 
@@ -69,3 +70,13 @@ def test_lengths_are_one_row(lens):
     q = torch.zeros(2, 2, 3, 64, dtype=BF)
     with pytest.raises(ValueError, match=r"lengths must be torch.int32 \[2\]"):
         _native._masked_args("x", q, q, q, q, None, 0.125, 0.0, None, True, lens=lens)
+
+
+def test_launches_of_2_32_threads_are_refused():
+    """A workgroup of 256 threads for each sequence and key head at least."""
+    one = dict(H=1, Hk=1, M=1, N=1)
+    assert _forward(B=1 << 24, **one) == _native.GPA_E_UNSUPPORTED
+    assert _backward(B=1 << 24, **one) == _native.GPA_E_UNSUPPORTED
+    # the join over a shared prefix: 64 threads a query and head
+    assert _forward(B=4, H=2, Hk=2, M=1 << 24, N=1, P=10, pk=FAKE, pv=FAKE, pk_sn=64, pv_sn=64, pk_sh=640,
+                    pv_sh=640) == _native.GPA_E_UNSUPPORTED
