@@ -140,22 +140,25 @@ __global__ __launch_bounds__(256) void attn_masked_delta_kernel(BwdArgs p) {
 
 constexpr float kPScale = 16384.0f;            // of P in fp16
 
-// The power of two by which a wave's dS are scaled in fp16: set by the first
-// values, lowered where later ones would pass the format's range.
+// The power of two by which a wave's dS are scaled in fp16: the largest one, lowered
+// where values would pass the format's range.
 struct DsScale {
-  float s = 0.f;
+  float s = 0x1p100f;
   // Whether it has to move for these values; `ratio` rescales the sums.
   __device__ __forceinline__ bool follow(const float (&ds)[16], float& ratio) {
     float mx = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(ds[i]));
-    if (!__builtin_amdgcn_ballot_w64(mx * s > 32768.0f || (s == 0.f && mx > 0.f))) return false;
+    if (!__builtin_amdgcn_ballot_w64(mx * s > 32768.0f)) return false;
+    // Infinities, of rows and keys that are lost, leave the scale to the others.
+    mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fabsf(ds[i]) < INFINITY ? fmaxf(mx, fabsf(ds[i])) : mx;
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) mx = fmaxf(mx, __shfl_xor(mx, i));
-    // 2^13 at most; a largest value that is not finite leaves the scale alone.
-    const int e = mx < INFINITY ? min(13 - __builtin_amdgcn_frexp_expf(mx), 100) : 0;
-    const float to = mx < INFINITY ? __builtin_amdgcn_ldexpf(1.0f, e) : s == 0.f ? 1.0f : s;
-    ratio = s == 0.f ? 1.0f : to / s;
+    if (!(mx * s > 32768.0f)) return false;
+    const float to = __builtin_amdgcn_ldexpf(1.0f, 13 - __builtin_amdgcn_frexp_expf(mx));   // 2^13 at most
+    ratio = to / s;
     s = to;
     return true;
   }
@@ -445,7 +448,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 2 : 1) void attn_masked_dkdv_
   }
 
   // The second half's sums by way of the ring, slots of 16 bytes a lane.
-  const float kx = (CAP != kNoCap ? 4.0f : 1.0f) * p.sm_scale * (F16 ? (sc.s == 0.f ? 0.f : 1.0f / sc.s) : 1.0f);
+  const float kx = (CAP != kNoCap ? 4.0f : 1.0f) * p.sm_scale * (F16 ? 1.0f / sc.s : 1.0f);
   const float vx = F16 ? 1.0f / kPScale : 1.0f;
 #pragma unroll
   for (int db = 0; db < DB; ++db) {
@@ -718,7 +721,7 @@ __global__ __launch_bounds__(kMThreads, 2) void attn_masked_dq_kernel(BwdArgs p)
     }
   }
   if (!live) return;
-  const float x = (CAP != kNoCap ? 4.0f : 1.0f) * p.sm_scale * (F16 ? (sc.s == 0.f ? 0.f : 1.0f / sc.s) : 1.0f);
+  const float x = (CAP != kNoCap ? 4.0f : 1.0f) * p.sm_scale * (F16 ? 1.0f / sc.s : 1.0f);
   if (piece.part >= 0) {
     float* P = p.qpart + ((int64_t)piece.part * kMRows + wave * 32 + l32) * HD;
 #pragma unroll

@@ -167,3 +167,30 @@ def test_windows_that_slide_over_a_sequence(dev):
         return [o.detach(), *torch.autograd.grad(o, x, d_o)]
     plain = [x.detach().contiguous().requires_grad_() for x in (q, k, v)]
     assert all(torch.equal(a, b) for a, b in zip(step(q, k, v), step(*plain)))
+
+
+# --- fp16 gradients beside infinite ones ------------------------------------------------
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [1e-4, 300.0])
+@pytest.mark.parametrize("lean", [1 / 128, 128.0])
+def test_small_fp16_gradients_beside_an_infinite_one(dev, lean, size, D):
+    """dS is scaled by a wave's largest value before it is rounded: of the finite ones.  An
+    infinite output gradient at row 100 reaches the keys up to 100, in the middle of
+    a block, and that row's dq; the others keep their accuracy.  Large keys (or
+    queries) bring what small dS make well above fp16's smallest step."""
+    q, k, v, d_o, _ = _inputs(1, 2, 1, 200, 200, D, HF, 95)
+    q, k, v, d_o = q * lean, k / lean, v / 64, d_o * size
+    ref = masked_attention(q, k, v, D ** -0.5, causal=True, d_o=d_o, u=2.0 ** -11)
+    d_o[:, :, 100, 5] = float("inf")
+    x = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(attention_masked(*x, D ** -0.5, causal=True), x, d_o.to(dev))
+    rows = torch.arange(200) != 100
+    _near("dq", dq[:, :, rows.to(dev)], ref.dq[:, :, rows], ref.dq_bound[:, :, rows], HF)
+    for name, got, want, bound in (("dk", dk, ref.dk, ref.dk_bound), ("dv", dv, ref.dv, ref.dv_bound)):
+        _near(name, got[:, :, 101:], want[:, :, 101:], bound[:, :, 101:], HF)
+    assert not torch.isfinite(dq[:, :, 100]).any() and not torch.isfinite(dk[:, :, :101]).any()
+    # in norm: P and dS rounded and the result, with its subnormal steps
+    for got, want in ((dq[:, :, rows.to(dev)], ref.dq[:, :, rows]), (dk[:, :, 101:], ref.dk[:, :, 101:])):
+        rel = ((got.cpu().double() - want).norm() / want.norm()).item()
+        assert rel <= 2 * 2.0 ** -11 + 2.0 ** -25 * want.numel() ** 0.5 / want.norm().item(), rel
