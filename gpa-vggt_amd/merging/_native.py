@@ -1205,7 +1205,7 @@ def _rows8(t):
     s = t.stride()
     if s[-1] == 1 and not t.data_ptr() & 15 and not any(x & 7 for x in s[:-1]):
         return t
-    return t if _rows_ok(t, 8) else t.contiguous()
+    return t if _rows_ok(t, 8) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _masked_shapes(what, q, k, v):

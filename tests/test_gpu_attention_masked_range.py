@@ -4,7 +4,7 @@ are the oracle's elementwise bounds, as in test_gpu_attention_masked.py."""
 import pytest
 import torch
 
-from merging.fused_attention import attention_masked
+from merging.fused_attention import attention_masked, attention_shared_prefix
 from oracle.masked_attention import masked_attention
 from test_gpu_attention_masked import BF, HF, _check, _inputs, _near
 from test_gpu_attention_shared_prefix import _check as _check_prefix
@@ -194,3 +194,21 @@ def test_small_fp16_gradients_beside_an_infinite_one(dev, lean, size, D):
     for got, want in ((dq[:, :, rows.to(dev)], ref.dq[:, :, rows]), (dk[:, :, 101:], ref.dk[:, :, 101:])):
         rel = ((got.cpu().double() - want).norm() / want.norm()).item()
         assert rel <= 2 * 2.0 ** -11 + 2.0 ** -25 * want.numel() ** 0.5 / want.norm().item(), rel
+
+
+# --- bases inside 16 bytes -------------------------------------------------------------
+
+def test_contiguous_operands_behind_odd_bases(dev):
+    g = torch.Generator(device=dev).manual_seed(97)
+    size = 2 * 30 * 64
+    flat = torch.randn(4, size + 8, generator=g, device=dev).to(BF)
+    at = lambda i: [x[i:i + size].view(1, 2, 30, 64) for x in flat]  # noqa: E731
+
+    def step(q, k, v, d_o):
+        x = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = attention_masked(*x, 0.125, causal=True)
+        shared = attention_shared_prefix(q, k[0], v[0], k, v, 0.125)
+        return [o.detach(), shared, *torch.autograd.grad(o, x, d_o)]
+    for i in (1, 4):
+        assert all(t.is_contiguous() for t in at(i))
+        assert all(torch.equal(a, b) for a, b in zip(step(*at(i)), step(*(t.clone() for t in at(i)))))

@@ -80,3 +80,11 @@ def test_launches_of_2_32_threads_are_refused():
     # the join over a shared prefix: 64 threads a query and head
     assert _forward(B=4, H=2, Hk=2, M=1 << 24, N=1, P=10, pk=FAKE, pv=FAKE, pk_sn=64, pv_sn=64, pk_sh=640,
                     pv_sh=640) == _native.GPA_E_UNSUPPORTED
+
+
+@pytest.mark.parametrize("at", [0, 1, 4])
+def test_rows_behind_any_base_are_aligned(at):
+    """A tensor that is contiguous but begins inside 16 bytes is copied too."""
+    t = torch.arange(512.0).to(BF)[at:at + 384].view(1, 2, 3, 64)
+    rows = _native._rows8(t)
+    assert torch.equal(rows, t) and _native._rows_ok(rows, 8)
