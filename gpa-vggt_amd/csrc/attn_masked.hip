@@ -36,12 +36,14 @@
 // each block's tiles, cut the longest and list the pieces by length, and
 // attn_masked_piece_kernel takes them in that order (`deals`).
 //
-// Measured (us): many rows, 340 at 16 heads of 64 and 10,992 tokens of four documents
-// (500 TFLOP/s), 101 at 2 x 16 heads of 128 on 2 x 4, 4,096 tokens of four causal
-// documents (490); bound by vector issue, 600 of the 800 cycles that a tile of 32 x 32
-// takes of a SIMD at head dim 64, the matrix instructions 256.  Few rows, 17 for one
-// token over 130,001 keys of 2 x 64 (4.0 TB/s) and 5 for the join; bound by
-// HBM and a launch's start and end.
+// Measured (us a kernel after 200 passes; the first ten of a process take a tenth to a
+// fifth longer): many rows, 289 at 16 heads of 64 and 10,992 tokens of four documents,
+// capped (590 TFLOP/s), 92 at 2 x 16 heads of 128 on 2 x 4, 4,096 tokens of four causal
+// documents, capped (540).  Bound by vector issue at head dim 64: four fifths of a busy
+// SIMD's time with a cap or slopes, 710 cycles a tile of 32 x 32, of which the matrix
+// instructions run 256.  At 128 vector issue takes 48 %, matrix instructions run 27 %, and
+// two waves a SIMD do not hide all of the rest.  Few rows, 16 for one token over 130,001
+// keys of 2 x 64 (4.1 TB/s) and 5 for the join; bound by HBM and a launch's start and end.
 //
 // A masked key's value does not reach a row: its weight is zero, and where
 // zero times it is not (an infinity or NaN), the workgroup (the wave, where it

@@ -41,14 +41,17 @@
 // take 505 us against 487 and 532 (2 x 16 heads of 128 on 2 x 4, 4,096 tokens), and
 // 545 against 500 and 582 (8 heads of 64, 8,191 tokens).  In fp16 small weights
 // would lose bits below 2^-14, so P is scaled by 2^14 and dS by a power of two that
-// follows its largest value; the sums are scaled back.
+// follows its largest finite value; the sums are scaled back.
 //
-// Measured (us): dk, dv 265 and dq 127 at 2 x 16 heads of 128 on 2 x 4, four causal
-// documents of 4,096 tokens in all (375 and 590 TFLOP/s, four and three products);
-// 225 and 203 at 8 of 64, 8,191 tokens, causal with a prefix and slopes (630 and
-// 520).  At head dim 128 dk and dv are bound by LDS reads, 1 KB a matrix
-// instruction, with one wave a SIMD (dK, dV, K and V fill 512 registers); at 64 by
-// vector issue.  delta reads 100 MB in 17.
+// Measured (us a kernel after 200 passes; the first ten of a process take a seventh
+// longer): dk, dv 235 and dq 114 at 2 x 16 heads of 128 on 2 x 4, four causal documents of
+// 4,096 tokens in all, capped (420 and 650 TFLOP/s, four and three products); 197 and 178
+// at 8 of 64, 8,191 tokens, causal with a prefix and slopes (720 and 590).  At head
+// dim 128 dk and dv are bound by latency: the ring's 135 KB leave one workgroup a CU, so
+// one wave a SIMD (416 registers, of which dK, dV, K and V are 192); it waits 43 % of its
+// time, vector issue takes 29 % of a SIMD's, matrix instructions run 23 %, and LDS is
+// busy 13 % of a CU's.  With two waves a SIMD, at 64, these are 35, 48, 37 and 34 %; dq
+// at 128 36, 47, 38 and 17 %.  delta reads 100 MB in 17.6.
 #include "attn_masked_deal.h"
 
 #include <algorithm>

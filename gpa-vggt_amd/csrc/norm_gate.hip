@@ -17,8 +17,8 @@
 // rows, then are added over its waves in LDS and over workgroups by a second
 // kernel, in a fixed order: two calls give the same bits.
 //
-// Measured at 16,384 x 4,096 bf16: forward 97 us (5.5 TB/s), backward 174 (4.6 TB/s)
-// and 11 for the column sums; at 8 rows of 2,048 the forward takes 4.1, a launch.
+// Measured at 16,384 x 4,096 bf16: forward 95 us (5.6 TB/s), backward 173 (4.7 TB/s)
+// and 11 for the column sums; at 8 rows of 2,048 the forward takes 4.2, a launch.
 #include "gpa_common.h"
 
 #include <math.h>

@@ -148,8 +148,8 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale
     no gradient.  Offsets are read on the GPU: they must not decrease, and
     what lies outside the tensors is cut to them.
 
-    Returns [B, H, M, D] in q's dtype and order of dimensions; with return_lse
-    also the log2 softmax denominators [B, H, M] fp32.
+    Returns [B, H, M, D] in q's dtype (of an fp32 q: what it was cast to) and order
+    of dimensions; with return_lse also the log2 softmax denominators [B, H, M] fp32.
     """
     what = "attention_masked"
     sm_scale, cap = _score_args(what, sm_scale, cap, slopes)

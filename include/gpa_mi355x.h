@@ -503,7 +503,7 @@ int gpa_residual_layernorm_f16(const void* x, const void* y, const void* gamma,
  * k and v [B, Hk, N, D], all bf16 or all fp16; D = 64 or 128; query head h
  * reads key head h / (H / Hk).
  *   x = sm_scale q.k;  s = cap > 0 ? cap tanh(x / cap) : x;
- *   s -= slopes[h] |at - j|                       (slopes != NULL)
+ *   s -= slopes[h] |at - j|                       (slopes != NULL; of either sign)
  *   o = sum_j softmax(s)_j v_j over the keys that the query sees;
  *   lse[b*lse_sb + h*lse_sh + m] = log2 sum_j e^s  (lse != NULL)
  * A query that sees no key gets zeros and -inf.
@@ -523,7 +523,9 @@ int gpa_residual_layernorm_f16(const void* x, const void* y, const void* gamma,
  * format.  The gradients take delta = dO . (o + o_rest) from it.
  * workspace: gpa_attn_masked_workspace_bytes(...) bytes, 16-byte aligned,
  * overwritten (0: none).  Key rows (k_sn, v_sn, pk_sn, pv_sn) are less than
- * 2^23 elements apart; a head's keys may span any distance.
+ * 2^23 elements apart; a head's keys may span any distance.  A call is refused
+ * where its launches would need 2^24 workgroups (one a batch element and key head
+ * at least) or, over a shared prefix, 2^26 queries and heads.
  */
 typedef struct gpa_attn_masked_args {
   const void *q, *k, *v;
@@ -553,9 +555,10 @@ int gpa_attn_masked(int dtype, const gpa_attn_masked_args* args, void* workspace
 /*
  * Its gradients, from the forward's output o and log2 LSE (args->o and
  * args->lse, both required), args->o_rest (NULL: taken as zero, which costs
- * where weights are sharp: dq and dk are then off by twice their rounding) and the output's gradient d_o, with d_lse the LSE's
- * (NULL: none; contiguous [B, H, M]): dq, dk and dv in the operands' format,
- * those of a shared key head summed over its query heads.  No shared prefix
+ * where weights are sharp: dq and dk are then off by twice their rounding) and
+ * the output's gradient d_o, with d_lse the LSE's (NULL: none; contiguous
+ * [B, H, M]): dq, dk and dv in the operands' format, those of a shared key head
+ * summed over its query heads.  No shared prefix
  * (P = 0, lens = NULL).  Sums run in a fixed order: two calls give the same
  * bits.  A batch element's query heads of one key head, and 65 tokens, span
  * less than 2^29 elements of q and of d_o.  workspace:
