@@ -63,6 +63,16 @@ the custom ops:
                        Tensor stats, float scale, bool layer)
                        -> (Tensor dx, Tensor dy, Tensor dpost_w, Tensor dpost_b,
                            Tensor dgate, Tensor dpre_w, Tensor dpre_b)
+    gpa::head_rotary(Tensor q, Tensor? k, Tensor? positions, Tensor? freqs,
+                     Tensor? axes, int pairing, int[] sections, Tensor? q_w,
+                     Tensor? k_w, Tensor? q_b, Tensor? k_b, int norm, float eps)
+                     -> (Tensor q, Tensor k)                       (differentiable)
+    gpa::head_rotary_bwd(Tensor? d_q, Tensor? d_k, Tensor q, Tensor? k,
+                         Tensor? positions, Tensor? freqs, Tensor? axes, int pairing,
+                         int[] sections, Tensor? q_w, Tensor? k_w, Tensor? q_b,
+                         Tensor? k_b, int norm, float eps)
+                         -> (Tensor dq, Tensor dk, Tensor dq_w, Tensor dk_w,
+                             Tensor dq_b, Tensor dk_b)
 
 All launch on torch's current stream of the input's device.  There is no
 fallback: a missing library or a non-GPU tensor raises.
@@ -74,12 +84,12 @@ import ctypes
 import struct
 import threading
 from pathlib import Path
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libgpa_mi355x.so"
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 GPA_OK = 0
 GPA_E_INVALID = -1
@@ -135,6 +145,16 @@ _NormArgs = _struct("_NormArgs", ("p: x y gate w1 b1 w2 b2 stats", "l: rows C gr
                                   "i: layer", "f: scale eps"))
 _NormGrads = _struct("_NormGrads", ("p: dh dout dx dy dgate dw1 db1 dw2 db2",
                                     "l: dh_sn dout_sn dx_sn dy_sn"))
+
+# gpa_head_rotary_args and gpa_head_rotary_grads.
+MAX_AXES = 8
+_RotaryArgs = _struct("_RotaryArgs", (
+    "p: q k", "l: B N H Hk D pairs q_sb q_sh q_sn k_sb k_sh k_sn", "p: positions", "l: pos_sb pos_sn",
+    "p: freqs axes q_w k_w q_b k_b", "i: positions_kind pairing norm sections_count", "f: eps",
+    "i: s0 s1 s2 s3 s4 s5 s6 s7"))
+_RotaryGrads = _struct("_RotaryGrads", (
+    "p: d_q_out d_k_out dq dk dq_w dk_w dq_b dk_b",
+    "l: dqo_sb dqo_sh dqo_sn dko_sb dko_sh dko_sn dq_sb dq_sh dq_sn dk_sb dk_sh dk_sn"))
 
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None
@@ -260,6 +280,13 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.gpa_norm_gate_bwd.restype = ctypes.c_int
     lib.gpa_norm_gate_bwd.argtypes = [ctypes.c_int, ctypes.c_int, _vp,
                                       _vp, _vp, ctypes.c_size_t, _vp]
+    lib.gpa_head_rotary.restype = ctypes.c_int
+    lib.gpa_head_rotary.argtypes = [ctypes.c_int, ctypes.c_int, _vp, _vp, _i64, _i64, _i64,
+                                    _vp, _i64, _i64, _i64, _vp]
+    lib.gpa_head_rotary_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.gpa_head_rotary_bwd_workspace_bytes.argtypes = [_i64] * 5 + [ctypes.c_int]
+    lib.gpa_head_rotary_bwd.restype = ctypes.c_int
+    lib.gpa_head_rotary_bwd.argtypes = [ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, ctypes.c_size_t, _vp]
     lib.gpa_merge_order.restype = ctypes.c_int
     lib.gpa_merge_order.argtypes = [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp]
     lib.gpa_merge_plan_workspace_bytes.restype = ctypes.c_size_t
@@ -316,7 +343,8 @@ def exported_symbols() -> Tuple[str, ...]:
             "gpa_attn_keybias_join", "gpa_qk_norm_rope_params",
             "gpa_attn_masked_workspace_bytes", "gpa_attn_masked",
             "gpa_attn_masked_bwd_workspace_bytes", "gpa_attn_masked_bwd", "gpa_norm_gate",
-            "gpa_norm_gate_bwd_workspace_bytes", "gpa_norm_gate_bwd")
+            "gpa_norm_gate_bwd_workspace_bytes", "gpa_norm_gate_bwd", "gpa_head_rotary",
+            "gpa_head_rotary_bwd_workspace_bytes", "gpa_head_rotary_bwd")
 
 
 def _check(rc: int, what: str) -> None:
@@ -1550,3 +1578,179 @@ def norm_gate_bwd(dh: Optional[torch.Tensor], dout: Optional[torch.Tensor], x: t
 def _norm_gate_bwd_fake(dh, dout, x, y, post_w, post_b, gate, pre_w, pre_b, stats, scale, layer):
     return (x.new_empty(x.shape), x.new_empty(x.shape),
             *(pre_w.new_empty((0,) if t is None else t.shape) for t in (post_w, post_b, gate, pre_w, pre_b)))
+
+
+# --------------------------------------------------------------------------
+# gpa::head_rotary and its gradients
+# --------------------------------------------------------------------------
+
+_POSITION_KINDS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _rotary_check(what, q, k, positions, freqs, axes, pairing, sections, params):
+    """Checks, and the parameters' type."""
+    if q.dtype not in _DTYPE_CODES:
+        raise ValueError(f"{what}: dtype {q.dtype} is not fp32, bf16 or fp16")
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.dtype != q.dtype or k.shape[0] != q.shape[0]
+                                           or k.shape[2:] != q.shape[2:])):
+        raise ValueError(f"{what}: q [B, H, N, D] and k [B, Hk, N, D] of one type, got {q.dtype} {tuple(q.shape)}"
+                         + ("" if k is None else f" and {k.dtype} {tuple(k.shape)}"))
+    B, _, N, D = q.shape
+    if (positions is None) != (freqs is None) or (freqs is None) != (axes is None):
+        raise ValueError(f"{what}: positions, freqs and axes go together")
+    if freqs is not None:
+        pairs = freqs.shape[0] if freqs.dim() == 1 else -1
+        if freqs.dtype != torch.float64 or axes.dtype != torch.int32 or axes.shape != freqs.shape or pairs < 0:
+            raise ValueError(f"{what}: freqs fp64 [pairs] and axes int32 [pairs], got {freqs.dtype} "
+                             f"{tuple(freqs.shape)} and {axes.dtype} {tuple(axes.shape)}")
+        if 2 * pairs > D:
+            raise ValueError(f"{what}: {pairs} pairs do not fit into heads of {D} features")
+        if not 1 <= len(sections) <= MAX_AXES or any(s < 0 for s in sections) or sum(sections) != pairs:
+            raise ValueError(f"{what}: sections {tuple(sections)} must be 1 to {MAX_AXES} counts that add to {pairs}")
+        if positions.dtype not in _POSITION_KINDS or positions.shape not in ((N, len(sections)), (B, N, len(sections))):
+            raise ValueError(f"{what}: positions must be int32, int64 or fp32 [{N}, {len(sections)}] or "
+                             f"[{B}, {N}, {len(sections)}], got {positions.dtype} {tuple(positions.shape)}")
+    if pairing not in (0, 1, 2):
+        raise ValueError(f"{what}: unknown pairing {pairing}")
+    given = [p for p in params if p is not None]
+    if any(p.shape != (D,) for p in given):
+        raise ValueError(f"{what}: parameters must be [{D}], got {[tuple(p.shape) for p in given]}")
+    if any(p.dtype != given[0].dtype or p.dtype not in (q.dtype, torch.float32) for p in given):
+        raise ValueError(f"{what}: parameters are all of the heads' type {q.dtype}, or all fp32, got "
+                         f"{[p.dtype for p in given]}")
+    return given[0].dtype if given else q.dtype
+
+
+def _features(t):
+    """t, or a copy, with contiguous features."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides3(t):
+    return t.stride()[:3] if t is not None else (0, 0, 0)
+
+
+def _rotary_args(q, k, positions, freqs, axes, pairing, sections, params, norm, eps):
+    """The filled gpa_head_rotary_args, and the tensors it points into."""
+    B, H, N, D = q.shape
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    params = [None if t is None else t.contiguous() for t in params]
+    pos_sb = pos_sn = pairs = kind = 0
+    if freqs is not None and freqs.shape[0] > 0:
+        freqs, axes, pairs = freqs.contiguous(), axes.contiguous(), freqs.shape[0]
+        if positions.stride(-1) != 1 and positions.shape[-1] > 1:
+            positions = positions.contiguous()
+        kind, pos_sn = _POSITION_KINDS[positions.dtype], positions.stride(-2)
+        pos_sb = positions.stride(0) if positions.dim() == 3 else 0
+    sizes = (*sections, *(0,) * (MAX_AXES - len(sections)))
+    a = _RotaryArgs.packed(
+        q.data_ptr(), ptr(k), B, N, H, 0 if k is None else k.shape[1], D, pairs, *q.stride()[:3], *_strides3(k),
+        ptr(positions), pos_sb, pos_sn, ptr(freqs), ptr(axes), *map(ptr, params), kind, pairing, norm, len(sections),
+        eps, *sizes)
+    return a, (q, k, positions, freqs, axes, params)
+
+
+def _rotary_setup(ctx, inputs, output):
+    q, k, positions, freqs, axes, pairing, sections, q_w, k_w, q_b, k_b, norm, eps = inputs
+    ctx.set_materialize_grads(False)
+    if k is None:
+        ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(*((q, k) if norm else (None, None)), positions, freqs, axes, q_w, k_w, q_b, k_b)
+    ctx.rest = (pairing, list(sections), norm, eps)
+
+
+def _rotary_backward(ctx, d_q, d_k):
+    q, k, positions, freqs, axes, q_w, k_w, q_b, k_b = ctx.saved_tensors
+    pairing, sections, norm, eps = ctx.rest
+    if d_q is None and d_k is None:
+        return (None,) * 13
+    if not norm:
+        q, k = (d_q if d_q is not None else d_k), d_k
+    got = head_rotary_bwd(d_q, d_k, q, k, positions, freqs, axes, pairing, sections, q_w, k_w, q_b, k_b, norm, eps)
+    dq, dk, dqw, dkw, dqb, dkb = got
+    some = lambda g, t, d: None if t is None or d is None else g  # noqa: E731
+    return (some(dq, q, d_q), some(dk, k, d_k), None, None, None, None, None, some(dqw, q_w, d_q), some(dkw, k_w, d_k),
+            some(dqb, q_b, d_q), some(dkb, k_b, d_k), None, None)
+
+
+def head_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[torch.Tensor],
+                freqs: Optional[torch.Tensor], axes: Optional[torch.Tensor], pairing: int, sections: List[int],
+                q_w: Optional[torch.Tensor], k_w: Optional[torch.Tensor], q_b: Optional[torch.Tensor],
+                k_b: Optional[torch.Tensor], norm: int, eps: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """gpa_head_rotary of q [B, H, N, D] and k [B, Hk, N, D] (None: an empty
+    tensor comes back): new tensors in their order of dimensions.  norm 0 none,
+    1 RMS, 2 LayerNorm; pairing as the header's GPA_PAIRS_*."""
+    what = "gpa::head_rotary"
+    params = (q_w, k_w, q_b, k_b)
+    dev = _require_gpu(*[t for t in (q, k, positions, freqs, axes, *params) if t is not None])
+    pdt = _rotary_check(what, q, k, positions, freqs, axes, pairing, sections, params)
+    q_out, k_out = _like(q), q.new_empty(0) if k is None else _like(k)
+    if q_out.numel() + k_out.numel() == 0:
+        return q_out, k_out
+    a, held = _rotary_args(_features(q), _features(k), positions, freqs, axes, pairing, sections, params, norm, eps)
+    with _on(dev):
+        rc = lib().gpa_head_rotary(_DTYPE_CODES[q.dtype], _DTYPE_CODES[pdt], a, q_out.data_ptr(), *q_out.stride()[:3],
+                                   k_out.data_ptr() if k is not None else None,
+                                   *((0, 0, 0) if k is None else k_out.stride()[:3]), _stream(dev))
+    _check(rc, what)
+    return q_out, k_out
+
+
+head_rotary = _op(head_rotary, _rotary_setup, _rotary_backward)
+
+
+@_fake("head_rotary")
+def _head_rotary_fake(q, k, positions, freqs, axes, pairing, sections, q_w, k_w, q_b, k_b, norm, eps):
+    return _like(q), q.new_empty(0) if k is None else _like(k)
+
+
+@_op
+def head_rotary_bwd(d_q: Optional[torch.Tensor], d_k: Optional[torch.Tensor], q: torch.Tensor,
+                    k: Optional[torch.Tensor], positions: Optional[torch.Tensor], freqs: Optional[torch.Tensor],
+                    axes: Optional[torch.Tensor], pairing: int, sections: List[int], q_w: Optional[torch.Tensor],
+                    k_w: Optional[torch.Tensor], q_b: Optional[torch.Tensor], k_b: Optional[torch.Tensor],
+                    norm: int, eps: float
+                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """gpa_head_rotary_bwd: the gradients of q, k, q_w, k_w, q_b and k_b (empty
+    tensors for absent ones, and where the output's gradient is None).  Without
+    a norm q and k give their sizes and order of dimensions alone."""
+    what = "gpa::head_rotary_bwd"
+    params = (q_w, k_w, q_b, k_b)
+    dev = _require_gpu(*[t for t in (q, k, d_q, d_k, positions, freqs, axes, *params) if t is not None])
+    pdt = _rotary_check(what, q, k, positions, freqs, axes, pairing, sections, params)
+    for name, d, t in (("d_q", d_q, q), ("d_k", d_k, k)):
+        if d is not None and (t is None or d.shape != t.shape or d.dtype != t.dtype):
+            raise ValueError(f"{what}: {name} {d.dtype} {tuple(d.shape)} does not match its tensor")
+    none = lambda: q.new_empty(0)  # noqa: E731
+    dq, dk = none() if d_q is None else _like(q), none() if d_k is None else _like(k)
+    grads = [none() if t is None or d is None else torch.empty(t.shape, device=dev, dtype=t.dtype)
+             for t, d in zip(params, (d_q, d_k, d_q, d_k))]
+    if dq.numel() + dk.numel() == 0:
+        return (dq, dk, *(g.zero_() for g in grads))
+    for i, d in enumerate((d_q, d_k, d_q, d_k)):
+        if d is not None and d.numel() == 0:
+            grads[i].zero_()
+    d_q, d_k = _features(d_q), _features(d_k)
+    a, held = _rotary_args(_features(q), _features(k), positions, freqs, axes, pairing, sections, params, norm, eps)
+    ptr = lambda t: 0 if t is None or t.numel() == 0 else t.data_ptr()  # noqa: E731
+    wanted = [ptr(g) if d is not None and d.numel() else 0 for g, d in zip(grads, (d_q, d_k, d_q, d_k))]
+    g = _RotaryGrads.packed(ptr(d_q), ptr(d_k), ptr(dq), ptr(dk), *wanted, *_strides3(d_q), *_strides3(d_k),
+                            *(dq.stride()[:3] if d_q is not None else (0, 0, 0)),
+                            *(dk.stride()[:3] if d_k is not None else (0, 0, 0)))
+    L = lib()
+    B, H, N, D = q.shape
+    ws_bytes = L.gpa_head_rotary_bwd_workspace_bytes(B, N, H, 0 if k is None else k.shape[1], D, norm) if any(wanted) else 0
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+    with _on(dev):
+        rc = L.gpa_head_rotary_bwd(_DTYPE_CODES[q.dtype], _DTYPE_CODES[pdt], a, g, None if ws is None else ws.data_ptr(),
+                                   ws_bytes, _stream(dev))
+    _check(rc, what)
+    return (dq, dk, *grads)
+
+
+@_fake("head_rotary_bwd")
+def _head_rotary_bwd_fake(d_q, d_k, q, k, positions, freqs, axes, pairing, sections, q_w, k_w, q_b, k_b, norm, eps):
+    none = lambda: q.new_empty(0)  # noqa: E731
+    return (none() if d_q is None else _like(q), none() if d_k is None else _like(k),
+            *(none() if t is None or d is None else t.new_empty(t.shape)
+              for t, d in zip((q_w, k_w, q_b, k_b), (d_q, d_k, d_q, d_k))))

@@ -71,7 +71,7 @@
 extern "C" {
 #endif
 
-#define GPA_ABI_VERSION 19
+#define GPA_ABI_VERSION 20
 
 enum {
   GPA_OK = 0,
@@ -612,6 +612,60 @@ size_t gpa_norm_gate_bwd_workspace_bytes(int64_t rows, int64_t C, int64_t groups
 int gpa_norm_gate_bwd(int dtype, int param_dtype, const gpa_norm_gate_args* args,
                       const gpa_norm_gate_grads* grads, void* workspace, size_t workspace_bytes,
                       void* stream);
+
+/*
+ * The norm of every head and its rotation by positions of several axes (no
+ * counterpart in the reference), of q [B, H, N, D] and, where Hk > 0, k [B, Hk, N, D]
+ * (features contiguous; D even, 2 to 256):
+ *   n = N(x) w + b;  y_a = n_a cos t - n_b sin t,  y_b = n_b cos t + n_a sin t
+ * for pair j of features (a, b), t = positions[axes[j]] freqs[j].  norm: 0 none, 1
+ * RMS, 2 LayerNorm over the head; parameters [D] of param_dtype (dtype or fp32; w
+ * NULL: 1, b NULL: 0).  pairing: feature j with pairs + j (halves), 2 j with 2 j + 1
+ * (neighbours), or halves of each axis's own block of 2 sections[i] features
+ * (blocks); features past 2 * pairs are not turned.  positions: element (b, n, axis)
+ * at b pos_sb + n pos_sn + axis, of positions_kind 0 int32, 1 int64, 2 fp32;
+ * sections_count axes.  axes and freqs are read on the GPU (an axis outside is
+ * cut to the range).  Angles are formed in 64 bits, everything else in 32,
+ * and each output is rounded once.
+ */
+enum { GPA_PAIRS_HALVES = 0, GPA_PAIRS_NEIGHBOURS = 1, GPA_PAIRS_BLOCKS = 2 };
+#define GPA_MAX_AXES 8
+
+typedef struct gpa_head_rotary_args {
+  const void *q, *k;
+  int64_t B, N, H, Hk, D, pairs;
+  int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn;
+  const void* positions;
+  int64_t pos_sb, pos_sn;
+  const double* freqs;            /* [pairs], radians a unit of position */
+  const int32_t* axes;            /* [pairs] */
+  const void *q_w, *k_w, *q_b, *k_b;
+  int32_t positions_kind, pairing, norm, sections_count;
+  float eps;
+  int32_t sections[GPA_MAX_AXES];
+} gpa_head_rotary_args;
+
+int gpa_head_rotary(int dtype, int param_dtype, const gpa_head_rotary_args* args, void* q_out,
+                    int64_t qo_sb, int64_t qo_sh, int64_t qo_sn, void* k_out, int64_t ko_sb,
+                    int64_t ko_sh, int64_t ko_sn, void* stream);
+
+/* Its gradients, from those of q_out and k_out (either NULL: that tensor has none, nor
+ * its parameters): dq and dk, and the parameters' (NULL: not wanted) in
+ * param_dtype.  Without a norm args->q and args->k are not read.  Sums run in a fixed
+ * order.  workspace: gpa_head_rotary_bwd_workspace_bytes(...), 16-byte aligned; none
+ * where no parameter's gradient is wanted. */
+typedef struct gpa_head_rotary_grads {
+  const void *d_q_out, *d_k_out;
+  void *dq, *dk, *dq_w, *dk_w, *dq_b, *dk_b;
+  int64_t dqo_sb, dqo_sh, dqo_sn, dko_sb, dko_sh, dko_sn;
+  int64_t dq_sb, dq_sh, dq_sn, dk_sb, dk_sh, dk_sn;
+} gpa_head_rotary_grads;
+
+size_t gpa_head_rotary_bwd_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t Hk, int64_t D,
+                                           int norm);
+int gpa_head_rotary_bwd(int dtype, int param_dtype, const gpa_head_rotary_args* args,
+                        const gpa_head_rotary_grads* grads, void* workspace, size_t workspace_bytes,
+                        void* stream);
 
 #ifdef __cplusplus
 }
