@@ -73,6 +73,11 @@ the custom ops:
                          Tensor? k_b, int norm, float eps)
                          -> (Tensor dq, Tensor dk, Tensor dq_w, Tensor dk_w,
                              Tensor dq_b, Tensor dk_b)
+    gpa::draft_tree(Tensor parents, Tensor lengths, Tensor? sizes)
+                    -> (Tensor positions, Tensor seen)
+    gpa::attn_tree(Tensor q, Tensor cache_k, Tensor cache_v, Tensor k, Tensor v,
+                   Tensor? lengths, Tensor seen, float sm_scale, float cap,
+                   Tensor? slopes, bool want_lse) -> (Tensor o, Tensor lse)
 
 All launch on torch's current stream of the input's device.  There is no
 fallback: a missing library or a non-GPU tensor raises.
@@ -145,6 +150,12 @@ _NormArgs = _struct("_NormArgs", ("p: x y gate w1 b1 w2 b2 stats", "l: rows C gr
                                   "i: layer", "f: scale eps"))
 _NormGrads = _struct("_NormGrads", ("p: dh dout dx dy dgate dw1 db1 dw2 db2",
                                     "l: dh_sn dout_sn dx_sn dy_sn"))
+
+# gpa_attn_tree_args.
+_TreeArgs = _struct("_TreeArgs", (
+    "p: q cache_k cache_v k v o lse", "l: B H Hk T N D",
+    "l: q_sb q_sh q_st ck_sb ck_sh ck_sn cv_sb cv_sh cv_sn k_sb k_sh k_st v_sb v_sh v_st o_sb o_sh o_st lse_sb lse_sh",
+    "p: lengths seen slopes", "l: slopes_sb", "f: sm_scale cap"))
 
 # gpa_head_rotary_args and gpa_head_rotary_grads.
 MAX_AXES = 8
@@ -280,6 +291,12 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.gpa_norm_gate_bwd.restype = ctypes.c_int
     lib.gpa_norm_gate_bwd.argtypes = [ctypes.c_int, ctypes.c_int, _vp,
                                       _vp, _vp, ctypes.c_size_t, _vp]
+    lib.gpa_draft_tree.restype = ctypes.c_int
+    lib.gpa_draft_tree.argtypes = [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp]
+    lib.gpa_attn_tree_workspace_bytes.restype = ctypes.c_size_t
+    lib.gpa_attn_tree_workspace_bytes.argtypes = [_i64] * 6
+    lib.gpa_attn_tree.restype = ctypes.c_int
+    lib.gpa_attn_tree.argtypes = [ctypes.c_int, _vp, _vp, ctypes.c_size_t, _vp]
     lib.gpa_head_rotary.restype = ctypes.c_int
     lib.gpa_head_rotary.argtypes = [ctypes.c_int, ctypes.c_int, _vp, _vp, _i64, _i64, _i64,
                                     _vp, _i64, _i64, _i64, _vp]
@@ -344,7 +361,8 @@ def exported_symbols() -> Tuple[str, ...]:
             "gpa_attn_masked_workspace_bytes", "gpa_attn_masked",
             "gpa_attn_masked_bwd_workspace_bytes", "gpa_attn_masked_bwd", "gpa_norm_gate",
             "gpa_norm_gate_bwd_workspace_bytes", "gpa_norm_gate_bwd", "gpa_head_rotary",
-            "gpa_head_rotary_bwd_workspace_bytes", "gpa_head_rotary_bwd")
+            "gpa_head_rotary_bwd_workspace_bytes", "gpa_head_rotary_bwd",
+            "gpa_draft_tree", "gpa_attn_tree_workspace_bytes", "gpa_attn_tree")
 
 
 def _check(rc: int, what: str) -> None:
@@ -1754,3 +1772,102 @@ def _head_rotary_bwd_fake(d_q, d_k, q, k, positions, freqs, axes, pairing, secti
     return (none() if d_q is None else _like(q), none() if d_k is None else _like(k),
             *(none() if t is None or d is None else t.new_empty(t.shape)
               for t, d in zip((q_w, k_w, q_b, k_b), (d_q, d_k, d_q, d_k))))
+
+
+# --------------------------------------------------------------------------
+# gpa::draft_tree and gpa::attn_tree
+# --------------------------------------------------------------------------
+
+MAX_DRAFT = 1024
+
+
+def _counts(what, name, t, B):
+    if t is not None and (t.dtype != torch.int32 or t.shape != (B,)):
+        raise ValueError(f"{what}: {name} must be torch.int32 [{B}], got {t.dtype} {tuple(t.shape)}")
+    return None if t is None else t.contiguous()
+
+
+@_op
+def draft_tree(parents: torch.Tensor, lengths: torch.Tensor,
+               sizes: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """gpa_draft_tree: positions int32 [B, T] and the seen tokens' bits int32
+    [B, T, ceil(T / 32)] of the trees that parents int32 [T] or [B, T] describe."""
+    what = "gpa::draft_tree"
+    dev = _require_gpu(*[t for t in (parents, lengths, sizes) if t is not None])
+    if lengths.dim() != 1:
+        raise ValueError(f"{what}: lengths must be torch.int32 [B], got {tuple(lengths.shape)}")
+    B = lengths.shape[0]
+    lengths, sizes = _counts(what, "lengths", lengths, B), _counts(what, "sizes", sizes, B)
+    if parents.dtype != torch.int32 or parents.dim() not in (1, 2) or (parents.dim() == 2 and parents.shape[0] != B):
+        raise ValueError(f"{what}: parents must be int32 [T] or [{B}, T], got {parents.dtype} {tuple(parents.shape)}")
+    T = parents.shape[-1]
+    if T > MAX_DRAFT:
+        raise NotImplementedError(f"{what}: {T} drafted tokens (up to {MAX_DRAFT})")
+    parents, sb = _table(what, "parents", parents, B, T, torch.int32)
+    positions = torch.empty(B, T, device=dev, dtype=torch.int32)
+    seen = torch.empty(B, T, (T + 31) // 32, device=dev, dtype=torch.int32)
+    with _on(dev):
+        rc = lib().gpa_draft_tree(parents.data_ptr(), sb, lengths.data_ptr(), None if sizes is None else sizes.data_ptr(),
+                                  B, T, positions.data_ptr(), seen.data_ptr(), _stream(dev))
+    _check(rc, what)
+    return positions, seen
+
+
+@_fake("draft_tree")
+def _draft_tree_fake(parents, lengths, sizes):
+    B, T = lengths.shape[0], parents.shape[-1]
+    return (parents.new_empty((B, T), dtype=torch.int32), parents.new_empty((B, T, (T + 31) // 32), dtype=torch.int32))
+
+
+def _tree_check(what, q, cache_k, cache_v, k, v, lengths, seen, slopes):
+    """Checks, and the tables as the kernel takes them."""
+    _masked_shapes(what, q, k, v)
+    B, H, T, D = q.shape
+    if k.shape[2] != T:
+        raise ValueError(f"{what}: {T} queries and {k.shape[2]} drafted keys")
+    for name, t in (("cache_k", cache_k), ("cache_v", cache_v)):
+        if t.dtype != q.dtype or t.dim() != 4 or t.shape != cache_k.shape \
+                or (*t.shape[:2], t.shape[3]) != (B, k.shape[1], D):
+            raise ValueError(f"{what}: {name} must be {q.dtype} [{B}, {k.shape[1]}, N, {D}], got {t.dtype} "
+                             f"{tuple(t.shape)}")
+    if T > MAX_DRAFT:
+        raise NotImplementedError(f"{what}: {T} drafted tokens (up to {MAX_DRAFT})")
+    if seen.dtype != torch.int32 or seen.shape != (B, T, (T + 31) // 32):
+        raise ValueError(f"{what}: seen must be int32 [{B}, {T}, {(T + 31) // 32}], got {seen.dtype} {tuple(seen.shape)}")
+    sl_sb = 0
+    if slopes is not None:
+        slopes, sl_sb = _table(what, "slopes", slopes, B, H, torch.float32)
+    return _counts(what, "lengths", lengths, B), seen.contiguous(), slopes, sl_sb
+
+
+@_op
+def attn_tree(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+              lengths: Optional[torch.Tensor], seen: torch.Tensor, sm_scale: float, cap: float,
+              slopes: Optional[torch.Tensor], want_lse: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """gpa_attn_tree: o like q, and the log2 LSE [B, H, T] fp32 if want_lse (else an
+    empty tensor).  cap 0: none."""
+    what = "gpa::attn_tree"
+    dev = _require_gpu(*[t for t in (q, cache_k, cache_v, k, v, lengths, seen, slopes) if t is not None])
+    lengths, seen, slopes, sl_sb = _tree_check(what, q, cache_k, cache_v, k, v, lengths, seen, slopes)
+    o = _like(q)
+    B, H, T, D = q.shape
+    lse = torch.empty((B, H, T) if want_lse else (0,), device=dev, dtype=torch.float32)
+    q, cache_k, cache_v, k, v = (_rows8(t) for t in (q, cache_k, cache_v, k, v))
+    N, Hk = cache_k.shape[2], k.shape[1]
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    a = _TreeArgs.packed(
+        *map(ptr, (q, cache_k, cache_v, k, v, o)), lse.data_ptr() if want_lse else 0, B, H, Hk, T, N, D,
+        *(s for t in (q, cache_k, cache_v, k, v, o) for s in t.stride()[:3]), *(lse.stride()[:2] if want_lse else (0, 0)),
+        ptr(lengths), seen.data_ptr(), ptr(slopes), sl_sb, sm_scale, cap)
+    L = lib()
+    ws_bytes = L.gpa_attn_tree_workspace_bytes(B, H, Hk, T, N, D)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+    with _on(dev):
+        rc = L.gpa_attn_tree(_DTYPE_CODES[q.dtype], a, None if ws is None else ws.data_ptr(), ws_bytes, _stream(dev))
+    _check(rc, what)
+    return o, lse
+
+
+@_fake("attn_tree")
+def _attn_tree_fake(q, cache_k, cache_v, k, v, lengths, seen, sm_scale, cap, slopes, want_lse):
+    return _like(q), q.new_empty(q.shape[:3] if want_lse else (0,), dtype=torch.float32)

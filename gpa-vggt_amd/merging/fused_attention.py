@@ -17,17 +17,19 @@ frame-special split path of vggt/layers/attention.py:148-176.
 reference) are the attention of language-model blocks: packed documents,
 causal and prefix masks, capped and distance-biased scores, shared key heads,
 gradients, and a prefix that a whole batch shares (`csrc/attn_masked.hip`).
+`draft_tree` and `attention_tree` check trees of drafted tokens against a cache
+(`csrc/attn_tree.hip`).
 """
 from __future__ import annotations
 
-from typing import Optional, Union
+from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _native
 
 __all__ = ["attention_keybias", "attention_join", "attention_masked", "attention_rows",
-           "attention_shared_prefix", "combine_by_lse", "LOG2E"]
+           "attention_shared_prefix", "attention_tree", "combine_by_lse", "draft_tree", "LOG2E"]
 
 LOG2E = 1.4426950408889634
 _F32_MIN, _F32_MAX = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
@@ -198,4 +200,45 @@ def attention_shared_prefix(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: t
     q, prefix_k, prefix_v, k, v = _half_operands(q, (prefix_k, prefix_v, k, v))
     o, lse = _native.attn_shared_prefix(q, prefix_k, prefix_v, k, v, lengths, sm_scale, cap, slopes,
                                         bool(return_lse))
+    return (o, lse) if return_lse else o
+
+
+def draft_tree(parents: torch.Tensor, lengths: torch.Tensor, *,
+               sizes: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Positions and sight of drafted tokens, a tree of them behind each sequence.
+
+    parents (int32 [B, T], or [T] for the same tree behind all; T up to 1,024): the
+    number of each token's parent, an earlier token of its sequence; anything else
+    hangs it on the last key of the cache.  lengths (int32 [B]): the caches'
+    keys; sizes (int32 [B]; None: T): how many of a sequence's tokens are there.
+    All are read on the GPU.
+
+    Returns (positions int32 [B, T], lengths[b] + depth, for the rotation of their
+    queries and keys; seen int32 [B, T, ceil(T / 32)], in whose row bit j (of
+    word j // 32) stands where a token sees token j: its ancestors and itself).
+    What lies behind a sequence's size has position 0 and sees nothing.  Both serve all
+    layers of a step.
+    """
+    return _native.draft_tree(parents, lengths, sizes)
+
+
+def attention_tree(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Tensor,
+                   v: torch.Tensor, sm_scale: float, *, seen: torch.Tensor,
+                   lengths: Optional[torch.Tensor] = None, cap: Optional[float] = None,
+                   slopes: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """Attention of drafted tokens over their sequence's cache and the drafted tokens
+    that they see.
+
+    q [B, H, T, D] and k, v [B, Hk, T, D]: the drafted tokens' (none of them in the cache
+    yet); cache_k, cache_v [B, Hk, N, D], of which every token sees the first
+    lengths[b] (int32 [B]; None: N) keys; seen: the bits from `draft_tree` (or
+    others of that form).  A token that sees no drafted one, not even itself, sees
+    nothing: zeros, LSE -inf.  Scores, dtypes, strides and results as in
+    `attention_masked`; with slopes a token lies |difference of positions| from a key,
+    as `draft_tree` counts them.  Forward only.
+    """
+    what = "attention_tree"
+    sm_scale, cap = _score_args(what, sm_scale, cap, slopes)
+    q, cache_k, cache_v, k, v = _half_operands(q, (cache_k, cache_v, k, v))
+    o, lse = _native.attn_tree(q, cache_k, cache_v, k, v, lengths, seen, sm_scale, cap, slopes, bool(return_lse))
     return (o, lse) if return_lse else o

@@ -667,6 +667,46 @@ int gpa_head_rotary_bwd(int dtype, int param_dtype, const gpa_head_rotary_args* 
                         const gpa_head_rotary_grads* grads, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/*
+ * A tree of drafted tokens for each of B sequences (no counterpart in the reference).
+ * parents int32 [B, T] (parents_sb between sequences, 0: the same tree for all): the
+ * number of a token's parent, an earlier one; anything else: the cache's last key.
+ * sizes int32 [B] (NULL: T): the tokens that are there.  positions int32 [B, T]:
+ * lengths[b] + depth; seen int32 [B, T, ceil(T / 32)]: bit j of a token's row (word j /
+ * 32, bit j % 32) where it sees token j, its ancestors and itself.  Tokens past a
+ * sequence's size get position 0 and no bit.  T <= 1,024.
+ */
+int gpa_draft_tree(const int32_t* parents, int64_t parents_sb, const int32_t* lengths,
+                   const int32_t* sizes, int64_t B, int64_t T, int32_t* positions, int32_t* seen,
+                   void* stream);
+
+/*
+ * Attention of drafted tokens q [B, H, T, D] over the first lengths[b] (int32 [B]; NULL: N)
+ * keys of cache_k, cache_v [B, Hk, N, D] and over the drafted k, v [B, Hk, T, D] that their
+ * rows of `seen` ([B, T, ceil(T / 32)], contiguous, as gpa_draft_tree makes) name.
+ * Scores, formats and results as gpa_attn_masked; the distance that a slope weighs
+ * is to position j of the cache from length + (bits of the row) - 1, and to a drafted
+ * token the number of seen tokens behind it.  A token with no bit gets zeros (LSE
+ * -inf).  D 64 or 128, T <= 1,024.  Sums run in a fixed order.  workspace:
+ * gpa_attn_tree_workspace_bytes(...), 16-byte aligned.
+ */
+typedef struct gpa_attn_tree_args {
+  const void *q, *cache_k, *cache_v, *k, *v;
+  void* o;
+  float* lse;
+  int64_t B, H, Hk, T, N, D;
+  int64_t q_sb, q_sh, q_st, ck_sb, ck_sh, ck_sn, cv_sb, cv_sh, cv_sn, k_sb, k_sh, k_st, v_sb, v_sh, v_st;
+  int64_t o_sb, o_sh, o_st, lse_sb, lse_sh;
+  const int32_t *lengths, *seen;
+  const float* slopes;            /* [H] or NULL; slopes_sb between batch elements (0: shared) */
+  int64_t slopes_sb;
+  float sm_scale, cap;
+} gpa_attn_tree_args;
+
+size_t gpa_attn_tree_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t T, int64_t N, int64_t D);
+int gpa_attn_tree(int dtype, const gpa_attn_tree_args* args, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif
