@@ -78,6 +78,12 @@ the custom ops:
     gpa::attn_tree(Tensor q, Tensor cache_k, Tensor cache_v, Tensor k, Tensor v,
                    Tensor? lengths, Tensor seen, float sm_scale, float cap,
                    Tensor? slopes, bool want_lse) -> (Tensor o, Tensor lse)
+    gpa::linear_gate(Tensor x, Tensor w, Tensor? bias, Tensor? gate, Tensor? residual,
+                     int act, bool want_z) -> (Tensor y, Tensor z)  (differentiable)
+    gpa::linear_gate_bwd(Tensor dy, Tensor? z, Tensor x, Tensor w, Tensor? bias,
+                         Tensor? gate, int act, bool want_x, bool want_w,
+                         bool want_bias, bool want_gate)
+                         -> (Tensor dx, Tensor dw, Tensor dbias, Tensor dgate)
 
 All launch on torch's current stream of the input's device.  There is no
 fallback: a missing library or a non-GPU tensor raises.
@@ -156,6 +162,10 @@ _TreeArgs = _struct("_TreeArgs", (
     "p: q cache_k cache_v k v o lse", "l: B H Hk T N D",
     "l: q_sb q_sh q_st ck_sb ck_sh ck_sn cv_sb cv_sh cv_sn k_sb k_sh k_st v_sb v_sh v_st o_sb o_sh o_st lse_sb lse_sh",
     "p: lengths seen slopes", "l: slopes_sb", "f: sm_scale cap"))
+
+# gpa_linear_gate_args and gpa_linear_gate_grads.
+_LinearArgs = _struct("_LinearArgs", ("p: x w bias gate residual", "l: M N K x_s w_s residual_s", "i: act"))
+_LinearGrads = _struct("_LinearGrads", ("p: dy z dx dw dbias dgate", "l: dy_s dx_s dw_s K_out"))
 
 # gpa_head_rotary_args and gpa_head_rotary_grads.
 MAX_AXES = 8
@@ -291,6 +301,14 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.gpa_norm_gate_bwd.restype = ctypes.c_int
     lib.gpa_norm_gate_bwd.argtypes = [ctypes.c_int, ctypes.c_int, _vp,
                                       _vp, _vp, ctypes.c_size_t, _vp]
+    lib.gpa_linear_gate_workspace_bytes.restype = ctypes.c_size_t
+    lib.gpa_linear_gate_workspace_bytes.argtypes = [_i64] * 3
+    lib.gpa_linear_gate.restype = ctypes.c_int
+    lib.gpa_linear_gate.argtypes = [ctypes.c_int, ctypes.c_int, _vp, _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp]
+    lib.gpa_linear_gate_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.gpa_linear_gate_bwd_workspace_bytes.argtypes = [_vp, _vp]
+    lib.gpa_linear_gate_bwd.restype = ctypes.c_int
+    lib.gpa_linear_gate_bwd.argtypes = [ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, ctypes.c_size_t, _vp]
     lib.gpa_draft_tree.restype = ctypes.c_int
     lib.gpa_draft_tree.argtypes = [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp]
     lib.gpa_attn_tree_workspace_bytes.restype = ctypes.c_size_t
@@ -362,7 +380,9 @@ def exported_symbols() -> Tuple[str, ...]:
             "gpa_attn_masked_bwd_workspace_bytes", "gpa_attn_masked_bwd", "gpa_norm_gate",
             "gpa_norm_gate_bwd_workspace_bytes", "gpa_norm_gate_bwd", "gpa_head_rotary",
             "gpa_head_rotary_bwd_workspace_bytes", "gpa_head_rotary_bwd",
-            "gpa_draft_tree", "gpa_attn_tree_workspace_bytes", "gpa_attn_tree")
+            "gpa_draft_tree", "gpa_attn_tree_workspace_bytes", "gpa_attn_tree",
+            "gpa_linear_gate_workspace_bytes", "gpa_linear_gate",
+            "gpa_linear_gate_bwd_workspace_bytes", "gpa_linear_gate_bwd")
 
 
 def _check(rc: int, what: str) -> None:
@@ -1871,3 +1891,151 @@ def attn_tree(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k: 
 @_fake("attn_tree")
 def _attn_tree_fake(q, cache_k, cache_v, k, v, lengths, seen, sm_scale, cap, slopes, want_lse):
     return _like(q), q.new_empty(q.shape[:3] if want_lse else (0,), dtype=torch.float32)
+
+
+# --------------------------------------------------------------------------
+# gpa::linear_gate and its gradients
+# --------------------------------------------------------------------------
+
+def _linear_check(what, x, w, bias, gate, residual, act):
+    """Checks, and the parameters' type."""
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{what} takes bf16 or fp16 x, got {x.dtype}")
+    if x.dim() != 2 or w.dim() != 2 or w.dtype != x.dtype or w.shape[1] != x.shape[1]:
+        raise ValueError(f"{what}: x [M, K] and weight [N, K] of one type, got {x.dtype} {tuple(x.shape)} and {w.dtype} "
+                         f"{tuple(w.shape)}")
+    N = w.shape[0]
+    given = [(n, t) for n, t in (("bias", bias), ("gate", gate)) if t is not None]
+    for name, t in given:
+        if t.shape != (N,):
+            raise ValueError(f"{what}: {name} must be [{N}], got {tuple(t.shape)}")
+        if t.dtype != given[0][1].dtype or t.dtype not in (x.dtype, torch.float32):
+            raise ValueError(f"{what}: bias and gate are both of x's type {x.dtype}, or both fp32, got {t.dtype}")
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != (x.shape[0], N)):
+        raise ValueError(f"{what}: residual must be {x.dtype} [{x.shape[0]}, {N}], got {residual.dtype} "
+                         f"{tuple(residual.shape)}")
+    if not 0 <= act <= 4:
+        raise ValueError(f"{what}: unknown activation {act}")
+    return given[0][1].dtype if given else x.dtype
+
+
+def _rows_of_8(t):
+    """t [R, C] of 16-bit values with C a multiple of 8 and rows that are 16-byte
+    aligned and do not overlap, padded with zero columns where it has no such form."""
+    R, C = t.shape
+    if C % 8 == 0 and C and _rows_ok(t, 8) and (R < 2 or 0 <= t.stride(0) < 1 << 21):
+        return t
+    new = t.new_zeros(R, max(8, -(-C // 8) * 8)) if C % 8 or not C else t.new_empty(R, C)
+    new[:, :C].copy_(t)
+    return new
+
+
+def _linear_args(x, w, bias, gate, residual, act):
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    return _LinearArgs.packed(x.data_ptr(), w.data_ptr(), ptr(bias), ptr(gate), ptr(residual), x.shape[0], w.shape[0],
+                              x.shape[1], x.stride(0), w.stride(0), 0 if residual is None else residual.stride(0), act)
+
+
+def _linear_setup(ctx, inputs, output):
+    x, w, bias, gate, residual, act, want_z = inputs
+    if (act or gate is not None) and not want_z:
+        raise RuntimeError("gpa::linear_gate: gradients need the sums before the activation (want_z)")
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(x, w, bias, gate, output[1] if want_z else None)
+    ctx.act = act
+
+
+def _linear_backward(ctx, dy, _):
+    x, w, bias, gate, z = ctx.saved_tensors
+    if dy is None:
+        return (None,) * 7
+    need = [ctx.needs_input_grad[i] and t is not None for i, t in enumerate((x, w, bias, gate))]
+    dx, dw, db, dg = linear_gate_bwd(dy, z, x, w, bias, gate, ctx.act, *need) if any(need) else (None,) * 4
+    some = lambda i, g: g if need[i] else None  # noqa: E731
+    return some(0, dx), some(1, dw), some(2, db), some(3, dg), dy if ctx.needs_input_grad[4] else None, None, None
+
+
+def linear_gate(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], gate: Optional[torch.Tensor],
+                residual: Optional[torch.Tensor], act: int, want_z: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """gpa_linear_gate: y [M, N] in x's type, and the sums before the activation, fp32
+    [M, N], if want_z (else an empty tensor), which gradients need where there is an
+    activation or a gate.  act as the header's GPA_ACT_*."""
+    what = "gpa::linear_gate"
+    dev = _require_gpu(*[t for t in (x, w, bias, gate, residual) if t is not None])
+    pdt = _linear_check(what, x, w, bias, gate, residual, act)
+    M, N = x.shape[0], w.shape[0]
+    y = torch.empty(M, N, device=dev, dtype=x.dtype)
+    z = torch.empty((M, N) if want_z else (0,), device=dev, dtype=torch.float32)
+    if M == 0 or N == 0:
+        return y, z
+    x, w = _rows_of_8(x), _rows_of_8(w)
+    bias, gate = (None if t is None else t.contiguous() for t in (bias, gate))
+    residual = residual if residual is None or residual.stride(1) == 1 or N == 1 else residual.contiguous()
+    L = lib()
+    ws_bytes = L.gpa_linear_gate_workspace_bytes(M, N, x.shape[1])
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+    with _on(dev):
+        rc = L.gpa_linear_gate(_DTYPE_CODES[x.dtype], _DTYPE_CODES[pdt], _linear_args(x, w, bias, gate, residual, act),
+                               y.data_ptr(), N, z.data_ptr() if want_z else None, None if ws is None else ws.data_ptr(),
+                               ws_bytes, _stream(dev))
+    _check(rc, what)
+    return y, z
+
+
+linear_gate = _op(linear_gate, _linear_setup, _linear_backward)
+
+
+@_fake("linear_gate")
+def _linear_gate_fake(x, w, bias, gate, residual, act, want_z):
+    size = (x.shape[0], w.shape[0])
+    return x.new_empty(size), x.new_empty(size if want_z else (0,), dtype=torch.float32)
+
+
+@_op
+def linear_gate_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: torch.Tensor, w: torch.Tensor,
+                    bias: Optional[torch.Tensor], gate: Optional[torch.Tensor], act: int, want_x: bool, want_w: bool,
+                    want_bias: bool, want_gate: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """gpa_linear_gate_bwd: the wanted gradients of x, w, bias and gate (empty tensors for
+    the others).  z: the forward's, with an activation or the gate's gradient."""
+    what = "gpa::linear_gate_bwd"
+    dev = _require_gpu(*[t for t in (dy, z, x, w, bias, gate) if t is not None])
+    pdt = _linear_check(what, x, w, bias, gate, dy, act)
+    (M, K), N = x.shape, w.shape[0]
+    if (want_bias and bias is None) or (want_gate and gate is None):
+        raise ValueError(f"{what}: no gradient of an absent bias or gate")
+    if z is None and (act or want_gate):
+        raise ValueError(f"{what}: an activation, and the gate's gradient, need z")
+    if z is not None and (z.dtype != torch.float32 or z.shape != (M, N) or not z.is_contiguous() or z.data_ptr() % 16):
+        raise ValueError(f"{what}: z must be contiguous fp32 [{M}, {N}], got {z.dtype} {tuple(z.shape)}")
+    none = lambda: x.new_empty(0)  # noqa: E731
+    dx = torch.empty(M, K, device=dev, dtype=x.dtype) if want_x else none()
+    dw = torch.empty(N, K, device=dev, dtype=w.dtype) if want_w else none()
+    db, dg = (torch.empty(N, device=dev, dtype=pdt) if want else none() for want in (want_bias, want_gate))
+    if M == 0 or N == 0 or K == 0:
+        dx.zero_(), dw.zero_()
+        if M == 0 or N == 0 or not (want_bias or want_gate):
+            return dx, dw, db.zero_(), dg.zero_()
+    x, w = _rows_of_8(x), _rows_of_8(w)
+    gate = None if gate is None else gate.contiguous()
+    dy = dy if dy.stride(1) == 1 or N == 1 else dy.contiguous()
+    ptr = lambda t: t.data_ptr() if t.numel() else 0  # noqa: E731
+    a = _linear_args(x, w, None, gate, None, act)
+    g = _LinearGrads.packed(dy.data_ptr(), 0 if z is None else z.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(dg), dy.stride(0),
+                            K, K, max(K, 1))
+    L = lib()
+    ws_bytes = L.gpa_linear_gate_bwd_workspace_bytes(a, g)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    with _on(dev):
+        rc = L.gpa_linear_gate_bwd(_DTYPE_CODES[x.dtype], _DTYPE_CODES[pdt], a, g, ws.data_ptr(), ws_bytes, _stream(dev))
+    _check(rc, what)
+    return dx, dw, db, dg
+
+
+@_fake("linear_gate_bwd")
+def _linear_gate_bwd_fake(dy, z, x, w, bias, gate, act, want_x, want_w, want_bias, want_gate):
+    none = lambda: x.new_empty(0)  # noqa: E731
+    pdt = next((t.dtype for t in (bias, gate) if t is not None), x.dtype)
+    return (torch.empty_like(x, memory_format=torch.contiguous_format) if want_x else none(),
+            torch.empty_like(w, memory_format=torch.contiguous_format) if want_w else none(),
+            *(x.new_empty(w.shape[0], dtype=pdt) if want else none() for want in (want_bias, want_gate)))

@@ -707,6 +707,46 @@ size_t gpa_attn_tree_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t T
 int gpa_attn_tree(int dtype, const gpa_attn_tree_args* args, void* workspace, size_t workspace_bytes,
                   void* stream);
 
+/*
+ * A projection with what follows it (no counterpart in the reference), rows of 16-bit
+ * x [M, K] and w [N, K]:
+ *   z = x w^T + bias;  y = residual + gate act(z)
+ * bias and gate [N] (of dtype or fp32) and residual [M, N] (dtype) may be NULL.  act:
+ * GPA_ACT_*.  fp32 inside (GELU's distribution is off by 8e-8 absolutely), y rounded once.
+ * K a multiple of 8 (pad with zeros), rows of x and w 16-byte aligned, of
+ * strides below 2^21.  z (NULL: not kept): fp32 [M, N] contiguous, 16-byte aligned, for
+ * the backward, which needs it with an activation or for the gate's gradient.
+ * workspace: gpa_linear_gate_workspace_bytes(...), 16-byte aligned.
+ */
+enum { GPA_ACT_NONE = 0, GPA_ACT_GELU = 1, GPA_ACT_GELU_TANH = 2, GPA_ACT_SILU = 3, GPA_ACT_RELU = 4 };
+
+typedef struct gpa_linear_gate_args {
+  const void *x, *w, *bias, *gate, *residual;
+  int64_t M, N, K, x_s, w_s, residual_s;
+  int32_t act;
+} gpa_linear_gate_args;
+
+size_t gpa_linear_gate_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate_args* args, void* y, int64_t y_s,
+                    float* z, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradients from y's, dy (any row stride): dx [M, K_out] and dw [N, K_out] in dtype, where
+ * K_out of K features are there (the others pad to a multiple of 8), dbias and dgate [N] in
+ * param_dtype, each NULL where it is not wanted; the residual's is dy.  Sums run in a
+ * fixed order.  N below 2^21.  workspace: gpa_linear_gate_bwd_workspace_bytes of the
+ * same arguments, 16-byte aligned. */
+typedef struct gpa_linear_gate_grads {
+  const void* dy;
+  const float* z;
+  void *dx, *dw, *dbias, *dgate;
+  int64_t dy_s, dx_s, dw_s, K_out;
+} gpa_linear_gate_grads;
+
+size_t gpa_linear_gate_bwd_workspace_bytes(const gpa_linear_gate_args* args, const gpa_linear_gate_grads* grads);
+int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_gate_args* args,
+                        const gpa_linear_gate_grads* grads, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

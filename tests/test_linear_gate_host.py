@@ -1,0 +1,111 @@
+"""Refusals of `linear_gate_residual` and its C entry points; none of this needs a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from merging import _native
+from merging.fused_linear import linear_gate_residual
+
+FAKE = 4096
+INV, UNS, WSP = _native.GPA_E_INVALID, _native.GPA_E_UNSUPPORTED, _native.GPA_E_WORKSPACE
+
+
+def _fields(struct, base, kw):
+    out = struct()
+    for name, x in {**base, **kw}.items():
+        setattr(out, name, x)
+    return out
+
+
+def _args(**kw):
+    return _fields(_native._LinearArgs, dict(x=FAKE, w=FAKE, bias=FAKE, gate=FAKE, residual=FAKE, M=300, N=64, K=128, x_s=128,
+                                             w_s=128, residual_s=64, act=1), kw)
+
+
+COMMON = [
+    (dict(dtype=0), INV), (dict(dtype=3), INV), (dict(dtype=1, pdtype=2), INV), (dict(dtype=2, pdtype=1), INV), (dict(M=-1), INV),
+    (dict(N=-1), INV), (dict(K=-8), INV), (dict(act=-1), INV), (dict(act=5), INV), (dict(K=0), INV), (dict(K=12), INV),
+    (dict(x=None), INV), (dict(w=None), INV), (dict(x=FAKE + 8), INV), (dict(w=FAKE + 2), INV), (dict(x_s=132), INV), (dict(w_s=4), INV),
+    (dict(x_s=1 << 21), UNS), (dict(w_s=1 << 21), UNS), (dict(x_s=-128), UNS), (dict(M=1 << 30), UNS), (dict(N=1 << 30), UNS),
+    (dict(K=1 << 21), UNS),
+]
+
+
+@pytest.mark.parametrize("kw,code", COMMON + [(dict(y=None), INV), (dict(z=FAKE + 4), INV)])
+def test_forward_argument_errors(kw, code):
+    kw = dict(kw)
+    dt, pdt, y, z = kw.pop("dtype", 1), kw.pop("pdtype", None), kw.pop("y", FAKE), kw.pop("z", FAKE)
+    rc = _native.lib().gpa_linear_gate(dt, dt if pdt is None else pdt, ctypes.byref(_args(**kw)), y, 64, z, FAKE, 1 << 30, None)
+    assert rc == code and _native.lib().gpa_last_error()
+
+
+def test_forward_workspace_errors():
+    """A product whose sum is cut needs room for the parts."""
+    L, a = _native.lib(), _args(M=70, N=70, K=8000, x_s=8000, w_s=8000)
+    need = L.gpa_linear_gate_workspace_bytes(70, 70, 8000)
+    assert need >= 2 * 70 * 72 * 4
+    for ws, size in ((None, need), (FAKE, need - 1), (FAKE + 8, need)):
+        assert L.gpa_linear_gate(1, 1, ctypes.byref(a), FAKE, 70, None, ws, size, None) == WSP
+    assert L.gpa_linear_gate_workspace_bytes(64, 70, 8000) == L.gpa_linear_gate_workspace_bytes(0, 70, 8000) == 0
+
+
+@pytest.mark.parametrize("kw,code", COMMON + [
+    (dict(g=dict(dy=None)), INV), (dict(g=dict(z=None)), INV), (dict(act=0, g=dict(z=None)), INV), (dict(gate=None), INV),
+    (dict(g=dict(z=FAKE + 4)), INV), (dict(g=dict(K_out=0)), INV), (dict(g=dict(K_out=129)), INV), (dict(g=dict(K_out=120)), INV),
+    (dict(M=0), INV), (dict(N=0), INV), (dict(N=1 << 21), UNS), (dict(ws=None), WSP), (dict(ws_bytes=64), WSP), (dict(ws=FAKE + 8), WSP),
+])
+def test_backward_argument_errors(kw, code):
+    kw = dict(kw)
+    dt, pdt, ws, ws_bytes = kw.pop("dtype", 1), kw.pop("pdtype", None), kw.pop("ws", FAKE), kw.pop("ws_bytes", 1 << 40)
+    g = _fields(_native._LinearGrads, dict(dy=FAKE, z=FAKE, dx=FAKE, dw=FAKE, dbias=FAKE, dgate=FAKE, dy_s=64, dx_s=128, dw_s=128,
+                                           K_out=128), kw.pop("g", {}))
+    rc = _native.lib().gpa_linear_gate_bwd(dt, dt if pdt is None else pdt, ctypes.byref(_args(**kw)), ctypes.byref(g), ws, ws_bytes, None)
+    assert rc == code and _native.lib().gpa_last_error()
+
+
+def test_nothing_to_do():
+    L = _native.lib()
+    none = _native._LinearGrads()
+    assert L.gpa_linear_gate(1, 1, None, FAKE, 64, None, None, 0, None) == INV
+    assert L.gpa_linear_gate_bwd(1, 1, ctypes.byref(_args()), None, FAKE, 1 << 30, None) == INV
+    assert L.gpa_linear_gate_bwd(1, 1, ctypes.byref(_args()), ctypes.byref(none), None, 0, None) == 0
+    for kw in (dict(M=0), dict(N=0)):
+        assert L.gpa_linear_gate(1, 1, ctypes.byref(_args(**kw)), None, 64, None, None, 0, None) == 0
+
+
+X, W = torch.zeros(5, 16, dtype=torch.bfloat16), torch.zeros(7, 16, dtype=torch.bfloat16)
+B = torch.zeros(7, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(activation="tanh"), "activation"), (dict(weight=W[:, :8]), "go together"), (dict(weight=B), "go together"),
+    (dict(residual=torch.zeros(5, 8)), "residual"), (dict(residual=torch.zeros(7)), "residual"), (dict(), "GPU"),
+])
+def test_python_refusals(kw, match):
+    a = {**dict(weight=W), **kw}
+    with pytest.raises(ValueError, match=match):
+        linear_gate_residual(X, a.pop("weight"), **a)
+    with pytest.raises(NotImplementedError, match="float64"):
+        linear_gate_residual(X.double(), W)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(x=X.float()), "bf16 or fp16"), (dict(w=W.half()), "one type"), (dict(x=X[0]), "one type"), (dict(bias=B[:6]), "bias"),
+    (dict(gate=B[None]), "gate"), (dict(bias=B.half()), "bias and gate"), (dict(bias=B.float(), gate=B), "bias and gate"),
+    (dict(residual=X), "residual"), (dict(residual=torch.zeros(5, 7)), "residual"), (dict(act=5), "activation"),
+])
+def test_op_refusals(kw, match):
+    a = {**dict(x=X, w=W, bias=None, gate=None, residual=None, act=0), **kw}
+    with pytest.raises(ValueError, match=match):
+        _native._linear_check("y", *a.values())
+
+
+@pytest.mark.parametrize("shape,begin", [((5, 16), 0), ((5, 16), 1), ((5, 13), 0), ((5, 0), 0), ((1, 3), 0), ((0, 16), 0)])
+def test_rows_of_8(shape, begin):
+    t = torch.arange(200.0).to(torch.bfloat16)[begin:begin + shape[0] * shape[1]].view(shape)
+    p = _native._rows_of_8(t)
+    assert p.shape[1] % 8 == 0 and p.shape[1] >= 8 and torch.equal(p[:, :shape[1]], t) and not p[:, shape[1]:].any()
+    assert _native._rows_ok(p, 8)
+    wide = torch.zeros(3, 1 << 21, dtype=torch.bfloat16)[:, :16]
+    assert _native._rows_of_8(wide).stride(0) == 16
