@@ -40,6 +40,7 @@ constexpr int kMaxD = 256;
 constexpr int kMaxChunks = 32;
 constexpr int kMaxTokens = 16;            // of a workgroup's tile
 constexpr int kCsFloats = 4096;           // cosines and sines of a tile
+constexpr int64_t kFwdWgs = 2048;
 constexpr int64_t kBwdWgs = 1024;
 
 // Eight pairs of a head: their features begin at o0 and o1 (neighbours: all at
@@ -54,6 +55,7 @@ struct Side {
   const void *w, *b;
   float* part;            // backward: [workgroup][2][D]
   int32_t heads, wgs;     // wgs: the backward's workgroups of this side
+  uint32_t magic;         // 2^32 / heads, rounded up
 };
 
 struct RotArgs {
@@ -63,7 +65,8 @@ struct RotArgs {
   const double* freqs;
   const int32_t* axes;
   int64_t N, tokens, tiles;
-  uint32_t rows_magic;    // 2^32 / heads of both, rounded up (one head: not used)
+  uint32_t rows_magic;    // 2^32 / heads of a row's tensors, rounded up (one head: not used)
+  uint32_t n_magic;       // 2^32 / N, rounded up (N == 1: not used)
   int32_t D, pairs, count, pos_kind, chunks, lanes, per_tile, norm, pf32;
   float eps, inv_d;
   Chunk chunk[kMaxChunks];
@@ -91,36 +94,44 @@ template <> struct Piece<float> { typedef f32x4 type; };
 template <> struct Piece<__bf16> { typedef bf16x8 type; };
 template <> struct Piece<_Float16> { typedef f16x8 type; };
 
-// A chunk's sixteen values as they lie in memory.
-template <typename T, bool VEC, bool INTER>
+// A chunk's sixteen values as they lie in memory, V of them at a time: 8 whole 16-byte
+// pieces, 2 a pair of values, 1 each by itself.
+template <typename T, int V, bool INTER>
 struct Raw {
-  typedef typename Piece<T>::type V;
+  typedef typename Piece<T>::type P16;
   static constexpr int PER = 16 / sizeof(T), HALF = 8 / PER;   // values of a piece; pieces of eight values
-  V v[2 * HALF];
+  P16 v[2 * HALF];
+  __device__ __forceinline__ void put(int i, T x) { v[i / PER][i % PER] = x; }
+  __device__ __forceinline__ T at(int i) const { return v[i / PER][i % PER]; }
   __device__ __forceinline__ void load(const T* row, const Chunk& c) {
-    if constexpr (VEC) {
-      const V* a = reinterpret_cast<const V*>(row + c.o0);
-      const V* b = INTER ? a + HALF : reinterpret_cast<const V*>(row + c.o1);
+    if constexpr (V == 8) {
+      const P16* a = reinterpret_cast<const P16*>(row + c.o0);
+      const P16* b = INTER ? a + HALF : reinterpret_cast<const P16*>(row + c.o1);
 #pragma unroll
-      for (int i = 0; i < HALF; ++i) v[i] = c.n ? a[i] : V{};
+      for (int i = 0; i < HALF; ++i) v[i] = c.n ? a[i] : P16{};
 #pragma unroll
-      for (int i = 0; i < HALF; ++i) v[HALF + i] = c.n ? b[i] : V{};
+      for (int i = 0; i < HALF; ++i) v[HALF + i] = c.n ? b[i] : P16{};
     } else {
+      typedef T Some __attribute__((ext_vector_type(2)));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool in = i < c.n;
-        put(INTER ? 2 * i : i, in ? row[c.o0 + (INTER ? 2 * i : i)] : (T)0.f);
-        put(INTER ? 2 * i + 1 : 8 + i, in ? row[INTER ? c.o0 + 2 * i + 1 : c.o1 + i] : (T)0.f);
+      for (int i = 0; i < 16; i += V) {        // value i of the chunk, in its order in registers
+        const bool in = (INTER ? i / 2 : i & 7) < c.n;
+        const T* from = row + (INTER || i < 8 ? c.o0 + i : c.o1 + i - 8);
+        if constexpr (V == 2) {
+          const Some x = in ? *reinterpret_cast<const Some*>(from) : Some{};
+          put(i, x[0]);
+          put(i + 1, x[1]);
+        } else {
+          put(i, in ? *from : (T)0.f);
+        }
       }
     }
   }
-  __device__ __forceinline__ void put(int i, T x) { v[i / PER][i % PER] = x; }
   __device__ __forceinline__ void get(float (&a)[8], float (&b)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int p = INTER ? 2 * i : i, q = INTER ? 2 * i + 1 : 8 + i;
-      a[i] = (float)v[p / PER][p % PER];
-      b[i] = (float)v[q / PER][q % PER];
+      a[i] = (float)at(INTER ? 2 * i : i);
+      b[i] = (float)at(INTER ? 2 * i + 1 : 8 + i);
     }
   }
   __device__ __forceinline__ void set(const float (&a)[8], const float (&b)[8]) {
@@ -131,21 +142,22 @@ struct Raw {
     }
   }
   __device__ __forceinline__ void store(T* row, const Chunk& c) const {
-    if constexpr (VEC) {
+    if constexpr (V == 8) {
       if (c.n == 0) return;
-      V* a = reinterpret_cast<V*>(row + c.o0);
-      V* b = INTER ? a + HALF : reinterpret_cast<V*>(row + c.o1);
+      P16* a = reinterpret_cast<P16*>(row + c.o0);
+      P16* b = INTER ? a + HALF : reinterpret_cast<P16*>(row + c.o1);
 #pragma unroll
       for (int i = 0; i < HALF; ++i) a[i] = v[i];
 #pragma unroll
       for (int i = 0; i < HALF; ++i) b[i] = v[HALF + i];
     } else {
+      typedef T Some __attribute__((ext_vector_type(2)));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i >= c.n) continue;
-        const int p = INTER ? 2 * i : i, q = INTER ? 2 * i + 1 : 8 + i;
-        row[c.o0 + p] = v[p / PER][p % PER];
-        row[INTER ? c.o0 + q : c.o1 + i] = v[q / PER][q % PER];
+      for (int i = 0; i < 16; i += V) {
+        if ((INTER ? i / 2 : i & 7) >= c.n) continue;
+        T* to = row + (INTER || i < 8 ? c.o0 + i : c.o1 + i - 8);
+        if constexpr (V == 2) *reinterpret_cast<Some*>(to) = Some{at(i), at(i + 1)};
+        else *to = at(i);
       }
     }
   }
@@ -161,40 +173,58 @@ __device__ __forceinline__ void take8(const float* p, float (&x)[8]) {
   }
 }
 
-struct Tile {
-  float cs[kCsFloats];    // [token][chunk][cos 8, sin 8]
-  int64_t at[kMaxTokens][2];   // a token's batch element and number
-};
-
-// The tokens of a tile, and the cosines and sines of their chunks.
-template <bool INTER>
-__device__ __forceinline__ void place_tile(const RotArgs& a, Tile& t, int64_t first, int live) {
-  for (int i = threadIdx.x; i < live; i += kThreads) {
-    const uint32_t tok = (uint32_t)(first + i), b = tok / (uint32_t)a.N;
-    t.at[i][0] = b;
-    t.at[i][1] = tok - b * (uint32_t)a.N;
-  }
-  const int width = a.chunks * 8;
-  for (int i = threadIdx.x; i < live * width; i += kThreads) {
-    const int k = i / width, c = i % width;
-    const Chunk ch = a.chunk[c >> 3];
-    if (ch.p0 < 0 || (c & 7) >= ch.n) continue;
-    const int j = ch.p0 + (c & 7);
-    const uint32_t tok = (uint32_t)(first + k), b = tok / (uint32_t)a.N, n = tok - b * (uint32_t)a.N;
-    int ax = a.axes[j];
-    ax = ax < 0 ? 0 : ax >= a.count ? a.count - 1 : ax;
-    const int64_t at = b * a.pos_sb + n * a.pos_sn + ax;
-    const double p = a.pos_kind == 0 ? (double)static_cast<const int32_t*>(a.pos)[at]
-                     : a.pos_kind == 1 ? (double)static_cast<const int64_t*>(a.pos)[at]
-                                       : (double)static_cast<const float*>(a.pos)[at];
-    const double turns = p * a.freqs[j] * 0.15915494309189533577;
-    const float rest = (float)(turns - __builtin_rint(turns));
-    float s, co;
-    sincospif(2.0f * rest, &s, &co);
-    t.cs[(k * a.chunks + (c >> 3)) * 16 + (c & 7)] = co;
-    t.cs[(k * a.chunks + (c >> 3)) * 16 + 8 + (c & 7)] = s;
-  }
+// Where a tile's tokens lie: its first one's batch element and number.
+struct Place { uint32_t b, n; };
+__device__ __forceinline__ Place place_of(const RotArgs& a, uint32_t first) {
+  const uint32_t b = first / (uint32_t)a.N;
+  return {b, first - b * (uint32_t)a.N};
 }
+// Token k (below kMaxTokens) of the tile.  (Sequences of kMaxTokens or more: it
+// lies in the first one's or the next.)
+__device__ __forceinline__ Place token_at(const RotArgs& a, Place p, uint32_t k) {
+  const uint32_t n = p.n + k, N = (uint32_t)a.N;
+  const uint32_t d = N >= kMaxTokens ? (n >= N ? 1 : 0) : N == 1 ? n : __umulhi(n, a.n_magic);
+  return {p.b + d, n - d * N};
+}
+
+// A thread's pair of features, whose angles it forms for every tile.
+struct Turner {
+  int pair, slot, slots, to;   // pair: -1 none; the tokens slot, slot + slots, ...
+  double speed;                // turns a unit of position
+  int64_t axis;
+  __device__ __forceinline__ explicit Turner(const RotArgs& a) {
+    const int width = a.lanes * 8, c = threadIdx.x % width;
+    slot = threadIdx.x / width;
+    slots = kThreads / width;
+    pair = -1;
+    to = 0;
+    speed = 0.0;
+    axis = 0;
+    if (c >= a.chunks * 8) return;
+    const Chunk ch = a.chunk[c >> 3];
+    if (ch.p0 < 0 || (c & 7) >= ch.n) return;
+    pair = ch.p0 + (c & 7);
+    to = (c >> 3) * 16 + (c & 7);
+    speed = a.freqs[pair] * 0.15915494309189533577;
+    const int ax = a.axes[pair];
+    axis = ax < 0 ? 0 : ax >= a.count ? a.count - 1 : ax;
+  }
+  __device__ __forceinline__ void turn(const RotArgs& a, Place first, int live, float* cs) const {
+    if (pair < 0) return;
+    for (int k = slot; k < live; k += slots) {
+      const Place t = token_at(a, first, k);
+      const int64_t at = t.b * a.pos_sb + t.n * a.pos_sn + axis;
+      const double p = a.pos_kind == 0 ? (double)static_cast<const int32_t*>(a.pos)[at]
+                       : a.pos_kind == 1 ? (double)static_cast<const int64_t*>(a.pos)[at]
+                                         : (double)static_cast<const float*>(a.pos)[at];
+      const double turns = p * speed;
+      float s, c;
+      sincospif(2.0f * (float)(turns - __builtin_rint(turns)), &s, &c);
+      cs[k * a.chunks * 16 + to] = c;
+      cs[k * a.chunks * 16 + to + 8] = s;
+    }
+  }
+};
 
 // A parameter in a lane's order: its sixteen values, `none` where there are none.
 template <typename T, bool INTER>
@@ -211,7 +241,8 @@ __device__ __forceinline__ void take_param(const RotArgs& a, const void* p, cons
 }
 
 // Both moments of a row; x, y centred under LayerNorm.  Returns 1 / sigma.
-__device__ __forceinline__ float moments(const RotArgs& a, const Chunk& c, bool vec, float (&x)[8], float (&y)[8]) {
+template <bool WHOLE>
+__device__ __forceinline__ float moments(const RotArgs& a, const Chunk& c, float (&x)[8], float (&y)[8]) {
   if (a.norm == kLayer) {
     float s = 0.f;
 #pragma unroll
@@ -219,7 +250,7 @@ __device__ __forceinline__ float moments(const RotArgs& a, const Chunk& c, bool 
     const float mean = row_sum(s, a.lanes) * a.inv_d;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {              // values that are not there stay 0
-      const bool in = vec ? c.n != 0 : i < c.n;
+      const bool in = WHOLE ? c.n != 0 : i < c.n;
       x[i] = in ? x[i] - mean : 0.f;
       y[i] = in ? y[i] - mean : 0.f;
     }
@@ -242,13 +273,69 @@ __device__ __forceinline__ Lane lane_of(const RotArgs& a) {
   return l;
 }
 
-template <typename T, bool VEC, bool INTER>
+// Rows of a workgroup: those of its tiles, `all` heads of each token, U * l.rows at a time; the next
+// ones' loads are issued before this one's arithmetic, a tile's first before its angles.
+struct Walk {
+  int64_t tile;
+  int r0, rows;           // the next rows' first, of `rows` of the tile
+  uint32_t first;         // the tile's first token
+  int live;
+  __device__ __forceinline__ void open(const RotArgs& a, int64_t at, int all) {
+    tile = at;
+    r0 = 0;
+    first = (uint32_t)(at * a.per_tile);
+    live = at < a.tiles ? (int)(a.tokens - first < a.per_tile ? a.tokens - first : a.per_tile) : 0;
+    rows = live * all;
+  }
+  // Whether the next rows are another tile's.
+  __device__ __forceinline__ bool on(const RotArgs& a, int step, int64_t stride, int all) {
+    r0 += step;
+    if (r0 < rows) return false;
+    open(a, tile + stride, all);
+    return true;
+  }
+};
+
+template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(kThreads) void head_rotary_kernel(RotArgs a) {
-  constexpr int U = sizeof(T) == 4 ? 2 : 4;    // rows a lane has in flight
-  __shared__ __attribute__((aligned(16))) Tile t;
+  constexpr int U = sizeof(T) == 4 ? 1 : 2;    // rows a lane has in flight, twice
+  __shared__ __attribute__((aligned(16))) float cs[kCsFloats];    // [token][chunk][cos 8, sin 8]
   __shared__ __attribute__((aligned(16))) float par[2][2][kMaxChunks * 16];
   const Lane l = lane_of(a);
-  const int at = threadIdx.x % a.lanes, both = a.side[0].heads + a.side[1].heads;
+  const int at = threadIdx.x % a.lanes, both = a.side[0].heads + a.side[1].heads, cat = at < a.chunks ? at : 0;
+  struct Some {
+    Raw<T, V, INTER> raw[U];
+    T* out[U];
+    int k[U];
+    bool which[U], fine[U];
+  };
+  // (Selected, not indexed: a lane's own index would be a load from the arguments.)
+  auto fetch = [&](const Walk& w, Some& m) __attribute__((always_inline)) {
+    const Place first = place_of(a, w.first);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = w.r0 + l.row + u * l.rows;
+      m.fine[u] = r < w.rows;
+      const int rc = m.fine[u] ? r : 0;
+      const int k = both == 1 ? rc : (int)__umulhi((uint32_t)rc, a.rows_magic), hh = rc - k * both;
+      const bool which = hh >= a.side[0].heads;
+      const int h = which ? hh - a.side[0].heads : hh;
+      const Side &s0 = a.side[0], &s1 = a.side[1];
+      const Place t = token_at(a, first, k);
+      m.k[u] = k;
+      m.which[u] = which;
+      m.out[u] = static_cast<T*>(which ? s1.out : s0.out) + t.b * (which ? s1.o_sb : s0.o_sb) +
+                 h * (which ? s1.o_sh : s0.o_sh) + t.n * (which ? s1.o_sn : s0.o_sn);
+      Chunk c = l.c;
+      if (!m.fine[u]) c.n = 0;
+      m.raw[u].load(static_cast<const T*>(which ? s1.x : s0.x) + t.b * (which ? s1.x_sb : s0.x_sb) +
+                        h * (which ? s1.x_sh : s0.x_sh) + t.n * (which ? s1.x_sn : s0.x_sn), c);
+    }
+  };
+  Walk w;
+  w.open(a, blockIdx.x, both);
+  Some now;
+  fetch(w, now);
   if (a.norm && l.row < 2) {                   // a row of lanes for each side (a wave has two at least)
     const Side& s = a.side[l.row];
     float x[8], y[8];
@@ -261,169 +348,156 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(RotArgs a) {
       }
     }
   }
-  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    const int64_t first = tile * a.per_tile;
-    const int live = (int)(a.tokens - first < a.per_tile ? a.tokens - first : a.per_tile);
-    const int rows = live * both;
-    __syncthreads();
-    place_tile<INTER>(a, t, first, live);
-    __syncthreads();
-    for (int r0 = l.row; r0 < rows + l.row; r0 += U * l.rows) {
-      Raw<T, VEC, INTER> raw[U];
-      T* out[U];
-      const float *cs[U], *w[U];
-      bool biased[U], fine[U];
+  const Turner turner(a);
+  bool fresh = true;
+  while (w.live > 0) {
+    if (fresh) {
+      __syncthreads();                         // the tile before is done with its angles
+      turner.turn(a, place_of(a, w.first), w.live, cs);
+      __syncthreads();
+    }
+    Some cur = now;
+    fresh = w.on(a, U * l.rows, gridDim.x, both);
+    if (w.live > 0) fetch(w, now);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * l.rows;
-        fine[u] = r < rows;
-        const int rc = fine[u] ? r : rows - 1;
-        const int k = both == 1 ? rc : (int)__umulhi((uint32_t)rc, a.rows_magic), hh = rc - k * both;
-        const bool which = hh >= a.side[0].heads;
-        const int h = which ? hh - a.side[0].heads : hh;
-        // Selected, not indexed: a lane's own index would be a load from the arguments.
-        const Side &s0 = a.side[0], &s1 = a.side[1];
-        const int64_t b = t.at[k][0], n = t.at[k][1];
-        raw[u].load(static_cast<const T*>(which ? s1.x : s0.x) + b * (which ? s1.x_sb : s0.x_sb) +
-                        h * (which ? s1.x_sh : s0.x_sh) + n * (which ? s1.x_sn : s0.x_sn), l.c);
-        out[u] = static_cast<T*>(which ? s1.out : s0.out) + b * (which ? s1.o_sb : s0.o_sb) +
-                 h * (which ? s1.o_sh : s0.o_sh) + n * (which ? s1.o_sn : s0.o_sn);
-        cs[u] = t.cs + (k * a.chunks + (at < a.chunks ? at : 0)) * 16;
-        w[u] = par[which][0] + at * 16;
-        biased[u] = which ? s1.b != nullptr : s0.b != nullptr;
-      }
+    for (int u = 0; u < U; ++u) {
+      float x[8], y[8];
+      cur.raw[u].get(x, y);
+      if (a.norm) {
+        const float inv = moments<V == 8>(a, l.c, x, y);
+        const float* pw = par[cur.which[u]][0] + at * 16;
+        float p[8], q[8];
+        take8(pw, p);
+        take8(pw + 8, q);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float x[8], y[8];
-        raw[u].get(x, y);
-        if (a.norm) {
-          const float inv = moments(a, l.c, VEC, x, y);
-          float p[8], q[8];
-          take8(w[u], p);
-          take8(w[u] + 8, q);
+        for (int i = 0; i < 8; ++i) {
+          x[i] = x[i] * inv * p[i];
+          y[i] = y[i] * inv * q[i];
+        }
+        if (a.side[0].b || a.side[1].b) {      // (of one alone: the other adds zeros)
+          take8(pw + kMaxChunks * 16, p);
+          take8(pw + kMaxChunks * 16 + 8, q);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            x[i] = x[i] * inv * p[i];
-            y[i] = y[i] * inv * q[i];
-          }
-          if (biased[u]) {
-            take8(w[u] + kMaxChunks * 16, p);
-            take8(w[u] + kMaxChunks * 16 + 8, q);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              x[i] += p[i];
-              y[i] += q[i];
-            }
+            x[i] += p[i];
+            y[i] += q[i];
           }
         }
-        if (l.c.p0 >= 0) {
-          float c[8], s[8];
-          take8(cs[u], c);
-          take8(cs[u] + 8, s);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float v = x[i];
-            x[i] = __builtin_fmaf(v, c[i], -(y[i] * s[i]));
-            y[i] = __builtin_fmaf(y[i], c[i], v * s[i]);
-          }
-        }
-        if (!fine[u]) continue;
-        raw[u].set(x, y);
-        raw[u].store(out[u], l.c);
       }
+      if (l.c.p0 >= 0) {
+        float c[8], s[8];
+        take8(cs + (cur.k[u] * a.chunks + cat) * 16, c);
+        take8(cs + (cur.k[u] * a.chunks + cat) * 16 + 8, s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float v = x[i];
+          x[i] = __builtin_fmaf(v, c[i], -(y[i] * s[i]));
+          y[i] = __builtin_fmaf(y[i], c[i], v * s[i]);
+        }
+      }
+      if (!cur.fine[u]) continue;
+      cur.raw[u].set(x, y);
+      cur.raw[u].store(cur.out[u], l.c);
     }
   }
 }
 
-template <typename T, bool VEC, bool INTER>
+template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(kThreads) void head_rotary_bwd_kernel(RotArgs a) {
-  constexpr int U = sizeof(T) == 4 ? 1 : 2;
-  __shared__ __attribute__((aligned(16))) Tile t;
+  __shared__ __attribute__((aligned(16))) float cs[kCsFloats];
   const Lane l = lane_of(a);
-  const int at = threadIdx.x % a.lanes;
+  const int at = threadIdx.x % a.lanes, cat = at < a.chunks ? at : 0;
   const int which = (int)blockIdx.x >= a.side[0].wgs;
   const Side& s = a.side[which];
   const int wg = which ? (int)blockIdx.x - a.side[0].wgs : (int)blockIdx.x;
+  struct Some {
+    Raw<T, V, INTER> x, dy;
+    T* out;
+    int k;
+    bool fine;
+  };
+  auto fetch = [&](const Walk& w, Some& m) __attribute__((always_inline)) {
+    const Place first = place_of(a, w.first);
+    const int r = w.r0 + l.row;
+    m.fine = r < w.rows;
+    const int rc = m.fine ? r : 0;
+    m.k = s.heads == 1 ? rc : (int)__umulhi((uint32_t)rc, s.magic);
+    const int h = rc - m.k * s.heads;
+    const Place t = token_at(a, first, m.k);
+    Chunk c = l.c;
+    if (!m.fine) c.n = 0;
+    m.dy.load(static_cast<const T*>(s.dy) + t.b * s.y_sb + h * s.y_sh + t.n * s.y_sn, c);
+    if (a.norm) m.x.load(static_cast<const T*>(s.x) + t.b * s.x_sb + h * s.x_sh + t.n * s.x_sn, c);
+    m.out = static_cast<T*>(s.out) + t.b * s.o_sb + h * s.o_sh + t.n * s.o_sn;
+  };
+  Walk w;
+  w.open(a, wg, s.heads);
+  Some now;
+  fetch(w, now);
+  const Turner turner(a);
   float wa[8], wb[8], dwa[8], dwb[8], dba[8], dbb[8];
   take_param<T, INTER>(a, s.w, l.c, 1.f, wa, wb);
 #pragma unroll
   for (int i = 0; i < 8; ++i) dwa[i] = dwb[i] = dba[i] = dbb[i] = 0.f;
-
-  for (int64_t tile = wg; tile < a.tiles; tile += s.wgs) {
-    const int64_t first = tile * a.per_tile;
-    const int live = (int)(a.tokens - first < a.per_tile ? a.tokens - first : a.per_tile);
-    const int rows = live * s.heads;
-    __syncthreads();
-    place_tile<INTER>(a, t, first, live);
-    __syncthreads();
-    for (int r0 = l.row; r0 < rows + l.row; r0 += U * l.rows) {
-      Raw<T, VEC, INTER> rx[U], ry[U];
-      T* out[U];
-      const float* cs[U];
-      bool fine[U];
+  bool fresh = true;
+  while (w.live > 0) {
+    if (fresh) {
+      __syncthreads();
+      turner.turn(a, place_of(a, w.first), w.live, cs);
+      __syncthreads();
+    }
+    Some cur = now;
+    fresh = w.on(a, l.rows, s.wgs, s.heads);
+    if (w.live > 0) fetch(w, now);
+    float ga[8], gb[8];
+    cur.dy.get(ga, gb);
+    if (l.c.p0 >= 0) {                         // turned back
+      float c[8], sn[8];
+      take8(cs + (cur.k * a.chunks + cat) * 16, c);
+      take8(cs + (cur.k * a.chunks + cat) * 16 + 8, sn);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * l.rows;
-        fine[u] = r < rows;
-        const int rc = fine[u] ? r : rows - 1, k = rc / s.heads, h = rc - k * s.heads;
-        ry[u].load(static_cast<const T*>(s.dy) + t.at[k][0] * s.y_sb + h * s.y_sh + t.at[k][1] * s.y_sn, l.c);
-        if (a.norm) rx[u].load(static_cast<const T*>(s.x) + t.at[k][0] * s.x_sb + h * s.x_sh + t.at[k][1] * s.x_sn, l.c);
-        out[u] = static_cast<T*>(s.out) + t.at[k][0] * s.o_sb + h * s.o_sh + t.at[k][1] * s.o_sn;
-        cs[u] = t.cs + (k * a.chunks + (at < a.chunks ? at : 0)) * 16;
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float ga[8], gb[8];
-        ry[u].get(ga, gb);
-        if (l.c.p0 >= 0) {                     // turned back
-          float c[8], sn[8];
-          take8(cs[u], c);
-          take8(cs[u] + 8, sn);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float v = ga[i];
-            ga[i] = __builtin_fmaf(v, c[i], gb[i] * sn[i]);
-            gb[i] = __builtin_fmaf(gb[i], c[i], -(v * sn[i]));
-          }
-        }
-        if (a.norm) {
-          float x[8], y[8];
-          rx[u].get(x, y);
-          const float inv = moments(a, l.c, VEC, x, y);
-          float s1 = 0.f, s0 = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            x[i] *= inv;
-            y[i] *= inv;
-            if (fine[u]) {
-              dwa[i] = __builtin_fmaf(ga[i], x[i], dwa[i]);
-              dwb[i] = __builtin_fmaf(gb[i], y[i], dwb[i]);
-              dba[i] += ga[i];
-              dbb[i] += gb[i];
-            }
-            ga[i] *= wa[i];
-            gb[i] *= wb[i];
-            s1 = __builtin_fmaf(ga[i], x[i], __builtin_fmaf(gb[i], y[i], s1));
-            s0 += ga[i] + gb[i];
-          }
-          s1 = row_sum(s1, a.lanes) * a.inv_d;
-          s0 = a.norm == kLayer ? row_sum(s0, a.lanes) * a.inv_d : 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            ga[i] = inv * (ga[i] - s0 - x[i] * s1);
-            gb[i] = inv * (gb[i] - s0 - y[i] * s1);
-          }
-        }
-        if (!fine[u]) continue;
-        ry[u].set(ga, gb);
-        ry[u].store(out[u], l.c);
+      for (int i = 0; i < 8; ++i) {
+        const float v = ga[i];
+        ga[i] = __builtin_fmaf(v, c[i], gb[i] * sn[i]);
+        gb[i] = __builtin_fmaf(gb[i], c[i], -(v * sn[i]));
       }
     }
+    if (a.norm) {
+      float x[8], y[8];
+      cur.x.get(x, y);
+      const float inv = moments<V == 8>(a, l.c, x, y);
+      float s1 = 0.f, s0 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] *= inv;
+        y[i] *= inv;
+        if (cur.fine) {
+          dwa[i] = __builtin_fmaf(ga[i], x[i], dwa[i]);
+          dwb[i] = __builtin_fmaf(gb[i], y[i], dwb[i]);
+          dba[i] += ga[i];
+          dbb[i] += gb[i];
+        }
+        ga[i] *= wa[i];
+        gb[i] *= wb[i];
+        s1 = __builtin_fmaf(ga[i], x[i], __builtin_fmaf(gb[i], y[i], s1));
+        s0 += ga[i] + gb[i];
+      }
+      s1 = row_sum(s1, a.lanes) * a.inv_d;
+      s0 = a.norm == kLayer ? row_sum(s0, a.lanes) * a.inv_d : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ga[i] = inv * (ga[i] - s0 - x[i] * s1);
+        gb[i] = inv * (gb[i] - s0 - y[i] * s1);
+      }
+    }
+    if (!cur.fine) continue;
+    cur.dy.set(ga, gb);
+    cur.dy.store(cur.out, l.c);
   }
   if (!s.part) return;
 
   // The rows' sums: over a wave's rows, then over the four waves in LDS.
-  float* red = t.cs;                           // [wave][lane of a row][4][8], at most 4 * 32 * 32 floats
+  float* red = cs;                             // [wave][lane of a row][4][8], at most 4 * 32 * 32 floats
   float* sums[4] = {dwa, dwb, dba, dbb};
 #pragma unroll
   for (int k = 0; k < 4; ++k)
@@ -572,8 +646,10 @@ int check(const char* fn, int dtype, int pdtype, const gpa_head_rotary_args* a) 
 
 struct Rows { const void* p; int64_t heads, sb, sh, sn; };
 
-// Fills everything but the outputs; returns whether chunks are whole 16-byte pieces.
-bool fill(const gpa_head_rotary_args* a, int dtype, int pdtype, std::initializer_list<Rows> all, RotArgs& r) {
+uint32_t magic_of(int64_t n) { return n < 2 ? 0 : (uint32_t)((((uint64_t)1 << 32) + n - 1) / n); }
+
+// Fills everything but the outputs; returns how many values can be loaded and stored together (8, 2, 1).
+int fill(const gpa_head_rotary_args* a, int dtype, int pdtype, std::initializer_list<Rows> all, RotArgs& r) {
   const int64_t esize = dtype == GPA_DTYPE_F32 ? 4 : 2, per16 = 16 / esize;
   auto st = [](int64_t n, int64_t s) { return n > 1 ? s : 0; };
   Side &q = r.side[0], &k = r.side[1];
@@ -589,49 +665,49 @@ bool fill(const gpa_head_rotary_args* a, int dtype, int pdtype, std::initializer
   r.D = (int32_t)a->D; r.pairs = (int32_t)a->pairs; r.count = a->sections_count;
   r.norm = a->norm; r.pf32 = pdtype == GPA_DTYPE_F32;
   r.eps = a->eps; r.inv_d = 1.0f / (float)a->D;
-  bool vec = true;
+  r.n_magic = magic_of(a->N);
+  q.magic = magic_of(a->H); k.magic = magic_of(a->Hk);
+  bool vec = true, two = true;
+  const bool next = a->pairing == GPA_PAIRS_NEIGHBOURS;
   for (int i = 0; i < r.chunks; ++i) {
     const Chunk& c = r.chunk[i];
-    vec = vec && c.n == 8 && c.o0 % 8 == 0 && (a->pairing == GPA_PAIRS_NEIGHBOURS || c.o1 % 8 == 0);
+    vec = vec && c.n == 8 && c.o0 % 8 == 0 && (next || c.o1 % 8 == 0);
+    two = two && (next || (c.n % 2 == 0 && c.o0 % 2 == 0 && c.o1 % 2 == 0));
   }
-  for (const Rows& x : all)
-    if (x.p && x.heads > 0)
-      vec = vec && (uintptr_t)x.p % 16 == 0 && st(a->B, x.sb) % per16 == 0 &&
-            st(x.heads, x.sh) % per16 == 0 && st(a->N, x.sn) % per16 == 0;
-  return vec;
+  for (const Rows& x : all) {
+    if (!x.p || x.heads == 0) continue;
+    const int64_t some = st(a->B, x.sb) | st(x.heads, x.sh) | st(a->N, x.sn);   // divisible by a power of two where all are
+    vec = vec && (uintptr_t)x.p % 16 == 0 && some % per16 == 0;
+    two = two && (uintptr_t)x.p % (2 * esize) == 0 && some % 2 == 0;
+  }
+  return vec ? 8 : two ? 2 : 1;
 }
 
-// Tokens of a workgroup's tile: four rounds of its rows, unless that leaves CUs
-// without a workgroup.  (Cosines and sines are formed for a whole tile at once.)
-int tile_tokens(const RotArgs& r, int64_t heads, int64_t rounds) {
-  const int64_t rows = kThreads / r.lanes;
-  int64_t n = std::min<int64_t>({rounds * rows / std::max<int64_t>(heads, 1), r.tokens / 1024, kMaxTokens,
-                                 kCsFloats / (16 * std::max(r.chunks, 1))});
+// Tokens of a workgroup's tile: what its angles' LDS holds, unless that leaves CUs idle.
+int tile_tokens(const RotArgs& r, int64_t wgs) {
+  const int64_t n = std::min<int64_t>({r.tokens / wgs, kMaxTokens, kCsFloats / (16 * std::max(r.chunks, 1))});
   return (int)std::max<int64_t>(n, 1);
 }
 
-template <typename T, bool VEC>
-hipError_t forward(const RotArgs& r, bool inter, hipStream_t s) {
-  const dim3 grid((unsigned)std::min<int64_t>(r.tiles, 1 << 22)), block(kThreads);
-  if (inter) hipLaunchKernelGGL((head_rotary_kernel<T, VEC, true>), grid, block, 0, s, r);
-  else hipLaunchKernelGGL((head_rotary_kernel<T, VEC, false>), grid, block, 0, s, r);
-  return hipGetLastError();
-}
-template <typename T, bool VEC>
-hipError_t backward(const RotArgs& r, bool inter, hipStream_t s) {
-  const dim3 grid((unsigned)(r.side[0].wgs + r.side[1].wgs)), block(kThreads);
-  if (inter) hipLaunchKernelGGL((head_rotary_bwd_kernel<T, VEC, true>), grid, block, 0, s, r);
-  else hipLaunchKernelGGL((head_rotary_bwd_kernel<T, VEC, false>), grid, block, 0, s, r);
+template <typename T, int V, bool BWD>
+hipError_t go(const RotArgs& r, bool inter, hipStream_t s) {
+  const dim3 grid((unsigned)(BWD ? r.side[0].wgs + r.side[1].wgs : std::min<int64_t>(r.tiles, 4 * kFwdWgs))), block(kThreads);
+  if constexpr (BWD) {
+    if (inter) hipLaunchKernelGGL((head_rotary_bwd_kernel<T, V, true>), grid, block, 0, s, r);
+    else hipLaunchKernelGGL((head_rotary_bwd_kernel<T, V, false>), grid, block, 0, s, r);
+  } else {
+    if (inter) hipLaunchKernelGGL((head_rotary_kernel<T, V, true>), grid, block, 0, s, r);
+    else hipLaunchKernelGGL((head_rotary_kernel<T, V, false>), grid, block, 0, s, r);
+  }
   return hipGetLastError();
 }
 template <bool BWD>
-hipError_t launch(const RotArgs& r, int dtype, bool vec, bool inter, hipStream_t s) {
-  auto go = [&](auto type) {
+hipError_t launch(const RotArgs& r, int dtype, int some, bool inter, hipStream_t s) {
+  auto of = [&](auto type) {
     typedef decltype(type) T;
-    if constexpr (BWD) return vec ? backward<T, true>(r, inter, s) : backward<T, false>(r, inter, s);
-    else return vec ? forward<T, true>(r, inter, s) : forward<T, false>(r, inter, s);
+    return some == 8 ? go<T, 8, BWD>(r, inter, s) : some == 2 ? go<T, 2, BWD>(r, inter, s) : go<T, 1, BWD>(r, inter, s);
   };
-  return dtype == GPA_DTYPE_F32 ? go(0.f) : dtype == GPA_DTYPE_BF16 ? go((__bf16)0.f) : go((_Float16)0.f);
+  return dtype == GPA_DTYPE_F32 ? of(0.f) : dtype == GPA_DTYPE_BF16 ? of((__bf16)0.f) : of((_Float16)0.f);
 }
 
 int refuse_launch(const char* fn, hipError_t e) {
@@ -672,16 +748,16 @@ extern "C" int gpa_head_rotary(int dtype, int param_dtype, const gpa_head_rotary
     gpa_set_error("%s: too many sections for this head dim", fn);
     return GPA_E_UNSUPPORTED;
   }
-  const bool vec = fill(a, dtype, param_dtype,
+  const int some = fill(a, dtype, param_dtype,
                         {{a->q, a->H, a->q_sb, a->q_sh, a->q_sn}, {a->k, a->Hk, a->k_sb, a->k_sh, a->k_sn},
                          {q_out, a->H, qo_sb, qo_sh, qo_sn}, {k_out, a->Hk, ko_sb, ko_sh, ko_sn}}, r);
   r.side[0].out = q_out; r.side[0].o_sb = qo_sb; r.side[0].o_sh = qo_sh; r.side[0].o_sn = qo_sn;
   r.side[1].out = k_out; r.side[1].o_sb = ko_sb; r.side[1].o_sh = ko_sh; r.side[1].o_sn = ko_sn;
   const int64_t both = a->H + a->Hk;
-  r.per_tile = tile_tokens(r, both, dtype == GPA_DTYPE_F32 ? 2 : 4);
+  r.per_tile = tile_tokens(r, kFwdWgs);
   r.tiles = (r.tokens + r.per_tile - 1) / r.per_tile;
-  r.rows_magic = both == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + both - 1) / both);
-  return refuse_launch(fn, launch<false>(r, dtype, vec, a->pairing == GPA_PAIRS_NEIGHBOURS, (hipStream_t)stream));
+  r.rows_magic = magic_of(both);
+  return refuse_launch(fn, launch<false>(r, dtype, some, a->pairing == GPA_PAIRS_NEIGHBOURS, (hipStream_t)stream));
 }
 
 extern "C" size_t gpa_head_rotary_bwd_workspace_bytes(int64_t B, int64_t N, int64_t H, int64_t Hk,
@@ -727,7 +803,7 @@ extern "C" int gpa_head_rotary_bwd(int dtype, int param_dtype, const gpa_head_ro
     return GPA_E_UNSUPPORTED;
   }
   const int64_t H = hq ? a->H : 0, Hk = hk ? a->Hk : 0;
-  const bool vec = fill(a, dtype, param_dtype,
+  const int some = fill(a, dtype, param_dtype,
                         {{a->norm ? a->q : nullptr, H, a->q_sb, a->q_sh, a->q_sn},
                          {a->norm ? a->k : nullptr, Hk, a->k_sb, a->k_sh, a->k_sn},
                          {g->d_q_out, H, g->dqo_sb, g->dqo_sh, g->dqo_sn}, {g->d_k_out, Hk, g->dko_sb, g->dko_sh, g->dko_sn},
@@ -744,10 +820,10 @@ extern "C" int gpa_head_rotary_bwd(int dtype, int param_dtype, const gpa_head_ro
     q.part = g->dq_w || g->dq_b ? (float*)workspace : nullptr;
     k.part = g->dk_w || g->dk_b ? (float*)workspace + w.q * 2 * a->D : nullptr;
   }
-  r.per_tile = tile_tokens(r, std::max(H, Hk), 2);
+  r.per_tile = tile_tokens(r, std::max(w.q, w.k));
   r.tiles = (r.tokens + r.per_tile - 1) / r.per_tile;
   const hipStream_t s = (hipStream_t)stream;
-  hipError_t e = launch<true>(r, dtype, vec, a->pairing == GPA_PAIRS_NEIGHBOURS, s);
+  hipError_t e = launch<true>(r, dtype, some, a->pairing == GPA_PAIRS_NEIGHBOURS, s);
   if (e == hipSuccess && sums) {
     SumArgs c{};
     c.part[0] = q.part; c.part[1] = k.part;
