@@ -13,18 +13,18 @@ enum Act { kActNone = 0, kActGelu = 1, kActGeluTanh = 2, kActSilu = 3, kActRelu 
 // How a product of I x J over K is cut: tiles (0: 256 x 256, 1: 128 x 256, 2: 128 x 128, 3: 64 x 64
 // of i and j), parts along k, and the fp32 partials' bytes.
 struct GemmPlan { int tile; int64_t ti, tj, splits; size_t bytes; };
-GemmPlan gemm_plan(int64_t I, int64_t J, int64_t K);
+GemmPlan gemm_plan(int64_t I, int64_t J, int64_t K, bool turned);
 
 // What becomes of a sum.
 struct Finish {
   void* out;              // 16-bit, rows out_s apart
   const void *bias, *gate;
   const void* residual;
-  float* z;               // the pre-activation, rows of J (nullable)
+  void* z;                // the sums before the activation, rows of J (nullable)
   const float* unscale;   // a factor (nullable)
   float* part;            // parts along k: [part][I][J rounded up to 8]
   int64_t out_s, res_s, I, J;
-  int32_t act, pf32;      // pf32: bias and gate are fp32
+  int32_t act, pf32, z16; // pf32: bias and gate are fp32; z16: z is fp16, else fp32
   int32_t wide;           // whole 16-byte groups of 8 can be loaded and stored
 };
 
@@ -49,16 +49,22 @@ __device__ __forceinline__ float logistic(float z) {
 }
 constexpr float kTanhC = 0.7978845608f, kTanhD = 0.044715f;   // gelu's tanh form: z logistic(2 c (z + d z^3))
 
-// act(z).  (An infinite z: -inf times the 0 of its distribution is 0, as the limit is.)
+// act(z).  (z is kept finite from below for the product: -inf times the 0 of its distribution
+// is 0, as the limit is.  A NaN comes out by the other factor.)
 template <int ACT>
 __device__ __forceinline__ float act_of(float z) {
   if constexpr (ACT == kActNone) return z;
   if constexpr (ACT == kActRelu) return z < 0.f ? 0.f : z;     // NaN stays
   float s, d;
-  if constexpr (ACT == kActGelu) s = normal_cdf(z, d);
-  else if constexpr (ACT == kActSilu) s = logistic(z);
-  else s = logistic(2.0f * kTanhC * z * __builtin_fmaf(kTanhD * z, z, 1.0f));
-  return s == 0.f ? 0.f : z * s;
+  if constexpr (ACT == kActGelu) {
+    s = normal_cdf(z, d);
+  } else {
+    constexpr float l2e = 1.44269504f;
+    float t = -l2e * z;
+    if constexpr (ACT == kActGeluTanh) t = z * __builtin_fmaf(z * z, -2.0f * l2e * kTanhC * kTanhD, -2.0f * l2e * kTanhC);
+    s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
+  }
+  return fmaxf(z, -3.0e38f) * s;
 }
 // act(z) and its derivative.
 template <int ACT>
@@ -113,6 +119,46 @@ __device__ __forceinline__ void param8(const void* p, int pf32, int wide, int64_
   }
 }
 
+// n sums (8: whole groups) kept at `at` of z for the backward.  In fp16 (where the gradients are
+// bf16's and no gate's sum is formed from it) a slope formed from z is off by 2^-11 of z times a
+// second derivative below one, an eighth of what rounding dz costs; beyond 65,504 it is
+// kept as infinite, where every slope is 0 or 1; a ReLU's sign is kept where z would round to 0.
+template <int ACT>
+__device__ __forceinline__ void keep8(const Finish& f, int64_t at, int n, const float (&v)[8]) {
+  if (!f.z16) {
+    float* z = static_cast<float*>(f.z) + at;
+    if (n == 8 && f.wide) {
+      reinterpret_cast<f32x4*>(z)[0] = f32x4{v[0], v[1], v[2], v[3]};
+      reinterpret_cast<f32x4*>(z)[1] = f32x4{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n) z[e] = v[e];
+    }
+    return;
+  }
+  __bf16* z = static_cast<__bf16*>(f.z) + at;  // fp16 by its bits
+  bf16x8 y;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    float a = v[e], b = v[e + 1];
+    if (ACT == kActRelu) {
+      a = a > 0.f ? fmaxf(a, 6e-8f) : a;
+      b = b > 0.f ? fmaxf(b, 6e-8f) : b;
+    }
+    const bf16x2 w = pack2<true>(a, b);
+    y[e] = w[0];
+    y[e + 1] = w[1];
+  }
+  if (n == 8 && f.wide) {
+    *reinterpret_cast<bf16x8*>(z) = y;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) z[e] = y[e];
+  }
+}
+
 template <int ACT>
 __device__ __forceinline__ void act8(float (&v)[8]) {
 #pragma unroll
@@ -142,15 +188,8 @@ __device__ __forceinline__ void finish8(const Finish& f, int64_t i, int64_t j, i
     for (int e = 0; e < 8; ++e) v[e] += x[e];
   }
   if (f.z) {
-    float* z = f.z + i * f.J + j;
-    if (f.wide) {
-      reinterpret_cast<f32x4*>(z)[0] = f32x4{v[0], v[1], v[2], v[3]};
-      reinterpret_cast<f32x4*>(z)[1] = f32x4{v[4], v[5], v[6], v[7]};
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < n) z[e] = v[e];
-    }
+    if (f.act == kActRelu) keep8<kActRelu>(f, i * f.J + j, n, v);
+    else keep8<kActNone>(f, i * f.J + j, n, v);
   }
   switch (f.act) {
     case kActGelu: act8<kActGelu>(v); break;

@@ -1,7 +1,7 @@
 // A projection with what follows it: y = residual + gate act(x w^T + bias), 16-bit
 // operands, fp32 from the products to the one rounding of y.  act: none, GELU (erf and
-// tanh forms), SiLU, ReLU.  For gradients the sum before the activation is kept in fp32: in
-// 16 bits its rounding alone would take what the gradient's own rounding takes.
+// tanh forms), SiLU, ReLU.  For gradients the sum before the activation is kept (z), in fp32 or,
+// where the gradients are coarser anyway, in fp16 (linear_gate.h, keep8).
 //
 // Many rows: linear_gemm.h.  Up to 64 rows (a decode step) the weight's bytes bound it,
 // and linear_rows_kernel streams them: 16 of its rows a workgroup, straight into the
@@ -11,27 +11,31 @@
 
 namespace gpa {
 
-// Time of a product in CU cycles: workgroups that a CU runs one after the other, each of
-// so many cycles a stage and at its ends.  (A stage's cycles: the matrix instructions',
-// or the LDS reads' where these take longer, as measured.)  Parts along k are taken
-// where tiles leave CUs idle; they cost writing and reading fp32 sums.
-GemmPlan gemm_plan(int64_t I, int64_t J, int64_t K) {
-  struct Shape { int64_t i, j; double stage, ends; int per_cu; };
-  static const Shape shapes[4] = {{256, 256, 1300, 9000, 1}, {128, 256, 700, 5000, 2}, {128, 128, 400, 4000, 2}, {64, 64, 140, 3000, 4}};
+// A product's time, roughly, in microseconds.  A CU has `held` workgroups at once; a stage of 32 k takes
+// one of them `alone`, and all together not less than `each` for every one; `ends` is what comes
+// before and after the stages.  As measured (8,192 x 4,096 x 4,096, us: 210, 252, 300, 500 by
+// tile; 2,048 x 2,048 x 1,024: 45, 22, 15, 19).  Parts along k pay where few tiles have long sums;
+// they cost a launch and their fp32 sums' bytes.
+GemmPlan gemm_plan(int64_t I, int64_t J, int64_t K, bool turned) {
+  struct Shape { int64_t i, j; int held; double alone, each, ends; };
+  static const Shape shapes[4] = {{256, 256, 1, 0.86, 0.86, 15}, {128, 256, 2, 0.62, 0.49, 7}, {128, 128, 3, 0.38, 0.27, 6},
+                                  {64, 64, 5, 0.2, 0.13, 2}};
   const int64_t nk = std::max<int64_t>((K + 31) / 32, 1);
   GemmPlan best{};
   double least = 0;
   for (int t = 0; t < 4; ++t) {
+    // Two turned operands' addresses do not fit beside 4 x 8 blocks: 440 to 710 us for 205.
+    if (t == 1 && turned) continue;
     const Shape& s = shapes[t];
     const int64_t ti = (I + s.i - 1) / s.i, tj = (J + s.j - 1) / s.j;
-    for (int64_t z = 1; z <= 16; z *= 2) {
-      if (z > 1 && nk / z < 4) break;
-      const double wgs = (double)ti * tj * z, rounds = std::max(1.0, std::ceil(wgs / (256.0 * s.per_cu)));
-      // The workgroups that a CU holds share its matrix cores, and hide each other's ends.
-      const double busy = std::ceil(wgs / 256.0) * s.stage * ((double)nk / z) + rounds * s.ends;
-      const double join = z > 1 ? 6000 + (double)I * J * 4 * (2 * z + 1) / 2000.0 : 0;   // a launch; bytes at 2,000 a cycle
-      if (best.ti == 0 || busy + join < least) {
-        least = busy + join;
+    for (int64_t z = 1; z <= 128 && (z == 1 || nk / z >= 8); z *= 2) {
+      const double n = std::ceil((double)ti * tj * z / 256), rounds = std::floor(n / s.held), rest = n - rounds * s.held;
+      const double stages = std::ceil((double)nk / z);
+      double time = rounds * (stages * std::max(s.alone, s.held * s.each) + s.ends);
+      if (rest > 0) time += stages * std::max(s.alone, rest * s.each) + s.ends;
+      if (z > 1) time += 5 + (double)I * J * 4 * (2 * z + 1) / 4e6;
+      if (best.ti == 0 || time < least) {
+        least = time;
         best = GemmPlan{t, ti, tj, z, z > 1 ? (size_t)z * I * ((J + 7) / 8 * 8) * sizeof(float) : 0};
       }
     }
@@ -157,24 +161,24 @@ using namespace gpa;
 
 extern "C" size_t gpa_linear_gate_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= kRowsMost || N <= 0 || K <= 0) return 0;
-  return gemm_plan(M, N, K).bytes;
+  return gemm_plan(M, N, K, false).bytes;
 }
 
-extern "C" int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate_args* a, void* y, int64_t y_s, float* z,
-                               void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate_args* a, void* y, int64_t y_s, void* z,
+                               int z_dtype, void* workspace, size_t workspace_bytes, void* stream) {
   const char* fn = "gpa_linear_gate";
   gpa_clear_error();
   const int rc = linear_check(fn, dtype, param_dtype, a);
   if (rc != GPA_OK || a->M == 0 || a->N == 0) return rc;
-  if (!y || (z && (uintptr_t)z % 16)) {
-    gpa_set_error("%s: null output, or z that is not 16-byte aligned", fn);
+  if (!y || (z && ((uintptr_t)z % 16 || (z_dtype != GPA_DTYPE_F32 && z_dtype != GPA_DTYPE_F16)))) {
+    gpa_set_error("%s: null output, or z that is not 16-byte aligned fp32 or fp16", fn);
     return GPA_E_INVALID;
   }
   const int64_t psize = param_dtype == GPA_DTYPE_F32 ? 4 : 2;
   Finish f{};
   f.out = y; f.out_s = y_s;
   f.bias = a->bias; f.gate = a->gate; f.residual = a->residual; f.res_s = a->residual_s;
-  f.z = z;
+  f.z = z; f.z16 = z_dtype == GPA_DTYPE_F16;
   f.I = a->M; f.J = a->N;
   f.act = a->act; f.pf32 = psize == 4;
   auto fine = [&](const void* p, int64_t s) { return !p || ((uintptr_t)p % 16 == 0 && (a->M < 2 || s % 8 == 0)); };
@@ -185,7 +189,7 @@ extern "C" int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate
   if (a->M <= kRowsMost) {
     e = f16 ? rows_launch<true>(a, f, s) : rows_launch<false>(a, f, s);
   } else {
-    const GemmPlan x = gemm_plan(a->M, a->N, a->K);
+    const GemmPlan x = gemm_plan(a->M, a->N, a->K, false);
     if (!linear_launchable(x, a->M, a->N)) {
       gpa_set_error("%s: problem exceeds the grid limit", fn);
       return GPA_E_UNSUPPORTED;

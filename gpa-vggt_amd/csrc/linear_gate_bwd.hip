@@ -17,13 +17,13 @@ namespace {
 
 struct DzArgs {
   const void* dy;
-  const float* z;
+  const void* z;
   const void* gate;
   const float* scale;     // fp16 with a gate: (scale, 1 / scale)
   void* dz;               // rows of J8, the columns past J zeros; null: sums alone
   float* part;            // [chunk][2][J]; null: no sums
   int64_t dy_s, I, J, J8, chunk;
-  int32_t pf32, wide;
+  int32_t pf32, wide, z16;
 };
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -72,7 +72,10 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
     for (int64_t i = i0 + wave; i < i1; i += 4) {
       float dy[8], z[8], out[8];
       param8<F16>(static_cast<const uint16_t*>(a.dy) + i * a.dy_s, 0, wide, j, n, dy);
-      if (a.z) param8<F16>(a.z + i * a.J, 1, wide, j, n, z);
+      if (a.z) {
+        if (a.z16) param8<true>(static_cast<const uint16_t*>(a.z) + i * a.J, 0, wide, j, n, z);
+        else param8<true>(static_cast<const float*>(a.z) + i * a.J, 1, wide, j, n, z);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float slope = 1.f;
@@ -146,8 +149,8 @@ BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, bool dz, bool sums, bool dx, b
   p.J8 = (N + 7) / 8 * 8;
   p.chunk = dz_chunk(M, N);
   p.chunks = (M + p.chunk - 1) / p.chunk;
-  if (dx) p.x = gemm_plan(M, K, N);
-  if (dw) p.w = gemm_plan(N, K, M);
+  if (dx) p.x = gemm_plan(M, K, N, true);
+  if (dw) p.w = gemm_plan(N, K, M, true);
   p.scale = dz ? (size_t)round16(M * p.J8 * 2) : 0;
   p.part = p.scale + 16;
   p.split = p.part + (sums ? (size_t)round16(p.chunks * 2 * N * 4) : 0);
@@ -206,7 +209,7 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
     gpa_set_error("%s: nothing to sum, so the gradients are zeros that the caller writes", fn);
     return GPA_E_INVALID;
   }
-  if (!g->dy || (g->dgate && !a->gate) || (g->z && (uintptr_t)g->z % 16) ||
+  if (!g->dy || (g->dgate && !a->gate) || (g->z && ((uintptr_t)g->z % 16 || (g->z_dtype != GPA_DTYPE_F32 && g->z_dtype != GPA_DTYPE_F16))) ||
       (!g->z && (a->act != kActNone || g->dgate))) {
     gpa_set_error("%s: dy is needed, z with an activation or the gate's gradient, and there is none of an absent gate", fn);
     return GPA_E_INVALID;
@@ -240,7 +243,7 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
   if (e == hipSuccess && (need_dz || sums)) {
     DzArgs d{};
     d.dy = g->dy; d.dy_s = a->M > 1 ? g->dy_s : 0;
-    d.z = g->z; d.gate = a->gate; d.scale = scale;
+    d.z = g->z; d.z16 = g->z_dtype == GPA_DTYPE_F16; d.gate = a->gate; d.scale = scale;
     d.dz = need_dz ? ws : nullptr;
     d.part = sums ? (float*)(ws + p.part) : nullptr;
     d.I = a->M; d.J = a->N; d.J8 = p.J8; d.chunk = p.chunk;

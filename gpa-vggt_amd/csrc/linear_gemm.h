@@ -281,30 +281,111 @@ __global__ __launch_bounds__(256, PER_CU) void linear_gemm_kernel(GemmArgs a) {
   const lds8 to[2] = {strip, own || WI == WJ ? strip + WJ * 1024 : (lds8)q1};
   const int quad = lane >> 4, l16 = lane & 15;
   const int64_t i0 = (int64_t)ti * FQ::T + wi * WI * 16, j0 = (int64_t)tj * FP::T + wj * WJ * 16;
-#pragma unroll
-  for (int h = 0; h < WI; h += 2) {
+  // A lane has the same eight columns throughout, and row r0 + RP it of a round's 32.
+  constexpr int RP = 32 / WJ, MASK = CH < 16 ? CH - 1 : 15;
+  const int c8 = lane % (WJ * 2), r0 = lane / (WJ * 2);
+  const int64_t j = j0 + c8 * 8;
+  auto down = [&](int h) __attribute__((always_inline)) {   // strips h, h + 1 into LDS
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int j = 0; j < WJ; ++j)
-        *(lds_f4)(to[s] + (l16 * CH + ((4 * j + quad) ^ (l16 & (CH < 16 ? CH - 1 : 15)))) * 16) = acc[h + s][j];
+      for (int b = 0; b < WJ; ++b) *(lds_f4)(to[s] + (l16 * CH + ((4 * b + quad) ^ (l16 & MASK))) * 16) = acc[h + s][b];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 2
-    for (int it = 0; it < WJ; ++it) {
-      const int idx = it * 64 + lane, row = idx / (WJ * 2), c = idx % (WJ * 2), r = row & 15;
-      const lds8 from = it * 2 / WJ ? to[1] : to[0];
-      const int x = r & (CH < 16 ? CH - 1 : 15);
-      const f32x4 lo = *(lds_f4)(from + (r * CH + ((2 * c) ^ x)) * 16);
-      const f32x4 hi = *(lds_f4)(from + (r * CH + ((2 * c + 1) ^ x)) * 16);
-      float v[8];
+  };
+  auto up = [&](int it, float (&v)[8]) __attribute__((always_inline)) {
+    const int row = it * RP + r0, r = row & 15, x = r & MASK;
+    const lds8 from = it * 2 / WJ ? to[1] : to[0];
+    const f32x4 lo = *(lds_f4)(from + (r * CH + ((2 * c8) ^ x)) * 16), hi = *(lds_f4)(from + (r * CH + ((2 * c8 + 1) ^ x)) * 16);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = lo[e];
-        v[4 + e] = hi[e];
-      }
-      finish8<F16>(a.out, i0 + h * 16 + row, j0 + c * 8, split, a.splits, v);
+    for (int e = 0; e < 4; ++e) {
+      v[e] = lo[e];
+      v[4 + e] = hi[e];
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  if (!a.out.wide || a.splits > 1) {
+#pragma unroll
+    for (int h = 0; h < WI; h += 2) {
+      down(h);
+#pragma unroll 1
+      for (int it = 0; it < WJ; ++it) {
+        float v[8];
+        up(it, v);
+        finish8<F16>(a.out, i0 + h * 16 + it * RP + r0, j, split, a.splits, v);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    return;
+  }
+  // Whole groups of eight columns: what a column has is loaded once, the residual a round ahead,
+  // before the stores of the round between, which a wait for it would wait for too.
+  const bool in = j < a.out.J;
+  float bias[8], gate[8];
+  if (a.out.bias && in) param8<F16>(a.out.bias, a.out.pf32, 1, j, 8, bias);
+  if (a.out.gate && in) param8<F16>(a.out.gate, a.out.pf32, 1, j, 8, gate);
+  const float factor = a.out.unscale ? *a.out.unscale : 1.f;
+  auto rounds = [&](auto which) __attribute__((always_inline)) {
+    constexpr int ACT = decltype(which)::value;
+    constexpr int SETS = WI == 8 ? 2 : 1;      // two waves a SIMD hide each other's waits
+    u32x4 res[SETS][WJ];
+    auto ahead = [&](int h) __attribute__((always_inline)) {
+      const int64_t i = i0 + h * 16 + r0;
+#pragma unroll
+      for (int it = 0; it < WJ; ++it)
+        if (in && i + it * RP < a.out.I)
+          res[h / 2 % SETS][it] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.out.residual) + (i + it * RP) * a.out.res_s + j);
+    };
+    if (SETS == 2 && a.out.residual) ahead(0);
+#pragma unroll
+    for (int h = 0; h < WI; h += 2) {
+      const int64_t i = i0 + h * 16 + r0;
+      if (a.out.residual && (SETS == 1 || h + 2 < WI)) ahead(SETS == 1 ? h : h + 2);
+      down(h);
+#pragma unroll
+      for (int it = 0; it < WJ; ++it) {
+        float v[8];
+        up(it, v);
+        if (!in || i + it * RP >= a.out.I) continue;
+        if (a.out.unscale) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= factor;
+        }
+        if (a.out.bias) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += bias[e];
+        }
+        if (a.out.z) keep8<ACT>(a.out, (i + it * RP) * a.out.J + j, 8, v);
+        act8<ACT>(v);
+        if (a.out.gate) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= gate[e];
+        }
+        if (a.out.residual) {
+          const bf16x8 x = __builtin_bit_cast(bf16x8, res[h / 2 % SETS][it]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += half_to_f32<F16>(x[e]);
+        }
+        bf16x8 y;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const bf16x2 w = pack2<F16>(v[e], v[e + 1]);
+          y[e] = w[0];
+          y[e + 1] = w[1];
+        }
+        *reinterpret_cast<bf16x8*>(static_cast<uint16_t*>(a.out.out) + (i + it * RP) * a.out.out_s + j) = y;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  };
+  if constexpr (PT) {                          // gradients: no activation
+    rounds(std::integral_constant<int, kActNone>{});
+  } else {
+    switch (a.out.act) {
+      case kActGelu: rounds(std::integral_constant<int, kActGelu>{}); break;
+      case kActGeluTanh: rounds(std::integral_constant<int, kActGeluTanh>{}); break;
+      case kActSilu: rounds(std::integral_constant<int, kActSilu>{}); break;
+      case kActRelu: rounds(std::integral_constant<int, kActRelu>{}); break;
+      default: rounds(std::integral_constant<int, kActNone>{});
+    }
   }
 }
 
@@ -341,10 +422,12 @@ hipError_t gemm_launch(const GemmArgs& a, hipStream_t s) {
 template <bool PT, bool QT, bool F16>
 hipError_t gemm(GemmArgs a, const GemmPlan& x, hipStream_t s) {
   a.ti = (int32_t)x.ti; a.tj = (int32_t)x.tj; a.splits = (int32_t)x.splits;
-  hipError_t e = x.tile == 0   ? gemm_launch<8, 8, 4, 1, PT, QT, F16>(a, s)
-                 : x.tile == 1 ? gemm_launch<4, 8, 3, 2, PT, QT, F16>(a, s)
-                 : x.tile == 2 ? gemm_launch<4, 4, 3, 2, PT, QT, F16>(a, s)
-                               : gemm_launch<2, 2, 4, 4, PT, QT, F16>(a, s);
+  hipError_t e;
+  if (x.tile == 0) e = gemm_launch<8, 8, 4, 1, PT, QT, F16>(a, s);
+  else if (x.tile == 2) e = gemm_launch<4, 4, 3, 2, PT, QT, F16>(a, s);
+  else if (x.tile == 3) e = gemm_launch<2, 2, 4, 4, PT, QT, F16>(a, s);
+  else if constexpr (!PT) e = gemm_launch<4, 8, 3, 2, PT, QT, F16>(a, s);
+  else return hipErrorInvalidValue;            // not planned for turned operands
   if (e != hipSuccess || x.splits == 1) return e;
   const int64_t threads = (a.out.J + 7) / 8 * a.out.I;
   hipLaunchKernelGGL((linear_join_kernel<F16>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a.out, (int)x.splits);

@@ -165,7 +165,7 @@ _TreeArgs = _struct("_TreeArgs", (
 
 # gpa_linear_gate_args and gpa_linear_gate_grads.
 _LinearArgs = _struct("_LinearArgs", ("p: x w bias gate residual", "l: M N K x_s w_s residual_s", "i: act"))
-_LinearGrads = _struct("_LinearGrads", ("p: dy z dx dw dbias dgate", "l: dy_s dx_s dw_s K_out"))
+_LinearGrads = _struct("_LinearGrads", ("p: dy z dx dw dbias dgate", "l: dy_s dx_s dw_s K_out", "i: z_dtype"))
 
 # gpa_head_rotary_args and gpa_head_rotary_grads.
 MAX_AXES = 8
@@ -304,7 +304,8 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.gpa_linear_gate_workspace_bytes.restype = ctypes.c_size_t
     lib.gpa_linear_gate_workspace_bytes.argtypes = [_i64] * 3
     lib.gpa_linear_gate.restype = ctypes.c_int
-    lib.gpa_linear_gate.argtypes = [ctypes.c_int, ctypes.c_int, _vp, _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp]
+    lib.gpa_linear_gate.argtypes = [ctypes.c_int, ctypes.c_int, _vp, _vp, _i64, _vp, ctypes.c_int, _vp, ctypes.c_size_t,
+                                    _vp]
     lib.gpa_linear_gate_bwd_workspace_bytes.restype = ctypes.c_size_t
     lib.gpa_linear_gate_bwd_workspace_bytes.argtypes = [_vp, _vp]
     lib.gpa_linear_gate_bwd.restype = ctypes.c_int
@@ -1956,17 +1957,23 @@ def _linear_backward(ctx, dy, _):
     return some(0, dx), some(1, dw), some(2, db), some(3, dg), dy if ctx.needs_input_grad[4] else None, None, None
 
 
+def _z_dtype(x, gate):
+    """What the sums are kept in: an eighth of what rounding dz costs, or nothing."""
+    return torch.float16 if x.dtype == torch.bfloat16 and gate is None else torch.float32
+
+
 def linear_gate(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], gate: Optional[torch.Tensor],
                 residual: Optional[torch.Tensor], act: int, want_z: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """gpa_linear_gate: y [M, N] in x's type, and the sums before the activation, fp32
+    """gpa_linear_gate: y [M, N] in x's type, and the sums before the activation
     [M, N], if want_z (else an empty tensor), which gradients need where there is an
-    activation or a gate.  act as the header's GPA_ACT_*."""
+    activation or a gate: fp32, but fp16 of bf16 operands without a gate.  act as
+    the header's GPA_ACT_*."""
     what = "gpa::linear_gate"
     dev = _require_gpu(*[t for t in (x, w, bias, gate, residual) if t is not None])
     pdt = _linear_check(what, x, w, bias, gate, residual, act)
     M, N = x.shape[0], w.shape[0]
     y = torch.empty(M, N, device=dev, dtype=x.dtype)
-    z = torch.empty((M, N) if want_z else (0,), device=dev, dtype=torch.float32)
+    z = torch.empty((M, N) if want_z else (0,), device=dev, dtype=_z_dtype(x, gate))
     if M == 0 or N == 0:
         return y, z
     x, w = _rows_of_8(x), _rows_of_8(w)
@@ -1977,8 +1984,8 @@ def linear_gate(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
     with _on(dev):
         rc = L.gpa_linear_gate(_DTYPE_CODES[x.dtype], _DTYPE_CODES[pdt], _linear_args(x, w, bias, gate, residual, act),
-                               y.data_ptr(), N, z.data_ptr() if want_z else None, None if ws is None else ws.data_ptr(),
-                               ws_bytes, _stream(dev))
+                               y.data_ptr(), N, z.data_ptr() if want_z else None, _DTYPE_CODES[z.dtype],
+                               None if ws is None else ws.data_ptr(), ws_bytes, _stream(dev))
     _check(rc, what)
     return y, z
 
@@ -1989,7 +1996,7 @@ linear_gate = _op(linear_gate, _linear_setup, _linear_backward)
 @_fake("linear_gate")
 def _linear_gate_fake(x, w, bias, gate, residual, act, want_z):
     size = (x.shape[0], w.shape[0])
-    return x.new_empty(size), x.new_empty(size if want_z else (0,), dtype=torch.float32)
+    return x.new_empty(size), x.new_empty(size if want_z else (0,), dtype=_z_dtype(x, gate))
 
 
 @_op
@@ -2006,8 +2013,8 @@ def linear_gate_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: torch.Tensor
         raise ValueError(f"{what}: no gradient of an absent bias or gate")
     if z is None and (act or want_gate):
         raise ValueError(f"{what}: an activation, and the gate's gradient, need z")
-    if z is not None and (z.dtype != torch.float32 or z.shape != (M, N) or not z.is_contiguous() or z.data_ptr() % 16):
-        raise ValueError(f"{what}: z must be contiguous fp32 [{M}, {N}], got {z.dtype} {tuple(z.shape)}")
+    if z is not None and (z.dtype not in (torch.float32, torch.float16) or z.shape != (M, N) or not z.is_contiguous() or z.data_ptr() % 16):
+        raise ValueError(f"{what}: z must be contiguous fp32 or fp16 [{M}, {N}], got {z.dtype} {tuple(z.shape)}")
     none = lambda: x.new_empty(0)  # noqa: E731
     dx = torch.empty(M, K, device=dev, dtype=x.dtype) if want_x else none()
     dw = torch.empty(N, K, device=dev, dtype=w.dtype) if want_w else none()
@@ -2022,7 +2029,7 @@ def linear_gate_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: torch.Tensor
     ptr = lambda t: t.data_ptr() if t.numel() else 0  # noqa: E731
     a = _linear_args(x, w, None, gate, None, act)
     g = _LinearGrads.packed(dy.data_ptr(), 0 if z is None else z.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(dg), dy.stride(0),
-                            K, K, max(K, 1))
+                            K, K, max(K, 1), 0 if z is None else _DTYPE_CODES[z.dtype])
     L = lib()
     ws_bytes = L.gpa_linear_gate_bwd_workspace_bytes(a, g)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)

@@ -6,7 +6,7 @@ step of fp16): a sum over K products of 16-bit values, exact in fp32, is off by 
 roundings) + 16 f, a logistic value s of t by s (1 - s) (|t| + 4) 4 f + 4 f s, and what
 comes in off moves an activation by at most 1.13 of it and its slope by 1.2 (GELU's
 second derivative is below 0.8, its tanh form's below 1, SiLU's 0.5; ReLU's slope is open
-where the sum's sign is).  dz is rounded once (fp16 with a gate: after a scaling that makes
+where the sum's sign is); without a gate a bf16 call's slopes come from sums kept in fp16.  dz is rounded once (fp16 with a gate: after a scaling that makes
 the gate's largest value one or more), sums over R rows add (R + 64) f of their terms.
 """
 import math
@@ -53,7 +53,8 @@ def _reference(x, w, bias, gate, residual, act, dy, u, tiny):
     got = [(y, u * y.abs() + ae * g.abs() + 4 * f * ((a * g).abs() + y.abs()) + tiny)]
     if dy is None:
         return got
-    se = se + 1.2 * ze + (((z.abs() <= ze) & (ze > 0)).double() if act == "relu" else 0)
+    kept = u == 2.0 ** -8 and gate is None and act        # z is kept in fp16
+    se = se + 1.2 * (ze + (2.0 ** -11 * z.abs() + 2.0 ** -25 if kept else 0)) + (((z.abs() <= ze) & (ze > 0)).double() if act == "relu" else 0)
     dz = dy * g * slope
     off = (dy * g).abs() * se + 4 * f * dz.abs() if act or gate is not None else dz * 0
     least = tiny * g.abs().max() if gate is not None else tiny

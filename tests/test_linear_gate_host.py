@@ -32,11 +32,11 @@ COMMON = [
 ]
 
 
-@pytest.mark.parametrize("kw,code", COMMON + [(dict(y=None), INV), (dict(z=FAKE + 4), INV)])
+@pytest.mark.parametrize("kw,code", COMMON + [(dict(y=None), INV), (dict(z=FAKE + 4), INV), (dict(z_dtype=1), INV)])
 def test_forward_argument_errors(kw, code):
     kw = dict(kw)
-    dt, pdt, y, z = kw.pop("dtype", 1), kw.pop("pdtype", None), kw.pop("y", FAKE), kw.pop("z", FAKE)
-    rc = _native.lib().gpa_linear_gate(dt, dt if pdt is None else pdt, ctypes.byref(_args(**kw)), y, 64, z, FAKE, 1 << 30, None)
+    dt, pdt, y, z, zdt = kw.pop("dtype", 1), kw.pop("pdtype", None), kw.pop("y", FAKE), kw.pop("z", FAKE), kw.pop("z_dtype", 0)
+    rc = _native.lib().gpa_linear_gate(dt, dt if pdt is None else pdt, ctypes.byref(_args(**kw)), y, 64, z, zdt, FAKE, 1 << 30, None)
     assert rc == code and _native.lib().gpa_last_error()
 
 
@@ -46,13 +46,13 @@ def test_forward_workspace_errors():
     need = L.gpa_linear_gate_workspace_bytes(70, 70, 8000)
     assert need >= 2 * 70 * 72 * 4
     for ws, size in ((None, need), (FAKE, need - 1), (FAKE + 8, need)):
-        assert L.gpa_linear_gate(1, 1, ctypes.byref(a), FAKE, 70, None, ws, size, None) == WSP
+        assert L.gpa_linear_gate(1, 1, ctypes.byref(a), FAKE, 70, None, 0, ws, size, None) == WSP
     assert L.gpa_linear_gate_workspace_bytes(64, 70, 8000) == L.gpa_linear_gate_workspace_bytes(0, 70, 8000) == 0
 
 
 @pytest.mark.parametrize("kw,code", COMMON + [
     (dict(g=dict(dy=None)), INV), (dict(g=dict(z=None)), INV), (dict(act=0, g=dict(z=None)), INV), (dict(gate=None), INV),
-    (dict(g=dict(z=FAKE + 4)), INV), (dict(g=dict(K_out=0)), INV), (dict(g=dict(K_out=129)), INV), (dict(g=dict(K_out=120)), INV),
+    (dict(g=dict(z=FAKE + 4)), INV), (dict(g=dict(z_dtype=1)), INV), (dict(g=dict(K_out=0)), INV), (dict(g=dict(K_out=129)), INV), (dict(g=dict(K_out=120)), INV),
     (dict(M=0), INV), (dict(N=0), INV), (dict(N=1 << 21), UNS), (dict(ws=None), WSP), (dict(ws_bytes=64), WSP), (dict(ws=FAKE + 8), WSP),
 ])
 def test_backward_argument_errors(kw, code):
@@ -67,11 +67,11 @@ def test_backward_argument_errors(kw, code):
 def test_nothing_to_do():
     L = _native.lib()
     none = _native._LinearGrads()
-    assert L.gpa_linear_gate(1, 1, None, FAKE, 64, None, None, 0, None) == INV
+    assert L.gpa_linear_gate(1, 1, None, FAKE, 64, None, 0, None, 0, None) == INV
     assert L.gpa_linear_gate_bwd(1, 1, ctypes.byref(_args()), None, FAKE, 1 << 30, None) == INV
     assert L.gpa_linear_gate_bwd(1, 1, ctypes.byref(_args()), ctypes.byref(none), None, 0, None) == 0
     for kw in (dict(M=0), dict(N=0)):
-        assert L.gpa_linear_gate(1, 1, ctypes.byref(_args(**kw)), None, 64, None, None, 0, None) == 0
+        assert L.gpa_linear_gate(1, 1, ctypes.byref(_args(**kw)), None, 64, None, 0, None, 0, None) == 0
 
 
 X, W = torch.zeros(5, 16, dtype=torch.bfloat16), torch.zeros(7, 16, dtype=torch.bfloat16)
