@@ -15,6 +15,19 @@ enum Act { kActNone = 0, kActGelu = 1, kActGeluTanh = 2, kActSilu = 3, kActRelu 
 struct GemmPlan { int tile; int64_t ti, tj, splits; size_t bytes; };
 GemmPlan gemm_plan(int64_t I, int64_t J, int64_t K, bool turned);
 
+// x and w as the products take them: K a multiple of 8 and rows that are 16-byte aligned, so or as
+// padded copies in the workspace (`bytes` of it, x's first).
+struct Laid {
+  int64_t K;
+  bool copy_x, copy_w;
+  size_t w_at, bytes;
+};
+Laid linear_laid(const gpa_linear_gate_args* a, bool x, bool w);
+struct Matrix { const uint16_t* p; int64_t stride; };
+hipError_t linear_lay(const gpa_linear_gate_args* a, const Laid& l, void* ws, Matrix& x, Matrix& w, hipStream_t s);
+int linear_check(const char* fn, int dtype, int pdtype, const gpa_linear_gate_args* a);
+bool linear_launchable(const GemmPlan& x, int64_t I, int64_t J);
+
 // What becomes of a sum.
 struct Finish {
   void* out;              // 16-bit, rows out_s apart
@@ -165,16 +178,64 @@ __device__ __forceinline__ void act8(float (&v)[8]) {
   for (int e = 0; e < 8; ++e) v[e] = act_of<ACT>(v[e]);
 }
 
+// act's eight values, chosen at run time.
+__device__ __forceinline__ void act8_of(int act, float (&v)[8]) {
+  switch (act) {
+    case kActGelu: act8<kActGelu>(v); break;
+    case kActGeluTanh: act8<kActGeluTanh>(v); break;
+    case kActSilu: act8<kActSilu>(v); break;
+    case kActRelu: act8<kActRelu>(v); break;
+    default: break;
+  }
+}
+
+// The sums v of row i, columns j .. j + 7 of a part.
+__device__ __forceinline__ void part8(const Finish& f, int64_t i, int64_t j, int split, const float (&v)[8]) {
+  if (i >= f.I || j >= f.J) return;
+  f32x4* to = reinterpret_cast<f32x4*>(f.part + ((int64_t)split * f.I + i) * ((f.J + 7) / 8 * 8) + j);
+  to[0] = f32x4{v[0], v[1], v[2], v[3]};
+  to[1] = f32x4{v[4], v[5], v[6], v[7]};
+}
+
+// The sums v of column j, rows i, i + STEP, ...
+template <bool F16, int STEP>
+__device__ __forceinline__ void finish_down(const Finish& f, int64_t i, int64_t j, float (&v)[8]) {
+  if (j >= f.J) return;
+  auto param = [&](const void* p) {
+    return f.pf32 ? static_cast<const float*>(p)[j] : half_to_f32<F16>(static_cast<const __bf16*>(p)[j]);
+  };
+  const float factor = f.unscale ? *f.unscale : 1.f, bias = f.bias ? param(f.bias) : 0.f, gate = f.gate ? param(f.gate) : 1.f;
+  const int n = f.I <= i ? 0 : (f.I - i + STEP - 1) / STEP < 8 ? (int)((f.I - i + STEP - 1) / STEP) : 8;
+  __bf16 res[8];
+  if (f.residual)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) res[e] = e < n ? static_cast<const __bf16*>(f.residual)[(i + e * STEP) * f.res_s + j] : (__bf16)0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (f.unscale) v[e] *= factor;
+    if (f.bias) v[e] += bias;
+  }
+  if (f.z)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float one[8] = {v[e]};
+      if (e >= n) continue;
+      if (f.act == kActRelu) keep8<kActRelu>(f, (i + e * STEP) * f.J + j, 1, one);
+      else keep8<kActNone>(f, (i + e * STEP) * f.J + j, 1, one);
+    }
+  act8_of(f.act, v);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (f.gate) v[e] *= gate;
+    if (f.residual) v[e] += half_to_f32<F16>(res[e]);
+    if (e < n) static_cast<__bf16*>(f.out)[(i + e * STEP) * f.out_s + j] = f32_to_half<F16>(v[e]);
+  }
+}
+
 // The sums v of row i, columns j .. j + 7.
 template <bool F16>
-__device__ __forceinline__ void finish8(const Finish& f, int64_t i, int64_t j, int split, int splits, float (&v)[8]) {
+__device__ __forceinline__ void finish8(const Finish& f, int64_t i, int64_t j, float (&v)[8]) {
   if (i >= f.I || j >= f.J) return;
-  if (splits > 1) {
-    f32x4* to = reinterpret_cast<f32x4*>(f.part + ((int64_t)split * f.I + i) * ((f.J + 7) / 8 * 8) + j);
-    to[0] = f32x4{v[0], v[1], v[2], v[3]};
-    to[1] = f32x4{v[4], v[5], v[6], v[7]};
-    return;
-  }
   const int n = f.J - j < 8 ? (int)(f.J - j) : 8;
   float x[8];
   if (f.unscale) {
@@ -191,13 +252,7 @@ __device__ __forceinline__ void finish8(const Finish& f, int64_t i, int64_t j, i
     if (f.act == kActRelu) keep8<kActRelu>(f, i * f.J + j, n, v);
     else keep8<kActNone>(f, i * f.J + j, n, v);
   }
-  switch (f.act) {
-    case kActGelu: act8<kActGelu>(v); break;
-    case kActGeluTanh: act8<kActGeluTanh>(v); break;
-    case kActSilu: act8<kActSilu>(v); break;
-    case kActRelu: act8<kActRelu>(v); break;
-    default: break;
-  }
+  act8_of(f.act, v);
   if (f.gate) {
     param8<F16>(f.gate, f.pf32, f.wide, j, n, x);
 #pragma unroll

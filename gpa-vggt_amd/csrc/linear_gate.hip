@@ -3,9 +3,9 @@
 // tanh forms), SiLU, ReLU.  For gradients the sum before the activation is kept (z), in fp32 or,
 // where the gradients are coarser anyway, in fp16 (linear_gate.h, keep8).
 //
-// Many rows: linear_gemm.h.  Up to 64 rows (a decode step) the weight's bytes bound it,
+// Many rows: linear_gemm.h.  Up to 16 rows (a decode step) the weight's bytes bound it,
 // and linear_rows_kernel streams them: 16 of its rows a workgroup, straight into the
-// matrix instructions' registers, the eight waves taking every eighth 32 features, so that
+// matrix instructions' registers, eight waves taking every eighth 32 features, so that
 // they read 512 bytes of a row together; the waves' sums meet in LDS.  x comes out of the L2.
 #include "linear_gemm.h"
 
@@ -45,67 +45,74 @@ GemmPlan gemm_plan(int64_t I, int64_t J, int64_t K, bool turned) {
 
 namespace {
 
-constexpr int kRowsMost = 64;
-constexpr int kRowWaves = 8;
+constexpr int kRowsMost = 16;
 
-template <int MB, bool F16>
-__global__ __launch_bounds__(kRowWaves * 64) void linear_rows_kernel(const uint16_t* x, int64_t x_s, const uint16_t* w, int64_t w_s,
-                                                                     int K, Finish f) {
-  constexpr int U = MB == 1 ? 8 : 4;           // steps whose loads are in flight together
-  __shared__ f32x4 sum[kRowWaves][MB][64];
+// Up to 16 rows.  WAVES waves take the steps of 32 k in turn.  Measured, us: 8 rows of 4,096 x 4,096
+// 10.5 (3.2 TB/s, launch and all; 256 workgroups, one a CU), 16,384 x 4,096 33 (4.1 TB/s), and of
+// 4,096 outputs over 16,384 features 43 with eight waves, 36 with sixteen.  More rows would
+// read x once for each 16 outputs: 32 and 64 rows took 16 and 23 us here, 64 x 64 tiles take 12 to 15.
+template <int WAVES, bool F16>
+__global__ __launch_bounds__(WAVES * 64) void linear_rows_kernel(Matrix x, Matrix w, int K, Finish f) {
+  constexpr int U = 4;                         // steps whose loads are in flight together
+  __shared__ f32x4 sum[WAVES][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quad = lane >> 4, l16 = lane & 15;
-  const int64_t n0 = (int64_t)blockIdx.x * 16, n = n0 + l16;
-  const uint16_t* W = w + n * w_s + 8 * quad;
-  f32x4 acc[MB];
-#pragma unroll
-  for (int b = 0; b < MB; ++b) acc[b] = f32x4{};
-  const int steps = (K + 31) / 32;
-  for (int s0 = wave; s0 < steps; s0 += U * kRowWaves) {
-    bf16x8 p[U], q[U][MB];
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const bool mine = n0 + l16 < f.J, row = l16 < f.I;
+  const uint16_t* W = w.p + (mine ? n0 + l16 : 0) * w.stride + 8 * quad;
+  const uint16_t* X = x.p + (row ? l16 : 0) * x.stride + 8 * quad;
+  f32x4 acc{};
+  for (int k0 = wave * 32; k0 < K; k0 += U * WAVES * 32) {
+    bf16x8 p[U], q[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = (s0 + u * kRowWaves) * 32;
+      const int k = k0 + u * WAVES * 32;
       const bool in = k + 8 * quad < K;
-      p[u] = in && n < f.J ? *reinterpret_cast<const bf16x8*>(W + k) : bf16x8{};
-#pragma unroll
-      for (int b = 0; b < MB; ++b)
-        q[u][b] = in && 16 * b + l16 < f.I ? *reinterpret_cast<const bf16x8*>(x + (16 * b + l16) * x_s + k + 8 * quad) : bf16x8{};
+      p[u] = in && mine ? *reinterpret_cast<const bf16x8*>(W + k) : bf16x8{};
+      q[u] = in && row ? *reinterpret_cast<const bf16x8*>(X + k) : bf16x8{};
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int b = 0; b < MB; ++b) acc[b] = mfma16x16x32_t<F16>(p[u], q[u][b], acc[b]);
+    for (int u = 0; u < U; ++u) acc = mfma16x16x32_t<F16>(p[u], q[u], acc);
   }
-#pragma unroll
-  for (int b = 0; b < MB; ++b) sum[wave][b][lane] = acc[b];
+  sum[wave][lane] = acc;
   __syncthreads();
-  // Lane (quad, l16) of block b has row 16 b + l16, columns 4 quad .. +3: eight of a row to a thread.
+  // Lane (quad, l16) has row l16, columns 4 quad .. +3: eight of a row to a thread.
   const int t = threadIdx.x;
-  if (t >= MB * 32) return;
-  const int b = t >> 5, half = t >> 4 & 1, at = half * 32 + (t & 15);
+  if (t >= 32) return;
+  const int half = t >> 4, at = half * 32 + (t & 15);
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.f;
 #pragma unroll
-  for (int i = 0; i < kRowWaves; ++i) {
-    const f32x4 lo = sum[i][b][at], hi = sum[i][b][at + 16];
+  for (int i = 0; i < WAVES; ++i) {
+    const f32x4 lo = sum[i][at], hi = sum[i][at + 16];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] += lo[e];
       v[4 + e] += hi[e];
     }
   }
-  finish8<F16>(f, 16 * b + (t & 15), n0 + 8 * half, 0, 1, v);
+  finish8<F16>(f, t & 15, n0 + 8 * half, v);
 }
 
 template <bool F16>
-hipError_t rows_launch(const gpa_linear_gate_args* a, const Finish& f, hipStream_t s) {
-  const dim3 grid((unsigned)((a->N + 15) / 16)), block(kRowWaves * 64);
-  const auto *x = (const uint16_t*)a->x, *w = (const uint16_t*)a->w;
-  if (a->M <= 16) hipLaunchKernelGGL((linear_rows_kernel<1, F16>), grid, block, 0, s, x, a->x_s, w, a->w_s, (int)a->K, f);
-  else if (a->M <= 32) hipLaunchKernelGGL((linear_rows_kernel<2, F16>), grid, block, 0, s, x, a->x_s, w, a->w_s, (int)a->K, f);
-  else hipLaunchKernelGGL((linear_rows_kernel<4, F16>), grid, block, 0, s, x, a->x_s, w, a->w_s, (int)a->K, f);
+hipError_t rows_launch(const Matrix& x, const Matrix& w, int64_t K, const Finish& f, hipStream_t s) {
+  const dim3 grid((unsigned)((f.J + 15) / 16));
+  if (K > 4096) hipLaunchKernelGGL((linear_rows_kernel<16, F16>), grid, dim3(1024), 0, s, x, w, (int)K, f);
+  else hipLaunchKernelGGL((linear_rows_kernel<8, F16>), grid, dim3(512), 0, s, x, w, (int)K, f);
   return hipGetLastError();
+}
+
+// Rows of C values to rows of C8, the columns past C zeros: x's, then w's.
+struct LayArgs { const uint16_t *x, *w; uint16_t *to_x, *to_w; int64_t x_rows, w_rows, x_s, w_s; int32_t C, C8; };
+__global__ __launch_bounds__(256) void linear_lay_kernel(LayArgs a) {
+  const int64_t wave = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (wave >= a.x_rows + a.w_rows) return;
+  const bool x = wave < a.x_rows;
+  const int64_t row = x ? wave : wave - a.x_rows;
+  const uint16_t* from = x ? a.x + row * a.x_s : a.w + row * a.w_s;
+  uint16_t* to = (x ? a.to_x : a.to_w) + row * a.C8;
+#pragma unroll 8
+  for (int c = threadIdx.x & 63; c < a.C8; c += 64) to[c] = c < a.C ? from[c] : (uint16_t)0;
 }
 
 }  // namespace
@@ -128,26 +135,42 @@ int linear_check(const char* fn, int dtype, int pdtype, const gpa_linear_gate_ar
     return GPA_E_INVALID;
   }
   const int64_t lim = (int64_t)1 << 21, most = (int64_t)1 << 30;
-  if (a->M >= most || a->N >= most || a->K >= lim) {
+  if (a->M >= most || a->N >= most || a->K >= lim - 8) {
     gpa_set_error("%s: %lld x %lld x %lld is too large (2^30 rows, 2^21 features)", fn, (long long)a->M, (long long)a->N, (long long)a->K);
     return GPA_E_UNSUPPORTED;
   }
   if (a->M == 0 || a->N == 0) return GPA_OK;
-  if (!a->x || !a->w) {
+  if (a->K > 0 && (!a->x || !a->w)) {
     gpa_set_error("%s: null pointer", fn);
     return GPA_E_INVALID;
   }
-  auto fine = [&](const void* p, int64_t n, int64_t s) { return (uintptr_t)p % 16 == 0 && (n < 2 || s % 8 == 0); };
-  if (a->K < 8 || a->K % 8 || !fine(a->x, a->M, a->x_s) || !fine(a->w, a->N, a->w_s)) {
-    gpa_set_error("%s: K must be a positive multiple of 8, rows of x and w 16-byte aligned", fn);
-    return GPA_E_INVALID;
-  }
-  // Rows of a tile are addressed by 32-bit offsets from its first one.
-  if ((a->M > 1 && (a->x_s < 0 || a->x_s >= lim)) || (a->N > 1 && (a->w_s < 0 || a->w_s >= lim))) {
-    gpa_set_error("%s: row strides from 0 to 2^21 are supported", fn);
-    return GPA_E_UNSUPPORTED;
-  }
   return GPA_OK;
+}
+
+Laid linear_laid(const gpa_linear_gate_args* a, bool x, bool w) {
+  Laid l{};
+  l.K = std::max<int64_t>((a->K + 7) / 8 * 8, 8);
+  // Rows of a tile are addressed by 32-bit offsets from its first one: strides below 2^21.
+  auto copied = [&](const void* p, int64_t n, int64_t st) {
+    return a->K != l.K || (uintptr_t)p % 16 || (n > 1 && (st % 8 || st < 0 || st >= (int64_t)1 << 21));
+  };
+  l.copy_x = x && copied(a->x, a->M, a->x_s);
+  l.copy_w = w && copied(a->w, a->N, a->w_s);
+  l.w_at = l.copy_x ? (size_t)a->M * l.K * 2 : 0;
+  l.bytes = l.w_at + (l.copy_w ? (size_t)a->N * l.K * 2 : 0);
+  return l;
+}
+
+hipError_t linear_lay(const gpa_linear_gate_args* a, const Laid& l, void* ws, Matrix& x, Matrix& w, hipStream_t s) {
+  char* const at = (char*)ws;
+  x = Matrix{(const uint16_t*)(l.copy_x ? at : a->x), l.copy_x || a->M < 2 ? l.K : a->x_s};
+  w = Matrix{(const uint16_t*)(l.copy_w ? at + l.w_at : a->w), l.copy_w || a->N < 2 ? l.K : a->w_s};
+  if (!l.copy_x && !l.copy_w) return hipSuccess;
+  const LayArgs p{(const uint16_t*)a->x, (const uint16_t*)a->w, (uint16_t*)x.p, (uint16_t*)w.p, l.copy_x ? a->M : 0, l.copy_w ? a->N : 0,
+                  a->M > 1 ? a->x_s : 0, a->N > 1 ? a->w_s : 0, (int32_t)a->K, (int32_t)l.K};
+  const int64_t wgs = (p.x_rows + p.w_rows + 3) / 4, most = (int64_t)1 << 22;
+  hipLaunchKernelGGL(linear_lay_kernel, dim3((unsigned)std::min(wgs, most), (unsigned)((wgs + most - 1) / most)), dim3(256), 0, s, p);
+  return hipGetLastError();
 }
 
 bool linear_launchable(const GemmPlan& x, int64_t I, int64_t J) {
@@ -159,9 +182,10 @@ bool linear_launchable(const GemmPlan& x, int64_t I, int64_t J) {
 
 using namespace gpa;
 
-extern "C" size_t gpa_linear_gate_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= kRowsMost || N <= 0 || K <= 0) return 0;
-  return gemm_plan(M, N, K, false).bytes;
+extern "C" size_t gpa_linear_gate_workspace_bytes(const gpa_linear_gate_args* a) {
+  if (!a || a->M <= 0 || a->N <= 0 || a->K < 0) return 0;
+  const Laid l = linear_laid(a, true, true);
+  return l.bytes + (a->M <= kRowsMost ? 0 : gemm_plan(a->M, a->N, l.K, false).bytes);
 }
 
 extern "C" int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate_args* a, void* y, int64_t y_s, void* z,
@@ -185,24 +209,28 @@ extern "C" int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate
   f.wide = a->N % 8 == 0 && fine(y, y_s) && fine(a->residual, a->residual_s) && fine(a->bias, 0) && fine(a->gate, 0);
   const hipStream_t s = (hipStream_t)stream;
   const bool f16 = dtype == GPA_DTYPE_F16;
-  hipError_t e;
-  if (a->M <= kRowsMost) {
-    e = f16 ? rows_launch<true>(a, f, s) : rows_launch<false>(a, f, s);
-  } else {
-    const GemmPlan x = gemm_plan(a->M, a->N, a->K, false);
-    if (!linear_launchable(x, a->M, a->N)) {
-      gpa_set_error("%s: problem exceeds the grid limit", fn);
-      return GPA_E_UNSUPPORTED;
-    }
-    if (x.bytes > 0 && (!workspace || workspace_bytes < x.bytes || (uintptr_t)workspace % 16)) {
-      gpa_set_error("%s: workspace of %zu bytes, 16-byte aligned, needed", fn, x.bytes);
-      return GPA_E_WORKSPACE;
-    }
+  const bool few = a->M <= kRowsMost;
+  const Laid l = linear_laid(a, true, true);
+  const GemmPlan x = few ? GemmPlan{} : gemm_plan(a->M, a->N, l.K, false);
+  if (!few && !linear_launchable(x, a->M, a->N)) {
+    gpa_set_error("%s: problem exceeds the grid limit", fn);
+    return GPA_E_UNSUPPORTED;
+  }
+  const size_t need = l.bytes + x.bytes;
+  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) {
+    gpa_set_error("%s: workspace of %zu bytes, 16-byte aligned, needed", fn, need);
+    return GPA_E_WORKSPACE;
+  }
+  Matrix mx, mw;
+  hipError_t e = linear_lay(a, l, workspace, mx, mw, s);
+  if (e == hipSuccess && few) {
+    e = f16 ? rows_launch<true>(mx, mw, l.K, f, s) : rows_launch<false>(mx, mw, l.K, f, s);
+  } else if (e == hipSuccess) {
     GemmArgs g{};
-    g.P = Operand{(const uint16_t*)a->w, a->N > 1 ? a->w_s : a->K, a->N, a->K};
-    g.Q = Operand{(const uint16_t*)a->x, a->M > 1 ? a->x_s : a->K, a->M, a->K};
-    g.nk = (int32_t)((a->K + 31) / 32);
-    f.part = (float*)workspace;
+    g.P = Operand{mw.p, mw.stride, a->N, l.K};
+    g.Q = Operand{mx.p, mx.stride, a->M, l.K};
+    g.nk = (int32_t)((l.K + 31) / 32);
+    f.part = (float*)((char*)workspace + l.bytes);
     g.out = f;
     e = f16 ? gemm<false, false, true>(g, x, s) : gemm<false, false, false>(g, x, s);
   }

@@ -19,89 +19,107 @@ struct DzArgs {
   const void* dy;
   const void* z;
   const void* gate;
-  const float* scale;     // fp16 with a gate: (scale, 1 / scale)
+  float* scale;           // fp16 with a gate: where the inverse of its scale goes
   void* dz;               // rows of J8, the columns past J zeros; null: sums alone
   float* part;            // [chunk][2][J]; null: no sums
   int64_t dy_s, I, J, J8, chunk;
-  int32_t pf32, wide, z16;
+  int32_t pf32, z16;
 };
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) v = fmaxf(v, __shfl_xor(v, i));
-  return v;
-}
-
-__global__ __launch_bounds__(1024) void linear_scale_kernel(const void* gate, int pf32, int64_t J, float* scale) {
-  __shared__ float top[16];
+// The power of two that makes the gate's largest finite value one to two, formed by a workgroup.
+__device__ __forceinline__ float gate_scale(const void* gate, int pf32, int64_t J, float* top) {
   float m = 0.f;
-  for (int64_t j = threadIdx.x; j < J; j += 1024) {
+  for (int64_t j = threadIdx.x; j < J; j += 256) {
     const float x = fabsf(pf32 ? static_cast<const float*>(gate)[j] : (float)static_cast<const _Float16*>(gate)[j]);
     m = x < INFINITY ? fmaxf(m, x) : m;
   }
-  m = wave_max(m);
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
   if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
   __syncthreads();
-  if (threadIdx.x > 0) return;
-  for (int i = 1; i < 16; ++i) m = fmaxf(m, top[i]);
+  m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   int e = 0;
   if (m > 0.f) frexpf(m, &e);                  // m = [0.5, 1) 2^e
-  e = min(max(e - 1, -100), 100);
-  scale[0] = ldexpf(1.0f, -e);
-  scale[1] = ldexpf(1.0f, e);
+  return ldexpf(1.0f, -min(max(e - 1, -100), 100));
 }
 
-// 512 columns (eight a lane) of `chunk` rows a workgroup, a wave every fourth row.
-template <int ACT, bool F16>
+// 512 columns (eight a lane: side by side where they come in aligned groups (WIDE), else each 64
+// from the next, so that a wave's loads lie together) of `chunk` rows a workgroup, a wave every
+// fourth row.
+template <int ACT, bool F16, bool WIDE, bool GATE>
 __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
   __shared__ __attribute__((aligned(16))) float red[4][2][512];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t j = (int64_t)blockIdx.x * 512 + lane * 8, i0 = blockIdx.y * a.chunk;
+  constexpr int STEP = WIDE ? 1 : 64;
+  const int64_t j = (int64_t)blockIdx.x * 512 + (WIDE ? lane * 8 : lane), i0 = blockIdx.y * a.chunk;
   const int64_t i1 = i0 + a.chunk < a.I ? i0 + a.chunk : a.I;
-  const int n = a.J - j >= 8 ? 8 : a.J > j ? (int)(a.J - j) : 0;
+  float scale = 1.f;
+  if (F16 && a.scale) {
+    scale = gate_scale(a.gate, a.pf32, a.J, &red[0][0][0]);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.scale = 1.0f / scale;
+  }
   float g[8], db[8], dg[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     g[e] = 1.f;
+    if (GATE && j + e * STEP < a.J)
+      g[e] = a.pf32 ? static_cast<const float*>(a.gate)[j + e * STEP] : half_to_f32<F16>(static_cast<const __bf16*>(a.gate)[j + e * STEP]);
     db[e] = dg[e] = 0.f;
   }
-  const bool wide = a.wide && n == 8;
-  if (a.gate) param8<F16>(a.gate, a.pf32, wide, j, n, g);
-  const float scale = a.scale ? *a.scale : 1.f;
-  if (n > 0)
+  if (j < a.J8)
     for (int64_t i = i0 + wave; i < i1; i += 4) {
       float dy[8], z[8], out[8];
-      param8<F16>(static_cast<const uint16_t*>(a.dy) + i * a.dy_s, 0, wide, j, n, dy);
-      if (a.z) {
-        if (a.z16) param8<true>(static_cast<const uint16_t*>(a.z) + i * a.J, 0, wide, j, n, z);
-        else param8<true>(static_cast<const float*>(a.z) + i * a.J, 1, wide, j, n, z);
+      const __bf16* DY = static_cast<const __bf16*>(a.dy) + i * a.dy_s + j;
+      if constexpr (WIDE) {
+        param8<F16>(DY, 0, 1, 0, 8, dy);
+        if (a.z && a.z16) param8<true>(static_cast<const uint16_t*>(a.z) + i * a.J + j, 0, 1, 0, 8, z);
+        else if (a.z) param8<true>(static_cast<const float*>(a.z) + i * a.J + j, 1, 1, 0, 8, z);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool in = j + e * 64 < a.J;
+          dy[e] = in ? half_to_f32<F16>(DY[e * 64]) : 0.f;
+          z[e] = 0.f;
+          if (!a.z || !in) continue;
+          z[e] = a.z16 ? half_to_f32<true>(static_cast<const __bf16*>(a.z)[i * a.J + j + e * 64])
+                       : static_cast<const float*>(a.z)[i * a.J + j + e * 64];
+        }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float slope = 1.f;
-        if (ACT != kActNone || a.z) {
+        if (ACT != kActNone || (GATE && a.z)) {
           const float v = act_both<ACT>(z[e], slope);
-          dg[e] = __builtin_fmaf(dy[e], v, dg[e]);
+          if (GATE) dg[e] = __builtin_fmaf(dy[e], v, dg[e]);
         }
         const float d = ACT != kActNone ? dy[e] * slope : dy[e];
-        db[e] = a.gate ? __builtin_fmaf(d, g[e], db[e]) : db[e] + d;
-        out[e] = a.gate ? d * (g[e] * scale) : d;
+        db[e] = GATE ? __builtin_fmaf(d, g[e], db[e]) : db[e] + d;
+        out[e] = GATE ? d * (g[e] * scale) : d;
       }
       if (!a.dz) continue;
-      bf16x8 y;
+      __bf16* DZ = static_cast<__bf16*>(a.dz) + i * a.J8 + j;
+      if constexpr (WIDE) {
+        bf16x8 y;
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const bf16x2 w = pack2<F16>(out[e], out[e + 1]);
-        y[e] = e < n ? w[0] : (__bf16)0.f;
-        y[e + 1] = e + 1 < n ? w[1] : (__bf16)0.f;
+        for (int e = 0; e < 8; e += 2) {
+          const bf16x2 w = pack2<F16>(out[e], out[e + 1]);
+          y[e] = w[0];
+          y[e + 1] = w[1];
+        }
+        *reinterpret_cast<bf16x8*>(DZ) = y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (j + e * 64 < a.J8) DZ[e * 64] = j + e * 64 < a.J ? f32_to_half<F16>(out[e]) : (__bf16)0.f;
       }
-      *reinterpret_cast<bf16x8*>(static_cast<uint16_t*>(a.dz) + i * a.J8 + j) = y;
     }
   if (!a.part) return;
+  if (F16) __syncthreads();                    // the gate's maximum is read
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    red[wave][0][lane * 8 + e] = db[e];
-    red[wave][1][lane * 8 + e] = dg[e];
+    const int at = WIDE ? lane * 8 + e : lane + e * 64;
+    red[wave][0][at] = db[e];
+    red[wave][1][at] = dg[e];
   }
   __syncthreads();
   for (int c = threadIdx.x; c < 1024; c += 256) {
@@ -132,20 +150,22 @@ __global__ __launch_bounds__(1024) void linear_cols_kernel(const float* part, in
   }
 }
 
-// Rows of a workgroup of the pass over dy: 1,024 workgroups in all, 16 rows at least.
+// Rows of a workgroup of the pass over dy: 1,024 workgroups in all, 8 rows at least.
 int64_t dz_chunk(int64_t I, int64_t J) {
   const int64_t cols = (J + 511) / 512, rows = std::max<int64_t>(1, 1024 / cols);
-  return std::max<int64_t>(16, (I + rows - 1) / rows);
+  return std::max<int64_t>(8, (I + rows - 1) / rows);
 }
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
 struct BwdPlan {
   GemmPlan x, w;
+  Laid laid;
   int64_t chunk, chunks, J8;
-  size_t dz, part, scale, split, bytes;        // where each begins
+  size_t part, scale, split, lay, bytes;       // where each begins, dz at 0
 };
-BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, bool dz, bool sums, bool dx, bool dw) {
+BwdPlan bwd_plan(const gpa_linear_gate_args* a, bool dz, bool sums, bool dx, bool dw) {
   BwdPlan p{};
+  const int64_t M = a->M, N = a->N, K = std::max<int64_t>(a->K, 1);
   p.J8 = (N + 7) / 8 * 8;
   p.chunk = dz_chunk(M, N);
   p.chunks = (M + p.chunk - 1) / p.chunk;
@@ -154,27 +174,34 @@ BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, bool dz, bool sums, bool dx, b
   p.scale = dz ? (size_t)round16(M * p.J8 * 2) : 0;
   p.part = p.scale + 16;
   p.split = p.part + (sums ? (size_t)round16(p.chunks * 2 * N * 4) : 0);
-  p.bytes = p.split + std::max(p.x.bytes, p.w.bytes);
+  p.laid = linear_laid(a, dw, dx);
+  p.lay = p.split + round16(std::max(p.x.bytes, p.w.bytes));
+  p.bytes = p.lay + p.laid.bytes;
   return p;
 }
 
 }  // namespace
 
-int linear_check(const char* fn, int dtype, int pdtype, const gpa_linear_gate_args* a);
-bool linear_launchable(const GemmPlan& x, int64_t I, int64_t J);
-
 namespace {
 
-template <bool F16>
-hipError_t dz_launch(const DzArgs& d, int act, dim3 grid, hipStream_t s) {
+template <bool F16, bool WIDE, bool GATE>
+void dz_go(const DzArgs& d, int act, dim3 grid, hipStream_t s) {
   const dim3 block(256);
   switch (act) {
-    case kActGelu: hipLaunchKernelGGL((linear_dz_kernel<kActGelu, F16>), grid, block, 0, s, d); break;
-    case kActGeluTanh: hipLaunchKernelGGL((linear_dz_kernel<kActGeluTanh, F16>), grid, block, 0, s, d); break;
-    case kActSilu: hipLaunchKernelGGL((linear_dz_kernel<kActSilu, F16>), grid, block, 0, s, d); break;
-    case kActRelu: hipLaunchKernelGGL((linear_dz_kernel<kActRelu, F16>), grid, block, 0, s, d); break;
-    default: hipLaunchKernelGGL((linear_dz_kernel<kActNone, F16>), grid, block, 0, s, d); break;
+    case kActGelu: hipLaunchKernelGGL((linear_dz_kernel<kActGelu, F16, WIDE, GATE>), grid, block, 0, s, d); break;
+    case kActGeluTanh: hipLaunchKernelGGL((linear_dz_kernel<kActGeluTanh, F16, WIDE, GATE>), grid, block, 0, s, d); break;
+    case kActSilu: hipLaunchKernelGGL((linear_dz_kernel<kActSilu, F16, WIDE, GATE>), grid, block, 0, s, d); break;
+    case kActRelu: hipLaunchKernelGGL((linear_dz_kernel<kActRelu, F16, WIDE, GATE>), grid, block, 0, s, d); break;
+    default: hipLaunchKernelGGL((linear_dz_kernel<kActNone, F16, WIDE, GATE>), grid, block, 0, s, d); break;
   }
+}
+template <bool F16, bool WIDE>
+void dz_gate(const DzArgs& d, int act, dim3 grid, hipStream_t s) {
+  d.gate ? dz_go<F16, WIDE, true>(d, act, grid, s) : dz_go<F16, WIDE, false>(d, act, grid, s);
+}
+hipError_t dz_launch(const DzArgs& d, int act, bool f16, bool wide, dim3 grid, hipStream_t s) {
+  if (f16) wide ? dz_gate<true, true>(d, act, grid, s) : dz_gate<true, false>(d, act, grid, s);
+  else wide ? dz_gate<false, true>(d, act, grid, s) : dz_gate<false, false>(d, act, grid, s);
   return hipGetLastError();
 }
 
@@ -190,8 +217,8 @@ static bool needs_dz(const gpa_linear_gate_args* a, const gpa_linear_gate_grads*
 }
 
 extern "C" size_t gpa_linear_gate_bwd_workspace_bytes(const gpa_linear_gate_args* a, const gpa_linear_gate_grads* g) {
-  if (!a || !g || a->M <= 0 || a->N <= 0 || a->K <= 0) return 0;
-  return bwd_plan(a->M, a->N, g->K_out, needs_dz(a, g), g->dbias || g->dgate, g->dx, g->dw).bytes;
+  if (!a || !g || a->M <= 0 || a->N <= 0 || a->K < 0) return 0;
+  return bwd_plan(a, needs_dz(a, g), g->dbias || g->dgate, g->dx, g->dw).bytes;
 }
 
 extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_gate_args* a, const gpa_linear_gate_grads* g,
@@ -214,8 +241,8 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
     gpa_set_error("%s: dy is needed, z with an activation or the gate's gradient, and there is none of an absent gate", fn);
     return GPA_E_INVALID;
   }
-  if (g->K_out < 1 || g->K_out > a->K || a->K - g->K_out >= 8) {
-    gpa_set_error("%s: %lld columns of gradients for K = %lld", fn, (long long)g->K_out, (long long)a->K);
+  if ((g->dx || g->dw) && a->K == 0) {
+    gpa_set_error("%s: no feature, so there are no gradients of x and w", fn);
     return GPA_E_INVALID;
   }
   if (a->N >= (int64_t)1 << 21) {
@@ -223,8 +250,8 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
     return GPA_E_UNSUPPORTED;
   }
   const bool f16 = dtype == GPA_DTYPE_F16, need_dz = needs_dz(a, g), sums = g->dbias || g->dgate;
-  const BwdPlan p = bwd_plan(a->M, a->N, g->K_out, need_dz, sums, g->dx, g->dw);
-  if ((g->dx && !linear_launchable(p.x, a->M, g->K_out)) || (g->dw && !linear_launchable(p.w, a->N, g->K_out))) {
+  const BwdPlan p = bwd_plan(a, need_dz, sums, g->dx, g->dw);
+  if ((g->dx && !linear_launchable(p.x, a->M, a->K)) || (g->dw && !linear_launchable(p.w, a->N, a->K))) {
     gpa_set_error("%s: problem exceeds the grid limit", fn);
     return GPA_E_UNSUPPORTED;
   }
@@ -235,11 +262,8 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
   char* ws = (char*)workspace;
   const hipStream_t s = (hipStream_t)stream;
   float* const scale = need_dz && f16 && a->gate ? (float*)(ws + p.scale) : nullptr;
-  hipError_t e = hipSuccess;
-  if (scale) {
-    hipLaunchKernelGGL(linear_scale_kernel, dim3(1), dim3(1024), 0, s, a->gate, (int)(param_dtype == GPA_DTYPE_F32), a->N, scale);
-    e = hipGetLastError();
-  }
+  Matrix x, w;
+  hipError_t e = linear_lay(a, p.laid, ws + p.lay, x, w, s);
   if (e == hipSuccess && (need_dz || sums)) {
     DzArgs d{};
     d.dy = g->dy; d.dy_s = a->M > 1 ? g->dy_s : 0;
@@ -248,9 +272,9 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
     d.part = sums ? (float*)(ws + p.part) : nullptr;
     d.I = a->M; d.J = a->N; d.J8 = p.J8; d.chunk = p.chunk;
     d.pf32 = param_dtype == GPA_DTYPE_F32;
-    d.wide = a->N % 8 == 0 && (uintptr_t)g->dy % 16 == 0 && d.dy_s % 8 == 0 && (uintptr_t)a->gate % 16 == 0;
+    const bool wide = a->N % 8 == 0 && (uintptr_t)g->dy % 16 == 0 && d.dy_s % 8 == 0;
     const dim3 grid((unsigned)((a->N + 511) / 512), (unsigned)p.chunks);
-    e = f16 ? dz_launch<true>(d, a->act, grid, s) : dz_launch<false>(d, a->act, grid, s);
+    e = dz_launch(d, a->act, f16, wide, grid, s);
     if (e == hipSuccess && sums) {
       const dim3 cols((unsigned)((a->N + 63) / 64), 2);
       auto go = [&](auto type) {
@@ -266,23 +290,23 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
   const Operand dz_rows{need_dz ? (const uint16_t*)ws : (const uint16_t*)g->dy, need_dz ? p.J8 : a->M > 1 ? g->dy_s : p.J8, a->M, p.J8};
   auto fine = [](const void* q, int64_t n, int64_t st) { return (uintptr_t)q % 16 == 0 && (n < 2 || st % 8 == 0); };
   GemmArgs m{};
-  m.out.unscale = scale ? scale + 1 : nullptr;
+  m.out.unscale = scale;
   m.out.part = (float*)(ws + p.split);
-  m.out.J = g->K_out;
+  m.out.J = a->K;
   if (e == hipSuccess && g->dx) {              // over the output features: w turned
-    m.P = Operand{(const uint16_t*)a->w, a->N > 1 ? a->w_s : a->K, a->N, a->K};
+    m.P = Operand{w.p, w.stride, a->N, p.laid.K};
     m.Q = dz_rows;
     m.nk = (int32_t)((p.J8 + 31) / 32);
     m.out.out = g->dx; m.out.out_s = g->dx_s; m.out.I = a->M;
-    m.out.wide = g->K_out % 8 == 0 && fine(g->dx, a->M, g->dx_s);
+    m.out.wide = a->K % 8 == 0 && fine(g->dx, a->M, g->dx_s);
     e = f16 ? gemm<true, false, true>(m, p.x, s) : gemm<true, false, false>(m, p.x, s);
   }
   if (e == hipSuccess && g->dw) {              // over the rows: both turned
-    m.P = Operand{(const uint16_t*)a->x, a->M > 1 ? a->x_s : a->K, a->M, a->K};
+    m.P = Operand{x.p, x.stride, a->M, p.laid.K};
     m.Q = dz_rows;
     m.nk = (int32_t)((a->M + 31) / 32);
     m.out.out = g->dw; m.out.out_s = g->dw_s; m.out.I = a->N;
-    m.out.wide = g->K_out % 8 == 0 && fine(g->dw, a->N, g->dw_s);
+    m.out.wide = a->K % 8 == 0 && fine(g->dw, a->N, g->dw_s);
     e = f16 ? gemm<true, true, true>(m, p.w, s) : gemm<true, true, false>(m, p.w, s);
   }
   if (e != hipSuccess) {

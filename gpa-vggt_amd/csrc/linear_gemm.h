@@ -302,15 +302,38 @@ __global__ __launch_bounds__(256, PER_CU) void linear_gemm_kernel(GemmArgs a) {
       v[4 + e] = hi[e];
     }
   };
-  if (!a.out.wide || a.splits > 1) {
+  if (a.splits > 1) {
+#pragma unroll
+    for (int h = 0; h < WI; h += 2) {
+      down(h);
+#pragma unroll 2
+      for (int it = 0; it < WJ; ++it) {
+        float v[8];
+        up(it, v);
+        part8(a.out, i0 + h * 16 + it * RP + r0, j, split, v);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    return;
+  }
+  // Columns that do not come in aligned groups of eight: a lane has one column of eight rows at a
+  // time, so that what a wave loads and stores at once lies together.
+  if (!a.out.wide) {
+    constexpr int W = WJ * 16 < 64 ? WJ * 16 : 64, DOWN = 64 / W;   // columns and rows of 64 lanes
 #pragma unroll
     for (int h = 0; h < WI; h += 2) {
       down(h);
 #pragma unroll 1
-      for (int it = 0; it < WJ; ++it) {
+      for (int it = 0; it < 32 / DOWN / 8 * (WJ * 16 / W); ++it) {
+        const int c = it % (WJ * 16 / W) * W + lane % W, first = it / (WJ * 16 / W) * 8 * DOWN + lane / W;
         float v[8];
-        up(it, v);
-        finish8<F16>(a.out, i0 + h * 16 + it * RP + r0, j, split, a.splits, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int row = first + e * DOWN, r = row & 15;
+          const lds8 from = row >> 4 ? to[1] : to[0];
+          v[e] = *(__attribute__((address_space(3))) float*)(from + (r * CH + ((c >> 2) ^ (r & MASK))) * 16 + (c & 3) * 4);
+        }
+        finish_down<F16, DOWN>(a.out, i0 + h * 16 + first, j0 + c, v);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
@@ -408,7 +431,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(Finish f, int splits) 
       v[4 + e] += hi[e];
     }
   }
-  finish8<F16>(f, i, j, 0, 1, v);
+  finish8<F16>(f, i, j, v);
 }
 
 template <int WI, int WJ, int R, int PER_CU, bool PT, bool QT, bool F16>

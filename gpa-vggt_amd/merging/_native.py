@@ -165,7 +165,7 @@ _TreeArgs = _struct("_TreeArgs", (
 
 # gpa_linear_gate_args and gpa_linear_gate_grads.
 _LinearArgs = _struct("_LinearArgs", ("p: x w bias gate residual", "l: M N K x_s w_s residual_s", "i: act"))
-_LinearGrads = _struct("_LinearGrads", ("p: dy z dx dw dbias dgate", "l: dy_s dx_s dw_s K_out", "i: z_dtype"))
+_LinearGrads = _struct("_LinearGrads", ("p: dy z dx dw dbias dgate", "l: dy_s dx_s dw_s", "i: z_dtype"))
 
 # gpa_head_rotary_args and gpa_head_rotary_grads.
 MAX_AXES = 8
@@ -302,7 +302,7 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.gpa_norm_gate_bwd.argtypes = [ctypes.c_int, ctypes.c_int, _vp,
                                       _vp, _vp, ctypes.c_size_t, _vp]
     lib.gpa_linear_gate_workspace_bytes.restype = ctypes.c_size_t
-    lib.gpa_linear_gate_workspace_bytes.argtypes = [_i64] * 3
+    lib.gpa_linear_gate_workspace_bytes.argtypes = [_vp]
     lib.gpa_linear_gate.restype = ctypes.c_int
     lib.gpa_linear_gate.argtypes = [ctypes.c_int, ctypes.c_int, _vp, _vp, _i64, _vp, ctypes.c_int, _vp, ctypes.c_size_t,
                                     _vp]
@@ -1920,15 +1920,9 @@ def _linear_check(what, x, w, bias, gate, residual, act):
     return given[0][1].dtype if given else x.dtype
 
 
-def _rows_of_8(t):
-    """t [R, C] of 16-bit values with C a multiple of 8 and rows that are 16-byte
-    aligned and do not overlap, padded with zero columns where it has no such form."""
-    R, C = t.shape
-    if C % 8 == 0 and C and _rows_ok(t, 8) and (R < 2 or 0 <= t.stride(0) < 1 << 21):
-        return t
-    new = t.new_zeros(R, max(8, -(-C // 8) * 8)) if C % 8 or not C else t.new_empty(R, C)
-    new[:, :C].copy_(t)
-    return new
+def _feature_rows(t):
+    """t [R, C], or a copy, with contiguous features."""
+    return t if t.stride(1) == 1 or t.shape[1] < 2 else t.contiguous()
 
 
 def _linear_args(x, w, bias, gate, residual, act):
@@ -1976,15 +1970,15 @@ def linear_gate(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
     z = torch.empty((M, N) if want_z else (0,), device=dev, dtype=_z_dtype(x, gate))
     if M == 0 or N == 0:
         return y, z
-    x, w = _rows_of_8(x), _rows_of_8(w)
+    x, w, residual = _feature_rows(x), _feature_rows(w), None if residual is None else _feature_rows(residual)
     bias, gate = (None if t is None else t.contiguous() for t in (bias, gate))
-    residual = residual if residual is None or residual.stride(1) == 1 or N == 1 else residual.contiguous()
+    a = _linear_args(x, w, bias, gate, residual, act)
     L = lib()
-    ws_bytes = L.gpa_linear_gate_workspace_bytes(M, N, x.shape[1])
+    ws_bytes = L.gpa_linear_gate_workspace_bytes(a)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
     with _on(dev):
-        rc = L.gpa_linear_gate(_DTYPE_CODES[x.dtype], _DTYPE_CODES[pdt], _linear_args(x, w, bias, gate, residual, act),
-                               y.data_ptr(), N, z.data_ptr() if want_z else None, _DTYPE_CODES[z.dtype],
+        rc = L.gpa_linear_gate(_DTYPE_CODES[x.dtype], _DTYPE_CODES[pdt], a, y.data_ptr(), N,
+                               z.data_ptr() if want_z else None, _DTYPE_CODES[z.dtype],
                                None if ws is None else ws.data_ptr(), ws_bytes, _stream(dev))
     _check(rc, what)
     return y, z
@@ -2023,13 +2017,12 @@ def linear_gate_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: torch.Tensor
         dx.zero_(), dw.zero_()
         if M == 0 or N == 0 or not (want_bias or want_gate):
             return dx, dw, db.zero_(), dg.zero_()
-    x, w = _rows_of_8(x), _rows_of_8(w)
+    x, w, dy = _feature_rows(x), _feature_rows(w), _feature_rows(dy)
     gate = None if gate is None else gate.contiguous()
-    dy = dy if dy.stride(1) == 1 or N == 1 else dy.contiguous()
     ptr = lambda t: t.data_ptr() if t.numel() else 0  # noqa: E731
     a = _linear_args(x, w, None, gate, None, act)
     g = _LinearGrads.packed(dy.data_ptr(), 0 if z is None else z.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(dg), dy.stride(0),
-                            K, K, max(K, 1), 0 if z is None else _DTYPE_CODES[z.dtype])
+                            K, K, 0 if z is None else _DTYPE_CODES[z.dtype])
     L = lib()
     ws_bytes = L.gpa_linear_gate_bwd_workspace_bytes(a, g)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)

@@ -32,8 +32,8 @@ def linear_gate_residual(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
     the result everything is fp32; it is rounded once.  Returns [..., N]; differentiable in all
     tensors (dz, the gradient before the activation, is rounded to x's type for its two products).
 
-    A product over a K that is no multiple of 8, or over rows that are not 16-byte
-    aligned, works on padded copies of x and weight.
+    Where K is no multiple of 8, or rows are not 16-byte aligned, x and weight are first
+    copied into padded rows.
     """
     what = "linear_gate_residual"
     if activation not in _ACTS:

@@ -713,8 +713,8 @@ int gpa_attn_tree(int dtype, const gpa_attn_tree_args* args, void* workspace, si
  *   z = x w^T + bias;  y = residual + gate act(z)
  * bias and gate [N] (of dtype or fp32) and residual [M, N] (dtype) may be NULL.  act:
  * GPA_ACT_*.  fp32 inside (GELU's distribution is off by 8e-8 absolutely), y rounded once.
- * K a multiple of 8 (pad with zeros), rows of x and w 16-byte aligned, of
- * strides below 2^21.  z (NULL: not kept): [M, N] contiguous, 16-byte aligned, z_dtype
+ * K that is no multiple of 8, rows of x or w that are not 16-byte aligned, and strides of
+ * 2^21 or more cost padded copies in the workspace.  z (NULL: not kept): [M, N] contiguous, 16-byte aligned, z_dtype
  * fp32 or fp16 (the nearest value, beyond the range infinite), for the backward, which
  * needs it with an activation or for the gate's gradient.
  * workspace: gpa_linear_gate_workspace_bytes(...), 16-byte aligned.
@@ -727,19 +727,18 @@ typedef struct gpa_linear_gate_args {
   int32_t act;
 } gpa_linear_gate_args;
 
-size_t gpa_linear_gate_workspace_bytes(int64_t M, int64_t N, int64_t K);
+size_t gpa_linear_gate_workspace_bytes(const gpa_linear_gate_args* args);
 int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate_args* args, void* y, int64_t y_s,
                     void* z, int z_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Its gradients from y's, dy (any row stride): dx [M, K_out] and dw [N, K_out] in dtype, where
- * K_out of K features are there (the others pad to a multiple of 8), dbias and dgate [N] in
- * param_dtype, each NULL where it is not wanted; the residual's is dy.  Sums run in a
+/* Its gradients from y's, dy (any row stride): dx [M, K] and dw [N, K] in dtype, dbias and
+ * dgate [N] in param_dtype, each NULL where it is not wanted; the residual's is dy.  Sums run in a
  * fixed order.  N below 2^21.  workspace: gpa_linear_gate_bwd_workspace_bytes of the
  * same arguments, 16-byte aligned. */
 typedef struct gpa_linear_gate_grads {
   const void *dy, *z;
   void *dx, *dw, *dbias, *dgate;
-  int64_t dy_s, dx_s, dw_s, K_out;
+  int64_t dy_s, dx_s, dw_s;
   int32_t z_dtype;
 } gpa_linear_gate_grads;
 

@@ -25,10 +25,8 @@ def _args(**kw):
 
 COMMON = [
     (dict(dtype=0), INV), (dict(dtype=3), INV), (dict(dtype=1, pdtype=2), INV), (dict(dtype=2, pdtype=1), INV), (dict(M=-1), INV),
-    (dict(N=-1), INV), (dict(K=-8), INV), (dict(act=-1), INV), (dict(act=5), INV), (dict(K=0), INV), (dict(K=12), INV),
-    (dict(x=None), INV), (dict(w=None), INV), (dict(x=FAKE + 8), INV), (dict(w=FAKE + 2), INV), (dict(x_s=132), INV), (dict(w_s=4), INV),
-    (dict(x_s=1 << 21), UNS), (dict(w_s=1 << 21), UNS), (dict(x_s=-128), UNS), (dict(M=1 << 30), UNS), (dict(N=1 << 30), UNS),
-    (dict(K=1 << 21), UNS),
+    (dict(N=-1), INV), (dict(K=-8), INV), (dict(act=-1), INV), (dict(act=5), INV), (dict(x=None), INV), (dict(w=None), INV),
+    (dict(M=1 << 30), UNS), (dict(N=1 << 30), UNS), (dict(K=1 << 21), UNS),
 ]
 
 
@@ -40,26 +38,35 @@ def test_forward_argument_errors(kw, code):
     assert rc == code and _native.lib().gpa_last_error()
 
 
-def test_forward_workspace_errors():
-    """A product whose sum is cut needs room for the parts."""
-    L, a = _native.lib(), _args(M=70, N=70, K=8000, x_s=8000, w_s=8000)
-    need = L.gpa_linear_gate_workspace_bytes(70, 70, 8000)
-    assert need >= 2 * 70 * 72 * 4
+@pytest.mark.parametrize("kw,least", [
+    (dict(M=70, N=70, K=80_000, x_s=80_000, w_s=80_000), 2 * 70 * 72 * 4),      # a sum that is cut has parts
+    (dict(K=127), (300 + 64) * 128 * 2), (dict(M=3, K=127), (3 + 64) * 128 * 2),  # padded copies of x and w
+    (dict(x=FAKE + 8), 300 * 128 * 2), (dict(w_s=130), 64 * 128 * 2), (dict(x_s=1 << 21), 300 * 128 * 2), (dict(w_s=-128), 64 * 128 * 2),
+    (dict(K=0), (300 + 64) * 8 * 2)])
+def test_forward_workspace(kw, least):
+    L, a = _native.lib(), _args(**kw)
+    need = L.gpa_linear_gate_workspace_bytes(ctypes.byref(a))
+    assert need >= least
     for ws, size in ((None, need), (FAKE, need - 1), (FAKE + 8, need)):
         assert L.gpa_linear_gate(1, 1, ctypes.byref(a), FAKE, 70, None, 0, ws, size, None) == WSP
-    assert L.gpa_linear_gate_workspace_bytes(64, 70, 8000) == L.gpa_linear_gate_workspace_bytes(0, 70, 8000) == 0
+
+
+def test_calls_without_a_workspace():
+    L = _native.lib()
+    for kw in (dict(M=16), dict(M=1, x_s=3), dict(M=0), dict(N=0), dict(M=-1)):
+        assert L.gpa_linear_gate_workspace_bytes(ctypes.byref(_args(**kw))) == 0
+    assert L.gpa_linear_gate_workspace_bytes(None) == 0
 
 
 @pytest.mark.parametrize("kw,code", COMMON + [
     (dict(g=dict(dy=None)), INV), (dict(g=dict(z=None)), INV), (dict(act=0, g=dict(z=None)), INV), (dict(gate=None), INV),
-    (dict(g=dict(z=FAKE + 4)), INV), (dict(g=dict(z_dtype=1)), INV), (dict(g=dict(K_out=0)), INV), (dict(g=dict(K_out=129)), INV), (dict(g=dict(K_out=120)), INV),
+    (dict(g=dict(z=FAKE + 4)), INV), (dict(g=dict(z_dtype=1)), INV), (dict(K=0), INV),
     (dict(M=0), INV), (dict(N=0), INV), (dict(N=1 << 21), UNS), (dict(ws=None), WSP), (dict(ws_bytes=64), WSP), (dict(ws=FAKE + 8), WSP),
 ])
 def test_backward_argument_errors(kw, code):
     kw = dict(kw)
     dt, pdt, ws, ws_bytes = kw.pop("dtype", 1), kw.pop("pdtype", None), kw.pop("ws", FAKE), kw.pop("ws_bytes", 1 << 40)
-    g = _fields(_native._LinearGrads, dict(dy=FAKE, z=FAKE, dx=FAKE, dw=FAKE, dbias=FAKE, dgate=FAKE, dy_s=64, dx_s=128, dw_s=128,
-                                           K_out=128), kw.pop("g", {}))
+    g = _fields(_native._LinearGrads, dict(dy=FAKE, z=FAKE, dx=FAKE, dw=FAKE, dbias=FAKE, dgate=FAKE, dy_s=64, dx_s=128, dw_s=128), kw.pop("g", {}))
     rc = _native.lib().gpa_linear_gate_bwd(dt, dt if pdt is None else pdt, ctypes.byref(_args(**kw)), ctypes.byref(g), ws, ws_bytes, None)
     assert rc == code and _native.lib().gpa_last_error()
 
@@ -99,13 +106,3 @@ def test_op_refusals(kw, match):
     a = {**dict(x=X, w=W, bias=None, gate=None, residual=None, act=0), **kw}
     with pytest.raises(ValueError, match=match):
         _native._linear_check("y", *a.values())
-
-
-@pytest.mark.parametrize("shape,begin", [((5, 16), 0), ((5, 16), 1), ((5, 13), 0), ((5, 0), 0), ((1, 3), 0), ((0, 16), 0)])
-def test_rows_of_8(shape, begin):
-    t = torch.arange(200.0).to(torch.bfloat16)[begin:begin + shape[0] * shape[1]].view(shape)
-    p = _native._rows_of_8(t)
-    assert p.shape[1] % 8 == 0 and p.shape[1] >= 8 and torch.equal(p[:, :shape[1]], t) and not p[:, shape[1]:].any()
-    assert _native._rows_ok(p, 8)
-    wide = torch.zeros(3, 1 << 21, dtype=torch.bfloat16)[:, :16]
-    assert _native._rows_of_8(wide).stride(0) == 16
