@@ -40,8 +40,12 @@ constexpr int kMaxD = 256;
 constexpr int kMaxChunks = 32;
 constexpr int kMaxTokens = 16;            // of a workgroup's tile
 constexpr int kCsFloats = 4096;           // cosines and sines of a tile
-constexpr int64_t kFwdWgs = 2048;
-constexpr int64_t kBwdWgs = 1024;
+// Workgroups: what 256 CUs hold at once, each walking its tiles with the next rows' loads in flight
+// (four to a CU forward; as many as tiles took 77 us for 71 at 16,384 tokens of 32 + 8 heads of
+// 128, and 38 for 28 at 10,992 of 16 + 16 of 64).
+constexpr int64_t kFwdWgs = 1024;
+constexpr int64_t kBwdWgs = 1024;        // three to a CU, 768, with a bias's sums or in fp32 (video: 51 us on 1,024, 41)
+
 
 // Eight pairs of a head: their features begin at o0 and o1 (neighbours: all at
 // o0), the first pair's number (-1: they are not turned), how many there are.
@@ -67,7 +71,7 @@ struct RotArgs {
   int64_t N, tokens, tiles;
   uint32_t rows_magic;    // 2^32 / heads of a row's tensors, rounded up (one head: not used)
   uint32_t n_magic;       // 2^32 / N, rounded up (N == 1: not used)
-  int32_t D, pairs, count, pos_kind, chunks, lanes, per_tile, norm, pf32;
+  int32_t D, pairs, count, pos_kind, chunks, lanes, per_tile, norm, pf32, bias;
   float eps, inv_d;
   Chunk chunk[kMaxChunks];
 };
@@ -297,7 +301,7 @@ struct Walk {
 };
 
 template <typename T, int V, bool INTER>
-__global__ __launch_bounds__(kThreads) void head_rotary_kernel(RotArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void head_rotary_kernel(RotArgs a) {
   constexpr int U = sizeof(T) == 4 ? 1 : 2;    // rows a lane has in flight, twice
   __shared__ __attribute__((aligned(16))) float cs[kCsFloats];    // [token][chunk][cos 8, sin 8]
   __shared__ __attribute__((aligned(16))) float par[2][2][kMaxChunks * 16];
@@ -402,7 +406,9 @@ __global__ __launch_bounds__(kThreads) void head_rotary_kernel(RotArgs a) {
   }
 }
 
-template <typename T, int V, bool INTER>
+// BIAS: a bias's gradient is wanted (its sums take 16 registers, with which a CU holds three
+// workgroups instead of four).
+template <typename T, int V, bool INTER, bool BIAS>
 __global__ __launch_bounds__(kThreads) void head_rotary_bwd_kernel(RotArgs a) {
   __shared__ __attribute__((aligned(16))) float cs[kCsFloats];
   const Lane l = lane_of(a);
@@ -474,8 +480,10 @@ __global__ __launch_bounds__(kThreads) void head_rotary_bwd_kernel(RotArgs a) {
         if (cur.fine) {
           dwa[i] = __builtin_fmaf(ga[i], x[i], dwa[i]);
           dwb[i] = __builtin_fmaf(gb[i], y[i], dwb[i]);
-          dba[i] += ga[i];
-          dbb[i] += gb[i];
+          if (BIAS) {
+            dba[i] += ga[i];
+            dbb[i] += gb[i];
+          }
         }
         ga[i] *= wa[i];
         gb[i] *= wb[i];
@@ -540,7 +548,7 @@ __global__ __launch_bounds__(1024) void head_rotary_sum_kernel(SumArgs a) {
   if (!out) return;
   float s = 0.f;
   if (c < a.D)
-#pragma unroll 4
+#pragma unroll 16
     for (int i = wave; i < a.wgs[side]; i += 16) s += a.part[side][((int64_t)i * 2 + k) * a.D + c];
   tot[wave][lane] = s;
   __syncthreads();
@@ -683,18 +691,34 @@ int fill(const gpa_head_rotary_args* a, int dtype, int pdtype, std::initializer_
   return vec ? 8 : two ? 2 : 1;
 }
 
-// Tokens of a workgroup's tile: what its angles' LDS holds, unless that leaves CUs idle.
-int tile_tokens(const RotArgs& r, int64_t wgs) {
-  const int64_t n = std::min<int64_t>({r.tokens / wgs, kMaxTokens, kCsFloats / (16 * std::max(r.chunks, 1))});
-  return (int)std::max<int64_t>(n, 1);
+// Tokens of a workgroup's tile.  Each has `heads` rows, `step` of them go at a time: of what the
+// angles' LDS holds and `wgs` workgroups leave to each, the number that leaves the fewest lanes idle
+// (5,476 tokens of 16 heads of 64 on 2,048 workgroups, 32 rows each where 128 go at a time: 15 us;
+// on 685, 128 each: 9.5).  Few tokens are spread over the chip.
+int tile_tokens(const RotArgs& r, int64_t heads, int64_t step, int64_t wgs) {
+  const int64_t most = std::min<int64_t>(kMaxTokens, kCsFloats / (16 * std::max(r.chunks, 1)));
+  const int64_t fill = std::min<int64_t>((step + heads - 1) / std::max<int64_t>(heads, 1), std::max<int64_t>(r.tokens / 256, 1));
+  const int64_t top = std::min(most, std::max((r.tokens + wgs - 1) / wgs, fill));
+  int64_t best = 1;
+  double least = 1e30;
+  for (int64_t n = 1; n <= top; ++n) {         // rounds a token; more tokens share a tile's ends
+    const double cost = (double)((n * heads + step - 1) / step) / n * (1.0 + 0.5 / n);
+    if (cost <= least) {
+      least = cost;
+      best = n;
+    }
+  }
+  return (int)best;
 }
 
 template <typename T, int V, bool BWD>
 hipError_t go(const RotArgs& r, bool inter, hipStream_t s) {
-  const dim3 grid((unsigned)(BWD ? r.side[0].wgs + r.side[1].wgs : std::min<int64_t>(r.tiles, 4 * kFwdWgs))), block(kThreads);
+  const dim3 grid((unsigned)(BWD ? r.side[0].wgs + r.side[1].wgs : std::min(r.tiles, kFwdWgs))), block(kThreads);
   if constexpr (BWD) {
-    if (inter) hipLaunchKernelGGL((head_rotary_bwd_kernel<T, V, true>), grid, block, 0, s, r);
-    else hipLaunchKernelGGL((head_rotary_bwd_kernel<T, V, false>), grid, block, 0, s, r);
+    if (inter && r.bias) hipLaunchKernelGGL((head_rotary_bwd_kernel<T, V, true, true>), grid, block, 0, s, r);
+    else if (inter) hipLaunchKernelGGL((head_rotary_bwd_kernel<T, V, true, false>), grid, block, 0, s, r);
+    else if (r.bias) hipLaunchKernelGGL((head_rotary_bwd_kernel<T, V, false, true>), grid, block, 0, s, r);
+    else hipLaunchKernelGGL((head_rotary_bwd_kernel<T, V, false, false>), grid, block, 0, s, r);
   } else {
     if (inter) hipLaunchKernelGGL((head_rotary_kernel<T, V, true>), grid, block, 0, s, r);
     else hipLaunchKernelGGL((head_rotary_kernel<T, V, false>), grid, block, 0, s, r);
@@ -718,11 +742,11 @@ int refuse_launch(const char* fn, hipError_t e) {
 
 // Workgroups of the backward's two sides, by their share of the heads; none has more than tiles.
 struct Wgs { int64_t q, k; };
-Wgs bwd_wgs(int64_t tokens, int64_t H, int64_t Hk, bool q, bool k) {
+Wgs bwd_wgs(int64_t tokens, int64_t H, int64_t Hk, bool q, bool k, int64_t total = kBwdWgs) {
   if (tokens <= 0) return {0, 0};
   const int64_t h = q ? H : 0, hk = k ? Hk : 0, all = std::max<int64_t>(h + hk, 1);
   auto share = [&](int64_t n) {
-    return n == 0 ? 0 : std::max<int64_t>(1, std::min(tokens, (kBwdWgs * n + all - 1) / all));
+    return n == 0 ? 0 : std::max<int64_t>(1, std::min(tokens, (total * n + all - 1) / all));
   };
   return {share(h), share(hk)};
 }
@@ -754,7 +778,7 @@ extern "C" int gpa_head_rotary(int dtype, int param_dtype, const gpa_head_rotary
   r.side[0].out = q_out; r.side[0].o_sb = qo_sb; r.side[0].o_sh = qo_sh; r.side[0].o_sn = qo_sn;
   r.side[1].out = k_out; r.side[1].o_sb = ko_sb; r.side[1].o_sh = ko_sh; r.side[1].o_sn = ko_sn;
   const int64_t both = a->H + a->Hk;
-  r.per_tile = tile_tokens(r, kFwdWgs);
+  r.per_tile = tile_tokens(r, both, (dtype == GPA_DTYPE_F32 ? 1 : 2) * (kThreads / r.lanes), kFwdWgs);
   r.tiles = (r.tokens + r.per_tile - 1) / r.per_tile;
   r.rows_magic = magic_of(both);
   return refuse_launch(fn, launch<false>(r, dtype, some, a->pairing == GPA_PAIRS_NEIGHBOURS, (hipStream_t)stream));
@@ -814,13 +838,14 @@ extern "C" int gpa_head_rotary_bwd(int dtype, int param_dtype, const gpa_head_ro
   k.dy = g->d_k_out; k.y_sb = g->dko_sb; k.y_sh = g->dko_sh; k.y_sn = g->dko_sn;
   q.out = g->dq; q.o_sb = g->dq_sb; q.o_sh = g->dq_sh; q.o_sn = g->dq_sn;
   k.out = g->dk; k.o_sb = g->dk_sb; k.o_sh = g->dk_sh; k.o_sn = g->dk_sn;
-  const Wgs w = bwd_wgs(r.tokens, a->H, a->Hk, hq, hk);
+  r.bias = g->dq_b || g->dk_b;
+  const Wgs w = bwd_wgs(r.tokens, a->H, a->Hk, hq, hk, r.bias || dtype == GPA_DTYPE_F32 ? kBwdWgs * 3 / 4 : kBwdWgs);
   q.wgs = (int32_t)w.q; k.wgs = (int32_t)w.k;
   if (sums) {
     q.part = g->dq_w || g->dq_b ? (float*)workspace : nullptr;
     k.part = g->dk_w || g->dk_b ? (float*)workspace + w.q * 2 * a->D : nullptr;
   }
-  r.per_tile = tile_tokens(r, std::max(w.q, w.k));
+  r.per_tile = tile_tokens(r, std::max(H, Hk), kThreads / r.lanes, std::max(w.q, w.k));
   r.tiles = (r.tokens + r.per_tile - 1) / r.per_tile;
   const hipStream_t s = (hipStream_t)stream;
   hipError_t e = launch<true>(r, dtype, some, a->pairing == GPA_PAIRS_NEIGHBOURS, s);
