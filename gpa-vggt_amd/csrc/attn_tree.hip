@@ -21,8 +21,8 @@
 //
 // Caches are of unequal length and known on the device alone.  Every workgroup adds
 // up the sequences' tiles and finds its own piece of one of them: pieces of at most S tiles, S so
-// that all together fill the chip once; a sequence in one piece writes its outputs itself,
-// the others' pieces are joined.  No list is made before, no order of arrival matters.
+// that all together fill the chip once (piece_tiles); a sequence in one piece writes its outputs
+// itself, the others' pieces are joined.  No list is made before, no order of arrival matters.
 #include "attn_masked.h"
 #include "attn_masked_rows.h"
 
@@ -40,7 +40,8 @@ struct TreeArgs {
   const uint32_t* seen;   // [B][T][words]
   int64_t seen_sb, seen_st;
   const int32_t* lens;    // nullable: all of the cache
-  int32_t T, words, R, blocks, target, join;
+  int32_t T, words, R, blocks, target, most;
+  int32_t* firsts;        // [B + 1]: a sequence's first piece, for the join (null: none)
 };
 
 struct Where { int b, z, count, first, tiles, len; };
@@ -52,22 +53,45 @@ __device__ __forceinline__ int cache_len(const TreeArgs& p, int b) {
 __device__ __forceinline__ int seq_tiles(const TreeArgs& p, int b) {
   return (cache_len(p, b) + kMTile - 1) / kMTile + (p.T + kMTile - 1) / kMTile;
 }
-// Tiles of a piece at most.  The pieces are no more than target where that is twice the
-// sequences or more (each sequence rounds up once).
+__device__ __forceinline__ int wave_sum(int v) {
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) v += __shfl_xor(v, i);
+  return __builtin_amdgcn_readfirstlane(v);
+}
+// Tiles of a piece at most.  With fewer sequences than `target` pieces to fill the chip with: the
+// least that gives no more than these (a sequence's last piece rounds up, so one even share is
+// seldom enough); otherwise the chip is full, and only sequences a quarter longer than the mean are
+// cut.  No sequence has more than `most` pieces.
 __device__ __forceinline__ int piece_tiles(const TreeArgs& p) {
   const int lane = threadIdx.x & 63;
-  int all = 0;
-  for (int b = lane; b < p.f.B; b += 64) all += seq_tiles(p, b);
+  int all = 0, top = 0;
+  for (int b = lane; b < p.f.B; b += 64) {
+    const int t = seq_tiles(p, b);
+    all += t;
+    top = max(top, t);
+  }
+  all = wave_sum(all);
 #pragma unroll
-  for (int i = 1; i < 64; i <<= 1) all += __shfl_xor(all, i);
-  const int parts = p.target >= 2 * p.f.B ? p.target - p.f.B : p.target;
-  return __builtin_amdgcn_readfirstlane(max(kLeastTiles, (all + parts - 1) / parts));
+  for (int i = 1; i < 64; i <<= 1) top = max(top, __shfl_xor(top, i));
+  top = __builtin_amdgcn_readfirstlane(top);
+  int S = max(kLeastTiles, (top + p.most - 1) / p.most);
+  if (p.f.B >= p.target) return max(S, (int)((5 * (int64_t)all / 4 + p.f.B - 1) / p.f.B));
+  S = max(S, (all + p.target - 1) / p.target);
+  while (S < top) {
+    int n = 0;
+    for (int b = lane; b < p.f.B; b += 64) n += (seq_tiles(p, b) + S - 1) / S;
+    n = wave_sum(n);
+    if (n <= p.target) break;
+    S = max(S + 1, (int)((int64_t)S * n / p.target));
+  }
+  return S;
 }
-// Piece `at` of all sequences' (b = -1: there are not so many).
-__device__ __forceinline__ Where find_piece(const TreeArgs& p, int at) {
+// Piece `at` of all sequences' (b = -1: there are not so many).  With `list` their firsts are written down.
+__device__ __forceinline__ Where find_piece(const TreeArgs& p, int at, bool list) {
   const int lane = threadIdx.x & 63, S = piece_tiles(p);
+  Where w{-1, 0, 0, 0, 0, 0};
   int before = 0;
-  for (int base = 0; base < p.f.B; base += 64) {
+  for (int base = 0; base < p.f.B && (list || w.b < 0); base += 64) {
     const int tiles = base + lane < p.f.B ? seq_tiles(p, base + lane) : 0, n = (tiles + S - 1) / S;
     int upto = n;                              // pieces up to this sequence's
 #pragma unroll
@@ -75,48 +99,42 @@ __device__ __forceinline__ Where find_piece(const TreeArgs& p, int at) {
       const int v = __shfl_up(upto, i);
       if (lane >= i) upto += v;
     }
+    if (list && base + lane < p.f.B) p.firsts[base + lane + 1] = before + upto;
     const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > at);
-    if (past) {
+    if (past && w.b < 0) {
       const int l = __builtin_ctzll(past);
-      Where w;
       w.b = base + l;
       w.count = __builtin_amdgcn_readlane(n, l);
       w.first = before + __builtin_amdgcn_readlane(upto, l) - w.count;
       w.z = at - w.first;
       w.tiles = __builtin_amdgcn_readlane(tiles, l);
       w.len = __builtin_amdgcn_readfirstlane(cache_len(p, w.b));
-      return w;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
   }
-  return Where{-1, 0, 0, 0, 0, 0};
+  if (list) p.firsts[0] = 0;
+  return w;
 }
 
-__device__ __forceinline__ Row locate_drafted(const TreeArgs& p, const Where& w, int kvh, int r, const uint32_t*& bits) {
-  Row x;
+// Row r; `blind`: it sees nothing, computes with a query of zeros, and its results are dropped (its
+// keys are not masked, so that the others' tiles need no mask for it).
+struct Drafted : Row { const uint32_t* bits; bool blind; };
+__device__ __forceinline__ Drafted locate_drafted(const TreeArgs& p, const Where& w, int kvh, int r) {
+  Drafted x;
   x.live = r < p.R;
   const int rc = x.live ? r : p.R - 1;
   x.kvh = kvh;
   x.b = w.b;
   x.tok = rc / p.f.G;
   x.h = kvh * p.f.G + rc % p.f.G;
-  bits = p.seen + x.b * p.seen_sb + x.tok * p.seen_st;
+  x.bits = p.seen + x.b * p.seen_sb + x.tok * p.seen_st;
   int n = 0;
-  for (int i = 0; i < p.words; ++i) n += __popc(i == p.words - 1 ? bits[i] & (0xffffffffu >> (31 & (32 * p.words - p.T))) : bits[i]);
-  const bool any = x.live && n > 0;            // a token that does not see itself sees nothing
-  x.lo = 0;
-  x.hi = any ? w.len : 0;
+  for (int i = 0; i < p.words; ++i) n += __popc(i == p.words - 1 ? x.bits[i] & (0xffffffffu >> (31 & (32 * p.words - p.T))) : x.bits[i]);
+  x.blind = !x.live || n == 0;                 // a token that does not see itself sees nothing
+  x.lo = x.w_lo = x.a_lo = 0;
+  x.hi = x.a_hi = w.len;
   x.at = w.len + n - 1;
-  x.w_lo = x.a_lo = 0;
-  x.w_hi = x.hi;
-  x.a_hi = !x.live ? 0x7fffffff : x.hi;
-#pragma unroll
-  for (int i = 1; i < 32; i <<= 1) {
-    x.w_hi = max(x.w_hi, __shfl_xor(x.w_hi, i));
-    x.a_hi = min(x.a_hi, __shfl_xor(x.a_hi, i));
-  }
-  x.w_hi = __builtin_amdgcn_readfirstlane(x.w_hi);
-  x.a_hi = __builtin_amdgcn_readfirstlane(x.a_hi);
+  x.w_hi = __builtin_amdgcn_ballot_w64(!x.blind) ? w.len : 0;
   return x;
 }
 
@@ -128,8 +146,19 @@ struct TreeRows : Rows<HD, F16, CAP, SLOPE> {
   const TreeArgs& p;
   const uint32_t* bits;
   bool live;
-  __device__ __forceinline__ TreeRows(const TreeArgs& args, const Row& x, const uint32_t* row_bits, int lane)
-      : Base(args.f, x, lane), p(args), bits(row_bits), live(x.live) {}
+  __device__ __forceinline__ TreeRows(const TreeArgs& args, const Drafted& x, int lane)
+      : Base(args.f, x, lane), p(args), bits(x.bits), live(!x.blind) {
+    if (x.blind)
+#pragma unroll
+      for (int ks = 0; ks < Base::KS; ++ks) Base::qf[ks] = bf16x8{};
+  }
+  __device__ __forceinline__ bool lost() const { return live && Base::odd(); }
+  __device__ __forceinline__ void drop_blind() {
+    if (live) return;
+    l = n = 0.f;
+#pragma unroll
+    for (int db = 0; db < Base::DB; ++db) o[db] = f32x16{};
+  }
 
   // This lane's bits of tile t of the drafted keys, its own half's keys at the bits
   // mfma_row(i, 0), and how many seen tokens lie behind the tile.
@@ -222,14 +251,13 @@ __global__ __launch_bounds__(kMThreads, kPerCu<HD>) void attn_tree_kernel(TreeAr
   constexpr int DJ = kMTile * CH / kMThreads;  // 16-byte DMAs per wave, tile and tensor
   __shared__ __attribute__((aligned(16))) Slot<HD> r0, r1, r2, r3;
   const Item it = tree_item(p, blockIdx.x);
-  const Where w = find_piece(p, it.piece);
+  const Where w = find_piece(p, it.piece, p.firsts && blockIdx.x == 0);
   if (w.b < 0) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = it.block * kMRows + wave * 32 + (lane & 31);
-  const uint32_t* bits;
-  const Row row = locate_drafted(p, w, it.kvh, r, bits);
-  TreeRows<HD, F16, CAP, SLOPE> R(p, row, bits, lane);
+  const Drafted row = locate_drafted(p, w, it.kvh, r);
+  TreeRows<HD, F16, CAP, SLOPE> R(p, row, lane);
   const int t_begin = share_of(w.tiles, w.z, w.count), t_end = share_of(w.tiles, w.z + 1, w.count);
   const int ct = (w.len + kMTile - 1) / kMTile;      // the cache's tiles
 
@@ -317,7 +345,7 @@ __global__ __launch_bounds__(kMThreads, kPerCu<HD>) void attn_tree_kernel(TreeAr
     __syncthreads();
     R.template slow<false>(r0.k, r0.v, t, ct, kUp<F16>);
   }
-  for (float up = kUp<F16>; __syncthreads_or(R.odd() && row.live); up = kDown) {
+  for (float up = kUp<F16>; __syncthreads_or(R.lost()); up = kDown) {
     R.restart();
     for (int t = t_begin; t < t_end; ++t) {
       __syncthreads();
@@ -329,6 +357,7 @@ __global__ __launch_bounds__(kMThreads, kPerCu<HD>) void attn_tree_kernel(TreeAr
     }
     if (F16 || up < 0.f) break;                // fp16's values times its weights are finite
   }
+  R.drop_blind();
   R.finish(p.f, row, tree_part<HD>(p, w, it.kvh, r), sum_halves(R.l), sum_halves(R.n));
 }
 
@@ -343,13 +372,12 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_tree_few_ker
   __shared__ __attribute__((aligned(16))) uint16_t vt[kMWaves][kMTile * HD];
   __shared__ float stat[kMWaves][2][32];
   const int kvh = blockIdx.x % p.f.Hk;
-  const Where w = find_piece(p, blockIdx.x / p.f.Hk);
+  const Where w = find_piece(p, blockIdx.x / p.f.Hk, p.firsts && blockIdx.x == 0);
   if (w.b < 0) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t* bits;
-  const Row row = locate_drafted(p, w, kvh, lane & 31, bits);
-  TreeRows<HD, F16, CAP, SLOPE> R(p, row, bits, lane);
+  const Drafted row = locate_drafted(p, w, kvh, lane & 31);
+  TreeRows<HD, F16, CAP, SLOPE> R(p, row, lane);
   const int t_begin = share_of(w.tiles, w.z, w.count) + wave, t_end = share_of(w.tiles, w.z + 1, w.count);
   const int ct = (w.len + kMTile - 1) / kMTile;
 
@@ -402,7 +430,7 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_tree_few_ker
     m_wait<0>();
     R.template slow<false>(kw, vw, t, ct, kUp<F16>);
   }
-  for (float up = kUp<F16>; __builtin_amdgcn_ballot_w64(R.odd() && row.live); up = kDown) {
+  for (float up = kUp<F16>; __builtin_amdgcn_ballot_w64(R.lost()); up = kDown) {
     R.restart();
     for (t = t_begin; t < t_end; t += kMWaves) {
       __builtin_amdgcn_s_waitcnt(0xc07f);
@@ -417,6 +445,8 @@ __global__ __launch_bounds__(kMThreads, HD == 64 ? 3 : 2) void attn_tree_few_ker
     }
     if (F16 || up < 0.f) break;
   }
+
+  R.drop_blind();
 
   // The four waves' results in wave 0, by way of K's buffers, all at one offset.
   float total = sum_halves(R.l);
@@ -480,12 +510,7 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs p) {
   const int per = (p.R + 4 / WAVES - 1) / (4 / WAVES);     // workgroups of a (sequence, key head)
   const int kvh = blockIdx.x / per % p.f.Hk, b = blockIdx.x / per / p.f.Hk;
   const int r = blockIdx.x % per * (4 / WAVES) + slot;
-  const int S = piece_tiles(p);
-  int first = 0;                               // pieces of the sequences before
-  for (int i = lane; i < b; i += 64) first += (seq_tiles(p, i) + S - 1) / S;
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) first += __shfl_xor(first, i);
-  const int count = (seq_tiles(p, b) + S - 1) / S;
+  const int first = p.firsts[b], count = p.firsts[b + 1] - first;
   if (count == 1) return;                      // the whole workgroup's
   const int rc = min(r, p.R - 1);
   auto at_piece = [&](int z) { return ((int64_t)(first + z) * p.f.Hk + kvh) * p.R + rc; };
@@ -586,7 +611,7 @@ __global__ __launch_bounds__(256) void draft_tree_kernel(DraftArgs p) {
   }
 }
 
-struct TreePlan { int blocks, target; bool few, join, many; int64_t pieces; size_t parts, bytes; };
+struct TreePlan { int blocks, target, most; bool few, join; int64_t pieces; size_t parts, bytes; };
 TreePlan tree_plan(int64_t B, int64_t Hk, int64_t G, int64_t T, int64_t N, int64_t D) {
   TreePlan x{};
   const int64_t R = T * G, tiles = (N + kMTile - 1) / kMTile + (T + kMTile - 1) / kMTile;
@@ -595,11 +620,12 @@ TreePlan tree_plan(int64_t B, int64_t Hk, int64_t G, int64_t T, int64_t N, int64
   // Workgroups that a CU holds, of the many-row kernel at head dim 64 three.
   const int64_t want = kTreeCus * (!x.few && D == 64 ? 3 : 2);
   x.target = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(1, x.blocks * Hk), kMaxPieces));
-  x.join = tiles > kLeastTiles && x.target > 1;
-  x.pieces = x.join ? x.target + B : B;
-  x.many = x.target > 64;                      // pieces of one sequence: no more than target
+  x.most = x.target > 64 ? kMaxPieces : 64;    // as the join's two forms hold
+  x.join = tiles > kLeastTiles && (x.target > 1 || B > 1);
+  // (piece_tiles: all / S and one of each sequence's, S being 5 / 4 of the mean)
+  x.pieces = !x.join ? B : B < x.target ? x.target : 2 * B;
   x.parts = x.join ? (size_t)(x.pieces * Hk * R) : 0;
-  x.bytes = x.parts * (D + 2) * sizeof(float);
+  x.bytes = x.join ? x.parts * (D + 2) * sizeof(float) + (B + 1) * sizeof(int32_t) : 0;
   return x;
 }
 
@@ -613,7 +639,7 @@ hipError_t tree_launch(const TreeArgs& a, const TreePlan& x, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !x.join) return e;
   const unsigned problems = (unsigned)(a.f.B * a.f.Hk);
-  if (x.many)
+  if (x.most > 64)
     hipLaunchKernelGGL((attn_tree_join_kernel<HD, F16, 4>), dim3(problems * a.R), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((attn_tree_join_kernel<HD, F16, 1>), dim3(problems * ((a.R + 3) / 4)), dim3(256), 0, s, a);
@@ -726,6 +752,7 @@ extern "C" int gpa_attn_tree(int dtype, const gpa_attn_tree_args* args, void* wo
   if (x.bytes > 0) {
     f.part = (float*)workspace;
     f.stat = f.part + x.parts * m.D;
+    a.firsts = (int32_t*)(f.stat + x.parts * 2);
   }
   FwdSet &c = f.set[0], &d = f.set[1];
   c.k = (const uint16_t*)m.k; c.v = (const uint16_t*)m.v; c.N = (int32_t)m.N;
@@ -737,7 +764,7 @@ extern "C" int gpa_attn_tree(int dtype, const gpa_attn_tree_args* args, void* wo
   a.T = (int32_t)m.M; a.words = (int32_t)((m.M + 31) / 32);
   a.seen_st = a.words; a.seen_sb = (int64_t)a.words * m.M;
   a.lens = m.lens;
-  a.R = (int32_t)R; a.blocks = x.blocks; a.target = x.target; a.join = x.join;
+  a.R = (int32_t)R; a.blocks = x.blocks; a.target = x.target; a.most = x.most;
   const bool f16 = dtype == GPA_DTYPE_F16, cap = m.cap > 0.f;
   const hipStream_t s = (hipStream_t)stream;
   const hipError_t e = m.D == 64 ? (f16 ? tree_go<64, true>(a, x, cap, s) : tree_go<64, false>(a, x, cap, s))

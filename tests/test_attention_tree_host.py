@@ -60,12 +60,12 @@ def test_draft_argument_errors(args, code):
 @pytest.mark.parametrize("B,H,Hk,T,N,D", [(1, 8, 2, 26, 130_001, 64), (8, 32, 8, 64, 8192, 128), (64, 16, 16, 16, 4096, 64),
                                           (300, 8, 1, 4, 100_000, 64), (1, 1, 1, 1024, 1 << 29, 128), (1, 4, 4, 1, 200, 64)])
 def test_workspace_stays_below_its_stated_size(B, H, Hk, T, N, D):
-    """8 (D + 2) bytes a row, 768 / (key heads and blocks of 128 rows) pieces more than
-    sequences."""
+    """4 (D + 2) bytes a row and piece, of 768 / (key heads and blocks of 128 rows) pieces, or two
+    for each sequence, and 4 a sequence."""
     R = T * (H // Hk)
     target = max(1, 768 // (Hk * -(-R // 128)))
     got = _native.lib().gpa_attn_tree_workspace_bytes(B, H, Hk, T, N, D)
-    assert got <= 4 * (D + 2) * (target + B) * Hk * R
+    assert got <= 4 * (D + 2) * max(target, 2 * B) * Hk * R + 4 * (B + 1)
     assert N > 200 or got == 0
 
 
