@@ -33,6 +33,10 @@ namespace {
 
 constexpr int kTreeCus = 256;
 constexpr int kLeastTiles = 8;           // of a piece
+// Longer sequences are cut.  A launch for the join is worth 30 tiles to up to 32 rows (22 tiles whole
+// 10.1 us, cut 11.9; 63 whole 15.5, cut 12.0) and 12 to more (head dim 64, 10 tiles 13.3 and 15.4, 17
+// tiles 16.6 and 15.5).
+constexpr int kSplitFew = 32, kSplitMany = 12;
 constexpr int64_t kMaxDraft = 1024;
 
 struct TreeArgs {
@@ -620,8 +624,8 @@ TreePlan tree_plan(int64_t B, int64_t Hk, int64_t G, int64_t T, int64_t N, int64
   // Workgroups that a CU holds, of the many-row kernel at head dim 64 three.
   const int64_t want = kTreeCus * (!x.few && D == 64 ? 3 : 2);
   x.target = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(1, x.blocks * Hk), kMaxPieces));
-  x.most = x.target > 64 ? kMaxPieces : 64;    // as the join's two forms hold
-  x.join = tiles > kLeastTiles && (x.target > 1 || B > 1);
+  x.join = tiles > (x.few ? kSplitFew : kSplitMany) && (x.target > 1 || B > 1);
+  x.most = !x.join ? 1 : x.target > 64 ? kMaxPieces : 64;   // as the join's two forms hold
   // (piece_tiles: all / S and one of each sequence's, S being 5 / 4 of the mean)
   x.pieces = !x.join ? B : B < x.target ? x.target : 2 * B;
   x.parts = x.join ? (size_t)(x.pieces * Hk * R) : 0;
