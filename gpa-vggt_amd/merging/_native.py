@@ -92,6 +92,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import struct
 import threading
 from pathlib import Path
@@ -398,14 +399,14 @@ def _check(rc: int, what: str) -> None:
 
 
 def _require_gpu(*tensors: torch.Tensor) -> torch.device:
-    dev = tensors[0].device
+    at = tensors[0].get_device()
     for t in tensors:
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise ValueError("the gfx950 merging kernels need GPU tensors, got device "
                              f"{t.device}")
-        if t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} vs {t.device}")
-    return dev
+        if t.get_device() != at:
+            raise ValueError(f"tensors on different devices: {tensors[0].device} vs {t.device}")
+    return tensors[0].device
 
 
 _NO_SWITCH = contextlib.nullcontext()
@@ -459,18 +460,29 @@ _LIB = torch.ops.gpa._library = torch.library.Library("gpa", "FRAGMENT")
 _Below = torch._C._AutoDispatchBelowAutograd
 
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _eager_stack():
+    """Whether no dispatch mode, functorch transform or trace looks on."""
+    return (torch._C._len_torch_dispatch_stack() == 0
+            and torch._C._functorch.peek_interpreter_stack() is None
+            and torch._C._get_tracing_state() is None)
+
+
 def _ordinary(args):
     """Whether these are plain tensors outside dispatch modes and functorch."""
     return (torch._C._len_torch_dispatch_stack() == 0
             and torch._C._functorch.peek_interpreter_stack() is None
-            and all(type(a) in (torch.Tensor, torch.nn.Parameter) for a in args
-                    if isinstance(a, torch.Tensor)))
+            and all(type(a) in _PLAIN for a in args if isinstance(a, torch.Tensor)))
 
 
-def _op(fn, setup_context=None, backward=None):
+def _op(fn, setup_context=None, backward=None, direct=False):
     """Define gpa::<name of fn> with fn as its implementation on every device
     (it refuses tensors that are not on a GPU) and, where it has gradients, its
-    backward; returns the callable."""
+    backward; returns the callable.  direct: its ordinary eager calls with GPU
+    tensors run fn itself, past the dispatcher (4 of such a call's 17 us, and 10 of a
+    backward's, which runs on the engine's thread)."""
     name = fn.__name__
     _LIB.define(name + torch.library.infer_schema(fn, mutates_args=()),
                 tags=(torch.Tag.pt2_compliant_tag,))
@@ -493,7 +505,7 @@ def _op(fn, setup_context=None, backward=None):
         @staticmethod
         def forward(ctx, *args):
             with _Below():
-                out = packets[name].default(*args)
+                out = (fn if direct else packets[name].default)(*args)
             setup_context(ctx, args, out)
             return out
 
@@ -504,10 +516,23 @@ def _op(fn, setup_context=None, backward=None):
         if torch.compiler.is_compiling():
             return getattr(ops, name).default(*args, **kwargs)
         op = packets[name].default
+        if direct and not kwargs and _eager_stack():
+            grad = False
+            for a in args:
+                if isinstance(a, torch.Tensor):
+                    if not a.is_cuda or type(a) not in _PLAIN:
+                        break
+                    grad = grad or a.requires_grad
+            else:
+                if not (grad and torch.is_grad_enabled()):
+                    with _Below():
+                        return fn(*args)
+                if backward is not None:
+                    return Eager.apply(*args)
         if torch.is_grad_enabled() and any(
                 isinstance(a, torch.Tensor) and a.requires_grad
                 for a in ((*args, *kwargs.values()) if kwargs else args)):
-            if backward is not None and not kwargs and _ordinary(args):
+            if backward is not None and not direct and not kwargs and _ordinary(args):
                 return Eager.apply(*args)
             return op(*args, **kwargs)
         with _Below():
@@ -1644,7 +1669,7 @@ def _rotary_check(what, q, k, positions, freqs, axes, pairing, sections, params)
                              f"{tuple(freqs.shape)} and {axes.dtype} {tuple(axes.shape)}")
         if 2 * pairs > D:
             raise ValueError(f"{what}: {pairs} pairs do not fit into heads of {D} features")
-        if not 1 <= len(sections) <= MAX_AXES or any(s < 0 for s in sections) or sum(sections) != pairs:
+        if not 1 <= len(sections) <= MAX_AXES or min(sections) < 0 or sum(sections) != pairs:
             raise ValueError(f"{what}: sections {tuple(sections)} must be 1 to {MAX_AXES} counts that add to {pairs}")
         if positions.dtype not in _POSITION_KINDS or positions.shape not in ((N, len(sections)), (B, N, len(sections))):
             raise ValueError(f"{what}: positions must be int32, int64 or fp32 [{N}, {len(sections)}] or "
@@ -1652,11 +1677,12 @@ def _rotary_check(what, q, k, positions, freqs, axes, pairing, sections, params)
     if pairing not in (0, 1, 2):
         raise ValueError(f"{what}: unknown pairing {pairing}")
     given = [p for p in params if p is not None]
-    if any(p.shape != (D,) for p in given):
-        raise ValueError(f"{what}: parameters must be [{D}], got {[tuple(p.shape) for p in given]}")
-    if any(p.dtype != given[0].dtype or p.dtype not in (q.dtype, torch.float32) for p in given):
-        raise ValueError(f"{what}: parameters are all of the heads' type {q.dtype}, or all fp32, got "
-                         f"{[p.dtype for p in given]}")
+    for p in given:
+        if p.shape != (D,):
+            raise ValueError(f"{what}: parameters must be [{D}], got {[tuple(p.shape) for p in given]}")
+        if p.dtype != given[0].dtype or p.dtype not in (q.dtype, torch.float32):
+            raise ValueError(f"{what}: parameters are all of the heads' type {q.dtype}, or all fp32, got "
+                             f"{[p.dtype for p in given]}")
     return given[0].dtype if given else q.dtype
 
 
@@ -1735,7 +1761,7 @@ def head_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[
     return q_out, k_out
 
 
-head_rotary = _op(head_rotary, _rotary_setup, _rotary_backward)
+head_rotary = _op(head_rotary, _rotary_setup, _rotary_backward, direct=True)
 
 
 @_fake("head_rotary")
@@ -1743,7 +1769,7 @@ def _head_rotary_fake(q, k, positions, freqs, axes, pairing, sections, q_w, k_w,
     return _like(q), q.new_empty(0) if k is None else _like(k)
 
 
-@_op
+@functools.partial(_op, direct=True)
 def head_rotary_bwd(d_q: Optional[torch.Tensor], d_k: Optional[torch.Tensor], q: torch.Tensor,
                     k: Optional[torch.Tensor], positions: Optional[torch.Tensor], freqs: Optional[torch.Tensor],
                     axes: Optional[torch.Tensor], pairing: int, sections: List[int], q_w: Optional[torch.Tensor],
@@ -1808,7 +1834,7 @@ def _counts(what, name, t, B):
     return None if t is None else t.contiguous()
 
 
-@_op
+@functools.partial(_op, direct=True)
 def draft_tree(parents: torch.Tensor, lengths: torch.Tensor,
                sizes: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
     """gpa_draft_tree: positions int32 [B, T] and the seen tokens' bits int32
@@ -1861,7 +1887,7 @@ def _tree_check(what, q, cache_k, cache_v, k, v, lengths, seen, slopes):
     return _counts(what, "lengths", lengths, B), seen.contiguous(), slopes, sl_sb
 
 
-@_op
+@functools.partial(_op, direct=True)
 def attn_tree(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
               lengths: Optional[torch.Tensor], seen: torch.Tensor, sm_scale: float, cap: float,
               slopes: Optional[torch.Tensor], want_lse: bool) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -1984,7 +2010,7 @@ def linear_gate(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
     return y, z
 
 
-linear_gate = _op(linear_gate, _linear_setup, _linear_backward)
+linear_gate = _op(linear_gate, _linear_setup, _linear_backward, direct=True)
 
 
 @_fake("linear_gate")
@@ -1993,7 +2019,7 @@ def _linear_gate_fake(x, w, bias, gate, residual, act, want_z):
     return x.new_empty(size), x.new_empty(size if want_z else (0,), dtype=_z_dtype(x, gate))
 
 
-@_op
+@functools.partial(_op, direct=True)
 def linear_gate_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: torch.Tensor, w: torch.Tensor,
                     bias: Optional[torch.Tensor], gate: Optional[torch.Tensor], act: int, want_x: bool, want_w: bool,
                     want_bias: bool, want_gate: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
