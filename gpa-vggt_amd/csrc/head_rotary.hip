@@ -46,7 +46,6 @@ constexpr int kCsFloats = 4096;           // cosines and sines of a tile
 constexpr int64_t kFwdWgs = 1024;
 constexpr int64_t kBwdWgs = 1024;        // three to a CU, 768, with a bias's sums or in fp32 (video: 51 us on 1,024, 41)
 
-
 // Eight pairs of a head: their features begin at o0 and o1 (neighbours: all at
 // o0), the first pair's number (-1: they are not turned), how many there are.
 struct Chunk { int16_t o0, o1, p0, n; };

@@ -9,7 +9,8 @@
 //
 // fp16: a gate may be as small as it likes (1e-5 is usual where it begins), and dz would
 // leave the format's range with it; the gate goes into dz times a power of two that makes its
-// largest value one to two, and the products are multiplied by its inverse.
+// largest value a half to one (dz is then no larger than 1.13 dy, whatever the activation), and the
+// products are multiplied by its inverse.
 #include "linear_gemm.h"
 
 namespace gpa {
@@ -26,7 +27,7 @@ struct DzArgs {
   int32_t pf32, z16;
 };
 
-// The power of two that makes the gate's largest finite value one to two, formed by a workgroup.
+// The power of two that makes the gate's largest finite value a half to one, formed by a workgroup.
 __device__ __forceinline__ float gate_scale(const void* gate, int pf32, int64_t J, float* top) {
   float m = 0.f;
   for (int64_t j = threadIdx.x; j < J; j += 256) {
@@ -40,7 +41,7 @@ __device__ __forceinline__ float gate_scale(const void* gate, int pf32, int64_t 
   m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   int e = 0;
   if (m > 0.f) frexpf(m, &e);                  // m = [0.5, 1) 2^e
-  return ldexpf(1.0f, -min(max(e - 1, -100), 100));
+  return ldexpf(1.0f, -min(max(e, -100), 100));
 }
 
 // 512 columns (eight a lane: side by side where they come in aligned groups (WIDE), else each 64

@@ -155,6 +155,21 @@ def test_gates_out_of_fp16s_middle(dev, act, gate_size):
     _check(dev, 150, 64, 80, dt=HF, pdt=F, act=act, gate=True, gate_size=gate_size)
 
 
+@pytest.mark.parametrize("gate_size", [0.95, 1.05, 1e-5])
+def test_gradients_near_fp16s_largest(dev, gate_size):
+    """dz of a gradient of 50,000 stays in range inside (1.13 times it at most), and dx with it: x's
+    gradient is dy gate w of one output, off by half a step for dz, w's product being exact, and for
+    itself (2 * 2^-11 of its value, and as much again for the product of both)."""
+    dy = torch.tensor([[50_000.0], [-49_000.0], [3.0]], device=dev, dtype=HF).repeat(20, 1)
+    x = torch.ones(60, 8, device=dev, dtype=HF, requires_grad=True)
+    w = torch.full((1, 8), 0.125, device=dev, dtype=HF)
+    gate = torch.tensor([gate_size], device=dev)
+    y = linear_gate_residual(x, w, gate=gate, activation="relu")
+    dx, = torch.autograd.grad(y, x, dy)
+    want = (dy.double() * gate.double() * 0.125).expand(-1, 8)
+    assert ((dx.double() - want).abs() <= want.abs() * (2.0 ** -10 + 2.0 ** -21) + 2.0 ** -25).all()
+
+
 @pytest.mark.parametrize("tile,M,N,K", [(0, 4096, 4096, 4096), (1, 8192, 2048, 1024), (2, 2048, 2048, 1024), (3, 700, 520, 256)])
 def test_every_tile_and_layout(dev, tile, M, N, K):
     """Sizes of each kind of tile, forward and (dx, dw) turned, with edges in both directions."""
