@@ -212,7 +212,8 @@ extern "C" int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate
   const bool few = a->M <= kRowsMost;
   const Laid l = linear_laid(a, true, true);
   const GemmPlan x = few ? GemmPlan{} : gemm_plan(a->M, a->N, l.K, false);
-  if (!few && !linear_launchable(x, a->M, a->N)) {
+  // (A launch has less than 2^32 threads: of a few rows up to 1,024 for 16 columns.)
+  if (few ? a->N > (int64_t)1 << 25 : !linear_launchable(x, a->M, a->N)) {
     gpa_set_error("%s: problem exceeds the grid limit", fn);
     return GPA_E_UNSUPPORTED;
   }

@@ -106,3 +106,11 @@ def test_op_refusals(kw, match):
     a = {**dict(x=X, w=W, bias=None, gate=None, residual=None, act=0), **kw}
     with pytest.raises(ValueError, match=match):
         _native._linear_check("y", *a.values())
+
+
+@pytest.mark.parametrize("M", [1, 16])
+@pytest.mark.parametrize("K", [8, 8192])
+def test_too_many_columns_of_few_rows(M, K):
+    """More than 2^32 threads, which a launch does not have."""
+    a = _args(M=M, N=(1 << 26) + 1, K=K, x_s=K, w_s=K)
+    assert _native.lib().gpa_linear_gate(1, 1, ctypes.byref(a), FAKE, 1 << 27, None, 0, None, 0, None) == UNS
