@@ -315,9 +315,28 @@ __global__ __launch_bounds__(kMThreads, kPerCu<HD>) void attn_tree_kernel(TreeAr
       const bool poly = R.settle(s, n0, edge);
       float x[16];
       R.template scores<false>(s, n0, poly, R.m, x);
-      const f32x16 next = R.products(nxt.k);   // beside the exponentials
+      __builtin_amdgcn_s_setprio(1);
+      const f32x16 next = R.products(nxt.k);     // beside the exponentials
+      // Both blocks in this order: what is read from LDS, arithmetic while it comes, then a product at a
+      // time; and a wave with products goes before one without (together 117 -> 113 us with a cap, 8
+      // sequences of 8,192 keys, 32 + 8 heads of 128, 64 drafted tokens; 67 -> 65 with heads of 64).
+      __builtin_amdgcn_sched_group_barrier(0x100, HD / 16, 0);
+      __builtin_amdgcn_sched_group_barrier(0x2, 16, 0);
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 256 / HD, 0);
+      }
       R.weigh(n0, edge, x);
       R.add(cur.v, x);
+      __builtin_amdgcn_sched_group_barrier(0x100, HD / 8, 0);
+      __builtin_amdgcn_sched_group_barrier(0x2, 24, 0);
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);
+      }
+      __builtin_amdgcn_s_setprio(0);
       s = next;
     } else {
       s = R.products(nxt.k);
