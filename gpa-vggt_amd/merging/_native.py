@@ -477,6 +477,17 @@ def _ordinary(args):
             and all(type(a) in _PLAIN for a in args if isinstance(a, torch.Tensor)))
 
 
+def _again(op, run, *args):
+    """A gradient op's call from a backward: `run`, which is the op without its checks, where
+    nothing but autograd looks on.  (The forward checked the saved tensors, and the engine holds
+    the outputs' gradients against the outputs.)"""
+    if torch.is_grad_enabled() or torch.compiler.is_compiling() or not _eager_stack() or not all(
+            type(a) in _PLAIN and a.is_cuda for a in args if isinstance(a, torch.Tensor)):
+        return op(*args)
+    with _Below():
+        return run(*args)
+
+
 def _op(fn, setup_context=None, backward=None, direct=False):
     """Define gpa::<name of fn> with fn as its implementation on every device
     (it refuses tensors that are not on a GPU) and, where it has gradients, its
@@ -1731,7 +1742,8 @@ def _rotary_backward(ctx, d_q, d_k):
         return (None,) * 13
     if not norm:
         q, k = (d_q if d_q is not None else d_k), d_k
-    got = head_rotary_bwd(d_q, d_k, q, k, positions, freqs, axes, pairing, sections, q_w, k_w, q_b, k_b, norm, eps)
+    got = _again(head_rotary_bwd, _rotary_grads, d_q, d_k, q, k, positions, freqs, axes, pairing, sections, q_w, k_w,
+                 q_b, k_b, norm, eps)
     dq, dk, dqw, dkw, dqb, dkb = got
     some = lambda g, t, d: None if t is None or d is None else g  # noqa: E731
     return (some(dq, q, d_q), some(dk, k, d_k), None, None, None, None, None, some(dqw, q_w, d_q), some(dkw, k_w, d_k),
@@ -1781,14 +1793,20 @@ def head_rotary_bwd(d_q: Optional[torch.Tensor], d_k: Optional[torch.Tensor], q:
     a norm q and k give their sizes and order of dimensions alone."""
     what = "gpa::head_rotary_bwd"
     params = (q_w, k_w, q_b, k_b)
-    dev = _require_gpu(*[t for t in (q, k, d_q, d_k, positions, freqs, axes, *params) if t is not None])
-    pdt = _rotary_check(what, q, k, positions, freqs, axes, pairing, sections, params)
+    _require_gpu(*[t for t in (q, k, d_q, d_k, positions, freqs, axes, *params) if t is not None])
+    _rotary_check(what, q, k, positions, freqs, axes, pairing, sections, params)
     for name, d, t in (("d_q", d_q, q), ("d_k", d_k, k)):
         if d is not None and (t is None or d.shape != t.shape or d.dtype != t.dtype):
             raise ValueError(f"{what}: {name} {d.dtype} {tuple(d.shape)} does not match its tensor")
+    return _rotary_grads(d_q, d_k, q, k, positions, freqs, axes, pairing, sections, q_w, k_w, q_b, k_b, norm, eps)
+
+
+def _rotary_grads(d_q, d_k, q, k, positions, freqs, axes, pairing, sections, q_w, k_w, q_b, k_b, norm, eps):
+    what, dev, params = "gpa::head_rotary_bwd", q.device, (q_w, k_w, q_b, k_b)
+    pdt = next((t.dtype for t in params if t is not None), q.dtype)
     none = lambda: q.new_empty(0)  # noqa: E731
     dq, dk = none() if d_q is None else _like(q), none() if d_k is None else _like(k)
-    grads = [none() if t is None or d is None else torch.empty(t.shape, device=dev, dtype=t.dtype)
+    grads = [none() if t is None or d is None else t.new_empty(t.shape)
              for t, d in zip(params, (d_q, d_k, d_q, d_k))]
     if dq.numel() + dk.numel() == 0:
         return (dq, dk, *(g.zero_() for g in grads))
@@ -1972,7 +1990,8 @@ def _linear_backward(ctx, dy, _):
     if dy is None:
         return (None,) * 7
     need = [ctx.needs_input_grad[i] and t is not None for i, t in enumerate((x, w, bias, gate))]
-    dx, dw, db, dg = linear_gate_bwd(dy, z, x, w, bias, gate, ctx.act, *need) if any(need) else (None,) * 4
+    dx, dw, db, dg = (_again(linear_gate_bwd, _linear_grads, dy, z, x, w, bias, gate, ctx.act, *need) if any(need)
+                      else (None,) * 4)
     some = lambda i, g: g if need[i] else None  # noqa: E731
     return some(0, dx), some(1, dw), some(2, db), some(3, dg), dy if ctx.needs_input_grad[4] else None, None, None
 
@@ -2026,15 +2045,21 @@ def linear_gate_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: torch.Tensor
     """gpa_linear_gate_bwd: the wanted gradients of x, w, bias and gate (empty tensors for
     the others).  z: the forward's, with an activation or the gate's gradient."""
     what = "gpa::linear_gate_bwd"
-    dev = _require_gpu(*[t for t in (dy, z, x, w, bias, gate) if t is not None])
-    pdt = _linear_check(what, x, w, bias, gate, dy, act)
-    (M, K), N = x.shape, w.shape[0]
+    _require_gpu(*[t for t in (dy, z, x, w, bias, gate) if t is not None])
+    _linear_check(what, x, w, bias, gate, dy, act)
+    M, N = x.shape[0], w.shape[0]
     if (want_bias and bias is None) or (want_gate and gate is None):
         raise ValueError(f"{what}: no gradient of an absent bias or gate")
     if z is None and (act or want_gate):
         raise ValueError(f"{what}: an activation, and the gate's gradient, need z")
     if z is not None and (z.dtype not in (torch.float32, torch.float16) or z.shape != (M, N) or not z.is_contiguous() or z.data_ptr() % 16):
         raise ValueError(f"{what}: z must be contiguous fp32 or fp16 [{M}, {N}], got {z.dtype} {tuple(z.shape)}")
+    return _linear_grads(dy, z, x, w, bias, gate, act, want_x, want_w, want_bias, want_gate)
+
+
+def _linear_grads(dy, z, x, w, bias, gate, act, want_x, want_w, want_bias, want_gate):
+    what, dev, (M, K), N = "gpa::linear_gate_bwd", x.device, x.shape, w.shape[0]
+    pdt = next((t.dtype for t in (bias, gate) if t is not None), x.dtype)
     none = lambda: x.new_empty(0)  # noqa: E731
     dx = torch.empty(M, K, device=dev, dtype=x.dtype) if want_x else none()
     dw = torch.empty(N, K, device=dev, dtype=w.dtype) if want_w else none()
