@@ -1306,7 +1306,8 @@ def _like(t):
 def _rows8(t):
     """t, or a copy, with rows of 16-bit values that are 16-byte aligned."""
     s = t.stride()
-    if s[-1] == 1 and not t.data_ptr() & 15 and not any(x & 7 for x in s[:-1]):
+    rows = s[0] | s[1] | s[2] if len(s) == 4 else s[0] | s[1] if len(s) == 3 else 1
+    if s[-1] == 1 and not rows & 7 and not t.data_ptr() & 15:
         return t
     return t if _rows_ok(t, 8) else t.clone(memory_format=torch.contiguous_format)
 
@@ -1887,14 +1888,12 @@ def _draft_tree_fake(parents, lengths, sizes):
 def _tree_check(what, q, cache_k, cache_v, k, v, lengths, seen, slopes):
     """Checks, and the tables as the kernel takes them."""
     _masked_shapes(what, q, k, v)
-    B, H, T, D = q.shape
-    if k.shape[2] != T:
-        raise ValueError(f"{what}: {T} queries and {k.shape[2]} drafted keys")
+    (B, H, T, D), (_, Hk, own, _), dt, cache = q.shape, k.shape, q.dtype, cache_k.shape
+    if own != T:
+        raise ValueError(f"{what}: {T} queries and {own} drafted keys")
     for name, t in (("cache_k", cache_k), ("cache_v", cache_v)):
-        if t.dtype != q.dtype or t.dim() != 4 or t.shape != cache_k.shape \
-                or (*t.shape[:2], t.shape[3]) != (B, k.shape[1], D):
-            raise ValueError(f"{what}: {name} must be {q.dtype} [{B}, {k.shape[1]}, N, {D}], got {t.dtype} "
-                             f"{tuple(t.shape)}")
+        if t.dtype != dt or len(cache) != 4 or t.shape != cache or cache[0] != B or cache[1] != Hk or cache[3] != D:
+            raise ValueError(f"{what}: {name} must be {dt} [{B}, {Hk}, N, {D}], got {t.dtype} {tuple(t.shape)}")
     if T > MAX_DRAFT:
         raise NotImplementedError(f"{what}: {T} drafted tokens (up to {MAX_DRAFT})")
     if seen.dtype != torch.int32 or seen.shape != (B, T, (T + 31) // 32):

@@ -120,7 +120,7 @@ def _half_operands(q, others):
         q = q.to(_autocast_dtype())
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise NotImplementedError(f"{q.dtype} is not supported; the gfx950 kernels run bf16 and fp16")
-    return (q, *(t.to(q.dtype) for t in others))
+    return (q, *[t if t.dtype == q.dtype else t.to(q.dtype) for t in others])
 
 
 def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale: float, *,

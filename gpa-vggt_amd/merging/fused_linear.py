@@ -44,9 +44,9 @@ def linear_gate_residual(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
     if residual is not None and residual.shape != (*lead, N):
         raise ValueError(f"{what}: residual {tuple(residual.shape)} must be {(*lead, N)}")
     x, weight = _half_operands(x, (weight,))
-    if residual is not None:
+    if residual is not None and residual.dtype != x.dtype:
         residual = residual.to(x.dtype)
-    if any(t is not None and t.dtype != x.dtype for t in (bias, gate)):
+    if (bias is not None and bias.dtype != x.dtype) or (gate is not None and gate.dtype != x.dtype):
         bias, gate = (None if t is None else t.float() for t in (bias, gate))
     act = _ACTS[activation]
     grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, gate, residual))
