@@ -2068,6 +2068,7 @@ def _linear_grads(dy, z, x, w, bias, gate, act, want_x, want_w, want_bias, want_
         if M == 0 or N == 0 or not (want_bias or want_gate):
             return dx, dw, db.zero_(), dg.zero_()
     x, w, dy = _feature_rows(x), _feature_rows(w), _feature_rows(dy)
+    z = z if z is None or z.is_contiguous() else z.contiguous()    # (saved, it may come back in other strides)
     gate = None if gate is None else gate.contiguous()
     ptr = lambda t: t.data_ptr() if t.numel() else 0  # noqa: E731
     a = _linear_args(x, w, None, gate, None, act)
