@@ -58,7 +58,8 @@ struct Side {
   int64_t x_sb, x_sh, x_sn, y_sb, y_sh, y_sn, o_sb, o_sh, o_sn;
   const void *w, *b;
   float* part;            // backward: [workgroup][2][D]
-  int32_t heads, wgs;     // wgs: the backward's workgroups of this side
+  int32_t heads, wgs, per_tile;   // wgs: the backward's workgroups of this side; per_tile: a tile's tokens
+  int64_t tiles;
   uint32_t magic;         // 2^32 / heads, rounded up
 };
 
@@ -68,10 +69,10 @@ struct RotArgs {
   int64_t pos_sb, pos_sn;
   const double* freqs;
   const int32_t* axes;
-  int64_t N, tokens, tiles;
+  int64_t N, tokens;
   uint32_t rows_magic;    // 2^32 / heads of a row's tensors, rounded up (one head: not used)
   uint32_t n_magic;       // 2^32 / N, rounded up (N == 1: not used)
-  int32_t D, pairs, count, pos_kind, chunks, lanes, per_tile, norm, pf32, bias;
+  int32_t D, pairs, count, pos_kind, chunks, lanes, norm, pf32, bias;
   float eps, inv_d;
   Chunk chunk[kMaxChunks];
 };
@@ -284,18 +285,18 @@ struct Walk {
   int r0, rows;           // the next rows' first, of `rows` of the tile
   uint32_t first;         // the tile's first token
   int live;
-  __device__ __forceinline__ void open(const RotArgs& a, int64_t at, int all) {
+  __device__ __forceinline__ void open(const RotArgs& a, const Side& s, int64_t at, int all) {
     tile = at;
     r0 = 0;
-    first = (uint32_t)(at * a.per_tile);
-    live = at < a.tiles ? (int)(a.tokens - first < a.per_tile ? a.tokens - first : a.per_tile) : 0;
+    first = (uint32_t)(at * s.per_tile);
+    live = at < s.tiles ? (int)(a.tokens - first < s.per_tile ? a.tokens - first : s.per_tile) : 0;
     rows = live * all;
   }
   // Whether the next rows are another tile's.
-  __device__ __forceinline__ bool on(const RotArgs& a, int step, int64_t stride, int all) {
+  __device__ __forceinline__ bool on(const RotArgs& a, const Side& s, int step, int64_t stride, int all) {
     r0 += step;
     if (r0 < rows) return false;
-    open(a, tile + stride, all);
+    open(a, s, tile + stride, all);
     return true;
   }
 };
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(kThreads, 4) void head_rotary_kernel(RotArgs a) {
     }
   };
   Walk w;
-  w.open(a, blockIdx.x, both);
+  w.open(a, a.side[0], blockIdx.x, both);     // (both sides together, in the first one's tiles)
   Some now;
   fetch(w, now);
   if (a.norm && l.row < 2) {                   // a row of lanes for each side (a wave has two at least)
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(kThreads, 4) void head_rotary_kernel(RotArgs a) {
       __syncthreads();
     }
     Some cur = now;
-    fresh = w.on(a, U * l.rows, gridDim.x, both);
+    fresh = w.on(a, a.side[0], U * l.rows, gridDim.x, both);
     if (w.live > 0) fetch(w, now);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -437,7 +438,7 @@ __global__ __launch_bounds__(kThreads) void head_rotary_bwd_kernel(RotArgs a) {
     m.out = static_cast<T*>(s.out) + t.b * s.o_sb + h * s.o_sh + t.n * s.o_sn;
   };
   Walk w;
-  w.open(a, wg, s.heads);
+  w.open(a, s, wg, s.heads);
   Some now;
   fetch(w, now);
   const Turner turner(a);
@@ -453,7 +454,7 @@ __global__ __launch_bounds__(kThreads) void head_rotary_bwd_kernel(RotArgs a) {
       __syncthreads();
     }
     Some cur = now;
-    fresh = w.on(a, l.rows, s.wgs, s.heads);
+    fresh = w.on(a, s, l.rows, s.wgs, s.heads);
     if (w.live > 0) fetch(w, now);
     float ga[8], gb[8];
     cur.dy.get(ga, gb);
@@ -507,11 +508,26 @@ __global__ __launch_bounds__(kThreads) void head_rotary_bwd_kernel(RotArgs a) {
   // The rows' sums: over a wave's rows, then over the four waves in LDS.
   float* red = cs;                             // [wave][lane of a row][4][8], at most 4 * 32 * 32 floats
   float* sums[4] = {dwa, dwb, dba, dbb};
+  auto each = [&](auto op) __attribute__((always_inline)) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < (BIAS ? 4 : 2); ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      for (int m = a.lanes; m < 64; m <<= 1) sums[k][i] += __shfl_xor(sums[k][i], m);
+      for (int i = 0; i < 8; ++i) sums[k][i] = op(sums[k][i]);
+  };
+  // (By DPP and swaps: 96 shuffles a wave through LDS took 10 us of a CU's.)
+  if (a.lanes <= 8) each([](float v) { return dpp_add<0x128>(v); });     // the lane eight on in a row of sixteen
+  if (a.lanes <= 4) each([](float v) { return dpp_add<0x124>(v); });
+  if (a.lanes <= 2) each([](float v) { return dpp_add<0x122>(v); });
+  if (a.lanes <= 1) each([](float v) { return dpp_add<0x121>(v); });
+  if (a.lanes <= 16)
+    each([](float v) {
+      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+      return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    });
+  each([](float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  });
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (lane < a.lanes)
@@ -695,7 +711,8 @@ int fill(const gpa_head_rotary_args* a, int dtype, int pdtype, std::initializer_
 // angles' LDS holds and `wgs` workgroups leave to each, the number that leaves the fewest lanes idle
 // (5,476 tokens of 16 heads of 64 on 2,048 workgroups, 32 rows each where 128 go at a time: 15 us;
 // on 685, 128 each: 9.5).  Few tokens are spread over the chip.
-int tile_tokens(const RotArgs& r, int64_t heads, int64_t step, int64_t wgs) {
+void tile(const RotArgs& r, Side& s, int64_t heads, int64_t step, int64_t wgs) {
+  wgs = std::max<int64_t>(wgs, 1);
   const int64_t most = std::min<int64_t>(kMaxTokens, kCsFloats / (16 * std::max(r.chunks, 1)));
   const int64_t fill = std::min<int64_t>((step + heads - 1) / std::max<int64_t>(heads, 1), std::max<int64_t>(r.tokens / 256, 1));
   const int64_t top = std::min(most, std::max((r.tokens + wgs - 1) / wgs, fill));
@@ -708,12 +725,13 @@ int tile_tokens(const RotArgs& r, int64_t heads, int64_t step, int64_t wgs) {
       best = n;
     }
   }
-  return (int)best;
+  s.per_tile = (int32_t)best;
+  s.tiles = (r.tokens + best - 1) / best;
 }
 
 template <typename T, int V, bool BWD>
 hipError_t go(const RotArgs& r, bool inter, hipStream_t s) {
-  const dim3 grid((unsigned)(BWD ? r.side[0].wgs + r.side[1].wgs : std::min(r.tiles, kFwdWgs))), block(kThreads);
+  const dim3 grid((unsigned)(BWD ? r.side[0].wgs + r.side[1].wgs : std::min(r.side[0].tiles, kFwdWgs))), block(kThreads);
   if constexpr (BWD) {
     if (inter && r.bias) hipLaunchKernelGGL((head_rotary_bwd_kernel<T, V, true, true>), grid, block, 0, s, r);
     else if (inter) hipLaunchKernelGGL((head_rotary_bwd_kernel<T, V, true, false>), grid, block, 0, s, r);
@@ -778,8 +796,7 @@ extern "C" int gpa_head_rotary(int dtype, int param_dtype, const gpa_head_rotary
   r.side[0].out = q_out; r.side[0].o_sb = qo_sb; r.side[0].o_sh = qo_sh; r.side[0].o_sn = qo_sn;
   r.side[1].out = k_out; r.side[1].o_sb = ko_sb; r.side[1].o_sh = ko_sh; r.side[1].o_sn = ko_sn;
   const int64_t both = a->H + a->Hk;
-  r.per_tile = tile_tokens(r, both, (dtype == GPA_DTYPE_F32 ? 1 : 2) * (kThreads / r.lanes), kFwdWgs);
-  r.tiles = (r.tokens + r.per_tile - 1) / r.per_tile;
+  tile(r, r.side[0], both, (dtype == GPA_DTYPE_F32 ? 1 : 2) * (kThreads / r.lanes), kFwdWgs);
   r.rows_magic = magic_of(both);
   return refuse_launch(fn, launch<false>(r, dtype, some, a->pairing == GPA_PAIRS_NEIGHBOURS, (hipStream_t)stream));
 }
@@ -845,8 +862,8 @@ extern "C" int gpa_head_rotary_bwd(int dtype, int param_dtype, const gpa_head_ro
     q.part = g->dq_w || g->dq_b ? (float*)workspace : nullptr;
     k.part = g->dk_w || g->dk_b ? (float*)workspace + w.q * 2 * a->D : nullptr;
   }
-  r.per_tile = tile_tokens(r, std::max(H, Hk), kThreads / r.lanes, std::max(w.q, w.k));
-  r.tiles = (r.tokens + r.per_tile - 1) / r.per_tile;
+  tile(r, q, H, kThreads / r.lanes, w.q);
+  tile(r, k, Hk, kThreads / r.lanes, w.k);
   const hipStream_t s = (hipStream_t)stream;
   hipError_t e = launch<true>(r, dtype, some, a->pairing == GPA_PAIRS_NEIGHBOURS, s);
   if (e == hipSuccess && sums) {
