@@ -72,7 +72,7 @@ struct RotArgs {
   int64_t N, tokens;
   uint32_t rows_magic;    // 2^32 / heads of a row's tensors, rounded up (one head: not used)
   uint32_t n_magic;       // 2^32 / N, rounded up (N == 1: not used)
-  int32_t D, pairs, count, pos_kind, chunks, lanes, norm, pf32, bias;
+  int32_t D, pairs, count, pos_kind, chunks, lanes, norm, pf32, bias, par16;   // par16: parameters are 16-byte aligned
   float eps, inv_d;
   Chunk chunk[kMaxChunks];
 };
@@ -232,14 +232,26 @@ struct Turner {
 };
 
 // A parameter in a lane's order: its sixteen values, `none` where there are none.
-template <typename T, bool INTER>
+template <typename T, int V, bool INTER>
 __device__ __forceinline__ void take_param(const RotArgs& a, const void* p, const Chunk& c, float none, float (&x)[8], float (&y)[8]) {
+  const bool wide = sizeof(T) == 4 || a.pf32;
+  if (V == 8 && a.par16 && p) {
+    if (wide) {
+      Raw<float, 8, INTER> r;
+      r.load(static_cast<const float*>(p), c);
+      r.get(x, y);
+    } else {
+      Raw<T, 8, INTER> r;
+      r.load(static_cast<const T*>(p), c);
+      r.get(x, y);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     x[i] = y[i] = none;
     if (!p || i >= c.n) continue;
     const int u = INTER ? c.o0 + 2 * i : c.o0 + i, v = INTER ? c.o0 + 2 * i + 1 : c.o1 + i;
-    const bool wide = sizeof(T) == 4 || a.pf32;
     x[i] = wide ? static_cast<const float*>(p)[u] : (float)static_cast<const T*>(p)[u];
     y[i] = wide ? static_cast<const float*>(p)[v] : (float)static_cast<const T*>(p)[v];
   }
@@ -345,7 +357,7 @@ __global__ __launch_bounds__(kThreads, 4) void head_rotary_kernel(RotArgs a) {
     const Side& s = a.side[l.row];
     float x[8], y[8];
     for (int k = 0; k < 2; ++k) {
-      take_param<T, INTER>(a, k ? s.b : s.w, l.c, k ? 0.f : 1.f, x, y);
+      take_param<T, V, INTER>(a, k ? s.b : s.w, l.c, k ? 0.f : 1.f, x, y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         par[l.row][k][at * 16 + i] = x[i];
@@ -410,7 +422,7 @@ __global__ __launch_bounds__(kThreads, 4) void head_rotary_kernel(RotArgs a) {
 // BIAS: a bias's gradient is wanted (its sums take 16 registers, with which a CU holds three
 // workgroups instead of four).
 template <typename T, int V, bool INTER, bool BIAS>
-__global__ __launch_bounds__(kThreads) void head_rotary_bwd_kernel(RotArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && V == 8 && !BIAS ? 4 : 3) void head_rotary_bwd_kernel(RotArgs a) {
   __shared__ __attribute__((aligned(16))) float cs[kCsFloats];
   const Lane l = lane_of(a);
   const int at = threadIdx.x % a.lanes, cat = at < a.chunks ? at : 0;
@@ -443,7 +455,7 @@ __global__ __launch_bounds__(kThreads) void head_rotary_bwd_kernel(RotArgs a) {
   fetch(w, now);
   const Turner turner(a);
   float wa[8], wb[8], dwa[8], dwb[8], dba[8], dbb[8];
-  take_param<T, INTER>(a, s.w, l.c, 1.f, wa, wb);
+  take_param<T, V, INTER>(a, s.w, l.c, 1.f, wa, wb);
 #pragma unroll
   for (int i = 0; i < 8; ++i) dwa[i] = dwb[i] = dba[i] = dbb[i] = 0.f;
   bool fresh = true;
@@ -688,6 +700,7 @@ int fill(const gpa_head_rotary_args* a, int dtype, int pdtype, std::initializer_
   r.N = a->N; r.tokens = a->B * a->N;
   r.D = (int32_t)a->D; r.pairs = (int32_t)a->pairs; r.count = a->sections_count;
   r.norm = a->norm; r.pf32 = pdtype == GPA_DTYPE_F32;
+  r.par16 = ((uintptr_t)a->q_w | (uintptr_t)a->k_w | (uintptr_t)a->q_b | (uintptr_t)a->k_b) % 16 == 0;
   r.eps = a->eps; r.inv_d = 1.0f / (float)a->D;
   r.n_magic = magic_of(a->N);
   q.magic = magic_of(a->H); k.magic = magic_of(a->Hk);

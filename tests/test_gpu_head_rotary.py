@@ -400,3 +400,22 @@ def test_registration(dev):
     args = (q, k, p, rot.freqs, rot.axes, 1, [3, 5], w, w.detach(), None, None, 1, 1e-6)
     torch.library.opcheck(torch.ops.gpa.head_rotary.default, args)
     torch.library.opcheck(torch.ops.gpa.head_rotary.default, (q, None, p, rot.freqs, rot.axes, 1, [3, 5], None, None, None, None, 0, 0.0))
+
+
+@pytest.mark.parametrize("dt,pdt", [(BF, BF), (BF, F), (F, F)])
+@pytest.mark.parametrize("pairing", ["half", "interleaved"])
+def test_parameters_at_any_address(dev, dt, pdt, pairing):
+    """Parameters that begin between 16-byte pieces, beside heads that do not: the same bits."""
+    g = torch.Generator(device=dev).manual_seed(3)
+    q, k, dq, dk = (torch.randn(2, h, 70, 64, generator=g, device=dev).to(dt) for h in (3, 2, 3, 2))
+    flat = torch.randn(4 * 64 + 1, generator=g, device=dev).to(pdt)
+    rotary, at = rotary_axes((32,), pairing=pairing), torch.arange(70, device=dev, dtype=torch.int32)[:, None]
+
+    def run(par):
+        leaves = [t.detach().requires_grad_() for t in (q, k, *par)]
+        x, y, qw, kw, qb, kb = leaves
+        out = qk_norm_rotate(x, y, at, rotary, q_weight=qw, k_weight=kw, q_bias=qb, k_bias=kb, kind="layer")
+        return [*out, *torch.autograd.grad(out, leaves, [dq, dk])]
+    views = [flat[1 + 64 * i:65 + 64 * i] for i in range(4)]
+    assert views[0].data_ptr() % 16 and not q.data_ptr() % 16
+    assert all(torch.equal(a, b) for a, b in zip(run(views), run([v.clone() for v in views])))
