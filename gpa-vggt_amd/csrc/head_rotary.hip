@@ -27,7 +27,7 @@
 // reads x and dy and writes dx (the moments are formed again, which costs less than
 // keeping them).  Parameters' gradients go through one fp32 partial a workgroup,
 // in a fixed order.  16,384 tokens of 32 + 8 heads of 128 in bf16: forward 74 us
-// (4.5 TB/s), backward 128 (3.9) and 6 for the sums; a copy runs at 4.9.
+// (4.5 TB/s), backward 117 (4.3) and 6 for the sums; a copy runs at 4.9.
 #include <algorithm>
 #include <math.h>
 
@@ -45,7 +45,8 @@ constexpr int kCsFloats = 4096;           // cosines and sines of a tile
 // (four to a CU forward; as many as tiles took 77 us for 71 at 16,384 tokens of 32 + 8 heads of
 // 128, and 38 for 28 at 10,992 of 16 + 16 of 64).
 constexpr int64_t kFwdWgs = 1024;
-constexpr int64_t kBwdWgs = 1024;        // three to a CU, 768, with a bias's sums or in fp32 (video: 51 us on 1,024, 41)
+constexpr int64_t kBwdWgs = 1024;        // three to a CU, 768, with a bias's sums or in fp32 (10,992 tokens of 16 + 16 heads of 64:
+                                         // 36.4 us on 1,024, 34.6; 20,000: 56, 51; fp32 12.6, 11.2)
 
 // Eight pairs of a head: their features begin at o0 and o1 (neighbours: all at
 // o0), the first pair's number (-1: they are not turned), how many there are.
@@ -526,7 +527,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && V == 8 && !BIAS ? 4 : 3
 #pragma unroll
       for (int i = 0; i < 8; ++i) sums[k][i] = op(sums[k][i]);
   };
-  // (By DPP and swaps: 96 shuffles a wave through LDS took 10 us of a CU's.)
+  // (By DPP and swaps: as shuffles through LDS these sums cost a pass 7 to 10 us.)
   if (a.lanes <= 8) each([](float v) { return dpp_add<0x128>(v); });     // the lane eight on in a row of sixteen
   if (a.lanes <= 4) each([](float v) { return dpp_add<0x124>(v); });
   if (a.lanes <= 2) each([](float v) { return dpp_add<0x122>(v); });
