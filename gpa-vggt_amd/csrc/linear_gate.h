@@ -16,13 +16,13 @@ struct GemmPlan { int tile; int64_t ti, tj, splits; size_t bytes; };
 GemmPlan gemm_plan(int64_t I, int64_t J, int64_t K, bool turned);
 
 // x and w as the products take them: K a multiple of 8 and rows that are 16-byte aligned, so or as
-// padded copies in the workspace (`bytes` of it, x's first).
+// padded copies in the workspace (`bytes` of it, x's first).  `turned`: as the gradients' products take them.
 struct Laid {
   int64_t K;
   bool copy_x, copy_w;
   size_t w_at, bytes;
 };
-Laid linear_laid(const gpa_linear_gate_args* a, bool x, bool w);
+Laid linear_laid(const gpa_linear_gate_args* a, bool x, bool w, bool turned);
 struct Matrix { const uint16_t* p; int64_t stride; };
 hipError_t linear_lay(const gpa_linear_gate_args* a, const Laid& l, void* ws, Matrix& x, Matrix& w, hipStream_t s);
 int linear_check(const char* fn, int dtype, int pdtype, const gpa_linear_gate_args* a);

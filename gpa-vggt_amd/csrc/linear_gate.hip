@@ -147,12 +147,14 @@ int linear_check(const char* fn, int dtype, int pdtype, const gpa_linear_gate_ar
   return GPA_OK;
 }
 
-Laid linear_laid(const gpa_linear_gate_args* a, bool x, bool w) {
+Laid linear_laid(const gpa_linear_gate_args* a, bool x, bool w, bool turned) {
   Laid l{};
   l.K = std::max<int64_t>((a->K + 7) / 8 * 8, 8);
-  // Rows of a tile are addressed by 32-bit offsets from its first one: strides below 2^21.
+  // Rows of a tile are addressed by 32-bit offsets from its first one: strides below 2^21.  Turned
+  // operands' rows lie apart (linear_gemm.h, Feed).
+  const int64_t least = turned ? l.K : 0;
   auto copied = [&](const void* p, int64_t n, int64_t st) {
-    return a->K != l.K || (uintptr_t)p % 16 || (n > 1 && (st % 8 || st < 0 || st >= (int64_t)1 << 21));
+    return a->K != l.K || (uintptr_t)p % 16 || (n > 1 && (st % 8 || st < least || st >= (int64_t)1 << 21));
   };
   l.copy_x = x && copied(a->x, a->M, a->x_s);
   l.copy_w = w && copied(a->w, a->N, a->w_s);
@@ -184,7 +186,7 @@ using namespace gpa;
 
 extern "C" size_t gpa_linear_gate_workspace_bytes(const gpa_linear_gate_args* a) {
   if (!a || a->M <= 0 || a->N <= 0 || a->K < 0) return 0;
-  const Laid l = linear_laid(a, true, true);
+  const Laid l = linear_laid(a, true, true, false);
   return l.bytes + (a->M <= kRowsMost ? 0 : gemm_plan(a->M, a->N, l.K, false).bytes);
 }
 
@@ -210,7 +212,7 @@ extern "C" int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate
   const hipStream_t s = (hipStream_t)stream;
   const bool f16 = dtype == GPA_DTYPE_F16;
   const bool few = a->M <= kRowsMost;
-  const Laid l = linear_laid(a, true, true);
+  const Laid l = linear_laid(a, true, true, false);
   const GemmPlan x = few ? GemmPlan{} : gemm_plan(a->M, a->N, l.K, false);
   // (A launch has less than 2^32 threads: of a few rows up to 1,024 for 16 columns.)
   if (few ? a->N > (int64_t)1 << 25 : !linear_launchable(x, a->M, a->N)) {

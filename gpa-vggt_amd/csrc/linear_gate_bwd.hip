@@ -175,7 +175,7 @@ BwdPlan bwd_plan(const gpa_linear_gate_args* a, bool dz, bool sums, bool dx, boo
   p.scale = dz ? (size_t)round16(M * p.J8 * 2) : 0;
   p.part = p.scale + 16;
   p.split = p.part + (sums ? (size_t)round16(p.chunks * 2 * N * 4) : 0);
-  p.laid = linear_laid(a, dw, dx);
+  p.laid = linear_laid(a, dw, dx, true);
   p.lay = p.split + round16(std::max(p.x.bytes, p.w.bytes));
   p.bytes = p.lay + p.laid.bytes;
   return p;
@@ -211,9 +211,10 @@ hipError_t dz_launch(const DzArgs& d, int act, bool f16, bool wide, dim3 grid, h
 
 using namespace gpa;
 
-// Whether dy itself is not dz as the products take it.
+// Whether dy itself is not dz as the products take it (turned, for dw: linear_gemm.h, Feed).
 static bool needs_dz(const gpa_linear_gate_args* a, const gpa_linear_gate_grads* g) {
-  const bool aligned = a->N % 8 == 0 && (uintptr_t)g->dy % 16 == 0 && (a->M < 2 || (g->dy_s % 8 == 0 && g->dy_s >= 0 && g->dy_s < 1 << 21));
+  const int64_t least = g->dw ? a->N : 0;
+  const bool aligned = a->N % 8 == 0 && (uintptr_t)g->dy % 16 == 0 && (a->M < 2 || (g->dy_s % 8 == 0 && g->dy_s >= least && g->dy_s < 1 << 21));
   return (g->dx || g->dw) && (a->act != kActNone || a->gate || !aligned);
 }
 

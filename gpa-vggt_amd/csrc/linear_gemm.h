@@ -49,7 +49,9 @@ __device__ __forceinline__ void wait_dma() {
 
 constexpr uint32_t kNowhere = 0x40000000u;     // a DMA offset outside every descriptor: zeros
 
-// One operand of a workgroup: BL blocks of 16 a wave, two waves' worth a tile.
+// One operand of a workgroup: BL blocks of 16 a wave, two waves' worth a tile.  Zeros past the last k:
+// by last_ok, or turned by the descriptor's end, behind which the rows past the last one begin (so
+// they may not lie over each other: stride >= cols).
 template <int BL, bool TURNED>
 struct Feed {
   static constexpr int T = 32 * BL;            // rows of i or j of a tile

@@ -733,8 +733,8 @@ int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate_args* args
 
 /* Its gradients from y's, dy (any row stride): dx [M, K] and dw [N, K] in dtype, dbias and
  * dgate [N] in param_dtype, each NULL where it is not wanted; the residual's is dy.  Sums run in a
- * fixed order.  N below 2^21.  workspace: gpa_linear_gate_bwd_workspace_bytes of the
- * same arguments, 16-byte aligned. */
+ * fixed order.  N below 2^21.  Rows of x, w and dy that lie over each other are copied.
+ * workspace: gpa_linear_gate_bwd_workspace_bytes of the same arguments, 16-byte aligned. */
 typedef struct gpa_linear_gate_grads {
   const void *dy, *z;
   void *dx, *dw, *dbias, *dgate;
