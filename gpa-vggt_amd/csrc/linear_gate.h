@@ -34,7 +34,7 @@ struct Finish {
   const void *bias, *gate;
   const void* residual;
   void* z;                // the sums before the activation, rows of J (nullable)
-  const float* unscale;   // a factor (nullable)
+  const float* unscale;   // a factor for each row (nullable)
   float* part;            // parts along k: [part][I][J rounded up to 8]
   int64_t out_s, res_s, I, J;
   int32_t act, pf32, z16; // pf32: bias and gate are fp32; z16: z is fp16, else fp32
@@ -204,7 +204,7 @@ __device__ __forceinline__ void finish_down(const Finish& f, int64_t i, int64_t 
   auto param = [&](const void* p) {
     return f.pf32 ? static_cast<const float*>(p)[j] : half_to_f32<F16>(static_cast<const __bf16*>(p)[j]);
   };
-  const float factor = f.unscale ? *f.unscale : 1.f, bias = f.bias ? param(f.bias) : 0.f, gate = f.gate ? param(f.gate) : 1.f;
+  const float bias = f.bias ? param(f.bias) : 0.f, gate = f.gate ? param(f.gate) : 1.f;
   const int n = f.I <= i ? 0 : (f.I - i + STEP - 1) / STEP < 8 ? (int)((f.I - i + STEP - 1) / STEP) : 8;
   __bf16 res[8];
   if (f.residual)
@@ -212,7 +212,7 @@ __device__ __forceinline__ void finish_down(const Finish& f, int64_t i, int64_t 
     for (int e = 0; e < 8; ++e) res[e] = e < n ? static_cast<const __bf16*>(f.residual)[(i + e * STEP) * f.res_s + j] : (__bf16)0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    if (f.unscale) v[e] *= factor;
+    if (f.unscale && e < n) v[e] *= f.unscale[i + e * STEP];
     if (f.bias) v[e] += bias;
   }
   if (f.z)
@@ -239,7 +239,7 @@ __device__ __forceinline__ void finish8(const Finish& f, int64_t i, int64_t j, f
   const int n = f.J - j < 8 ? (int)(f.J - j) : 8;
   float x[8];
   if (f.unscale) {
-    const float s = *f.unscale;
+    const float s = f.unscale[i];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] *= s;
   }

@@ -7,10 +7,13 @@
 // parts.  Without activation and gate dz is dy as it lies.  Both products take w and x as they
 // lie in memory, turned on their way out of LDS (linear_gemm.h): no transposed copy.
 //
-// fp16: a gate may be as small as it likes (1e-5 is usual where it begins), and dz would
-// leave the format's range with it; the gate goes into dz times a power of two that makes its
-// largest value a half to one (dz is then no larger than 1.13 dy, whatever the activation), and the
-// products are multiplied by its inverse.
+// fp16: a gate may be as small as it likes (1e-5 is usual where it begins), or of any size in
+// one column and another, and dz would leave the format's range with it.  A row of dw has one gate: its
+// product takes dy act'(z), and the gate multiplies the sums.  A row of dx has them all: its dz are
+// scaled by a power of two that brings the row's largest dy gate (dz is no larger than 1.13 of it,
+// whatever the activation) to 2^13 .. 2^14, and the sums by its inverse; what lies 2^27 below
+// the largest keeps every bit.  (One scale for both products, by the largest gate: under gates of 300 and 0.3
+// and a dy of 1e-3 the small one's row of dw was off by 3 % of its norm.)
 #include "linear_gemm.h"
 
 namespace gpa {
@@ -20,28 +23,44 @@ struct DzArgs {
   const void* dy;
   const void* z;
   const void* gate;
-  float* scale;           // fp16 with a gate: where the inverse of its scale goes
-  void* dz;               // rows of J8, the columns past J zeros; null: sums alone
+  void* dz;               // rows of J8, the columns past J zeros; null: not wanted
+  void* bare;             // fp16 with a gate: dw's, without it; null: not wanted
+  float* unscale;         // fp16 with a gate: the inverse of each row's scale in dz
+  float* gate32;          // where the gate goes, the scales of dw's rows; null: not wanted
   float* part;            // [chunk][2][J]; null: no sums
   int64_t dy_s, I, J, J8, chunk;
-  int32_t pf32, z16;
+  int32_t pf32, z16, gate_wide;
 };
 
-// The power of two that makes the gate's largest finite value a half to one, formed by a workgroup.
-__device__ __forceinline__ float gate_scale(const void* gate, int pf32, int64_t J, float* top) {
+// The scale of each row of dz in fp16, by its largest finite dy gate: a wave a row.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void linear_scale_kernel(DzArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (i >= a.I) return;
+  const __bf16* DY = static_cast<const __bf16*>(a.dy) + i * a.dy_s;
   float m = 0.f;
-  for (int64_t j = threadIdx.x; j < J; j += 256) {
-    const float x = fabsf(pf32 ? static_cast<const float*>(gate)[j] : (float)static_cast<const _Float16*>(gate)[j]);
-    m = x < INFINITY ? fmaxf(m, x) : m;
+  constexpr int AT = WIDE ? 8 : 1;
+  for (int64_t j = lane * AT; j < a.J; j += 64 * AT) {
+    float dy[8], g[8];
+    if constexpr (WIDE) {
+      param8<true>(DY + j, 0, 1, 0, 8, dy);
+      param8<true>(a.gate, a.pf32, a.gate_wide, j, 8, g);
+    } else {
+      dy[0] = half_to_f32<true>(DY[j]);
+      g[0] = a.pf32 ? static_cast<const float*>(a.gate)[j] : half_to_f32<true>(static_cast<const __bf16*>(a.gate)[j]);
+    }
+#pragma unroll
+    for (int e = 0; e < AT; ++e) {
+      const float x = fabsf(dy[e] * g[e]);
+      m = x < INFINITY ? fmaxf(m, x) : m;
+    }
   }
 #pragma unroll
-  for (int i = 1; i < 64; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
-  if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  int e = 0;
+  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+  int e = 14;
   if (m > 0.f) frexpf(m, &e);                  // m = [0.5, 1) 2^e
-  return ldexpf(1.0f, -min(max(e, -100), 100));
+  if (lane == 0) a.unscale[i] = ldexpf(1.0f, max(e - 14, -126));
 }
 
 // 512 columns (eight a lane: side by side where they come in aligned groups (WIDE), else each 64
@@ -54,11 +73,6 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
   constexpr int STEP = WIDE ? 1 : 64;
   const int64_t j = (int64_t)blockIdx.x * 512 + (WIDE ? lane * 8 : lane), i0 = blockIdx.y * a.chunk;
   const int64_t i1 = i0 + a.chunk < a.I ? i0 + a.chunk : a.I;
-  float scale = 1.f;
-  if (F16 && a.scale) {
-    scale = gate_scale(a.gate, a.pf32, a.J, &red[0][0][0]);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.scale = 1.0f / scale;
-  }
   float g[8], db[8], dg[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -66,10 +80,28 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
     if (GATE && j + e * STEP < a.J)
       g[e] = a.pf32 ? static_cast<const float*>(a.gate)[j + e * STEP] : half_to_f32<F16>(static_cast<const __bf16*>(a.gate)[j + e * STEP]);
     db[e] = dg[e] = 0.f;
+    if (GATE && F16 && a.gate32 && blockIdx.y == 0 && wave == 0 && j + e * STEP < a.J) a.gate32[j + e * STEP] = g[e];
   }
+  auto put = [&](void* rows, int64_t i, const float (&v)[8]) __attribute__((always_inline)) {
+    __bf16* to = static_cast<__bf16*>(rows) + i * a.J8 + j;
+    if constexpr (WIDE) {
+      bf16x8 y;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const bf16x2 w = pack2<F16>(v[e], v[e + 1]);
+        y[e] = w[0];
+        y[e + 1] = w[1];
+      }
+      *reinterpret_cast<bf16x8*>(to) = y;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (j + e * 64 < a.J8) to[e * 64] = j + e * 64 < a.J ? f32_to_half<F16>(v[e]) : (__bf16)0.f;
+    }
+  };
   if (j < a.J8)
     for (int64_t i = i0 + wave; i < i1; i += 4) {
-      float dy[8], z[8], out[8];
+      float dy[8], z[8], d[8];
       const __bf16* DY = static_cast<const __bf16*>(a.dy) + i * a.dy_s + j;
       if constexpr (WIDE) {
         param8<F16>(DY, 0, 1, 0, 8, dy);
@@ -93,29 +125,23 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
           const float v = act_both<ACT>(z[e], slope);
           if (GATE) dg[e] = __builtin_fmaf(dy[e], v, dg[e]);
         }
-        const float d = ACT != kActNone ? dy[e] * slope : dy[e];
-        db[e] = GATE ? __builtin_fmaf(d, g[e], db[e]) : db[e] + d;
-        out[e] = GATE ? d * (g[e] * scale) : d;
+        d[e] = ACT != kActNone ? dy[e] * slope : dy[e];
+      }
+      if (GATE && F16 && a.bare) put(a.bare, i, d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        db[e] = GATE ? __builtin_fmaf(d[e], g[e], db[e]) : db[e] + d[e];
+        if (GATE) d[e] *= g[e];
       }
       if (!a.dz) continue;
-      __bf16* DZ = static_cast<__bf16*>(a.dz) + i * a.J8 + j;
-      if constexpr (WIDE) {
-        bf16x8 y;
+      if (GATE && F16) {
+        const float scale = 1.0f / a.unscale[i];
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const bf16x2 w = pack2<F16>(out[e], out[e + 1]);
-          y[e] = w[0];
-          y[e + 1] = w[1];
-        }
-        *reinterpret_cast<bf16x8*>(DZ) = y;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (j + e * 64 < a.J8) DZ[e * 64] = j + e * 64 < a.J ? f32_to_half<F16>(out[e]) : (__bf16)0.f;
+        for (int e = 0; e < 8; ++e) d[e] *= scale;
       }
+      put(a.dz, i, d);
     }
   if (!a.part) return;
-  if (F16) __syncthreads();                    // the gate's maximum is read
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int at = WIDE ? lane * 8 + e : lane + e * 64;
@@ -162,7 +188,7 @@ struct BwdPlan {
   GemmPlan x, w;
   Laid laid;
   int64_t chunk, chunks, J8;
-  size_t part, scale, split, lay, bytes;       // where each begins, dz at 0
+  size_t bare, rows, gate, part, split, lay, bytes;   // where each begins, dz at 0
 };
 BwdPlan bwd_plan(const gpa_linear_gate_args* a, bool dz, bool sums, bool dx, bool dw) {
   BwdPlan p{};
@@ -172,8 +198,13 @@ BwdPlan bwd_plan(const gpa_linear_gate_args* a, bool dz, bool sums, bool dx, boo
   p.chunks = (M + p.chunk - 1) / p.chunk;
   if (dx) p.x = gemm_plan(M, K, N, true);
   if (dw) p.w = gemm_plan(N, K, M, true);
-  p.scale = dz ? (size_t)round16(M * p.J8 * 2) : 0;
-  p.part = p.scale + 16;
+  // (With a gate as fp16 needs it: the formats are not known here.)
+  const size_t one = dz ? (size_t)round16(M * p.J8 * 2) : 0;
+  const bool gate = dz && a->gate;
+  p.bare = gate && dx ? one : 0;
+  p.rows = gate && dx && dw ? 2 * one : one;
+  p.gate = p.rows + (gate ? round16(M * 4) : 0);
+  p.part = p.gate + (gate ? round16(N * 4) : 0);
   p.split = p.part + (sums ? (size_t)round16(p.chunks * 2 * N * 4) : 0);
   p.laid = linear_laid(a, dw, dx, true);
   p.lay = p.split + round16(std::max(p.x.bytes, p.w.bytes));
@@ -201,6 +232,14 @@ void dz_gate(const DzArgs& d, int act, dim3 grid, hipStream_t s) {
   d.gate ? dz_go<F16, WIDE, true>(d, act, grid, s) : dz_go<F16, WIDE, false>(d, act, grid, s);
 }
 hipError_t dz_launch(const DzArgs& d, int act, bool f16, bool wide, dim3 grid, hipStream_t s) {
+  if (d.dz && d.unscale) {
+    const int64_t wgs = (d.I + 3) / 4, most = (int64_t)1 << 22;   // (a launch has less than 2^32 threads, also of one dimension)
+    const dim3 rows((unsigned)std::min(wgs, most), (unsigned)((wgs + most - 1) / most));
+    if (wide) hipLaunchKernelGGL((linear_scale_kernel<true>), rows, dim3(256), 0, s, d);
+    else hipLaunchKernelGGL((linear_scale_kernel<false>), rows, dim3(256), 0, s, d);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   if (f16) wide ? dz_gate<true, true>(d, act, grid, s) : dz_gate<true, false>(d, act, grid, s);
   else wide ? dz_gate<false, true>(d, act, grid, s) : dz_gate<false, false>(d, act, grid, s);
   return hipGetLastError();
@@ -257,20 +296,25 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
     gpa_set_error("%s: problem exceeds the grid limit", fn);
     return GPA_E_UNSUPPORTED;
   }
-  if (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16) {
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || (uintptr_t)workspace % 16)) {
     gpa_set_error("%s: workspace of %zu bytes, 16-byte aligned, needed", fn, p.bytes);
     return GPA_E_WORKSPACE;
   }
   char* ws = (char*)workspace;
   const hipStream_t s = (hipStream_t)stream;
-  float* const scale = need_dz && f16 && a->gate ? (float*)(ws + p.scale) : nullptr;
+  const bool apart = need_dz && f16 && a->gate;          // dw's dz without the gate, dx's with its rows' scales
+  float* const rows = apart && g->dx ? (float*)(ws + p.rows) : nullptr;
+  float* const gates = apart && g->dw ? (float*)(ws + p.gate) : nullptr;
   Matrix x, w;
   hipError_t e = linear_lay(a, p.laid, ws + p.lay, x, w, s);
   if (e == hipSuccess && (need_dz || sums)) {
     DzArgs d{};
     d.dy = g->dy; d.dy_s = a->M > 1 ? g->dy_s : 0;
-    d.z = g->z; d.z16 = g->z_dtype == GPA_DTYPE_F16; d.gate = a->gate; d.scale = scale;
-    d.dz = need_dz ? ws : nullptr;
+    d.z = g->z; d.z16 = g->z_dtype == GPA_DTYPE_F16; d.gate = a->gate;
+    d.gate_wide = (uintptr_t)a->gate % 16 == 0;
+    d.dz = need_dz && (!apart || g->dx) ? ws : nullptr;
+    d.bare = gates ? ws + p.bare : nullptr;
+    d.unscale = rows; d.gate32 = gates;
     d.part = sums ? (float*)(ws + p.part) : nullptr;
     d.I = a->M; d.J = a->N; d.J8 = p.J8; d.chunk = p.chunk;
     d.pf32 = param_dtype == GPA_DTYPE_F32;
@@ -289,10 +333,10 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
       e = hipGetLastError();
     }
   }
-  const Operand dz_rows{need_dz ? (const uint16_t*)ws : (const uint16_t*)g->dy, need_dz ? p.J8 : a->M > 1 ? g->dy_s : p.J8, a->M, p.J8};
+  Operand dz_rows{need_dz ? (const uint16_t*)ws : (const uint16_t*)g->dy, need_dz ? p.J8 : a->M > 1 ? g->dy_s : p.J8, a->M, p.J8};
   auto fine = [](const void* q, int64_t n, int64_t st) { return (uintptr_t)q % 16 == 0 && (n < 2 || st % 8 == 0); };
   GemmArgs m{};
-  m.out.unscale = scale;
+  m.out.unscale = rows;
   m.out.part = (float*)(ws + p.split);
   m.out.J = a->K;
   if (e == hipSuccess && g->dx) {              // over the output features: w turned
@@ -305,7 +349,9 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
   }
   if (e == hipSuccess && g->dw) {              // over the rows: both turned
     m.P = Operand{x.p, x.stride, a->M, p.laid.K};
+    if (apart) dz_rows.p = (const uint16_t*)(ws + p.bare);
     m.Q = dz_rows;
+    m.out.unscale = gates;
     m.nk = (int32_t)((a->M + 31) / 32);
     m.out.out = g->dw; m.out.out_s = g->dw_s; m.out.I = a->N;
     m.out.wide = a->K % 8 == 0 && fine(g->dw, a->N, g->dw_s);

@@ -352,7 +352,6 @@ __global__ __launch_bounds__(256, PER_CU) void linear_gemm_kernel(GemmArgs a) {
   float bias[8], gate[8];
   if (a.out.bias && in) param8<F16>(a.out.bias, a.out.pf32, 1, j, 8, bias);
   if (a.out.gate && in) param8<F16>(a.out.gate, a.out.pf32, 1, j, 8, gate);
-  const float factor = a.out.unscale ? *a.out.unscale : 1.f;
   auto rounds = [&](auto which) __attribute__((always_inline)) {
     constexpr int ACT = decltype(which)::value;
     constexpr int SETS = WI == 8 ? 2 : 1;      // two waves a SIMD hide each other's waits
@@ -376,6 +375,7 @@ __global__ __launch_bounds__(256, PER_CU) void linear_gemm_kernel(GemmArgs a) {
         up(it, v);
         if (!in || i + it * RP >= a.out.I) continue;
         if (a.out.unscale) {
+          const float factor = a.out.unscale[i + it * RP];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] *= factor;
         }
