@@ -99,6 +99,7 @@ from pathlib import Path
 from typing import List, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libgpa_mi355x.so"
 ABI_VERSION = 20
@@ -477,6 +478,14 @@ def _ordinary(args):
             and all(type(a) in _PLAIN for a in args if isinstance(a, torch.Tensor)))
 
 
+def _no_tangents(name, args):
+    """Refuses tensors that carry a tangent of forward-mode differentiation, which none of the ops has:
+    below autograd it would be dropped.  (Outside a dual level none does.)"""
+    if forward_ad._current_level >= 0 and any(isinstance(a, torch.Tensor) and forward_ad.unpack_dual(a).tangent is not None
+                                              for a in args):
+        raise NotImplementedError(f"gpa::{name} has no forward-mode derivative (jvp); use reverse mode")
+
+
 def _again(op, run, *args):
     """A gradient op's call from a backward: `run`, which is the op without its checks, where
     nothing but autograd looks on.  (The forward checked the saved tensors, and the engine holds
@@ -484,6 +493,7 @@ def _again(op, run, *args):
     if torch.is_grad_enabled() or torch.compiler.is_compiling() or not _eager_stack() or not all(
             type(a) in _PLAIN and a.is_cuda for a in args if isinstance(a, torch.Tensor)):
         return op(*args)
+    _no_tangents(op.__name__, args)
     with _Below():
         return run(*args)
 
@@ -509,6 +519,16 @@ def _op(fn, setup_context=None, backward=None, direct=False):
     getattr(ops, name)                   # so that the namespace holds it
     packets = vars(ops)
 
+    # The registered op sees tangents here alone (transforms take them off what they call below).
+    def refusing(below):
+        def autograd(keys, *args, **kwargs):
+            _no_tangents(name, (*args, *kwargs.values()))
+            return below.call_boxed(keys, *args, **kwargs)
+        return autograd
+
+    for key in ("AutogradCUDA", "AutogradCPU"):
+        _LIB.impl(name, refusing(torch.library.get_kernel(f"gpa::{name}", key)), key, with_keyset=True)
+
     # Gradients in ordinary eager calls go through this Function, without the
     # dispatcher's generated one around the op's own (an op and its backward:
     # 125 and 130 us of a training step's host time).
@@ -527,6 +547,9 @@ def _op(fn, setup_context=None, backward=None, direct=False):
         if torch.compiler.is_compiling():
             return getattr(ops, name).default(*args, **kwargs)
         op = packets[name].default
+        if torch._C._functorch.peek_interpreter_stack() is not None:
+            return op(*args, **kwargs)
+        _no_tangents(name, (*args, *kwargs.values()) if kwargs else args)
         if direct and not kwargs and _eager_stack():
             grad = False
             for a in args:
