@@ -26,7 +26,9 @@ def linear_gate_residual(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
     """residual + gate * activation(x weight^T + bias).
 
     x [..., K], weight [N, K] (GPU, bf16 or fp16; an fp32 x is cast to the autocast dtype or
-    bf16, and weight and residual with it; any strides), bias and gate [N], residual [..., N].
+    bf16, and residual with it; weight is used in x's type; any strides), bias and gate [N],
+    residual [..., N] of x's type (a wider one would lose what it has more: it is refused, and
+    added outside).
     activation: None, "gelu" (the normal distribution's), "gelu_tanh", "silu" or "relu".  bias
     and gate are of x's type, or any is fp32 and both are used so.  From the products to
     the result everything is fp32; it is rounded once.  Returns [..., N]; differentiable in all
@@ -43,6 +45,8 @@ def linear_gate_residual(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
     N, lead = weight.shape[0], x.shape[:-1]
     if residual is not None and residual.shape != (*lead, N):
         raise ValueError(f"{what}: residual {tuple(residual.shape)} must be {(*lead, N)}")
+    if residual is not None and residual.dtype != x.dtype and x.dtype in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{what}: residual is {residual.dtype} beside x in {x.dtype}; cast one of them")
     x, weight = _half_operands(x, (weight,))
     if residual is not None and residual.dtype != x.dtype:
         residual = residual.to(x.dtype)
