@@ -33,11 +33,11 @@ struct Finish {
   void* out;              // 16-bit, rows out_s apart
   const void *bias, *gate;
   const void* residual;
-  void* z;                // the sums before the activation, rows of J (nullable)
+  float* z;               // the sums before the activation, rows of J (nullable)
   const float* unscale;   // a factor for each row (nullable)
   float* part;            // parts along k: [part][I][J rounded up to 8]
   int64_t out_s, res_s, I, J;
-  int32_t act, pf32, z16; // pf32: bias and gate are fp32; z16: z is fp16, else fp32
+  int32_t act, pf32;      // pf32: bias and gate are fp32
   int32_t wide;           // whole 16-byte groups of 8 can be loaded and stored
 };
 
@@ -132,43 +132,18 @@ __device__ __forceinline__ void param8(const void* p, int pf32, int wide, int64_
   }
 }
 
-// n sums (8: whole groups) kept at `at` of z for the backward.  In fp16 (where the gradients are
-// bf16's and no gate's sum is formed from it) a slope formed from z is off by 2^-11 of z times a
-// second derivative below one, an eighth of what rounding dz costs; beyond 65,504 it is
-// kept as infinite, where every slope is 0 or 1; a ReLU's sign is kept where z would round to 0.
-template <int ACT>
+// n sums (8: whole groups) kept at `at` of z for the backward, in fp32: a slope takes the relative error of
+// z times z act'' / act', which is 5 and more where an activation runs out (as fp16, half the bytes, sums of -10
+// cost a SiLU's gradients up to 0.4 %, as much as rounding dz to bf16, and alike in all rows of a column).
 __device__ __forceinline__ void keep8(const Finish& f, int64_t at, int n, const float (&v)[8]) {
-  if (!f.z16) {
-    float* z = static_cast<float*>(f.z) + at;
-    if (n == 8 && f.wide) {
-      reinterpret_cast<f32x4*>(z)[0] = f32x4{v[0], v[1], v[2], v[3]};
-      reinterpret_cast<f32x4*>(z)[1] = f32x4{v[4], v[5], v[6], v[7]};
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < n) z[e] = v[e];
-    }
-    return;
-  }
-  __bf16* z = static_cast<__bf16*>(f.z) + at;  // fp16 by its bits
-  bf16x8 y;
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    float a = v[e], b = v[e + 1];
-    if (ACT == kActRelu) {
-      a = a > 0.f ? fmaxf(a, 6e-8f) : a;
-      b = b > 0.f ? fmaxf(b, 6e-8f) : b;
-    }
-    const bf16x2 w = pack2<true>(a, b);
-    y[e] = w[0];
-    y[e + 1] = w[1];
-  }
+  float* z = f.z + at;
   if (n == 8 && f.wide) {
-    *reinterpret_cast<bf16x8*>(z) = y;
+    reinterpret_cast<f32x4*>(z)[0] = f32x4{v[0], v[1], v[2], v[3]};
+    reinterpret_cast<f32x4*>(z)[1] = f32x4{v[4], v[5], v[6], v[7]};
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < n) z[e] = y[e];
+      if (e < n) z[e] = v[e];
   }
 }
 
@@ -217,12 +192,8 @@ __device__ __forceinline__ void finish_down(const Finish& f, int64_t i, int64_t 
   }
   if (f.z)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float one[8] = {v[e]};
-      if (e >= n) continue;
-      if (f.act == kActRelu) keep8<kActRelu>(f, (i + e * STEP) * f.J + j, 1, one);
-      else keep8<kActNone>(f, (i + e * STEP) * f.J + j, 1, one);
-    }
+    for (int e = 0; e < 8; ++e)
+      if (e < n) f.z[(i + e * STEP) * f.J + j] = v[e];
   act8_of(f.act, v);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -248,10 +219,7 @@ __device__ __forceinline__ void finish8(const Finish& f, int64_t i, int64_t j, f
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += x[e];
   }
-  if (f.z) {
-    if (f.act == kActRelu) keep8<kActRelu>(f, i * f.J + j, n, v);
-    else keep8<kActNone>(f, i * f.J + j, n, v);
-  }
+  if (f.z) keep8(f, i * f.J + j, n, v);
   act8_of(f.act, v);
   if (f.gate) {
     param8<F16>(f.gate, f.pf32, f.wide, j, n, x);

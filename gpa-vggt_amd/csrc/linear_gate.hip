@@ -1,7 +1,6 @@
 // A projection with what follows it: y = residual + gate act(x w^T + bias), 16-bit
 // operands, fp32 from the products to the one rounding of y.  act: none, GELU (erf and
-// tanh forms), SiLU, ReLU.  For gradients the sum before the activation is kept (z), in fp32 or,
-// where the gradients are coarser anyway, in fp16 (linear_gate.h, keep8).
+// tanh forms), SiLU, ReLU.  For gradients the sum before the activation is kept (z, fp32).
 //
 // Many rows: linear_gemm.h.  Up to 16 rows (a decode step) the weight's bytes bound it,
 // and linear_rows_kernel streams them: 16 of its rows a workgroup, straight into the
@@ -196,15 +195,15 @@ extern "C" int gpa_linear_gate(int dtype, int param_dtype, const gpa_linear_gate
   gpa_clear_error();
   const int rc = linear_check(fn, dtype, param_dtype, a);
   if (rc != GPA_OK || a->M == 0 || a->N == 0) return rc;
-  if (!y || (z && ((uintptr_t)z % 16 || (z_dtype != GPA_DTYPE_F32 && z_dtype != GPA_DTYPE_F16)))) {
-    gpa_set_error("%s: null output, or z that is not 16-byte aligned fp32 or fp16", fn);
+  if (!y || (z && ((uintptr_t)z % 16 || z_dtype != GPA_DTYPE_F32))) {
+    gpa_set_error("%s: null output, or z that is not 16-byte aligned fp32", fn);
     return GPA_E_INVALID;
   }
   const int64_t psize = param_dtype == GPA_DTYPE_F32 ? 4 : 2;
   Finish f{};
   f.out = y; f.out_s = y_s;
   f.bias = a->bias; f.gate = a->gate; f.residual = a->residual; f.res_s = a->residual_s;
-  f.z = z; f.z16 = z_dtype == GPA_DTYPE_F16;
+  f.z = (float*)z;
   f.I = a->M; f.J = a->N;
   f.act = a->act; f.pf32 = psize == 4;
   auto fine = [&](const void* p, int64_t s) { return !p || ((uintptr_t)p % 16 == 0 && (a->M < 2 || s % 8 == 0)); };

@@ -21,7 +21,7 @@ namespace {
 
 struct DzArgs {
   const void* dy;
-  const void* z;
+  const float* z;
   const void* gate;
   void* dz;               // rows of J8, the columns past J zeros; null: not wanted
   void* bare;             // fp16 with a gate: dw's, without it; null: not wanted
@@ -29,7 +29,7 @@ struct DzArgs {
   float* gate32;          // where the gate goes, the scales of dw's rows; null: not wanted
   float* part;            // [chunk][2][J]; null: no sums
   int64_t dy_s, I, J, J8, chunk;
-  int32_t pf32, z16, gate_wide;
+  int32_t pf32, gate_wide;
 };
 
 // The scale of each row of dz in fp16, by its largest finite dy gate: a wave a row.
@@ -105,17 +105,13 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzArgs a) {
       const __bf16* DY = static_cast<const __bf16*>(a.dy) + i * a.dy_s + j;
       if constexpr (WIDE) {
         param8<F16>(DY, 0, 1, 0, 8, dy);
-        if (a.z && a.z16) param8<true>(static_cast<const uint16_t*>(a.z) + i * a.J + j, 0, 1, 0, 8, z);
-        else if (a.z) param8<true>(static_cast<const float*>(a.z) + i * a.J + j, 1, 1, 0, 8, z);
+        if (a.z) param8<F16>(a.z + i * a.J + j, 1, 1, 0, 8, z);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const bool in = j + e * 64 < a.J;
           dy[e] = in ? half_to_f32<F16>(DY[e * 64]) : 0.f;
-          z[e] = 0.f;
-          if (!a.z || !in) continue;
-          z[e] = a.z16 ? half_to_f32<true>(static_cast<const __bf16*>(a.z)[i * a.J + j + e * 64])
-                       : static_cast<const float*>(a.z)[i * a.J + j + e * 64];
+          z[e] = a.z && in ? a.z[i * a.J + j + e * 64] : 0.f;
         }
       }
 #pragma unroll
@@ -277,7 +273,7 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
     gpa_set_error("%s: nothing to sum, so the gradients are zeros that the caller writes", fn);
     return GPA_E_INVALID;
   }
-  if (!g->dy || (g->dgate && !a->gate) || (g->z && ((uintptr_t)g->z % 16 || (g->z_dtype != GPA_DTYPE_F32 && g->z_dtype != GPA_DTYPE_F16))) ||
+  if (!g->dy || (g->dgate && !a->gate) || (g->z && ((uintptr_t)g->z % 16 || g->z_dtype != GPA_DTYPE_F32)) ||
       (!g->z && (a->act != kActNone || g->dgate))) {
     gpa_set_error("%s: dy is needed, z with an activation or the gate's gradient, and there is none of an absent gate", fn);
     return GPA_E_INVALID;
@@ -310,7 +306,7 @@ extern "C" int gpa_linear_gate_bwd(int dtype, int param_dtype, const gpa_linear_
   if (e == hipSuccess && (need_dz || sums)) {
     DzArgs d{};
     d.dy = g->dy; d.dy_s = a->M > 1 ? g->dy_s : 0;
-    d.z = g->z; d.z16 = g->z_dtype == GPA_DTYPE_F16; d.gate = a->gate;
+    d.z = (const float*)g->z; d.gate = a->gate;
     d.gate_wide = (uintptr_t)a->gate % 16 == 0;
     d.dz = need_dz && (!apart || g->dx) ? ws : nullptr;
     d.bare = gates ? ws + p.bare : nullptr;

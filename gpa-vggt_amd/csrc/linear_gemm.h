@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256, PER_CU) void linear_gemm_kernel(GemmArgs a) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] += bias[e];
         }
-        if (a.out.z) keep8<ACT>(a.out, (i + it * RP) * a.out.J + j, 8, v);
+        if (a.out.z) keep8(a.out, (i + it * RP) * a.out.J + j, 8, v);
         act8<ACT>(v);
         if (a.out.gate) {
 #pragma unroll

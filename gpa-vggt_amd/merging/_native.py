@@ -2018,23 +2018,17 @@ def _linear_backward(ctx, dy, _):
     return some(0, dx), some(1, dw), some(2, db), some(3, dg), dy if ctx.needs_input_grad[4] else None, None, None
 
 
-def _z_dtype(x, gate):
-    """What the sums are kept in: an eighth of what rounding dz costs, or nothing."""
-    return torch.float16 if x.dtype == torch.bfloat16 and gate is None else torch.float32
-
-
 def linear_gate(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], gate: Optional[torch.Tensor],
                 residual: Optional[torch.Tensor], act: int, want_z: bool) -> Tuple[torch.Tensor, torch.Tensor]:
     """gpa_linear_gate: y [M, N] in x's type, and the sums before the activation
-    [M, N], if want_z (else an empty tensor), which gradients need where there is an
-    activation or a gate: fp32, but fp16 of bf16 operands without a gate.  act as
-    the header's GPA_ACT_*."""
+    fp32 [M, N], if want_z (else an empty tensor), which gradients need where there is an
+    activation or a gate.  act as the header's GPA_ACT_*."""
     what = "gpa::linear_gate"
     dev = _require_gpu(*[t for t in (x, w, bias, gate, residual) if t is not None])
     pdt = _linear_check(what, x, w, bias, gate, residual, act)
     M, N = x.shape[0], w.shape[0]
     y = torch.empty(M, N, device=dev, dtype=x.dtype)
-    z = torch.empty((M, N) if want_z else (0,), device=dev, dtype=_z_dtype(x, gate))
+    z = torch.empty((M, N) if want_z else (0,), device=dev, dtype=torch.float32)
     if M == 0 or N == 0:
         return y, z
     x, w, residual = _feature_rows(x), _feature_rows(w), None if residual is None else _feature_rows(residual)
@@ -2057,7 +2051,7 @@ linear_gate = _op(linear_gate, _linear_setup, _linear_backward, direct=True)
 @_fake("linear_gate")
 def _linear_gate_fake(x, w, bias, gate, residual, act, want_z):
     size = (x.shape[0], w.shape[0])
-    return x.new_empty(size), x.new_empty(size if want_z else (0,), dtype=_z_dtype(x, gate))
+    return x.new_empty(size), x.new_empty(size if want_z else (0,), dtype=torch.float32)
 
 
 @functools.partial(_op, direct=True)
@@ -2074,8 +2068,8 @@ def linear_gate_bwd(dy: torch.Tensor, z: Optional[torch.Tensor], x: torch.Tensor
         raise ValueError(f"{what}: no gradient of an absent bias or gate")
     if z is None and (act or want_gate):
         raise ValueError(f"{what}: an activation, and the gate's gradient, need z")
-    if z is not None and (z.dtype not in (torch.float32, torch.float16) or z.shape != (M, N) or not z.is_contiguous() or z.data_ptr() % 16):
-        raise ValueError(f"{what}: z must be contiguous fp32 or fp16 [{M}, {N}], got {z.dtype} {tuple(z.shape)}")
+    if z is not None and (z.dtype != torch.float32 or z.shape != (M, N) or not z.is_contiguous() or z.data_ptr() % 16):
+        raise ValueError(f"{what}: z must be contiguous fp32 [{M}, {N}], got {z.dtype} {tuple(z.shape)}")
     return _linear_grads(dy, z, x, w, bias, gate, act, want_x, want_w, want_bias, want_gate)
 
 

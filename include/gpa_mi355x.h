@@ -714,9 +714,8 @@ int gpa_attn_tree(int dtype, const gpa_attn_tree_args* args, void* workspace, si
  * bias and gate [N] (of dtype or fp32) and residual [M, N] (dtype) may be NULL.  act:
  * GPA_ACT_*.  fp32 inside (GELU's distribution is off by 8e-8 absolutely), y rounded once.
  * K that is no multiple of 8, rows of x or w that are not 16-byte aligned, and strides of
- * 2^21 or more cost padded copies in the workspace.  z (NULL: not kept): [M, N] contiguous, 16-byte aligned, z_dtype
- * fp32 or fp16 (the nearest value, beyond the range infinite), for the backward, which
- * needs it with an activation or for the gate's gradient.
+ * 2^21 or more cost padded copies in the workspace.  z (NULL: not kept): [M, N] contiguous, 16-byte aligned
+ * fp32 (z_dtype GPA_DTYPE_F32), for the backward, which needs it with an activation or for the gate's gradient.
  * workspace: gpa_linear_gate_workspace_bytes(...), 16-byte aligned.
  */
 enum { GPA_ACT_NONE = 0, GPA_ACT_GELU = 1, GPA_ACT_GELU_TANH = 2, GPA_ACT_SILU = 3, GPA_ACT_RELU = 4 };

@@ -114,3 +114,12 @@ def test_too_many_columns_of_few_rows(M, K):
     """More than 2^32 threads, which a launch does not have."""
     a = _args(M=M, N=(1 << 26) + 1, K=K, x_s=K, w_s=K)
     assert _native.lib().gpa_linear_gate(1, 1, ctypes.byref(a), FAKE, 1 << 27, None, 0, None, 0, None) == UNS
+
+
+def test_kept_sums_are_fp32():
+    L, a = _native.lib(), _args(act=1)
+    for zdt in (_native._DTYPE_CODES[torch.bfloat16], _native._DTYPE_CODES[torch.float16]):
+        assert L.gpa_linear_gate(1, 1, ctypes.byref(a), FAKE, 64, FAKE, zdt, FAKE, 1 << 30, None) == INV
+        g = _fields(_native._LinearGrads, dict(dy=FAKE, z=FAKE, dx=FAKE, dy_s=64, dx_s=128, z_dtype=zdt), {})
+        assert L.gpa_linear_gate_bwd(1, 1, ctypes.byref(a), ctypes.byref(g), FAKE, 1 << 40, None) == INV
+    assert torch.ops.gpa.linear_gate.default(X.to("meta"), W.to("meta"), None, None, None, 1, True)[1].dtype == torch.float32
