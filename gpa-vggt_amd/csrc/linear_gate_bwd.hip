@@ -32,16 +32,17 @@ struct DzArgs {
   int32_t pf32, gate_wide;
 };
 
-// The scale of each row of dz in fp16, by its largest finite dy gate: a wave a row.
+// The scale of each row of dz in fp16, by its largest finite dy gate: a workgroup a row (a wave a
+// row: 8.4 us for 4.3 at 1,374 rows of 1,001).
 template <bool WIDE>
 __global__ __launch_bounds__(256) void linear_scale_kernel(DzArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
+  __shared__ float top[4];
+  const int64_t i = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
   if (i >= a.I) return;
   const __bf16* DY = static_cast<const __bf16*>(a.dy) + i * a.dy_s;
   float m = 0.f;
   constexpr int AT = WIDE ? 8 : 1;
-  for (int64_t j = lane * AT; j < a.J; j += 64 * AT) {
+  for (int64_t j = threadIdx.x * AT; j < a.J; j += 256 * AT) {
     float dy[8], g[8];
     if constexpr (WIDE) {
       param8<true>(DY + j, 0, 1, 0, 8, dy);
@@ -58,9 +59,12 @@ __global__ __launch_bounds__(256) void linear_scale_kernel(DzArgs a) {
   }
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+  if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
   int e = 14;
   if (m > 0.f) frexpf(m, &e);                  // m = [0.5, 1) 2^e
-  if (lane == 0) a.unscale[i] = ldexpf(1.0f, max(e - 14, -126));
+  if (threadIdx.x == 0) a.unscale[i] = ldexpf(1.0f, max(e - 14, -126));
 }
 
 // 512 columns (eight a lane: side by side where they come in aligned groups (WIDE), else each 64
@@ -229,7 +233,7 @@ void dz_gate(const DzArgs& d, int act, dim3 grid, hipStream_t s) {
 }
 hipError_t dz_launch(const DzArgs& d, int act, bool f16, bool wide, dim3 grid, hipStream_t s) {
   if (d.dz && d.unscale) {
-    const int64_t wgs = (d.I + 3) / 4, most = (int64_t)1 << 22;   // (a launch has less than 2^32 threads, also of one dimension)
+    const int64_t wgs = d.I, most = (int64_t)1 << 22;   // (a dimension has less than 2^32 threads)
     const dim3 rows((unsigned)std::min(wgs, most), (unsigned)((wgs + most - 1) / most));
     if (wide) hipLaunchKernelGGL((linear_scale_kernel<true>), rows, dim3(256), 0, s, d);
     else hipLaunchKernelGGL((linear_scale_kernel<false>), rows, dim3(256), 0, s, d);
