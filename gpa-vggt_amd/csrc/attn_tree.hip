@@ -7,7 +7,8 @@
 //
 // Positions: key j of the cache stands at j, a drafted token at length + depth, its depth
 // being one less than its bits; so token i lies as far from a drafted token j that it sees
-// as it sees tokens behind j, which the bits alone tell.
+// as it sees tokens behind j, which the bits alone tell.  (Of a tree's bits, in which a row has its token's
+// ancestors and itself.  Any others are taken as masks; by a slope they are weighed as if they were a tree's.)
 //
 // gpa_draft_tree makes the bits and the positions from the tokens' parents, once a step:
 // a thread a token walks up its ancestors, whose numbers fall, so its words fill from the
@@ -37,9 +38,10 @@ namespace {
 
 constexpr int kTreeCus = 256;
 constexpr int kLeastTiles = 8;           // of a piece
-// Longer sequences are cut.  A launch for the join is worth 30 tiles to up to 32 rows (22 tiles whole
-// 10.1 us, cut 11.9; 63 whole 15.5, cut 12.0) and 12 to more (head dim 64, 10 tiles 13.3 and 15.4, 17
-// tiles 16.6 and 15.5).
+// Sequences are cut where the caches' buffer has more tiles than this: the host knows its size and not
+// the lengths, so short sequences in a long buffer are cut and joined too.  A launch for the join is worth
+// 30 tiles to up to 32 rows (22 tiles whole 10.1 us, cut 11.9; 63 whole 15.5, cut 12.0) and 12 to more
+// (head dim 64, 10 tiles 13.3 and 15.4, 17 tiles 16.6 and 15.5).
 constexpr int kSplitFew = 32, kSplitMany = 12;
 constexpr int64_t kMaxDraft = 1024;
 
@@ -138,7 +140,7 @@ __device__ __forceinline__ Drafted locate_drafted(const TreeArgs& p, const Where
   x.bits = p.seen + x.b * p.seen_sb + x.tok * p.seen_st;
   int n = 0;
   for (int i = 0; i < p.words; ++i) n += __popc(i == p.words - 1 ? x.bits[i] & (0xffffffffu >> (31 & (32 * p.words - p.T))) : x.bits[i]);
-  x.blind = !x.live || n == 0;                 // a token that does not see itself sees nothing
+  x.blind = !x.live || n == 0;                 // a token that sees no drafted one sees nothing
   x.lo = x.w_lo = x.a_lo = 0;
   x.hi = x.a_hi = w.len;
   x.at = w.len + n - 1;

@@ -17,7 +17,7 @@
 // What bounds it: the matrix instructions, by the power that they take.  8,192 x 4,096 x 4,096 in bf16:
 // 210 to 221 us (1,240 to 1,310 TFLOP/s; 1,594 is what a product of 16,384^3 reaches in the vendor's
 // library, which takes 218 to 222 us here), its turned forms 207 to 237 (the library 254 and 287);
-// bias, tanh GELU, residual and the sums kept for the backward add 60 to 75 us of stores and arithmetic.
+// bias, tanh GELU, residual and the fp32 sums kept for the backward add 65 to 75 us of stores and arithmetic.
 #pragma once
 
 #include <type_traits>

@@ -235,7 +235,8 @@ def attention_tree(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
     others of that form).  A token that sees no drafted one, not even itself, sees
     nothing: zeros, LSE -inf.  Scores, dtypes, strides and results as in
     `attention_masked`; with slopes a token lies |difference of positions| from a key,
-    as `draft_tree` counts them.  Forward only.
+    as `draft_tree` counts them, which the bits tell if they are a tree's (a token's ancestors
+    and itself): with slopes they have to be.  Forward only.
     """
     what = "attention_tree"
     sm_scale, cap = _score_args(what, sm_scale, cap, slopes)

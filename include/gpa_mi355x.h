@@ -686,8 +686,9 @@ int gpa_draft_tree(const int32_t* parents, int64_t parents_sb, const int32_t* le
  * rows of `seen` ([B, T, ceil(T / 32)], contiguous, as gpa_draft_tree makes) name.
  * Scores, formats and results as gpa_attn_masked; the distance that a slope weighs
  * is to position j of the cache from length + (bits of the row) - 1, and to a drafted
- * token the number of seen tokens behind it.  A token with no bit gets zeros (LSE
- * -inf).  D 64 or 128, T <= 1,024.  Sums run in a fixed order.  workspace:
+ * token the number of seen tokens behind it (the differences of positions where the bits are a tree's,
+ * a token's ancestors and itself).  A token with no bit gets zeros (LSE -inf).  D 64 or
+ * 128, T <= 1,024.  Sums run in a fixed order.  workspace:
  * gpa_attn_tree_workspace_bytes(...), 16-byte aligned.
  */
 typedef struct gpa_attn_tree_args {
